@@ -53,7 +53,8 @@ typedef enum tropnn_b200_dtype {
   TROPNN_B200_BF16 = 2,
   TROPNN_B200_U8 = 3,  /* packed route indices (cells <= 256) */
   TROPNN_B200_I16 = 4, /* packed route indices (cells <= 32767) */
-  TROPNN_B200_I64 = 5  /* route indices otherwise */
+  TROPNN_B200_I64 = 5, /* route indices otherwise */
+  TROPNN_B200_I32 = 6  /* token indices of the distillation operators */
 } tropnn_b200_dtype;
 
 /* STE surrogates of layers/surrogate.py:9-17. */
@@ -607,6 +608,105 @@ TROPNN_B200_API int tropnn_b200_trop_backward(const float *grad_hidden, const fl
                               const float *margins, float code_scale, int training,
                               float *grad_latent, void *grad_router_weight, void *grad_router_bias,
                               void *grad_code, void *workspace, size_t workspace_bytes, void *stream);
+
+/* -------------------------------------------------------- token operators
+ *
+ * What a token model of routed layers needs around them; no reference counterpart.
+ */
+
+/*
+ * Gated linear recurrence over [batch, steps, dim], per channel, with a = sigmoid(gate):
+ *   h_t = keep_t a_t h_{t-1} + (1 - a_t) value_t,  keep_t = 0 where reset[b, t] != 0, else 1
+ * gate and value in `dtype` (F32/F16/BF16) with strides in elements over batch and steps and unit
+ * stride over dim; h0 f32 [batch, dim] (NULL: zeros), reset u8 [batch, steps] (NULL: none). h
+ * [batch, steps, dim] contiguous in `dtype`, h_last f32 [batch, dim] (h0 when steps is 0). The
+ * state is f32 throughout. `saved` (NULL: not kept) receives the f32 states that the backward
+ * starts from, tropnn_b200_recurrence_saved_size bytes. Deterministic; no workspace.
+ */
+TROPNN_B200_API size_t tropnn_b200_recurrence_saved_size(int64_t batch, int64_t steps, int64_t dim);
+TROPNN_B200_API int tropnn_b200_recurrence_forward(const void *gate, int64_t gate_batch_stride, int64_t gate_step_stride,
+                                   const void *value, int64_t value_batch_stride, int64_t value_step_stride,
+                                   int dtype, const float *h0, const uint8_t *reset, int64_t batch, int64_t steps,
+                                   int64_t dim, void *h, float *h_last, float *saved, size_t saved_bytes,
+                                   void *stream);
+
+/*
+ * Its backward: grad [batch, steps, dim] contiguous in `dtype` (NULL: zeros) and grad_last f32
+ * [batch, dim] (NULL: zeros) are the gradients of h and h_last; grad_gate and grad_value
+ * (contiguous, `dtype`) and grad_h0 (f32 [batch, dim], NULL: skipped) are written. `saved` is the
+ * forward's. Deterministic.
+ */
+TROPNN_B200_API int tropnn_b200_recurrence_backward(const void *gate, int64_t gate_batch_stride, int64_t gate_step_stride,
+                                    const void *value, int64_t value_batch_stride, int64_t value_step_stride,
+                                    int dtype, const uint8_t *reset, int64_t batch, int64_t steps, int64_t dim,
+                                    const float *saved, size_t saved_bytes, const void *grad,
+                                    const float *grad_last, void *grad_gate, void *grad_value, float *grad_h0,
+                                    void *stream);
+
+/*
+ * One token of the recurrence: state (f32 [batch, dim], row stride in elements) is updated in
+ * place, h [batch, dim] contiguous receives it rounded to `dtype`. reset u8 [batch] or NULL.
+ */
+TROPNN_B200_API int tropnn_b200_recurrence_step(const void *gate, int64_t gate_stride, const void *value, int64_t value_stride,
+                                int dtype, const uint8_t *reset, int64_t batch, int64_t dim, float *state,
+                                int64_t state_stride, void *h, void *stream);
+
+/*
+ * Distillation from a teacher's top logits, mixed with the label cross-entropy. For row n:
+ *   q = softmax(teacher / T) over the row's entries with an index in [0, vocab) and a logit above
+ *   -inf, p = softmax(logits / T), p1 = softmax(logits)
+ *   loss = (1 - w) T^2 sum_k q_k (log q_k - log p[index_k]) + w (-log p1[label])
+ * w = label_weight. A label that is ignore_index or outside [0, vocab) gives no label term, a row
+ * without entries no teacher term; a row with neither ("without a target") has loss 0 and gradient
+ * 0. Entries of one index add up. logits: row n of `vocab` elements at
+ * (n / inner) * outer_stride + (n % inner) * inner_stride; teacher [rows, top] and indices
+ * [rows, top] (I32/I64) contiguous, top <= 1024; labels int64 [rows] or NULL. losses f32 [rows];
+ * stats f32 [rows, 4], 16-byte aligned (NULL: not kept), for distill_reduce and distill_grad.
+ */
+TROPNN_B200_API int tropnn_b200_distill_loss(const void *logits, int dtype, int64_t rows, int64_t inner, int64_t outer_stride,
+                             int64_t inner_stride, int64_t vocab, const void *teacher, int teacher_dtype,
+                             const void *indices, int index_dtype, int64_t top, const int64_t *labels,
+                             int64_t ignore_index, float temperature, float label_weight, float *losses,
+                             float *stats, void *stream);
+
+/* *loss = sum of losses in a fixed order, over the rows with a target if mean != 0 (0 where none
+ * has one); *count = the divisor (1 for a sum). */
+TROPNN_B200_API int tropnn_b200_distill_reduce(const float *losses, const float *stats, int64_t rows, int mean, float *loss,
+                               float *count, void *stream);
+
+/* The gradient of sum_n scale_n loss_n, scale_n = row_scale[n, or 0 unless scale_per_row] /
+ * max(*count, 1) (row_scale NULL: 1, count NULL: 1), into grad [rows, vocab] contiguous, dtype of
+ * the logits. `stats` is distill_loss's. */
+TROPNN_B200_API int tropnn_b200_distill_grad(const void *logits, int dtype, int64_t rows, int64_t inner, int64_t outer_stride,
+                             int64_t inner_stride, int64_t vocab, const void *teacher, int teacher_dtype,
+                             const void *indices, int index_dtype, int64_t top, const int64_t *labels,
+                             int64_t ignore_index, float temperature, float label_weight, const float *stats,
+                             const float *row_scale, int scale_per_row, const float *count, void *grad,
+                             void *stream);
+
+/* distill_loss and distill_grad (count 1) in one launch. */
+TROPNN_B200_API int tropnn_b200_distill_loss_grad(const void *logits, int dtype, int64_t rows, int64_t inner,
+                                  int64_t outer_stride, int64_t inner_stride, int64_t vocab, const void *teacher,
+                                  int teacher_dtype, const void *indices, int index_dtype, int64_t top,
+                                  const int64_t *labels, int64_t ignore_index, float temperature,
+                                  float label_weight, const float *row_scale, int scale_per_row, float *losses,
+                                  void *grad, void *stream);
+
+/*
+ * One token id a row from logits (rows as in distill_loss) and a uniform number in [0, 1) a row.
+ * Tokens rank by (logit descending, index ascending) and weigh round(2^31 exp((x - max) / T)), a
+ * whole number; kept are the first top_k of them (<= 0: all), of those the ones with less than
+ * top_p of their weight before them, of those the ones with exp((x - max) / T) >= min_p, and the
+ * first one always. The token is the first in index order whose running kept weight exceeds
+ * floor(u * total). temperature <= 0: the first of the ranking. A row with a NaN, or with nothing
+ * above -inf, gives -1. Each setting comes as a device array of one a row (top_k I32/I64) or, where
+ * that is NULL, as a value. Deterministic and independent of the batch.
+ */
+TROPNN_B200_API int tropnn_b200_sample_tokens(const void *logits, int dtype, int64_t rows, int64_t inner, int64_t outer_stride,
+                              int64_t inner_stride, int64_t vocab, const float *uniforms,
+                              const float *temperature, float temperature_value, const void *top_k,
+                              int top_k_dtype, int64_t top_k_value, const float *top_p, float top_p_value,
+                              const float *min_p, float min_p_value, int64_t *tokens, void *stream);
 
 #ifdef __cplusplus
 }

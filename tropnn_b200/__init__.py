@@ -6,6 +6,9 @@ Public surface:
     layers with the reference's constructor arguments, parameters and ``state_dict``.
   * ``trop_route_hidden_b200``, ``pairwise_b200`` — the operator-level entry points
     (mirroring ``trop_route_hidden_tilelang`` / ``pairwise_tilelang``).
+  * ``gated_recurrence_b200``, ``gated_recurrence_step_b200``, ``distill_loss_b200``,
+    ``distill_loss_grad_b200``, ``sample_tokens_b200`` — what a token model of routed layers
+    needs around them: the sequence mixer, its training loss and its sampler.
   * ``register(tropnn)`` — lets the reference package's own classes accept
     ``backend="b200"``.
   * ``tropnn_b200.distributed`` — batch-row sharding and gradient all-reduce for
@@ -32,16 +35,28 @@ from .ops import (
     trop_route_hidden_b200,
     trop_route_hidden_packed,
 )
+from .token_ops import (
+    distill_loss_b200,
+    distill_loss_grad_b200,
+    gated_recurrence_b200,
+    gated_recurrence_step_b200,
+    sample_tokens_b200,
+)
 
 __all__ = [
     "PairwiseLinear",
     "RoutedLinearBase",
     "TropFanLinear",
     "TropLinear",
+    "distill_loss_b200",
+    "distill_loss_grad_b200",
+    "gated_recurrence_b200",
+    "gated_recurrence_step_b200",
     "packed_route_index_dtype",
     "pairwise_anchor_index",
     "pairwise_b200",
     "register",
+    "sample_tokens_b200",
     "trop_route_hidden_b200",
     "trop_route_hidden_packed",
 ]

@@ -17,10 +17,10 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libtropnn_b200.so"
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 # tropnn_b200_dtype
-F32, F16, BF16, U8, I16, I64 = 0, 1, 2, 3, 4, 5
+F32, F16, BF16, U8, I16, I64, I32 = 0, 1, 2, 3, 4, 5, 6
 # tropnn_b200_surrogate
 SURROGATES = {"fast_sigmoid_odd": 0, "izhikevich": 1}
 
@@ -41,6 +41,11 @@ _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
+
+# The rows, targets and weights that the three distillation entry points share.
+_DISTILL_ROWS: list[object] = [
+    _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _i32, _p, _i32, _i64, _p, _i64, _f32, _f32
+]
 
 # name -> (restype, argtypes), in the order of include/tropnn_b200.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -129,6 +134,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tropnn_b200_trop_backward": (
         _i32,
         [_p, _p, _i64, _i64, _p, _p, _i32, _i64, _i64, _p, _p, _i32, _p, _f32, _i32, _p, _p, _p, _p, _p, _sz, _p],
+    ),
+    "tropnn_b200_recurrence_saved_size": (_sz, [_i64, _i64, _i64]),
+    "tropnn_b200_recurrence_forward": (
+        _i32, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _i64, _i64, _i64, _p, _p, _p, _sz, _p]
+    ),
+    "tropnn_b200_recurrence_backward": (
+        _i32,
+        [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64, _i64, _p, _sz, _p, _p, _p, _p, _p, _p],
+    ),
+    "tropnn_b200_recurrence_step": (_i32, [_p, _i64, _p, _i64, _i32, _p, _i64, _i64, _p, _i64, _p, _p]),
+    "tropnn_b200_distill_loss": (_i32, [*_DISTILL_ROWS, _p, _p, _p]),
+    "tropnn_b200_distill_reduce": (_i32, [_p, _p, _i64, _i32, _p, _p, _p]),
+    "tropnn_b200_distill_grad": (_i32, [*_DISTILL_ROWS, _p, _p, _i32, _p, _p, _p]),
+    "tropnn_b200_distill_loss_grad": (_i32, [*_DISTILL_ROWS, _p, _i32, _p, _p, _p]),
+    "tropnn_b200_sample_tokens": (
+        _i32,
+        [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _i32, _i64, _p, _f32, _p, _f32, _p, _p],
     ),
 }
 

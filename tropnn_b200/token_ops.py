@@ -1,0 +1,456 @@
+"""Operators of a token model around the routed layers, over the sm_100a C ABI.
+
+* ``gated_recurrence_b200`` / ``gated_recurrence_step_b200``: the sequence mixer, for whole
+  sequences (differentiable) and for one decoded token.
+* ``distill_loss_b200`` / ``distill_loss_grad_b200``: the loss of a student's logits against a
+  teacher's top logits, through autograd or with the gradient in the same launch.
+* ``sample_tokens_b200``: temperature, top-k, top-p and min-p sampling from given uniform numbers.
+
+The reference has no counterpart of these. They keep the conventions of the other operators:
+CUDA tensors only (``ValueError`` otherwise, there is no CPU path), ``TypeError`` for a dtype,
+kernels on ``torch.cuda.current_stream()``, buffers from PyTorch's caching allocator, no host
+synchronisation, deterministic results.
+"""
+
+from __future__ import annotations
+
+import math
+from contextlib import AbstractContextManager, nullcontext
+from typing import Any
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _native as nat
+from .ops import _launch, _require_cuda
+
+__all__ = [
+    "distill_loss_b200",
+    "distill_loss_grad_b200",
+    "gated_recurrence_b200",
+    "gated_recurrence_step_b200",
+    "sample_tokens_b200",
+]
+
+MAX_TEACHER_TOP = 1024
+_REDUCTIONS = ("mean", "sum", "none")
+
+
+def _on(device: torch.device) -> AbstractContextManager[Any]:
+    """The device's context, without the cost of entering it where it is current."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _same_device(device: torch.device, **tensors: Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _require_cuda(t, name)
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _unit_last(t: Tensor) -> Tensor:
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+# ---------------------------------------------------------------------------
+# gated linear recurrence
+# ---------------------------------------------------------------------------
+
+
+class _GatedRecurrenceFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(  # type: ignore[override]
+        ctx: Any, gate: Tensor, value: Tensor, h0: Tensor | None, reset: Tensor | None, keep: bool
+    ) -> tuple[Tensor, Tensor]:
+        batch, steps, dim = gate.shape
+        dev = gate.device
+        lib = nat.load()
+        h = torch.empty((batch, steps, dim), device=dev, dtype=gate.dtype)
+        h_last = torch.empty((batch, dim), device=dev, dtype=torch.float32)
+        saved_bytes = lib.tropnn_b200_recurrence_saved_size(batch, steps, dim) if keep else 0
+        saved = torch.empty(saved_bytes // 4, device=dev, dtype=torch.float32) if keep else None
+        with _on(dev):
+            _launch(
+                "recurrence_forward", lib.tropnn_b200_recurrence_forward, gate.data_ptr(), gate.stride(0),
+                gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype),
+                nat.ptr(h0), nat.ptr(reset), batch, steps, dim, h.data_ptr(), h_last.data_ptr(), nat.ptr(saved),
+                saved_bytes, nat.stream_handle(dev),
+            )
+        if keep:
+            ctx.save_for_backward(gate, value, reset, saved)
+            ctx.saved_bytes = saved_bytes
+            ctx.set_materialize_grads(False)
+        return h, h_last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad_h: Tensor | None, grad_last: Tensor | None) -> tuple[Any, ...]:
+        gate, value, reset, saved = ctx.saved_tensors
+        if grad_h is None and grad_last is None:
+            return None, None, None, None, None
+        batch, steps, dim = gate.shape
+        dev = gate.device
+        lib = nat.load()
+        grad_h = None if grad_h is None else grad_h.contiguous()
+        grad_last = None if grad_last is None else grad_last.contiguous()
+        grad_gate = torch.empty((batch, steps, dim), device=dev, dtype=gate.dtype)
+        grad_value = torch.empty((batch, steps, dim), device=dev, dtype=gate.dtype)
+        grad_h0 = torch.empty((batch, dim), device=dev, dtype=torch.float32) if ctx.needs_input_grad[2] else None
+        with _on(dev):
+            _launch(
+                "recurrence_backward", lib.tropnn_b200_recurrence_backward, gate.data_ptr(), gate.stride(0),
+                gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype),
+                nat.ptr(reset), batch, steps, dim, saved.data_ptr(), ctx.saved_bytes, nat.ptr(grad_h),
+                nat.ptr(grad_last), grad_gate.data_ptr(), grad_value.data_ptr(), nat.ptr(grad_h0),
+                nat.stream_handle(dev),
+            )
+        return grad_gate, grad_value, grad_h0, None, None
+
+
+def _check_gate_value(gate: Tensor, value: Tensor, ndim: int) -> None:
+    _require_cuda(gate, "gate")
+    _same_device(gate.device, value=value)
+    if gate.ndim != ndim or value.shape != gate.shape:
+        want = "[batch, steps, dim]" if ndim == 3 else "[batch, dim]"
+        raise ValueError(f"gate and value must both have shape {want}, got {tuple(gate.shape)} and {tuple(value.shape)}")
+    nat.float_code(gate.dtype)
+    if value.dtype != gate.dtype:
+        raise TypeError(f"gate and value must have one dtype, got {gate.dtype} and {value.dtype}")
+
+
+def _check_reset(reset: Tensor | None, shape: tuple[int, ...], device: torch.device) -> Tensor | None:
+    if reset is None:
+        return None
+    _same_device(device, reset=reset)
+    if reset.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f"reset must be bool or uint8, got {reset.dtype}")
+    if reset.shape != shape:
+        raise ValueError(f"reset must have shape {shape}, got {tuple(reset.shape)}")
+    return reset.contiguous()
+
+
+def gated_recurrence_b200(
+    gate: Tensor, value: Tensor, h0: Tensor | None = None, *, reset: Tensor | None = None
+) -> tuple[Tensor, Tensor]:
+    """Gated linear recurrence over whole sequences, per channel:
+
+        h_t = keep_t * a_t * h_{t-1} + (1 - a_t) * value_t,   a = sigmoid(gate)
+
+    ``gate`` and ``value`` are ``[batch, steps, dim]`` in one of f32/f16/bf16, any batch and step
+    strides (the two halves of one projection's output are read in place). ``h0`` ``[batch, dim]``
+    is the state before the first token (zeros by default), ``reset`` ``[batch, steps]`` marks the
+    tokens that start a document: nothing of the state before them is kept. Returns ``(h, h_last)``:
+    ``h`` in the inputs' dtype and the last state in f32, which continues a sequence as ``h0`` of
+    the next call or as the state of ``gated_recurrence_step_b200``. The state is f32 throughout.
+    Differentiable in gate, value and h0 (once); the backward scans the states again from one in 64
+    saved ones instead of reading ``h``.
+    """
+    _check_gate_value(gate, value, 3)
+    batch, steps, dim = gate.shape
+    if h0 is not None:
+        _same_device(gate.device, h0=h0)
+        if h0.shape != (batch, dim):
+            raise ValueError(f"h0 must have shape {(batch, dim)}, got {tuple(h0.shape)}")
+        nat.float_code(h0.dtype)
+        h0 = h0.to(torch.float32).contiguous()
+    reset = _check_reset(reset, (batch, steps), gate.device)
+    gate, value = _unit_last(gate), _unit_last(value)
+    keep = torch.is_grad_enabled() and (
+        gate.requires_grad or value.requires_grad or (h0 is not None and h0.requires_grad)
+    )
+    return _GatedRecurrenceFunction.apply(gate, value, h0, reset, keep)
+
+
+def gated_recurrence_step_b200(gate: Tensor, value: Tensor, state: Tensor, *, reset: Tensor | None = None) -> Tensor:
+    """One token of ``gated_recurrence_b200`` for every row: ``gate`` and ``value`` ``[batch, dim]``,
+    ``state`` f32 ``[batch, dim]``, updated in place; ``reset`` ``[batch]`` clears a row's state
+    first. Returns the new state rounded to the inputs' dtype. Not differentiable."""
+    _check_gate_value(gate, value, 2)
+    _same_device(gate.device, state=state)
+    if state.shape != gate.shape:
+        raise ValueError(f"state must have shape {tuple(gate.shape)}, got {tuple(state.shape)}")
+    if state.dtype != torch.float32:
+        raise TypeError(f"state must be float32, got {state.dtype}")
+    batch, dim = gate.shape
+    if (dim > 1 and state.stride(1) != 1) or (batch > 1 and state.stride(0) < dim):
+        raise ValueError("state must have unit stride over dim and rows of its own")
+    if torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or state.requires_grad):
+        raise ValueError("gated_recurrence_step_b200 is not differentiable: call it under torch.no_grad()")
+    reset = _check_reset(reset, (batch,), gate.device)
+    gate, value = _unit_last(gate), _unit_last(value)
+    h = torch.empty((batch, dim), device=gate.device, dtype=gate.dtype)
+    with _on(gate.device):
+        _launch(
+            "recurrence_step", nat.load().tropnn_b200_recurrence_step, gate.data_ptr(), gate.stride(0),
+            value.data_ptr(), value.stride(0), nat.float_code(gate.dtype), nat.ptr(reset), batch, dim,
+            state.data_ptr(), state.stride(0), h.data_ptr(), nat.stream_handle(gate.device),
+        )
+    return h
+
+
+# ---------------------------------------------------------------------------
+# logits as rows
+# ---------------------------------------------------------------------------
+
+
+def _logit_rows(logits: Tensor) -> tuple[Tensor, int, int, int, int]:
+    """``(logits, rows, inner, outer_stride, inner_stride)``: row n of ``logits[..., vocab]`` starts
+    at element ``(n // inner) * outer_stride + (n % inner) * inner_stride``. A slice such as
+    ``logits[:, :-1]`` of a batch of sequences is read in place; other layouts are copied."""
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        logits = logits.contiguous()
+    shape, stride = logits.shape[:-1], logits.stride()[:-1]
+    if len(shape) == 2:
+        return logits, shape[0] * shape[1], max(1, shape[1]), stride[0], stride[1]
+    if len(shape) == 1:
+        return logits, shape[0], 1, stride[0], 0
+    logits = logits.contiguous()
+    rows = math.prod(shape)
+    return logits, rows, 1, logits.shape[-1], 0
+
+
+# ---------------------------------------------------------------------------
+# distillation
+# ---------------------------------------------------------------------------
+
+
+class _Distill:
+    """Checked arguments of one call, in the order of the C entry points."""
+
+    def __init__(
+        self, logits: Tensor, teacher: Tensor, indices: Tensor, labels: Tensor | None, temperature: float,
+        label_weight: float, ignore_index: int,
+    ) -> None:
+        _require_cuda(logits, "logits")
+        _same_device(logits.device, teacher_logits=teacher, teacher_indices=indices, labels=labels)
+        nat.float_code(logits.dtype)
+        nat.float_code(teacher.dtype)
+        if logits.ndim < 1 or logits.shape[-1] < 1:
+            raise ValueError(f"logits must have shape [..., vocab] with vocab >= 1, got {tuple(logits.shape)}")
+        lead = logits.shape[:-1]
+        if teacher.ndim != logits.ndim or teacher.shape[:-1] != lead or indices.shape != teacher.shape:
+            raise ValueError(
+                f"teacher_logits and teacher_indices must both have shape {(*lead, 'top')}, got {tuple(teacher.shape)} "
+                f"and {tuple(indices.shape)}"
+            )
+        if teacher.shape[-1] > MAX_TEACHER_TOP:
+            raise ValueError(f"at most {MAX_TEACHER_TOP} teacher entries a row, got {teacher.shape[-1]}")
+        if indices.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"teacher_indices must be int64 or int32, got {indices.dtype}")
+        if labels is not None:
+            if labels.shape != lead:
+                raise ValueError(f"labels must have shape {tuple(lead)}, got {tuple(labels.shape)}")
+            if labels.dtype not in (torch.int64, torch.int32):
+                raise TypeError(f"labels must be int64 or int32, got {labels.dtype}")
+        temperature, label_weight = float(temperature), float(label_weight)
+        if not (0.0 < temperature < math.inf):
+            raise ValueError(f"temperature must be positive and finite, got {temperature}")
+        if not (0.0 <= label_weight <= 1.0):
+            raise ValueError(f"label_weight must be in [0, 1], got {label_weight}")
+        if label_weight > 0.0 and labels is None:
+            raise ValueError("label_weight > 0 needs labels")
+        self.lead = lead
+        self.logits, self.rows, inner, outer_stride, inner_stride = _logit_rows(logits.detach())
+        self.teacher = teacher.detach().contiguous()
+        self.indices = indices.contiguous()
+        self.labels = None if labels is None else labels.to(torch.int64).contiguous()
+        self.args = (
+            self.logits.data_ptr(), nat.float_code(logits.dtype), self.rows, inner, outer_stride, inner_stride,
+            logits.shape[-1], self.teacher.data_ptr(), nat.float_code(teacher.dtype), self.indices.data_ptr(),
+            nat.I64 if indices.dtype == torch.int64 else nat.I32, teacher.shape[-1], nat.ptr(self.labels),
+            int(ignore_index), temperature, label_weight,
+        )
+
+    def grad_like(self) -> Tensor:
+        return torch.empty(self.logits.shape, device=self.logits.device, dtype=self.logits.dtype)
+
+
+class _DistillLossFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, logits: Tensor, call: _Distill, reduction: str) -> Tensor:  # type: ignore[override]
+        dev = logits.device
+        lib = nat.load()
+        losses = torch.empty(call.lead, device=dev, dtype=torch.float32)
+        stats = torch.empty((call.rows, 4), device=dev, dtype=torch.float32)
+        with _on(dev):
+            stream = nat.stream_handle(dev)
+            _launch("distill_loss", lib.tropnn_b200_distill_loss, *call.args, losses.data_ptr(), stats.data_ptr(), stream)
+            loss, count = losses, None
+            if reduction != "none":
+                loss = torch.empty((), device=dev, dtype=torch.float32)
+                count = torch.empty((), device=dev, dtype=torch.float32)
+                _launch("distill_reduce", lib.tropnn_b200_distill_reduce, losses.data_ptr(), stats.data_ptr(),
+                        call.rows, int(reduction == "mean"), loss.data_ptr(), count.data_ptr(), stream)
+        # The call holds its tensors' addresses; saving them finds out a change in place.
+        ctx.save_for_backward(logits, stats, count, call.teacher, call.indices, call.labels)
+        ctx.call = call
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad_loss: Tensor) -> tuple[Any, ...]:
+        logits, stats, count, *_ = ctx.saved_tensors
+        call = ctx.call
+        dev = logits.device
+        grad = call.grad_like()
+        scale = grad_loss.to(torch.float32).contiguous()
+        with _on(dev):
+            _launch("distill_grad", nat.load().tropnn_b200_distill_grad, *call.args, stats.data_ptr(), scale.data_ptr(),
+                    int(count is None), nat.ptr(count), grad.data_ptr(), nat.stream_handle(dev))
+        return grad, None, None
+
+
+def distill_loss_b200(
+    logits: Tensor,
+    teacher_logits: Tensor,
+    teacher_indices: Tensor,
+    labels: Tensor | None = None,
+    *,
+    temperature: float = 1.0,
+    label_weight: float = 0.0,
+    ignore_index: int = -100,
+    reduction: str = "mean",
+) -> Tensor:
+    """Loss of a student's ``logits`` ``[..., vocab]`` against a teacher's top logits.
+
+    ``teacher_logits`` and ``teacher_indices`` ``[..., top]`` (top <= 1024) are the teacher's
+    largest logits and their tokens; an index outside ``[0, vocab)`` (such as -1) or a logit of
+    -inf is padding. With ``q = softmax(teacher_logits / T)`` over a row's entries, ``p =
+    softmax(logits / T)`` and ``w = label_weight``::
+
+        loss = (1 - w) * T**2 * KL(q || p) + w * cross_entropy(logits, label)
+
+    A row without entries has no teacher term; a label that is ``ignore_index`` or outside ``[0,
+    vocab)`` gives no label term; a row with neither has loss 0 and gradient 0 and does not count in
+    the "mean" (which is 0 where no row counts). ``reduction`` is "mean", "sum" or "none" (a loss a
+    row). Everything is computed in f32 and the loss is f32; logits of f32/f16/bf16, sliced rows and
+    steps in place. Differentiable (once) in the logits; the teacher gets no gradient. The backward
+    reads the logits again: ``distill_loss_grad_b200`` does both in one pass.
+    """
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
+    call = _Distill(logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
+    return _DistillLossFunction.apply(logits, call, reduction)
+
+
+def distill_loss_grad_b200(
+    logits: Tensor,
+    teacher_logits: Tensor,
+    teacher_indices: Tensor,
+    labels: Tensor | None = None,
+    *,
+    temperature: float = 1.0,
+    label_weight: float = 0.0,
+    ignore_index: int = -100,
+    row_scale: Tensor | float | None = None,
+) -> tuple[Tensor, Tensor]:
+    """The losses of ``distill_loss_b200`` a row (f32 ``[...]``) and the gradient of ``sum(row_scale
+    * losses)`` in the logits (their dtype, contiguous), in one launch. ``row_scale`` is a number, a
+    one-element f32 tensor, or f32 ``[...]``: the upstream gradient with the divisor of a mean and
+    a loss scale in it, so that a gradient in f16 is scaled before it is rounded. For training
+    loops that call the head's backward themselves, such as a head in chunks of rows."""
+    call = _Distill(logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
+    dev = logits.device
+    scale: Tensor | None = None
+    if isinstance(row_scale, Tensor):
+        _same_device(dev, row_scale=row_scale)
+        if row_scale.dtype != torch.float32:
+            raise TypeError(f"row_scale must be float32, got {row_scale.dtype}")
+        if row_scale.numel() != 1 and row_scale.shape != call.lead:
+            raise ValueError(f"row_scale must have one element or shape {tuple(call.lead)}, got {tuple(row_scale.shape)}")
+        scale = row_scale.detach().contiguous()
+    elif row_scale is not None:
+        scale = torch.full((1,), float(row_scale), device=dev, dtype=torch.float32)
+    per_row = scale is not None and scale.shape == call.lead
+    losses = torch.empty(call.lead, device=dev, dtype=torch.float32)
+    grad = call.grad_like()
+    with _on(dev):
+        _launch("distill_loss_grad", nat.load().tropnn_b200_distill_loss_grad, *call.args, nat.ptr(scale), int(per_row),
+                losses.data_ptr(), grad.data_ptr(), nat.stream_handle(dev))
+    return losses, grad
+
+
+# ---------------------------------------------------------------------------
+# sampling
+# ---------------------------------------------------------------------------
+
+
+def _setting(
+    value: Tensor | float, name: str, lead: torch.Size, device: torch.device, lo: float, hi: float
+) -> tuple[Tensor | None, float]:
+    """A sampling setting as (one a row, or None; the value where it is one for all)."""
+    if isinstance(value, Tensor):
+        _same_device(device, **{name: value})
+        if value.dtype != torch.float32:
+            raise TypeError(f"{name} must be a number or float32, got {value.dtype}")
+        if value.shape != lead:
+            raise ValueError(f"{name} must be a number or have shape {tuple(lead)}, got {tuple(value.shape)}")
+        return value.contiguous(), 0.0
+    number = float(value)
+    if not (lo <= number <= hi):
+        raise ValueError(f"{name} must be in [{lo:g}, {hi:g}], got {number}")
+    return None, number
+
+
+def sample_tokens_b200(
+    logits: Tensor,
+    uniforms: Tensor,
+    *,
+    temperature: Tensor | float = 1.0,
+    top_k: Tensor | int = 0,
+    top_p: Tensor | float = 1.0,
+    min_p: Tensor | float = 0.0,
+) -> Tensor:
+    """One token (int64 ``[...]``) a row of ``logits`` ``[..., vocab]`` from ``uniforms`` (f32
+    ``[...]``, in [0, 1)).
+
+    Tokens rank by (logit descending, index ascending). Kept are the ``top_k`` first (0: all); of
+    those the ones with less than ``top_p`` of their probability before them; of those the ones with
+    at least ``min_p`` of the likeliest one's probability; the likeliest one always. The token is
+    where ``uniforms`` falls in the kept probabilities, in index order. ``temperature`` 0 takes the
+    likeliest. Each setting is a number or a tensor of one a row (f32, ``top_k`` int32/int64), whose
+    values are not checked: temperatures <= 0 are greedy and top_k <= 0 keeps all. A row with a NaN, or
+    with nothing above -inf, gives -1.
+
+    Probabilities are whole numbers (2^31 for the likeliest token) and add up exactly, so a row's
+    token depends on its logits and settings alone: not on the batch, the strides or the run.
+    """
+    _require_cuda(logits, "logits")
+    nat.float_code(logits.dtype)
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must have shape [..., vocab] with vocab >= 1, got {tuple(logits.shape)}")
+    lead, dev, vocab = logits.shape[:-1], logits.device, logits.shape[-1]
+    _same_device(dev, uniforms=uniforms)
+    if uniforms.dtype != torch.float32:
+        raise TypeError(f"uniforms must be float32, got {uniforms.dtype}")
+    if uniforms.shape != lead:
+        raise ValueError(f"uniforms must have shape {tuple(lead)}, got {tuple(uniforms.shape)}")
+    t, t_value = _setting(temperature, "temperature", lead, dev, 0.0, 3.4e38)
+    p, p_value = _setting(top_p, "top_p", lead, dev, 0.0, 1.0)
+    floor, floor_value = _setting(min_p, "min_p", lead, dev, 0.0, 1.0)
+    k, k_value, k_code = None, 0, nat.I64
+    if isinstance(top_k, Tensor):
+        _same_device(dev, top_k=top_k)
+        if top_k.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"top_k must be a number or int32/int64, got {top_k.dtype}")
+        if top_k.shape != lead:
+            raise ValueError(f"top_k must be a number or have shape {tuple(lead)}, got {tuple(top_k.shape)}")
+        k, k_code = top_k.contiguous(), nat.I64 if top_k.dtype == torch.int64 else nat.I32
+    else:
+        k_value = int(top_k)
+        if k_value < 0:
+            raise ValueError(f"top_k must be >= 0, got {k_value}")
+        k_value = min(k_value, vocab)
+    logits, rows, inner, outer_stride, inner_stride = _logit_rows(logits.detach())
+    uniforms = uniforms.contiguous()
+    tokens = torch.empty(lead, device=dev, dtype=torch.int64)
+    with _on(dev):
+        _launch(
+            "sample_tokens", nat.load().tropnn_b200_sample_tokens, logits.data_ptr(), nat.float_code(logits.dtype),
+            rows, inner, outer_stride, inner_stride, vocab, uniforms.data_ptr(), nat.ptr(t), t_value, nat.ptr(k), k_code,
+            k_value, nat.ptr(p), p_value, nat.ptr(floor), floor_value, tokens.data_ptr(), nat.stream_handle(dev),
+        )
+    return tokens
