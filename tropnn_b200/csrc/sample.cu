@@ -34,10 +34,12 @@ constexpr int kBins = 2048;
 constexpr int kDigitBits = 11;
 constexpr int kList = 2048;
 constexpr int kBinsPerThread = kBins / kThreads;
+constexpr int kFew = 256;
 // W >= 1 needs z >= ln(0.5 / 2^31) = -22.18: the bins cover the tokens that weigh anything.
-constexpr float kBinScale = kBins / 22.25f;
-constexpr int64_t kSliceTwoPerSm = 64 * 1024;  // bytes of logits a CTA, two CTAs on an SM
-constexpr int64_t kSliceMost = 168 * 1024;     // one CTA on an SM
+constexpr float kLowestZ = -22.25f;
+constexpr float kBinScale = kBins / -kLowestZ;
+constexpr int64_t kSliceShared = 64 * 1024 + 64;  // bytes of logits a CTA, two (without a search three) on an SM
+constexpr int64_t kSliceMost = 168 * 1024;        // one CTA on an SM
 
 struct SampleArgs {
   const void *logits;
@@ -71,7 +73,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN where eithe
 
 // One row's distribution.
 struct Scale {
-  float best, inv_t;
+  float best, inv_t, temperature;
   bool only_best;  // an infinite best logit, or 1 / T past f32: nothing else weighs anything
   __device__ __forceinline__ float z(float x) const { return (x - best) * inv_t; }
   __device__ __forceinline__ float e(float x) const {
@@ -79,18 +81,25 @@ struct Scale {
     return expf(z(x));
   }
   __device__ __forceinline__ static uint32_t weight(float e) { return __float2uint_rn(e * 2147483648.f); }
+  // kBins and above: weighs nothing.
   __device__ __forceinline__ int bin(float x) const {
-    if (only_best) return 0;  // only the tokens at best weigh anything
-    return min(static_cast<int>(z(x) * -kBinScale), kBins - 1);
+    if (only_best) return x == best ? 0 : kBins;
+    return static_cast<int>(fminf(z(x) * -kBinScale, float(kBins)));
+  }
+  // A logit that every x with z(x) >= z0 is above, rounding included.
+  __device__ __forceinline__ float below(float z0) const {
+    if (only_best) return best;
+    const float d = z0 * temperature;
+    return best + d - 1e-5f * (fabsf(best) + fabsf(d));
   }
 };
 
 // What the cluster's first CTA tells the others to do next.
-enum Command { kDone = 0, kGather = 1, kRefine = 2 };
+enum Command { kDone = 0, kGather = 1, kRefine = 2, kFinish = 3 };
 struct Order {
   int command;
   int bin;
-  int shift;           // tokens of the bin with (key >> shift) == prefix; 64: all of the bin
+  int shift;           // kGather, kRefine: tokens of the bin with (key >> shift) == prefix; 64: all of the bin
   uint64_t prefix;
   float cut_logit;     // kDone: kept are x > cut_logit, and x == cut_logit up to cut_index
   uint32_t cut_index;
@@ -105,11 +114,9 @@ struct Shared {
   Order order;
   uint32_t listed;
   // the first CTA's search
-  int found_bin;
-  uint32_t found_count;
-  uint64_t found_before;
-  uint32_t found_count_before;
-  uint64_t total;
+  int found;
+  uint32_t found_count, found_count_before;
+  uint64_t found_before, found_upto;
 };
 
 struct Histogram {
@@ -147,6 +154,25 @@ struct Vec {
     }
   }
 };
+// The largest element of a vector; PROPAGATE: NaN if one is.
+template <typename T, bool PROPAGATE>
+__device__ __forceinline__ float vec_max(const uint4 &q) {
+  if constexpr (std::is_same<T, float>::value) {
+    const float a = __uint_as_float(q.x), b = __uint_as_float(q.y), c = __uint_as_float(q.z), d = __uint_as_float(q.w);
+    if constexpr (PROPAGATE) return max_nan(max_nan(a, b), max_nan(c, d));
+    return fmaxf(fmaxf(a, b), fmaxf(c, d));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 a = *reinterpret_cast<const __half2 *>(&q.x), b = *reinterpret_cast<const __half2 *>(&q.y),
+                  c = *reinterpret_cast<const __half2 *>(&q.z), d = *reinterpret_cast<const __half2 *>(&q.w);
+    const __half2 m = __hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d));
+    return max_nan(__low2float(m), __high2float(m));
+  } else {
+    const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162 *>(&q.x), b = *reinterpret_cast<const __nv_bfloat162 *>(&q.y),
+                         c = *reinterpret_cast<const __nv_bfloat162 *>(&q.z), d = *reinterpret_cast<const __nv_bfloat162 *>(&q.w);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d));
+    return max_nan(__low2float(m), __high2float(m));
+  }
+}
 template <typename T>
 __device__ __forceinline__ T lowest_logit();
 template <>
@@ -177,16 +203,80 @@ __device__ __forceinline__ void cluster_sync(int ranks) {
   else __syncthreads();
 }
 
+// Inclusive prefix sums of a count and a weight over the block's threads, and their totals.
+__device__ __forceinline__ void block_scan(uint32_t &count, uint64_t &weight, uint32_t &all_count, uint64_t &all_weight,
+                                           Shared &sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t c = __shfl_up_sync(0xffffffffu, count, o);
+    const uint64_t w = __shfl_up_sync(0xffffffffu, weight, o);
+    if (lane >= o) {
+      count += c;
+      weight += w;
+    }
+  }
+  __syncthreads();
+  if (lane == 31) {
+    sh.warp_count[warp] = count;
+    sh.warp_sum[warp] = weight;
+  }
+  __syncthreads();
+  uint32_t c = sh.warp_count[lane % kWarps];
+  uint64_t w = sh.warp_sum[lane % kWarps];
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const uint32_t cb = __shfl_up_sync(0xffffffffu, c, o, kWarps);
+    const uint64_t wb = __shfl_up_sync(0xffffffffu, w, o, kWarps);
+    if ((lane % kWarps) >= o) {
+      c += cb;
+      w += wb;
+    }
+  }
+  all_count = __shfl_sync(0xffffffffu, c, kWarps - 1);
+  all_weight = __shfl_sync(0xffffffffu, w, kWarps - 1);
+  const uint32_t cb = __shfl_sync(0xffffffffu, c, warp == 0 ? 0 : warp - 1);
+  const uint64_t wb = __shfl_sync(0xffffffffu, w, warp == 0 ? 0 : warp - 1);
+  if (warp > 0) {
+    count += cb;
+    weight += wb;
+  }
+}
+
+// The first n entries of `list` (room for kList), largest first; zeros fill up the power of two.
+__device__ __forceinline__ void sort_list(uint64_t *list, uint32_t n) {
+  uint32_t size = 2;
+  while (size < n) size <<= 1;
+  for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+  __syncthreads();
+  for (uint32_t span = 2; span <= size; span <<= 1) {
+    for (uint32_t d = span >> 1; d > 0; d >>= 1) {
+      for (uint32_t i = threadIdx.x; i < size / 2; i += kThreads) {
+        const uint32_t lo = ((i & ~(d - 1)) << 1) | (i & (d - 1)), hi = lo + d;
+        const uint64_t p = list[lo], q = list[hi];
+        if ((p < q) == ((lo & span) == 0)) {
+          list[lo] = q;
+          list[hi] = p;
+        }
+      }
+      // Up to d = 32 a warp's pairs stay within its own 64 entries.
+      if (d > 32 || d == 1) __syncthreads();
+      else __syncwarp();
+    }
+  }
+}
+
 // RESIDENT: the slice stays in shared memory; else every pass reads global memory (L2) again.
-template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs g) {
+// SEARCH: some row may have a top-k or a top-p.
+template <typename T, bool RESIDENT, bool SEARCH>
+__global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const SampleArgs g) {
   constexpr int kN = Vec<T>::kN;
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared sh;
   Histogram &hist = *reinterpret_cast<Histogram *>(dynamic);
   uint64_t *list = reinterpret_cast<uint64_t *>(dynamic);
   Merged &merged = *reinterpret_cast<Merged *>(dynamic + sizeof(Histogram));
-  uint4 *kept_slice = reinterpret_cast<uint4 *>(dynamic + kSearchBytes);
+  uint4 *kept_slice = reinterpret_cast<uint4 *>(dynamic + (SEARCH ? kSearchBytes : 0));
 
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -206,18 +296,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs g)
   const float temperature = g.temperature != nullptr ? g.temperature[row] : g.temperature_value;
   float top_p = g.top_p != nullptr ? g.top_p[row] : g.top_p_value;
   float min_p = g.min_p != nullptr ? g.min_p[row] : g.min_p_value;
-  if (!(min_p <= 1.f)) top_p = min_p = 0.f;  // no token reaches it: the first one alone
   int64_t top_k = g.top_k_value;
   if (g.top_k != nullptr)
     top_k = g.top_k_dtype == TROPNN_B200_I64 ? static_cast<const int64_t *>(g.top_k)[row] : static_cast<const int32_t *>(g.top_k)[row];
-  const bool by_count = top_k > 0 && top_k < g.vocab;
-  const bool by_weight = !(top_p >= 1.f);
-
+  // No token reaches a min-p above 1 (or NaN): the first one alone, as a top-p of 0 leaves it.
+  if (!(min_p <= 1.f)) top_p = min_p = 0.f;
+  const bool by_count = SEARCH && top_k > 0 && top_k < g.vocab;
+  const bool by_weight = SEARCH && !(top_p >= 1.f);
   if (ranks > 1) cluster_arrive();
 
   // The slice, and the row's maximum (NaN where a logit is).
   float m = -INFINITY;
-  constexpr int kAhead = 4;
+  constexpr int kAhead = SEARCH ? 8 : 4;
   for (int v0 = tid; v0 < vecs; v0 += kThreads * kAhead) {
     uint4 q[kAhead];
 #pragma unroll
@@ -227,23 +317,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs g)
     for (int i = 0; i < kAhead; ++i) {
       if (v0 + i * kThreads < vecs) {
         if constexpr (RESIDENT) kept_slice[v0 + i * kThreads] = q[i];
-        float f[kN];
-        Vec<T>::unpack(q[i], f);
-#pragma unroll
-        for (int j = 0; j < kN; ++j) m = max_nan(m, f[j]);
+        m = max_nan(m, vec_max<T, true>(q[i]));
       }
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) sh.warp_sum[warp] = __float_as_uint(m);
+  if (lane == 0) sh.warp_count[warp] = __float_as_uint(m);
   __syncthreads();
   if (ranks > 1) cluster_wait();
-  if (tid < ranks) {
-    m = __uint_as_float(static_cast<uint32_t>(sh.warp_sum[0]));
+  if (warp == 0) {
+    m = __uint_as_float(sh.warp_count[lane % kWarps]);
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) m = max_nan(m, __uint_as_float(static_cast<uint32_t>(sh.warp_sum[w])));
-    *cluster.map_shared_rank(&sh.maxima[rank], tid) = m;
+    for (int o = kWarps / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane < ranks) *cluster.map_shared_rank(&sh.maxima[rank], lane) = m;
   }
   cluster_sync(ranks);
   Scale scale;
@@ -256,8 +343,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs g)
   if (!(temperature > 0.f)) {
     uint32_t first = 0xFFFFFFFFu;
     for (int v = tid; v < vecs; v += kThreads) {
+      const uint4 q = at(v);
+      if (vec_max<T, false>(q) < scale.best) continue;
       float f[kN];
-      Vec<T>::unpack(at(v), f);
+      Vec<T>::unpack(q, f);
 #pragma unroll
       for (int j = kN - 1; j >= 0; --j)
         if (f[j] == scale.best) first = min(first, index0(v) + j);
@@ -277,220 +366,199 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs g)
     }
     return;
   }
+  scale.temperature = temperature;
   scale.inv_t = 1.f / temperature;
   scale.only_best = scale.best == INFINITY || scale.inv_t == INFINITY;
+  const float uniform = g.uniforms[row];
+  auto target_of = [&](uint64_t total) -> uint64_t {
+    const double place = floor(static_cast<double>(uniform) * static_cast<double>(total));
+    const uint64_t target = place >= 1.0 ? static_cast<uint64_t>(place) : 0;
+    return target > total - 1 ? total - 1 : target;
+  };
 
   float cut_logit = -INFINITY;
   uint32_t cut_index = 0xFFFFFFFFu;
-  if (by_count || by_weight) {
-    // The first CTA's search: first for the top-k's end, then for the top-p's.
-    bool counting = by_count;  // which of the two
-    uint64_t limit_count = by_count ? static_cast<uint64_t>(top_k) : 0;
-    double limit_weight = 0.0;
+  if constexpr (SEARCH) if (by_count || by_weight) {
+    // State of the first CTA's search: for the top-k's end, then for the top-p's.
+    bool counting = by_count;
+    const uint64_t limit_count = by_count ? static_cast<uint64_t>(top_k) : 0;
+    double limit_weight = -1.0;  // not known yet
+    auto limit_of = [&](uint64_t all) { return fmax(static_cast<double>(top_p) * static_cast<double>(all), 0.5); };
     uint64_t cut = 0;  // rank key of the last kept token
     uint32_t base_count = 0;
     uint64_t base_weight = 0;  // before the bin or digit in question
     int bin = -1, shift = 64;
     uint64_t prefix = 0;
-    bool fresh = true;  // histogram over all bins
     for (;;) {
-      // A histogram: of all tokens by z, or of one bin's by the next bits of their keys.
+      // A histogram: of all tokens by z (fresh), or of one bin's by the next bits of their keys.
+      const bool fresh = bin < 0;
       for (int i = tid; i < kBins; i += kThreads) hist.count[i] = hist.low[i] = hist.high[i] = 0;
       __syncthreads();
       const int next_shift = shift == 64 ? 64 - kDigitBits : max(shift - kDigitBits, 0);
+      const uint32_t digit_mask = (1u << ((shift == 64 ? 64 : shift) - next_shift)) - 1u;
+      const float floor_x = scale.below(fresh ? kLowestZ : -(bin + 1) / kBinScale);
       for (int v = tid; v < vecs; v += kThreads) {
+        const uint4 q = at(v);
+        if (vec_max<T, false>(q) < floor_x) continue;
         float f[kN];
-        Vec<T>::unpack(at(v), f);
+        Vec<T>::unpack(q, f);
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
-          const uint32_t w = Scale::weight(scale.e(f[j]));
-          if (w == 0) continue;
           int b = scale.bin(f[j]);
+          if (b >= kBins) continue;
           if (!fresh) {
             if (b != bin) continue;
             const uint64_t key = rank_key(f[j], index0(v) + j);
             if (shift < 64 && (key >> shift) != prefix) continue;
-            // larger keys rank first: digits count down
-            b = kBins - 1 - static_cast<int>((key >> next_shift) & ((1u << (shift == 64 ? kDigitBits : shift - next_shift)) - 1u));
+            b = kBins - 1 - static_cast<int>(static_cast<uint32_t>(key >> next_shift) & digit_mask);  // larger keys first
           }
-          atomicAdd(&hist.count[b], 1u);
-          const uint32_t old = atomicAdd(&hist.low[b], w);
-          if (old + w < old) atomicAdd(&hist.high[b], 1u);
+          if (by_count) atomicAdd(&hist.count[b], 1u);
+          if (by_weight) {
+            const uint32_t w = Scale::weight(scale.e(f[j]));
+            const uint32_t old = atomicAdd(&hist.low[b], w);
+            if (old + w < old) atomicAdd(&hist.high[b], 1u);
+          }
         }
       }
       cluster_sync(ranks);
       for (int i = rank * kThreads + tid; i < kBins; i += ranks * kThreads) {
         uint32_t c = 0;
         uint64_t w = 0;
-        for (int r = 0; r < ranks; ++r) {
-          const Histogram *h = cluster.map_shared_rank(&hist, r);
-          c += h->count[i];
-          w += (uint64_t(h->high[i]) << 32) + h->low[i];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+          if (r < ranks) {
+            const Histogram *h = cluster.map_shared_rank(&hist, r);
+            c += h->count[i];
+            w += (uint64_t(h->high[i]) << 32) + h->low[i];
+          }
         }
         Merged *to = cluster.map_shared_rank(&merged, 0);
         to->count[i] = c;
         to->weight[i] = w;
       }
       cluster_sync(ranks);
-      bool listing = false;
+      bool listing = false;  // the first CTA has the bin's tokens
+      Order o;
       do {
         if (rank == 0) {
-          // The bin where the running count or weight reaches the limit.
-          uint32_t c[kBinsPerThread], cs = 0;
-          uint64_t w[kBinsPerThread], ws = 0;
-          if (!listing) {
-#pragma unroll
-            for (int i = 0; i < kBinsPerThread; ++i) {
-              c[i] = merged.count[tid * kBinsPerThread + i];
-              w[i] = merged.weight[tid * kBinsPerThread + i];
-              cs += c[i];
-              ws += w[i];
+          o.command = kDone;
+          bool again;
+          do {
+            again = false;
+            const uint32_t n = listing ? sh.listed : 0;
+            if (n > kList) {  // known by its weight alone, the bin held too many
+              o.command = kRefine;
+              break;
             }
-          } else {
-            // The listed tokens, sorted: each takes the place of a bin.
-            const uint32_t n = sh.listed;
-            uint32_t size = 1;
-            while (size < n) size <<= 1;
-            for (uint32_t i = n + tid; i < size; i += kThreads) list[i] = 0;
-            __syncthreads();
-            for (uint32_t span = 2; span <= size; span <<= 1) {
-              for (uint32_t d = span >> 1; d > 0; d >>= 1) {
-                for (uint32_t i = tid; i < size / 2; i += kThreads) {
-                  const uint32_t lo = 2 * d * (i / d) + i % d, hi = lo + d;
-                  const uint64_t p = list[lo], q = list[hi];
-                  if ((p < q) == ((lo & span) == 0)) {
-                    list[lo] = q;
-                    list[hi] = p;
-                  }
-                }
-                __syncthreads();
-              }
-            }
+            if (listing) sort_list(list, n);
+            // The place where the running count or weight reaches the limit: a bin, or a token.
+            uint32_t c[kBinsPerThread], cs = 0;
+            uint64_t w[kBinsPerThread], ws = 0;
 #pragma unroll
             for (int i = 0; i < kBinsPerThread; ++i) {
               const uint32_t k = tid * kBinsPerThread + i;
-              c[i] = k < n ? 1u : 0u;
-              w[i] = k < n ? Scale::weight(scale.e(logit_of(list[k]))) : 0u;
+              if (listing) {
+                c[i] = k < n ? 1u : 0u;
+                w[i] = k < n ? Scale::weight(scale.e(logit_of(list[k]))) : 0u;
+              } else {
+                c[i] = merged.count[k];
+                w[i] = merged.weight[k];
+              }
               cs += c[i];
               ws += w[i];
             }
-          }
-          uint32_t ci = cs;
-          uint64_t wi = ws;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t cb = __shfl_up_sync(0xffffffffu, ci, o);
-            const uint64_t wb = __shfl_up_sync(0xffffffffu, wi, o);
-            if (lane >= o) {
-              ci += cb;
-              wi += wb;
+            uint32_t upto_c = cs, all_count;
+            uint64_t upto_w = ws, all_weight;
+            block_scan(upto_c, upto_w, all_count, all_weight, sh);
+            if (fresh && !listing) {
+              if (counting && all_count < limit_count) counting = false;  // all that weigh anything stay
+              if (!counting && limit_weight < 0.0) limit_weight = limit_of(all_weight);
             }
-          }
-          __syncthreads();
-          if (lane == 31) {
-            sh.warp_count[warp] = ci;
-            sh.warp_sum[warp] = wi;
-          }
-          if (tid == 0) sh.found_bin = -1;
-          __syncthreads();
-          uint32_t cb = ci - cs;
-          uint64_t wb = wi - ws, all = 0;
-          uint32_t all_count = 0;
-          for (int i = 0; i < kWarps; ++i) {
-            if (i < warp) {
-              cb += sh.warp_count[i];
-              wb += sh.warp_sum[i];
-            }
-            all += sh.warp_sum[i];
-            all_count += sh.warp_count[i];
-          }
-          // A top-k past the tokens that weigh anything cuts nothing; the top-p then follows on
-          // the same histogram.
-          if (counting && fresh && !listing && all_count < limit_count) {
-            counting = false;
-            if (by_weight) limit_weight = fmax(static_cast<double>(top_p) * static_cast<double>(all), 0.5);
-          } else if (!counting && fresh && !listing && limit_weight == 0.0) {
-            limit_weight = fmax(static_cast<double>(top_p) * static_cast<double>(all), 0.5);  // 0.5: the first one alone
-          }
-          const bool searching = counting || by_weight;
-          if (searching) {
+            if (tid == 0) sh.found = -1;
+            __syncthreads();
+            const bool searching = counting || by_weight;
+            if (searching) {
+              uint64_t before_c = uint64_t(base_count) + (upto_c - cs), before_w = base_weight + (upto_w - ws);
 #pragma unroll
-            for (int i = 0; i < kBinsPerThread; ++i) {
-              const uint64_t before_c = base_count + cb, before_w = base_weight + wb;
-              const bool open = counting ? before_c < limit_count : static_cast<double>(before_w) < limit_weight;
-              const bool shut = counting ? before_c + c[i] >= limit_count
-                                         : !(static_cast<double>(before_w + w[i]) < limit_weight);
-              if (open && shut) {  // one bin of all
-                sh.found_bin = tid * kBinsPerThread + i;
-                sh.found_count = c[i];
-                sh.found_count_before = static_cast<uint32_t>(before_c);
-                sh.found_before = before_w;
-                sh.total = before_w + w[i];
+              for (int i = 0; i < kBinsPerThread; ++i) {
+                const bool open = counting ? before_c < limit_count : static_cast<double>(before_w) < limit_weight;
+                const bool shut = counting ? before_c + c[i] >= limit_count
+                                           : !(static_cast<double>(before_w + w[i]) < limit_weight);
+                if (open && shut) {  // one of all
+                  sh.found = tid * kBinsPerThread + i;
+                  sh.found_count = c[i];
+                  sh.found_count_before = static_cast<uint32_t>(before_c);
+                  sh.found_before = before_w;
+                  sh.found_upto = before_w + w[i];
+                }
+                before_c += c[i];
+                before_w += w[i];
               }
-              cb += c[i];
-              wb += w[i];
             }
-          }
-          __syncthreads();
-          Order o;
-          o.command = kDone;
-          o.bin = bin;
-          o.shift = shift;
-          o.prefix = prefix;
-          const int f = sh.found_bin;
-          if (searching && f >= 0) {
+            __syncthreads();
+            const int f = sh.found;
+            if (!searching || f < 0) break;
             if (listing) {
               cut = list[f];
               if (counting && by_weight) {
-                // The top-k ends here; its weight sets the top-p's limit, from the first bin again.
+                // The top-k ends here; its weight sets the top-p's limit, searched from the first bin.
                 counting = false;
-                limit_weight = fmax(static_cast<double>(top_p) * static_cast<double>(sh.total), 0.5);
+                limit_weight = limit_of(sh.found_upto);
                 base_count = 0;
                 base_weight = 0;
                 bin = -1;
                 shift = 64;
-                o.command = kRefine;
-                o.bin = -1;
-                o.shift = 64;
+                if (fresh) again = true;  // the histogram of all tokens is still there
+                else o.command = kRefine;
+                listing = false;
               }
-            } else {
-              base_count = sh.found_count_before;
-              base_weight = sh.found_before;
-              if (fresh) {
-                bin = f;
-              } else {
-                const int bits = shift == 64 ? kDigitBits : shift - next_shift;
-                prefix = (shift == 64 ? 0 : prefix << bits) | static_cast<uint64_t>(kBins - 1 - f);
-                shift = next_shift;
-              }
-              o.command = sh.found_count <= kList ? kGather : kRefine;
-              o.bin = bin;
-              o.shift = shift;
-              o.prefix = prefix;
+              __syncthreads();  // sh.found and the list have been read
+              continue;
             }
-          }
+            if (fresh && counting && sh.found_count_before + sh.found_count <= kFew) {
+              bin = f;
+              o.command = kFinish;
+              break;
+            }
+            base_count = sh.found_count_before;
+            base_weight = sh.found_before;
+            if (fresh) {
+              bin = f;
+            } else {
+              const int bits = (shift == 64 ? 64 : shift) - next_shift;
+              prefix = (shift == 64 ? 0 : prefix << bits) | static_cast<uint64_t>(kBins - 1 - f);
+              shift = next_shift;
+            }
+            o.command = by_count && sh.found_count > kList ? kRefine : kGather;
+          } while (again);
+          o.bin = bin;
+          o.shift = shift;
+          o.prefix = prefix;
           o.cut_logit = cut == 0 ? -INFINITY : logit_of(cut);
           o.cut_index = cut == 0 ? 0xFFFFFFFFu : index_of(cut);
+          __syncthreads();
           if (tid < ranks) *cluster.map_shared_rank(&sh.order, tid) = o;
           if (tid == 0) sh.listed = 0;
         }
         cluster_sync(ranks);
-        const Order o = sh.order;
+        o = sh.order;
         bin = o.bin;
         shift = o.shift;
         prefix = o.prefix;
-        cut_logit = o.cut_logit;
-        cut_index = o.cut_index;
-        listing = o.command == kGather;
+        listing = o.command == kGather || o.command == kFinish;
         if (listing) {
           uint32_t *listed = cluster.map_shared_rank(&sh.listed, 0);
           uint64_t *to = cluster.map_shared_rank(list, 0);
+          const float floor_bin = scale.below(-(bin + 1) / kBinScale);
           for (int v = tid; v < vecs; v += kThreads) {
+            const uint4 q = at(v);
+            if (vec_max<T, false>(q) < floor_bin) continue;
             float f[kN];
-            Vec<T>::unpack(at(v), f);
+            Vec<T>::unpack(q, f);
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-              if (f[j] == -INFINITY || scale.bin(f[j]) != bin || Scale::weight(scale.e(f[j])) == 0) continue;
+              const int b = scale.bin(f[j]);
+              if (o.command == kFinish ? b > bin : b != bin) continue;
               const uint64_t key = rank_key(f[j], index0(v) + j);
               if (shift < 64 && (key >> shift) != prefix) continue;
               const uint32_t place = atomicAdd(listed, 1u);
@@ -498,60 +566,112 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs g)
             }
           }
           cluster_sync(ranks);
+          if (o.command == kFinish) {
+            if (rank != 0) return;
+            // All that can be kept is here: rank each of the few tokens, keep, draw.
+            const int n = static_cast<int>(sh.listed);
+            uint32_t *weights = merged.count;
+            uint64_t key = 0;
+            float e = 0.f;
+            uint32_t w = 0;
+            if (tid < n) {
+              key = list[tid];
+              e = scale.e(logit_of(key));
+              w = Scale::weight(e);
+              weights[tid] = w;
+            }
+            __syncthreads();
+            uint32_t place = 0;
+            uint64_t before = 0;
+            if (tid < n) {
+              for (int i = 0; i < n; ++i) {
+                const bool ahead = list[i] > key;
+                place += ahead ? 1u : 0u;
+                before += ahead ? weights[i] : 0u;
+              }
+            }
+            const bool top = tid < n && place < limit_count;
+            uint32_t scratch_c = 0, all_c;
+            uint64_t scratch_w = top ? w : 0u, all;
+            block_scan(scratch_c, scratch_w, all_c, all, sh);
+            bool keep = top && (!by_weight || static_cast<double>(before) < limit_of(all)) && e >= min_p;
+            keep |= tid < n && place == 0;
+            w = keep ? w : 0u;
+            __syncthreads();
+            if (tid < n) weights[tid] = w;
+            scratch_w = w;
+            block_scan(scratch_c, scratch_w, all_c, all, sh);
+            if (keep) {
+              const uint32_t index = index_of(key);
+              uint64_t upto = 0;
+              for (int i = 0; i < n; ++i) upto += index_of(list[i]) <= index ? weights[i] : 0u;
+              const uint64_t target = target_of(all);
+              if (upto > target && upto - w <= target) g.tokens[row] = index;  // one of all
+            }
+            return;
+          }
         }
       } while (listing);
-      if (sh.order.command == kDone) break;
-      fresh = bin < 0;
-      __syncthreads();
+      if (o.command == kDone) {
+        cut_logit = o.cut_logit;
+        cut_index = o.cut_index;
+        break;
+      }
     }
   }
 
   // The kept weights of each warp's stretch of the slice, of each CTA, of the row.
-  auto kept = [&](float f, uint32_t i) -> uint32_t {
-    const float e = scale.e(f);
-    const bool in = (f > cut_logit || (f == cut_logit && i <= cut_index)) && (e >= min_p || f == scale.best);
-    return in ? Scale::weight(e) : 0u;
+  const bool cutting = cut_logit > -INFINITY;
+  const float floor_x = fmaxf(cut_logit, scale.below(fmaxf(kLowestZ, logf(min_p) - 1e-3f)));
+  auto kept = [&](const uint4 &q, int v, uint32_t (&w)[kN]) {
+    float f[kN];
+    Vec<T>::unpack(q, f);
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+      const float e = scale.e(f[j]);
+      bool in = e >= min_p;
+      if (SEARCH && cutting) in &= f[j] > cut_logit || (f[j] == cut_logit && index0(v) + j <= cut_index);
+      w[j] = in ? Scale::weight(e) : 0u;
+    }
   };
   const int per_warp = (vecs + kThreads - 1) / kThreads * 32;
   const int begin = min(warp * per_warp, vecs), stop = min(begin + per_warp, vecs);
   uint64_t sum = 0;
   for (int v = begin + lane; v < stop; v += 32) {
-    float f[kN];
-    Vec<T>::unpack(at(v), f);
+    const uint4 q = at(v);
+    if (vec_max<T, false>(q) < floor_x) continue;
+    uint32_t w[kN];
+    kept(q, v, w);
 #pragma unroll
-    for (int j = 0; j < kN; ++j) sum += kept(f[j], index0(v) + j);
+    for (int j = 0; j < kN; ++j) sum += w[j];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   __syncthreads();
   if (lane == 0) sh.warp_sum[warp] = sum;
   __syncthreads();
-  if (tid < ranks) {
-    uint64_t all = 0;
+  uint64_t all = sh.warp_sum[lane % kWarps], before = lane < warp ? all : 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) all += sh.warp_sum[w];
-    *cluster.map_shared_rank(&sh.sums[rank], tid) = all;
-  }
+  for (int o = kWarps / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (tid < ranks) *cluster.map_shared_rank(&sh.sums[rank], tid) = all;
   cluster_sync(ranks);
-  uint64_t total = 0, before = 0;
+  uint64_t total = 0;
   for (int r = 0; r < ranks; ++r) {
-    if (r == rank) before = total;
+    if (r < rank) before += sh.sums[r];
     total += sh.sums[r];
   }
-  for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
-  const double place = floor(static_cast<double>(g.uniforms[row]) * static_cast<double>(total));
-  uint64_t target = place >= 1.0 ? static_cast<uint64_t>(place) : 0;
-  target = target > total - 1 ? total - 1 : target;
+  const uint64_t target = target_of(total);
   if (target < before || target >= before + sum) return;  // one warp of the cluster goes on
   for (int v0 = begin; v0 < stop; v0 += 32) {
     const int v = v0 + lane;
     uint32_t w[kN];
     uint64_t mine = 0;
     if (v < stop) {
-      float f[kN];
-      Vec<T>::unpack(at(v), f);
+      kept(at(v), v, w);
 #pragma unroll
-      for (int j = 0; j < kN; ++j) mine += w[j] = kept(f[j], index0(v) + j);
+      for (int j = 0; j < kN; ++j) mine += w[j];
     }
     uint64_t upto = mine;
 #pragma unroll
@@ -584,16 +704,20 @@ int launch_sample(const char *what, SampleArgs g, int64_t rows, cudaStream_t str
   // The fewest CTAs a row that keep its slices at two CTAs an SM, more while SMs are idle.
   const int64_t row_bytes = g.vocab * int64_t(sizeof(T)) + 32;
   int ranks = 1;
-  while (ranks < kMaxCluster && (row_bytes > ranks * kSliceTwoPerSm || (rows * ranks * 2 <= sms && row_bytes > ranks * 4096)))
+  while (ranks < kMaxCluster && (row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 4096)))
     ranks *= 2;
   const int64_t vecs = row_bytes / 16;
   const int64_t slice = ceil_div(vecs, ranks);
   const bool resident = slice * 16 <= kSliceMost;
+  const bool search = g.top_k != nullptr || g.top_k_value > 0 || g.top_p != nullptr || g.top_p_value < 1.f || g.min_p != nullptr ||
+                      !(g.min_p_value <= 1.f);
   TB_REQUIRE(rows * ranks <= 0x7fffffffLL && slice <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: too many rows", what);
   g.slice_vecs = static_cast<int>(slice);
-  const size_t smem = kSearchBytes + 16 + (resident ? static_cast<size_t>(slice) * 16 : 0);
-  const void *kernel = resident ? reinterpret_cast<const void *>(sample_kernel<T, true>)
-                                : reinterpret_cast<const void *>(sample_kernel<T, false>);
+  const size_t smem = (search ? kSearchBytes : 0) + 16 + (resident ? static_cast<size_t>(slice) * 16 : 0);
+  const void *kernel = resident ? (search ? reinterpret_cast<const void *>(sample_kernel<T, true, true>)
+                                          : reinterpret_cast<const void *>(sample_kernel<T, true, false>))
+                                : (search ? reinterpret_cast<const void *>(sample_kernel<T, false, true>)
+                                          : reinterpret_cast<const void *>(sample_kernel<T, false, false>));
   TB_CHECK(ensure_dynamic_smem(kernel, smem, what));
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(rows * ranks));
