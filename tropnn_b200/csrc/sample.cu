@@ -13,10 +13,14 @@
 // or with a NaN, gives -1.
 //
 // A row belongs to a cluster of 1 to 8 CTAs, each of which keeps its slice of the logits in shared
-// memory: HBM is read once. The end of the prefix is found without sorting the row: a histogram
-// over 2048 bins of z (counts and weights) names the bin that holds it, the few tokens of that bin
-// go to the cluster's first CTA, which sorts them. A bin of more than 2048 tokens (equal or nearly
-// equal logits) is first refined by the bits of its tokens' rank keys, 11 at a time.
+// memory: HBM is read once. The end of the prefix is found without sorting: a histogram over 2048
+// bins of z (counts and weights) names the bin that holds it, further ones over the rank keys of
+// that bin's tokens name the logit; how many tokens of that logit stay is arithmetic, and which ones
+// a running count in index order, taken together with the final sums. Where a top-k leaves at most
+// 256 tokens, they go to the cluster's first CTA, which does the rest. Passes after the first skip
+// vectors whose largest logit lies below what they look for.
+#include <cfloat>
+
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -32,7 +36,6 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 2048;
 constexpr int kDigitBits = 11;
-constexpr int kList = 2048;
 constexpr int kBinsPerThread = kBins / kThreads;
 constexpr int kFew = 256;
 // W >= 1 needs z >= ln(0.5 / 2^31) = -22.18: the bins cover the tokens that weigh anything.
@@ -54,16 +57,14 @@ struct SampleArgs {
   int slice_vecs;  // 16-byte vectors of a CTA's slice
 };
 
-__device__ __forceinline__ uint64_t rank_key(float x, uint32_t i) {
-  const uint32_t b = __float_as_uint(x + 0.f);  // -0 ranks as +0
-  const uint32_t key = b ^ ((b >> 31) != 0u ? 0xFFFFFFFFu : 0x80000000u);
-  return (uint64_t(key) << 32) | (0xFFFFFFFFu - i);
+// Larger for larger logits; -0 as +0.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ ((b >> 31) != 0u ? 0xFFFFFFFFu : 0x80000000u);
 }
-__device__ __forceinline__ float logit_of(uint64_t key) {
-  const uint32_t k = static_cast<uint32_t>(key >> 32);
+__device__ __forceinline__ float logit_of(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) != 0u ? 0x80000000u : 0xFFFFFFFFu));
 }
-__device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is
   float r;
@@ -74,64 +75,65 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN where eithe
 // One row's distribution.
 struct Scale {
   float best, inv_t, temperature;
-  bool only_best;  // an infinite best logit, or 1 / T past f32: nothing else weighs anything
-  __device__ __forceinline__ float z(float x) const { return (x - best) * inv_t; }
-  __device__ __forceinline__ float e(float x) const {
-    if (only_best) return x == best ? 1.f : 0.f;
-    return expf(z(x));
-  }
+  // The minimum makes z(best) = 0 of a NaN: of inf - inf, or of 0 times an infinite 1 / T.
+  __device__ __forceinline__ float z(float x) const { return fminf((x - best) * inv_t, 0.f); }
   __device__ __forceinline__ static uint32_t weight(float e) { return __float2uint_rn(e * 2147483648.f); }
-  // kBins and above: weighs nothing.
-  __device__ __forceinline__ int bin(float x) const {
-    if (only_best) return x == best ? 0 : kBins;
-    return static_cast<int>(fminf(z(x) * -kBinScale, float(kBins)));
+  // -z in steps of 1 / kBinScale, to the nearest: adding it to 2^23 leaves the number in the low bits.
+  // kBins (and nothing above): weighs nothing.
+  __device__ __forceinline__ static int bin(float z) {
+    return __float_as_int(fminf(fmaf(z, -kBinScale, 8388608.f), 8388608.f + kBins)) - 0x4B000000;
   }
-  // A logit that every x with z(x) >= z0 is above, rounding included.
+  // A logit that every x with z(x) >= z0 is above, and one that it is below, rounding included.
   __device__ __forceinline__ float below(float z0) const {
-    if (only_best) return best;
     const float d = z0 * temperature;
-    return best + d - 1e-5f * (fabsf(best) + fabsf(d));
+    return fminf(best + d - 1e-5f * (fabsf(best) + fabsf(d)), best);
   }
+  __device__ __forceinline__ float above(float z0) const {
+    const float d = z0 * temperature;
+    return fminf(best + d + 1e-5f * (fabsf(best) + fabsf(d)), best);
+  }
+  __device__ __forceinline__ float bin_low(int b) const { return below(-(b + 1) / kBinScale); }
+  __device__ __forceinline__ float bin_high(int b) const { return above(-(b - 1) / kBinScale); }
 };
 
 // What the cluster's first CTA tells the others to do next.
-enum Command { kDone = 0, kGather = 1, kRefine = 2, kFinish = 3 };
+enum Command { kDone = 0, kRefine = 1, kFresh = 2, kFinish = 3 };
 struct Order {
   int command;
   int bin;
-  int shift;           // kGather, kRefine: tokens of the bin with (key >> shift) == prefix; 64: all of the bin
-  uint64_t prefix;
-  float cut_logit;     // kDone: kept are x > cut_logit, and x == cut_logit up to cut_index
-  uint32_t cut_index;
+  uint32_t key_low, key_high;  // kRefine: the keys in question; kDone: those of the cut's logit
+  uint32_t ties;               // kDone: how many tokens of that logit stay
 };
 
 struct Shared {
   uint64_t warp_sum[kWarps];
+  uint32_t warp_count[kWarps];
   uint64_t sums[kMaxCluster];
+  uint32_t ties[kMaxCluster], tie_weight[kMaxCluster];
   float maxima[kMaxCluster];
   uint32_t first_index[kMaxCluster];
-  uint32_t warp_count[kWarps];
   Order order;
-  uint32_t listed;
+  uint32_t listed, tied;
   // the first CTA's search
   int found;
   uint32_t found_count, found_count_before;
-  uint64_t found_before, found_upto;
+  uint64_t found_before, found_weight;
 };
 
 struct Histogram {
   uint32_t count[kBins], low[kBins], high[kBins];
 };
-struct Merged {
-  uint32_t count[kBins];
-  uint64_t weight[kBins];
+struct Few {  // over the first CTA's histogram
+  uint64_t key[kFew];  // rank keys: logit, then index
+  uint32_t weight[kFew];
 };
-constexpr size_t kSearchBytes = sizeof(Histogram) + sizeof(Merged);
-static_assert(sizeof(Histogram) >= kList * sizeof(uint64_t), "the list lies over the histogram");
+static_assert(sizeof(Few) <= sizeof(Histogram), "the list lies over the histogram");
 
 template <typename T>
 struct Vec {
   static constexpr int kN = 16 / sizeof(T);
+  // Keys of different logits are at least this far apart (a 16-bit logit leaves low f32 bits empty).
+  static constexpr uint32_t kKeyStep = std::is_same<T, float>::value ? 1u : std::is_same<T, __half>::value ? 1u << 13 : 1u << 16;
   __device__ __forceinline__ static void unpack(const uint4 &q, float (&v)[kN]) {
     if constexpr (std::is_same<T, float>::value) {
       v[0] = __uint_as_float(q.x);
@@ -243,29 +245,6 @@ __device__ __forceinline__ void block_scan(uint32_t &count, uint64_t &weight, ui
   }
 }
 
-// The first n entries of `list` (room for kList), largest first; zeros fill up the power of two.
-__device__ __forceinline__ void sort_list(uint64_t *list, uint32_t n) {
-  uint32_t size = 2;
-  while (size < n) size <<= 1;
-  for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
-  __syncthreads();
-  for (uint32_t span = 2; span <= size; span <<= 1) {
-    for (uint32_t d = span >> 1; d > 0; d >>= 1) {
-      for (uint32_t i = threadIdx.x; i < size / 2; i += kThreads) {
-        const uint32_t lo = ((i & ~(d - 1)) << 1) | (i & (d - 1)), hi = lo + d;
-        const uint64_t p = list[lo], q = list[hi];
-        if ((p < q) == ((lo & span) == 0)) {
-          list[lo] = q;
-          list[hi] = p;
-        }
-      }
-      // Up to d = 32 a warp's pairs stay within its own 64 entries.
-      if (d > 32 || d == 1) __syncthreads();
-      else __syncwarp();
-    }
-  }
-}
-
 // RESIDENT: the slice stays in shared memory; else every pass reads global memory (L2) again.
 // SEARCH: some row may have a top-k or a top-p.
 template <typename T, bool RESIDENT, bool SEARCH>
@@ -274,9 +253,8 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared sh;
   Histogram &hist = *reinterpret_cast<Histogram *>(dynamic);
-  uint64_t *list = reinterpret_cast<uint64_t *>(dynamic);
-  Merged &merged = *reinterpret_cast<Merged *>(dynamic + sizeof(Histogram));
-  uint4 *kept_slice = reinterpret_cast<uint4 *>(dynamic + (SEARCH ? kSearchBytes : 0));
+  Few &few = *reinterpret_cast<Few *>(dynamic);
+  uint4 *kept_slice = reinterpret_cast<uint4 *>(dynamic + (SEARCH ? sizeof(Histogram) : 0));
 
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -367,8 +345,7 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
     return;
   }
   scale.temperature = temperature;
-  scale.inv_t = 1.f / temperature;
-  scale.only_best = scale.best == INFINITY || scale.inv_t == INFINITY;
+  scale.inv_t = fmaxf(1.f / temperature, FLT_MIN);  // not 0: -inf has to stay at -inf
   const float uniform = g.uniforms[row];
   auto target_of = [&](uint64_t total) -> uint64_t {
     const double place = floor(static_cast<double>(uniform) * static_cast<double>(total));
@@ -376,303 +353,342 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
     return target > total - 1 ? total - 1 : target;
   };
 
-  float cut_logit = -INFINITY;
-  uint32_t cut_index = 0xFFFFFFFFu;
+  // Kept are the logits above cut_high and the first `ties` from cut_low to it (one value).
+  float cut_low = -INFINITY, cut_high = -INFINITY;
+  uint32_t ties = 0;
   if constexpr (SEARCH) if (by_count || by_weight) {
     // State of the first CTA's search: for the top-k's end, then for the top-p's.
     bool counting = by_count;
     const uint64_t limit_count = by_count ? static_cast<uint64_t>(top_k) : 0;
     double limit_weight = -1.0;  // not known yet
     auto limit_of = [&](uint64_t all) { return fmax(static_cast<double>(top_p) * static_cast<double>(all), 0.5); };
-    uint64_t cut = 0;  // rank key of the last kept token
-    uint32_t base_count = 0;
-    uint64_t base_weight = 0;  // before the bin or digit in question
-    int bin = -1, shift = 64;
-    uint64_t prefix = 0;
+    uint64_t base_count = 0, base_weight = 0;  // before the keys in question
+    Order o;
+    o.command = kFresh;
+    o.bin = 0;
+    o.key_low = o.key_high = 0;
     for (;;) {
-      // A histogram: of all tokens by z (fresh), or of one bin's by the next bits of their keys.
-      const bool fresh = bin < 0;
+      // A histogram: of all tokens by z, or of one bin's, between two keys, by the rest of their keys.
+      const bool fresh = o.command == kFresh;
+      const uint32_t range = o.key_high - o.key_low;  // keys, less one
+      const int shift = max(0, 32 - __clz(range) - kDigitBits);
       for (int i = tid; i < kBins; i += kThreads) hist.count[i] = hist.low[i] = hist.high[i] = 0;
       __syncthreads();
-      const int next_shift = shift == 64 ? 64 - kDigitBits : max(shift - kDigitBits, 0);
-      const uint32_t digit_mask = (1u << ((shift == 64 ? 64 : shift) - next_shift)) - 1u;
-      const float floor_x = scale.below(fresh ? kLowestZ : -(bin + 1) / kBinScale);
+      const float floor_x = fresh ? scale.below(kLowestZ) : logit_of(o.key_low);
       for (int v = tid; v < vecs; v += kThreads) {
         const uint4 q = at(v);
         if (vec_max<T, false>(q) < floor_x) continue;
         float f[kN];
         Vec<T>::unpack(q, f);
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          int b = scale.bin(f[j]);
-          if (b >= kBins) continue;
-          if (!fresh) {
-            if (b != bin) continue;
-            const uint64_t key = rank_key(f[j], index0(v) + j);
-            if (shift < 64 && (key >> shift) != prefix) continue;
-            b = kBins - 1 - static_cast<int>(static_cast<uint32_t>(key >> next_shift) & digit_mask);  // larger keys first
-          }
-          if (by_count) atomicAdd(&hist.count[b], 1u);
+        if (fresh) {
           if (by_weight) {
-            const uint32_t w = Scale::weight(scale.e(f[j]));
-            const uint32_t old = atomicAdd(&hist.low[b], w);
-            if (old + w < old) atomicAdd(&hist.high[b], 1u);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+              const float z = scale.z(f[j]);
+              const int b = Scale::bin(z);
+              const uint32_t w = Scale::weight(expf(z));
+              if (b < kBins) {
+                const uint32_t old = atomicAdd(&hist.low[b], w);
+                if (old + w < old) atomicAdd(&hist.high[b], 1u);
+                if (by_count) atomicAdd(&hist.count[b], 1u);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+              const int b = Scale::bin(scale.z(f[j]));
+              if (b < kBins) atomicAdd(&hist.count[b], 1u);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            const uint32_t down = o.key_high - key_of(f[j]);  // larger keys first
+            const float z = scale.z(f[j]);
+            if (down <= range && Scale::bin(z) == o.bin) {
+              const uint32_t w = Scale::weight(expf(z));
+              const uint32_t old = atomicAdd(&hist.low[down >> shift], w);
+              if (old + w < old) atomicAdd(&hist.high[down >> shift], 1u);
+              atomicAdd(&hist.count[down >> shift], 1u);
+            }
           }
         }
       }
       cluster_sync(ranks);
-      for (int i = rank * kThreads + tid; i < kBins; i += ranks * kThreads) {
-        uint32_t c = 0;
-        uint64_t w = 0;
+      if (rank == 0) {
+        // All CTAs' bins (four a thread), and where the running count or weight reaches the limit.
+        static_assert(kBinsPerThread == 4, "a bin a component");
+        uint32_t c[4] = {0, 0, 0, 0};
+        uint64_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int r = 0; r < kMaxCluster; ++r) {
           if (r < ranks) {
             const Histogram *h = cluster.map_shared_rank(&hist, r);
-            c += h->count[i];
-            w += (uint64_t(h->high[i]) << 32) + h->low[i];
+            const uint4 hc = reinterpret_cast<const uint4 *>(h->count)[tid], hl = reinterpret_cast<const uint4 *>(h->low)[tid],
+                        hh = reinterpret_cast<const uint4 *>(h->high)[tid];
+            c[0] += hc.x;
+            c[1] += hc.y;
+            c[2] += hc.z;
+            c[3] += hc.w;
+            w[0] += (uint64_t(hh.x) << 32) + hl.x;
+            w[1] += (uint64_t(hh.y) << 32) + hl.y;
+            w[2] += (uint64_t(hh.z) << 32) + hl.z;
+            w[3] += (uint64_t(hh.w) << 32) + hl.w;
           }
         }
-        Merged *to = cluster.map_shared_rank(&merged, 0);
-        to->count[i] = c;
-        to->weight[i] = w;
+        const uint32_t cs = c[0] + c[1] + c[2] + c[3];
+        const uint64_t ws = w[0] + w[1] + w[2] + w[3];
+        uint32_t upto_c = cs, all_count;
+        uint64_t upto_w = ws, all_weight;
+        if (tid == 0) sh.found = -1;
+        block_scan(upto_c, upto_w, all_count, all_weight, sh);
+        if (fresh) {
+          if (counting && all_count < limit_count) counting = false;  // all that weigh anything stay
+          if (!counting && limit_weight < 0.0) limit_weight = limit_of(all_weight);
+        }
+        const bool searching = counting || by_weight;
+        if (searching) {
+          uint64_t before_c = base_count + (upto_c - cs), before_w = base_weight + (upto_w - ws);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool open = counting ? before_c < limit_count : static_cast<double>(before_w) < limit_weight;
+            const bool shut = counting ? before_c + c[i] >= limit_count
+                                       : !(static_cast<double>(before_w + w[i]) < limit_weight);
+            if (open && shut) {  // one of all
+              sh.found = tid * 4 + i;
+              sh.found_count = c[i];
+              sh.found_count_before = static_cast<uint32_t>(before_c);
+              sh.found_before = before_w;
+              sh.found_weight = w[i];
+            }
+            before_c += c[i];
+            before_w += w[i];
+          }
+        }
+        __syncthreads();
+        const int f = sh.found;
+        Order next = o;
+        if (!searching || f < 0) {
+          next.command = kDone;
+          next.key_low = next.key_high = 0;
+        } else {
+          base_count = sh.found_count_before;
+          base_weight = sh.found_before;
+          if (fresh) {
+            next.bin = f;
+            next.command = counting && base_count + sh.found_count <= kFew ? kFinish : kRefine;
+            next.key_high = key_of(scale.bin_high(f));
+            next.key_low = key_of(scale.bin_low(f));
+          } else {
+            next.command = kRefine;
+            next.key_high = o.key_high - (static_cast<uint32_t>(f) << shift);
+            const uint32_t left = next.key_high - o.key_low, span = (1u << shift) - 1u;
+            next.key_low = next.key_high - min(left, span);
+            if (next.key_high - next.key_low < Vec<T>::kKeyStep) {
+              // One logit: its tokens weigh the same, and the first of them in index order stay.
+              const uint64_t weight = sh.found_weight / sh.found_count;
+              uint64_t stay = 0;
+              if (counting) {
+                stay = limit_count - base_count;
+              } else {
+                const double more = (limit_weight - static_cast<double>(base_weight)) / fmax(static_cast<double>(weight), 1.0);
+                stay = more > 2.0 ? static_cast<uint64_t>(more) - 1 : 0;
+                while (stay < sh.found_count && static_cast<double>(base_weight + stay * weight) < limit_weight) ++stay;
+                while (stay > 1 && !(static_cast<double>(base_weight + (stay - 1) * weight) < limit_weight)) --stay;
+              }
+              next.command = kDone;
+              next.ties = static_cast<uint32_t>(stay);
+              if (counting && by_weight) {
+                // The top-k's weight sets the top-p's limit, searched from the first bin.
+                limit_weight = limit_of(base_weight + stay * weight);
+                counting = false;
+                base_count = base_weight = 0;
+                next.command = kFresh;
+              }
+            }
+          }
+        }
+        if (tid < ranks) *cluster.map_shared_rank(&sh.order, tid) = next;
+        if (tid == 0) sh.listed = 0;
       }
       cluster_sync(ranks);
-      bool listing = false;  // the first CTA has the bin's tokens
-      Order o;
-      do {
-        if (rank == 0) {
-          o.command = kDone;
-          bool again;
-          do {
-            again = false;
-            const uint32_t n = listing ? sh.listed : 0;
-            if (n > kList) {  // known by its weight alone, the bin held too many
-              o.command = kRefine;
-              break;
-            }
-            if (listing) sort_list(list, n);
-            // The place where the running count or weight reaches the limit: a bin, or a token.
-            uint32_t c[kBinsPerThread], cs = 0;
-            uint64_t w[kBinsPerThread], ws = 0;
+      o = sh.order;
+      if (o.command == kDone) break;
+      if (o.command == kFinish) {
+        Few *to = cluster.map_shared_rank(&few, 0);
+        uint32_t *listed = cluster.map_shared_rank(&sh.listed, 0);
+        const float floor_bin = scale.bin_low(o.bin);
+        for (int v = tid; v < vecs; v += kThreads) {
+          const uint4 q = at(v);
+          if (vec_max<T, false>(q) < floor_bin) continue;
+          float f[kN];
+          Vec<T>::unpack(q, f);
 #pragma unroll
-            for (int i = 0; i < kBinsPerThread; ++i) {
-              const uint32_t k = tid * kBinsPerThread + i;
-              if (listing) {
-                c[i] = k < n ? 1u : 0u;
-                w[i] = k < n ? Scale::weight(scale.e(logit_of(list[k]))) : 0u;
-              } else {
-                c[i] = merged.count[k];
-                w[i] = merged.weight[k];
-              }
-              cs += c[i];
-              ws += w[i];
-            }
-            uint32_t upto_c = cs, all_count;
-            uint64_t upto_w = ws, all_weight;
-            block_scan(upto_c, upto_w, all_count, all_weight, sh);
-            if (fresh && !listing) {
-              if (counting && all_count < limit_count) counting = false;  // all that weigh anything stay
-              if (!counting && limit_weight < 0.0) limit_weight = limit_of(all_weight);
-            }
-            if (tid == 0) sh.found = -1;
-            __syncthreads();
-            const bool searching = counting || by_weight;
-            if (searching) {
-              uint64_t before_c = uint64_t(base_count) + (upto_c - cs), before_w = base_weight + (upto_w - ws);
-#pragma unroll
-              for (int i = 0; i < kBinsPerThread; ++i) {
-                const bool open = counting ? before_c < limit_count : static_cast<double>(before_w) < limit_weight;
-                const bool shut = counting ? before_c + c[i] >= limit_count
-                                           : !(static_cast<double>(before_w + w[i]) < limit_weight);
-                if (open && shut) {  // one of all
-                  sh.found = tid * kBinsPerThread + i;
-                  sh.found_count = c[i];
-                  sh.found_count_before = static_cast<uint32_t>(before_c);
-                  sh.found_before = before_w;
-                  sh.found_upto = before_w + w[i];
-                }
-                before_c += c[i];
-                before_w += w[i];
-              }
-            }
-            __syncthreads();
-            const int f = sh.found;
-            if (!searching || f < 0) break;
-            if (listing) {
-              cut = list[f];
-              if (counting && by_weight) {
-                // The top-k ends here; its weight sets the top-p's limit, searched from the first bin.
-                counting = false;
-                limit_weight = limit_of(sh.found_upto);
-                base_count = 0;
-                base_weight = 0;
-                bin = -1;
-                shift = 64;
-                if (fresh) again = true;  // the histogram of all tokens is still there
-                else o.command = kRefine;
-                listing = false;
-              }
-              __syncthreads();  // sh.found and the list have been read
-              continue;
-            }
-            if (fresh && counting && sh.found_count_before + sh.found_count <= kFew) {
-              bin = f;
-              o.command = kFinish;
-              break;
-            }
-            base_count = sh.found_count_before;
-            base_weight = sh.found_before;
-            if (fresh) {
-              bin = f;
-            } else {
-              const int bits = (shift == 64 ? 64 : shift) - next_shift;
-              prefix = (shift == 64 ? 0 : prefix << bits) | static_cast<uint64_t>(kBins - 1 - f);
-              shift = next_shift;
-            }
-            o.command = by_count && sh.found_count > kList ? kRefine : kGather;
-          } while (again);
-          o.bin = bin;
-          o.shift = shift;
-          o.prefix = prefix;
-          o.cut_logit = cut == 0 ? -INFINITY : logit_of(cut);
-          o.cut_index = cut == 0 ? 0xFFFFFFFFu : index_of(cut);
-          __syncthreads();
-          if (tid < ranks) *cluster.map_shared_rank(&sh.order, tid) = o;
-          if (tid == 0) sh.listed = 0;
+          for (int j = 0; j < kN; ++j) {
+            if (Scale::bin(scale.z(f[j])) > o.bin) continue;
+            const uint32_t place = atomicAdd(listed, 1u);
+            if (place < kFew) to->key[place] = (uint64_t(key_of(f[j])) << 32) | (0xFFFFFFFFu - (index0(v) + j));
+          }
         }
         cluster_sync(ranks);
-        o = sh.order;
-        bin = o.bin;
-        shift = o.shift;
-        prefix = o.prefix;
-        listing = o.command == kGather || o.command == kFinish;
-        if (listing) {
-          uint32_t *listed = cluster.map_shared_rank(&sh.listed, 0);
-          uint64_t *to = cluster.map_shared_rank(list, 0);
-          const float floor_bin = scale.below(-(bin + 1) / kBinScale);
-          for (int v = tid; v < vecs; v += kThreads) {
-            const uint4 q = at(v);
-            if (vec_max<T, false>(q) < floor_bin) continue;
-            float f[kN];
-            Vec<T>::unpack(q, f);
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-              const int b = scale.bin(f[j]);
-              if (o.command == kFinish ? b > bin : b != bin) continue;
-              const uint64_t key = rank_key(f[j], index0(v) + j);
-              if (shift < 64 && (key >> shift) != prefix) continue;
-              const uint32_t place = atomicAdd(listed, 1u);
-              if (place < kList) to[place] = key;
-            }
-          }
-          cluster_sync(ranks);
-          if (o.command == kFinish) {
-            if (rank != 0) return;
-            // All that can be kept is here: rank each of the few tokens, keep, draw.
-            const int n = static_cast<int>(sh.listed);
-            uint32_t *weights = merged.count;
-            uint64_t key = 0;
-            float e = 0.f;
-            uint32_t w = 0;
-            if (tid < n) {
-              key = list[tid];
-              e = scale.e(logit_of(key));
-              w = Scale::weight(e);
-              weights[tid] = w;
-            }
-            __syncthreads();
-            uint32_t place = 0;
-            uint64_t before = 0;
-            if (tid < n) {
-              for (int i = 0; i < n; ++i) {
-                const bool ahead = list[i] > key;
-                place += ahead ? 1u : 0u;
-                before += ahead ? weights[i] : 0u;
-              }
-            }
-            const bool top = tid < n && place < limit_count;
-            uint32_t scratch_c = 0, all_c;
-            uint64_t scratch_w = top ? w : 0u, all;
-            block_scan(scratch_c, scratch_w, all_c, all, sh);
-            bool keep = top && (!by_weight || static_cast<double>(before) < limit_of(all)) && e >= min_p;
-            keep |= tid < n && place == 0;
-            w = keep ? w : 0u;
-            __syncthreads();
-            if (tid < n) weights[tid] = w;
-            scratch_w = w;
-            block_scan(scratch_c, scratch_w, all_c, all, sh);
-            if (keep) {
-              const uint32_t index = index_of(key);
-              uint64_t upto = 0;
-              for (int i = 0; i < n; ++i) upto += index_of(list[i]) <= index ? weights[i] : 0u;
-              const uint64_t target = target_of(all);
-              if (upto > target && upto - w <= target) g.tokens[row] = index;  // one of all
-            }
-            return;
+        if (rank != 0) return;
+        // All that can be kept is here: rank each of the few tokens, keep, draw.
+        const int n = static_cast<int>(min(sh.listed, uint32_t(kFew)));
+        uint64_t key = 0;
+        float e = 0.f;
+        uint32_t w = 0;
+        if (tid < n) {
+          key = few.key[tid];
+          e = expf(scale.z(logit_of(static_cast<uint32_t>(key >> 32))));
+          w = Scale::weight(e);
+          few.weight[tid] = w;
+        }
+        __syncthreads();
+        uint32_t place = 0;
+        uint64_t before = 0;
+        if (tid < n) {
+          for (int i = 0; i < n; ++i) {
+            const bool ahead = few.key[i] > key;
+            place += ahead ? 1u : 0u;
+            before += ahead ? few.weight[i] : 0u;
           }
         }
-      } while (listing);
-      if (o.command == kDone) {
-        cut_logit = o.cut_logit;
-        cut_index = o.cut_index;
-        break;
+        const bool top = tid < n && place < limit_count;
+        uint32_t scratch_c = 0, all_c;
+        uint64_t scratch_w = top ? w : 0u, all;
+        block_scan(scratch_c, scratch_w, all_c, all, sh);
+        bool keep = top && (!by_weight || static_cast<double>(before) < limit_of(all)) && e >= min_p;
+        keep |= tid < n && place == 0;
+        w = keep ? w : 0u;
+        if (tid < n) few.weight[tid] = w;
+        scratch_w = w;
+        block_scan(scratch_c, scratch_w, all_c, all, sh);
+        if (keep) {
+          const uint32_t low = static_cast<uint32_t>(key);  // larger for lower indices
+          uint64_t upto = 0;
+          for (int i = 0; i < n; ++i) upto += static_cast<uint32_t>(few.key[i]) >= low ? few.weight[i] : 0u;
+          const uint64_t target = target_of(all);
+          if (upto > target && upto - w <= target) g.tokens[row] = 0xFFFFFFFFu - low;  // one of all
+        }
+        return;
       }
+    }
+    if (o.key_high != 0) {
+      cut_low = logit_of(o.key_low);
+      cut_high = logit_of(o.key_high);
+      ties = o.ties;
     }
   }
 
-  // The kept weights of each warp's stretch of the slice, of each CTA, of the row.
-  const bool cutting = cut_logit > -INFINITY;
-  const float floor_x = fmaxf(cut_logit, scale.below(fmaxf(kLowestZ, logf(min_p) - 1e-3f)));
-  auto kept = [&](const uint4 &q, int v, uint32_t (&w)[kN]) {
+  // The kept weights above the cut, and the tokens at it, of each warp's stretch of the slice, of each
+  // CTA, of the row.
+  const bool cutting = SEARCH && cut_high > -INFINITY;
+  const float floor_x = fmaxf(cut_low, scale.below(fmaxf(kLowestZ, logf(min_p) - 1e-3f)));
+  auto kept = [&](const uint4 &q, uint32_t (&w)[kN], uint32_t &at_cut) {  // at_cut: a bit an element
     float f[kN];
     Vec<T>::unpack(q, f);
+    at_cut = 0;
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
-      const float e = scale.e(f[j]);
-      bool in = e >= min_p;
-      if (SEARCH && cutting) in &= f[j] > cut_logit || (f[j] == cut_logit && index0(v) + j <= cut_index);
+      const float e = expf(scale.z(f[j]));
+      const bool in = e >= min_p && (!cutting || f[j] >= cut_low);
       w[j] = in ? Scale::weight(e) : 0u;
+      if (cutting) at_cut |= in && f[j] <= cut_high ? 1u << j : 0u;
     }
   };
   const int per_warp = (vecs + kThreads - 1) / kThreads * 32;
   const int begin = min(warp * per_warp, vecs), stop = min(begin + per_warp, vecs);
   uint64_t sum = 0;
+  uint32_t tied = 0, tie_weight = 0;
   for (int v = begin + lane; v < stop; v += 32) {
     const uint4 q = at(v);
     if (vec_max<T, false>(q) < floor_x) continue;
-    uint32_t w[kN];
-    kept(q, v, w);
+    uint32_t w[kN], at_cut;
+    kept(q, w, at_cut);
+    if (at_cut != 0) {
+      tied += __popc(at_cut);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        if ((at_cut >> j) & 1u) {
+          tie_weight = w[j];  // the same for all
+          w[j] = 0;
+        }
+      }
+    }
 #pragma unroll
     for (int j = 0; j < kN; ++j) sum += w[j];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  tied = __reduce_add_sync(0xffffffffu, tied);
+  tie_weight = __reduce_max_sync(0xffffffffu, tie_weight);
   __syncthreads();
-  if (lane == 0) sh.warp_sum[warp] = sum;
+  if (tid == 0) sh.tied = 0;
+  if (lane == 0) {
+    sh.warp_sum[warp] = sum;
+    sh.warp_count[warp] = tied;
+  }
   __syncthreads();
+  if (lane == 0 && tie_weight != 0) atomicMax(&sh.tied, tie_weight);
   uint64_t all = sh.warp_sum[lane % kWarps], before = lane < warp ? all : 0;
+  const uint32_t each = sh.warp_count[lane % kWarps];
+  uint32_t ties_before = __reduce_add_sync(0xffffffffu, lane < warp ? each : 0u);
+  const uint32_t all_ties = __reduce_add_sync(0xffffffffu, lane < kWarps ? each : 0u);
 #pragma unroll
   for (int o = kWarps / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  if (tid < ranks) *cluster.map_shared_rank(&sh.sums[rank], tid) = all;
+  __syncthreads();
+  if (tid < ranks) {
+    *cluster.map_shared_rank(&sh.sums[rank], tid) = all;
+    *cluster.map_shared_rank(&sh.ties[rank], tid) = all_ties;
+    *cluster.map_shared_rank(&sh.tie_weight[rank], tid) = sh.tied;
+  }
   cluster_sync(ranks);
   uint64_t total = 0;
+  uint32_t ties_total = 0;
+  tie_weight = 0;
   for (int r = 0; r < ranks; ++r) {
-    if (r < rank) before += sh.sums[r];
+    if (r < rank) {
+      before += sh.sums[r];
+      ties_before += sh.ties[r];
+    }
     total += sh.sums[r];
+    ties_total += sh.ties[r];
+    tie_weight = max(tie_weight, sh.tie_weight[r]);
   }
+  total += uint64_t(min(ties_total, ties)) * tie_weight;
+  before += uint64_t(min(ties_before, ties)) * tie_weight;
+  sum += uint64_t(min(ties_before + tied, ties) - min(ties_before, ties)) * tie_weight;
   const uint64_t target = target_of(total);
   if (target < before || target >= before + sum) return;  // one warp of the cluster goes on
   for (int v0 = begin; v0 < stop; v0 += 32) {
     const int v = v0 + lane;
-    uint32_t w[kN];
-    uint64_t mine = 0;
+    uint32_t w[kN], at_cut = 0;
     if (v < stop) {
-      kept(at(v), v, w);
+      kept(at(v), w, at_cut);
+    } else {
 #pragma unroll
-      for (int j = 0; j < kN; ++j) mine += w[j];
+      for (int j = 0; j < kN; ++j) w[j] = 0;
     }
+    uint32_t rank_in = __popc(at_cut);  // of the lane's first token at the cut
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t below = __shfl_up_sync(0xffffffffu, rank_in, o);
+      if (lane >= o) rank_in += below;
+    }
+    const uint32_t passed = __shfl_sync(0xffffffffu, rank_in, 31);
+    rank_in += ties_before - __popc(at_cut);
+    uint64_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+      if ((at_cut >> j) & 1u) {
+        if (rank_in >= ties) w[j] = 0;
+        ++rank_in;
+      }
+      mine += w[j];
+    }
+    ties_before += passed;
     uint64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -713,7 +729,7 @@ int launch_sample(const char *what, SampleArgs g, int64_t rows, cudaStream_t str
                       !(g.min_p_value <= 1.f);
   TB_REQUIRE(rows * ranks <= 0x7fffffffLL && slice <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: too many rows", what);
   g.slice_vecs = static_cast<int>(slice);
-  const size_t smem = (search ? kSearchBytes : 0) + 16 + (resident ? static_cast<size_t>(slice) * 16 : 0);
+  const size_t smem = (search ? sizeof(Histogram) : 0) + 16 + (resident ? static_cast<size_t>(slice) * 16 : 0);
   const void *kernel = resident ? (search ? reinterpret_cast<const void *>(sample_kernel<T, true, true>)
                                           : reinterpret_cast<const void *>(sample_kernel<T, true, false>))
                                 : (search ? reinterpret_cast<const void *>(sample_kernel<T, false, true>)
