@@ -621,14 +621,17 @@ TROPNN_B200_API int tropnn_b200_trop_backward(const float *grad_hidden, const fl
  * stride over dim; h0 f32 [batch, dim] (NULL: zeros), reset u8 [batch, steps] (NULL: none). h
  * [batch, steps, dim] contiguous in `dtype`, h_last f32 [batch, dim] (h0 when steps is 0). The
  * state is f32 throughout. `saved` (NULL: not kept) receives the f32 states that the backward
- * starts from, tropnn_b200_recurrence_saved_size bytes. Deterministic; no workspace.
+ * starts from, tropnn_b200_recurrence_saved_size bytes. The workspace (that of the forward or of the
+ * backward call alone, 0 bytes unless a long sequence is cut into chunks) is
+ * tropnn_b200_recurrence_workspace_size bytes, 8-byte aligned. Deterministic.
  */
 TROPNN_B200_API size_t tropnn_b200_recurrence_saved_size(int64_t batch, int64_t steps, int64_t dim);
+TROPNN_B200_API size_t tropnn_b200_recurrence_workspace_size(int64_t batch, int64_t steps, int64_t dim, int dtype);
 TROPNN_B200_API int tropnn_b200_recurrence_forward(const void *gate, int64_t gate_batch_stride, int64_t gate_step_stride,
                                    const void *value, int64_t value_batch_stride, int64_t value_step_stride,
                                    int dtype, const float *h0, const uint8_t *reset, int64_t batch, int64_t steps,
                                    int64_t dim, void *h, float *h_last, float *saved, size_t saved_bytes,
-                                   void *stream);
+                                   void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * Its backward: grad [batch, steps, dim] contiguous in `dtype` (NULL: zeros) and grad_last f32
@@ -641,7 +644,7 @@ TROPNN_B200_API int tropnn_b200_recurrence_backward(const void *gate, int64_t ga
                                     int dtype, const uint8_t *reset, int64_t batch, int64_t steps, int64_t dim,
                                     const float *saved, size_t saved_bytes, const void *grad,
                                     const float *grad_last, void *grad_gate, void *grad_value, float *grad_h0,
-                                    void *stream);
+                                    void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * One token of the recurrence: state (f32 [batch, dim], row stride in elements) is updated in

@@ -42,7 +42,7 @@ def test_c_entries_refuse_before_any_device_work(lib) -> None:
 
     def recurrence(dtype=nat.F32, batch=1, steps=1, dim=4):
         return lib.tropnn_b200_recurrence_forward(null, 0, 0, null, 0, 0, dtype, null, null, batch, steps, dim, null, null,
-                                                  null, 0, null)
+                                                  null, 0, null, 0, null)
 
     def distill(dtype=nat.F32, rows=1, vocab=8, top=2, index=nat.I64, temperature=1.0, weight=0.0):
         return lib.tropnn_b200_distill_loss(null, dtype, rows, 1, vocab, 0, vocab, null, nat.F32, null, index, top, null,

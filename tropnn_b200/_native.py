@@ -136,12 +136,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _p, _i64, _i64, _p, _p, _i32, _i64, _i64, _p, _p, _i32, _p, _f32, _i32, _p, _p, _p, _p, _p, _sz, _p],
     ),
     "tropnn_b200_recurrence_saved_size": (_sz, [_i64, _i64, _i64]),
+    "tropnn_b200_recurrence_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),
     "tropnn_b200_recurrence_forward": (
-        _i32, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _i64, _i64, _i64, _p, _p, _p, _sz, _p]
+        _i32, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _i64, _i64, _i64, _p, _p, _p, _sz, _p, _sz, _p]
     ),
     "tropnn_b200_recurrence_backward": (
         _i32,
-        [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64, _i64, _p, _sz, _p, _p, _p, _p, _p, _p],
+        [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64, _i64, _p, _sz, _p, _p, _p, _p, _p, _p, _sz, _p],
     ),
     "tropnn_b200_recurrence_step": (_i32, [_p, _i64, _p, _i64, _i32, _p, _i64, _i64, _p, _i64, _p, _p]),
     "tropnn_b200_distill_loss": (_i32, [*_DISTILL_ROWS, _p, _p, _p]),

@@ -4,11 +4,18 @@
 //   h_t = keep_t a_t h_{t-1} + c_t x_t                          (keep_t = 0 at a reset, else 1)
 //
 // The recurrence is linear, so a run of steps maps the state before it to P h + H with P the
-// product of its keep_t a_t. A warp owns kRun consecutive steps of 64 channels (two a lane): it
+// product of its keep_t a_t. A warp owns a run of consecutive steps of 64 channels (two a lane): it
 // scans them in registers from h = 0 for (P, H), hands those to the other warps through shared
 // memory, composes the runs before its own into its incoming state and scans again from there.
-// A tile is 8 warps' runs; a CTA walks the tiles of its 64 channels in order. One read of gate
-// and value, one write of h: the kernels are bound by HBM traffic.
+// A CTA's 8 warps take a tile of 8 runs. One read of gate and value, one write of h: the kernels are
+// bound by HBM traffic where enough CTAs are at work:
+//  - a cluster of up to 8 CTAs takes as many consecutive tiles at once and exchanges their maps
+//    through distributed shared memory, while the next tiles' loads are under way;
+//  - with too few channels for that (a long sequence of a small batch) the sequence is cut into
+//    chunks: a first launch computes each chunk's map, and every chunk composes those before its own.
+//    The inputs are then read twice, the second time largely from L2.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -18,11 +25,14 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kChan = 64;                    // channels of a CTA, two a lane
-constexpr int kRunFwd = 16;                  // steps of a warp's run, forward
-constexpr int kRunBwd = 8;                   // ... backward (more live values a step)
-constexpr int kTileFwd = kWarps * kRunFwd;   // 128
-constexpr int kTileBwd = kWarps * kRunBwd;   // 64: also the distance of the saved states
-static_assert(kTileFwd % kTileBwd == 0 && kTileBwd % kRunFwd == 0, "saved states start at a run of the forward");
+// Steps of a warp's run: what leaves room for the next tile's values in 128 registers a thread.
+template <typename T>
+constexpr int kRunFwd = sizeof(T) == 2 ? 16 : 8;
+constexpr int kRunBwd = 8;
+constexpr int kTileBwd = kWarps * kRunBwd;  // 64: also the distance of the saved states
+static_assert(kTileBwd % kRunFwd<float> == 0 && kTileBwd % kRunFwd<__half> == 0, "saved states start at a run");
+constexpr int kMaxCluster = 8;
+constexpr int kSlots = 2 * 148;  // CTAs at once
 
 // Two channels of one step as they lie in memory.
 template <typename T>
@@ -129,6 +139,10 @@ struct RecurrenceArgs {
   const uint8_t *reset;
   int64_t steps, dim;
   int channel_blocks;
+  int ranks;            // CTAs of a cluster
+  int chunks;           // of the sequence, each a launch-grid row
+  int64_t chunk_tiles;  // tiles of a chunk
+  float2 *maps;         // chunks > 1: (P, H) or (P, R) of [batch, chunk, dim]
   void *h;
   float *h_last;
   float *saved;  // [batch, saved_tiles, dim]: the state before each 64-step tile; NULL: not kept
@@ -139,6 +153,89 @@ struct RecurrenceArgs {
   void *grad_gate, *grad_value;
   float *grad_h0;
 };
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// Exchange of run maps: (P, H) of the CTA's warps and of the cluster's CTAs, two lane channels each.
+struct Exchange {
+  float2 p[2][kWarps][32], h[2][kWarps][32];
+  float4 rank[2][kMaxCluster][32];
+};
+
+// The chunks' maps before (FORWARD) or after this one, composed onto `state`: the warps take a share
+// each, in order.
+template <bool PAIRED, bool FORWARD>
+__device__ __forceinline__ float2 through_chunks(const RecurrenceArgs &g, int64_t batch, int64_t ch, bool on0, bool on1,
+                                                 int chunk, float2 state, Exchange &ex) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int count = FORWARD ? chunk : g.chunks - 1 - chunk;
+  const int share = (count + kWarps - 1) / kWarps;
+  const int first = min(warp * share, count), stop = min(first + share, count);
+  float2 p = make_float2(1.f, 1.f), h = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int i = first; i < stop; ++i) {
+    const int q = FORWARD ? i : g.chunks - 1 - i;
+    const float2 *m = g.maps + (batch * g.chunks + q) * g.dim + ch;
+    float2 a = make_float2(1.f, 0.f), b = make_float2(1.f, 0.f);
+    if (on0) a = __ldg(m);
+    if (on1) b = __ldg(m + kSecond<PAIRED>);
+    const float2 mp = make_float2(a.x, b.x);
+    h = apply_run(mp, h, make_float2(a.y, b.y));
+    p = mul2(mp, p);
+  }
+  ex.p[0][warp][lane] = p;
+  ex.h[0][warp][lane] = h;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) state = apply_run(ex.p[0][w][lane], state, ex.h[0][w][lane]);
+  __syncthreads();
+  return state;
+}
+
+// Hands this warp's (p, h) around: returns the state before its run, and moves `state` past the
+// cluster's tiles. ORDER 1: the runs follow one another by warp, -1: from the last warp back.
+template <int ORDER>
+__device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, float2 h, float2 &state, int ranks, int rank) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ex.p[buf][warp][lane] = p;
+  ex.h[buf][warp][lane] = h;
+  __syncthreads();
+  float2 in = state;
+  if (ranks == 1) {
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const int w = ORDER > 0 ? i : kWarps - 1 - i;
+      if (w == warp) in = state;
+      state = apply_run(ex.p[buf][w][lane], state, ex.h[buf][w][lane]);
+    }
+    return in;
+  }
+  if (warp < ranks) {  // the CTA's map, to one CTA a warp
+    float2 cp = make_float2(1.f, 1.f), ch = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const int w = ORDER > 0 ? i : kWarps - 1 - i;
+      const float2 pw = ex.p[buf][w][lane];
+      ch = apply_run(pw, ch, ex.h[buf][w][lane]);
+      cp = mul2(cp, pw);
+    }
+    *cooperative_groups::this_cluster().map_shared_rank(&ex.rank[buf][rank][lane], warp) = make_float4(cp.x, cp.y, ch.x, ch.y);
+  }
+  cluster_arrive();
+  cluster_wait();
+  for (int r = 0; r < ranks; ++r) {
+    if (r == rank) in = state;
+    const float4 m = ex.rank[buf][r][lane];
+    state = apply_run(make_float2(m.x, m.y), state, make_float2(m.z, m.w));
+  }
+#pragma unroll
+  for (int i = 0; i < kWarps - 1; ++i) {
+    const int w = ORDER > 0 ? i : kWarps - 1 - i;
+    if (ORDER > 0 ? w < warp : w > warp) in = apply_run(ex.p[buf][w][lane], in, ex.h[buf][w][lane]);
+  }
+  return in;
+}
 
 // The reset flags of `n` consecutive steps as bits.
 __device__ __forceinline__ uint32_t reset_bits(const uint8_t *row, int64_t t0, int n) {
@@ -152,40 +249,51 @@ __device__ __forceinline__ uint32_t reset_bits(const uint8_t *row, int64_t t0, i
 
 template <typename T, bool PAIRED>
 __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const RecurrenceArgs g) {
-  __shared__ float2 run_p[2][kWarps][32], run_h[2][kWarps][32];
+  constexpr int kRun = kRunFwd<T>, kTile = kWarps * kRun;
+  __shared__ Exchange ex;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t batch = blockIdx.x / g.channel_blocks;
-  const int64_t ch = int64_t(blockIdx.x % g.channel_blocks) * kChan + first_channel<PAIRED>(lane);
+  const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
+  const int unit = blockIdx.x / g.ranks;
+  const int64_t batch = unit / g.channel_blocks;
+  const int64_t ch = int64_t(unit % g.channel_blocks) * kChan + first_channel<PAIRED>(lane);
   const bool on0 = ch < g.dim, on1 = ch + kSecond<PAIRED> < g.dim;
   const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + ch;
   const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + ch;
   T *out = static_cast<T *>(g.h) + batch * g.steps * g.dim + ch;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
+  const int64_t first = chunk * g.chunk_tiles * kTile, stop = min64(g.steps, first + g.chunk_tiles * kTile);
+  if (g.ranks > 1) cluster_arrive();
 
-  float2 state = make_float2(0.f, 0.f);  // the state before the tile, the same in every warp
+  Raw<T> rf[kRun], rx[kRun];
+  auto load = [&](int64_t t0) {
+    const int n = static_cast<int>(t0 >= stop ? 0 : min64(kRun, stop - t0));
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const bool in = j < n;
+      rf[j] = load_raw<T, PAIRED>(gate + (t0 + j) * g.gate_step, in && on0, in && on1);
+      rx[j] = load_raw<T, PAIRED>(value + (t0 + j) * g.value_step, in && on0, in && on1);
+    }
+  };
+  load(first + rank * kTile + warp * kRun);
+  float2 state = make_float2(0.f, 0.f);  // the state before the cluster's tiles, the same in every warp
   if (g.h0 != nullptr) {
     const float *p = g.h0 + batch * g.dim + ch;
     if (on0) state.x = p[0];
     if (on1) state.y = p[kSecond<PAIRED>];
   }
+  if (chunk > 0) state = through_chunks<PAIRED, true>(g, batch, ch, on0, on1, chunk, state, ex);
+  if (g.ranks > 1) cluster_wait();
 
   int buf = 0;
-  for (int64_t tile = 0; tile < g.steps; tile += kTileFwd, buf ^= 1) {
-    const int64_t t0 = tile + warp * kRunFwd;
-    const int n = static_cast<int>(t0 >= g.steps ? 0 : min64(kRunFwd, g.steps - t0));
-    Raw<T> rf[kRunFwd], rx[kRunFwd];
-#pragma unroll
-    for (int j = 0; j < kRunFwd; ++j) {
-      const bool in = j < n;
-      rf[j] = load_raw<T, PAIRED>(gate + (t0 + j) * g.gate_step, in && on0, in && on1);
-      rx[j] = load_raw<T, PAIRED>(value + (t0 + j) * g.value_step, in && on0, in && on1);
-    }
+  for (int64_t tile = first; tile < stop; tile += int64_t(g.ranks) * kTile, buf ^= 1) {
+    const int64_t t0 = tile + rank * kTile + warp * kRun;
+    const int n = static_cast<int>(t0 >= stop ? 0 : min64(kRun, stop - t0));
     const uint32_t cut = reset_bits(reset, t0, n);
     const float2 zero = make_float2(0.f, 0.f);
     float2 h = zero, p = make_float2(1.f, 1.f);
-    float2 a[kRunFwd], b[kRunFwd];
+    float2 a[kRun], b[kRun];
 #pragma unroll
-    for (int j = 0; j < kRunFwd; ++j) {
+    for (int j = 0; j < kRun; ++j) {
       const float2 f = unpack<T>(rf[j]), x = unpack<T>(rx[j]);
       float2 c;
       gates(f.x, a[j].x, c.x);
@@ -197,24 +305,15 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
         p = mul2(p, a[j]);
       }
     }
-    run_p[buf][warp][lane] = p;
-    run_h[buf][warp][lane] = h;
-    __syncthreads();
-    // The state before this warp's run, and before the next tile.
-    float2 in = state;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) in = state;
-      const float2 pw = run_p[buf][w][lane], hw = run_h[buf][w][lane];
-      state = apply_run(pw, state, hw);
-    }
-    if (g.saved != nullptr && (warp * kRunFwd) % kTileBwd == 0 && n > 0) {
+    load(t0 + int64_t(g.ranks) * kTile);
+    float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank);
+    if (g.saved != nullptr && (warp * kRun) % kTileBwd == 0 && n > 0) {
       float *s = g.saved + (batch * g.saved_tiles + t0 / kTileBwd) * g.dim + ch;
       if (on0) s[0] = in.x;
       if (on1) s[kSecond<PAIRED>] = in.y;
     }
 #pragma unroll
-    for (int j = 0; j < kRunFwd; ++j) {
+    for (int j = 0; j < kRun; ++j) {
       if (j < n) {
         if ((cut >> j) & 1u) in = zero;
         in = fma2(a[j], in, b[j]);
@@ -222,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
       }
     }
   }
-  if (warp == 0) {
+  if (warp == 0 && rank == 0 && chunk == g.chunks - 1) {
     float *p = g.h_last + batch * g.dim + ch;
     if (on0) p[0] = state.x;
     if (on1) p[kSecond<PAIRED>] = state.y;
@@ -232,116 +331,192 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
 // Backward. With r_t = keep_t a_t ds_t the part of step t's gradient that reaches h_{t-1}:
 //   ds_t = grad_t + r_{t+1},  grad_value = c ds,  grad_gate = a c (keep h_{t-1} - x) ds
 // h_{t-1} is scanned again from the state saved before the tile (in 32 bits; h itself is not
-// read), the same way as forward, and ds the same way from the tile's end: both exchanges of run
-// maps share one barrier, and both have the same P.
+// read), the same way as forward within the tile; r comes from the sequence's end, across the
+// cluster's tiles. Both have the same P.
 template <typename T, bool PAIRED>
 __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const RecurrenceArgs g) {
-  __shared__ float2 run_p[2][kWarps][32], run_h[2][kWarps][32], run_r[2][kWarps][32];
+  constexpr int kRun = kRunBwd, kTile = kTileBwd;
+  __shared__ Exchange ex;
+  __shared__ float2 run_h[2][kWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t batch = blockIdx.x / g.channel_blocks;
-  const int64_t ch = int64_t(blockIdx.x % g.channel_blocks) * kChan + first_channel<PAIRED>(lane);
+  const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
+  const int unit = blockIdx.x / g.ranks;
+  const int64_t batch = unit / g.channel_blocks;
+  const int64_t ch = int64_t(unit % g.channel_blocks) * kChan + first_channel<PAIRED>(lane);
   const bool on0 = ch < g.dim, on1 = ch + kSecond<PAIRED> < g.dim;
   const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + ch;
   const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + ch;
   const T *grad = g.grad != nullptr ? static_cast<const T *>(g.grad) + batch * g.steps * g.dim + ch : nullptr;
+  const bool on0_g = on0 && grad != nullptr, on1_g = on1 && grad != nullptr;
   T *grad_gate = static_cast<T *>(g.grad_gate) + batch * g.steps * g.dim + ch;
   T *grad_value = static_cast<T *>(g.grad_value) + batch * g.steps * g.dim + ch;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
+  const int64_t first = chunk * g.chunk_tiles, stop = min64(g.saved_tiles, first + g.chunk_tiles);
+  if (g.ranks > 1) cluster_arrive();
 
-  float2 back = make_float2(0.f, 0.f);  // r of the step after the tile
+  Raw<T> rf[kRun], rx[kRun], rg[kRun];
+  float2 before;
+  auto steps_of = [&](int64_t k) -> int {
+    const int64_t t0 = k * kTile + warp * kRun;
+    return static_cast<int>(k < first || t0 >= g.steps ? 0 : min64(kRun, g.steps - t0));
+  };
+  auto load = [&](int64_t k) {
+    const int64_t t0 = k * kTile + warp * kRun;
+    const int n = steps_of(k);
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const bool in = j < n;
+      rf[j] = load_raw<T, PAIRED>(gate + (t0 + j) * g.gate_step, in && on0, in && on1);
+      rx[j] = load_raw<T, PAIRED>(value + (t0 + j) * g.value_step, in && on0, in && on1);
+      rg[j] = load_raw<T, PAIRED>(grad + (t0 + j) * g.dim, in && on0_g, in && on1_g);
+    }
+    before = make_float2(0.f, 0.f);
+    const float *p = g.saved + (batch * g.saved_tiles + k) * g.dim + ch;
+    if (n > 0 && on0) before.x = __ldg(p);
+    if (n > 0 && on1) before.y = __ldg(p + kSecond<PAIRED>);
+  };
+  load(stop - 1 - rank);
+  float2 back = make_float2(0.f, 0.f);  // r of the step after the cluster's tiles
   if (g.grad_last != nullptr) {
     const float *p = g.grad_last + batch * g.dim + ch;
     if (on0) back.x = p[0];
     if (on1) back.y = p[kSecond<PAIRED>];
   }
+  if (chunk < g.chunks - 1) back = through_chunks<PAIRED, false>(g, batch, ch, on0, on1, chunk, back, ex);
+  if (g.ranks > 1) cluster_wait();
 
   int buf = 0;
-  for (int64_t k = g.saved_tiles - 1; k >= 0; --k, buf ^= 1) {
-    const int64_t t0 = k * kTileBwd + warp * kRunBwd;
-    const int n = static_cast<int>(t0 >= g.steps ? 0 : min64(kRunBwd, g.steps - t0));
-    Raw<T> rf[kRunBwd], rx[kRunBwd], rg[kRunBwd];
-#pragma unroll
-    for (int j = 0; j < kRunBwd; ++j) {
-      const bool in = j < n;
-      rf[j] = load_raw<T, PAIRED>(gate + (t0 + j) * g.gate_step, in && on0, in && on1);
-      rx[j] = load_raw<T, PAIRED>(value + (t0 + j) * g.value_step, in && on0, in && on1);
-      rg[j] = load_raw<T, PAIRED>(grad + (t0 + j) * g.dim, in && on0 && grad != nullptr, in && on1 && grad != nullptr);
-    }
-    float2 before = make_float2(0.f, 0.f);
-    {
-      const float *p = g.saved + (batch * g.saved_tiles + k) * g.dim + ch;
-      if (on0) before.x = __ldg(p);
-      if (on1) before.y = __ldg(p + kSecond<PAIRED>);
-    }
+  for (int64_t last = stop - 1; last >= first; last -= g.ranks, buf ^= 1) {
+    const int64_t k = last - rank, t0 = k * kTile + warp * kRun;
+    const int n = steps_of(k);
     const uint32_t cut = reset_bits(reset, t0, n);
 
     const float2 zero = make_float2(0.f, 0.f);
-    float2 h = zero, p = make_float2(1.f, 1.f), r = zero;
-    float2 a[kRunBwd], c[kRunBwd];
+    float2 h = zero, p = make_float2(1.f, 1.f), r = zero, h_in = before;
+    float2 a[kRun], c[kRun], x[kRun], gt[kRun];
 #pragma unroll
-    for (int j = 0; j < kRunBwd; ++j) {
-      const float2 f = unpack<T>(rf[j]), x = unpack<T>(rx[j]);
+    for (int j = 0; j < kRun; ++j) {
+      const float2 f = unpack<T>(rf[j]);
+      x[j] = unpack<T>(rx[j]);
+      gt[j] = unpack<T>(rg[j]);
       gates(f.x, a[j].x, c[j].x);
       gates(f.y, a[j].y, c[j].y);
       if (j < n) {
         if ((cut >> j) & 1u) h = p = zero;
-        h = fma2(a[j], h, mul2(c[j], x));
+        h = fma2(a[j], h, mul2(c[j], x[j]));
         p = mul2(p, a[j]);
       }
     }
 #pragma unroll
-    for (int j = kRunBwd - 1; j >= 0; --j) {
+    for (int j = kRun - 1; j >= 0; --j) {
       if (j < n) {
-        const float2 gt = unpack<T>(rg[j]);
-        r = mul2(a[j], make_float2(gt.x + r.x, gt.y + r.y));
+        r = mul2(a[j], make_float2(gt[j].x + r.x, gt[j].y + r.y));
         if ((cut >> j) & 1u) r = zero;
       }
     }
-    run_p[buf][warp][lane] = p;
+    load(k - g.ranks);
     run_h[buf][warp][lane] = h;
-    run_r[buf][warp][lane] = r;
-    __syncthreads();
-    float2 h_in = before, r_in = back;
+    float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) {
-        const float2 pw = run_p[buf][w][lane], hw = run_h[buf][w][lane];
-        h_in = apply_run(pw, h_in, hw);
-      }
+    for (int w = 0; w < kWarps - 1; ++w) {
+      if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane]);
     }
 #pragma unroll
-    for (int w = kWarps - 1; w >= 0; --w) {
-      if (w == warp) r_in = back;
-      const float2 pw = run_p[buf][w][lane], rw = run_r[buf][w][lane];
-      back = apply_run(pw, back, rw);
-    }
-    float2 u[kRunBwd];  // keep h_{t-1} - x
-#pragma unroll
-    for (int j = 0; j < kRunBwd; ++j) {
+    for (int j = 0; j < kRun; ++j) {
       if (j < n) {
-        const float2 x = unpack<T>(rx[j]);
+        const float2 v = x[j];
         if ((cut >> j) & 1u) h_in = zero;
-        u[j] = make_float2(h_in.x - x.x, h_in.y - x.y);
-        h_in = fma2(a[j], h_in, mul2(c[j], x));
+        x[j] = make_float2(h_in.x - v.x, h_in.y - v.y);  // keep h_{t-1} - x from here on
+        h_in = fma2(a[j], h_in, mul2(c[j], v));
       }
     }
 #pragma unroll
-    for (int j = kRunBwd - 1; j >= 0; --j) {
+    for (int j = kRun - 1; j >= 0; --j) {
       if (j < n) {
-        const float2 gt = unpack<T>(rg[j]);
-        const float2 ds = make_float2(gt.x + r_in.x, gt.y + r_in.y);
+        const float2 ds = make_float2(gt[j].x + r_in.x, gt[j].y + r_in.y);
         const float2 gx = mul2(c[j], ds);
         r_in = mul2(a[j], ds);
         store_pair<T, PAIRED>(grad_value + (t0 + j) * g.dim, gx, on0, on1);
-        store_pair<T, PAIRED>(grad_gate + (t0 + j) * g.dim, mul2(mul2(a[j], gx), u[j]), on0, on1);
+        store_pair<T, PAIRED>(grad_gate + (t0 + j) * g.dim, mul2(mul2(a[j], gx), x[j]), on0, on1);
         if ((cut >> j) & 1u) r_in = zero;
       }
     }
   }
-  if (warp == 0 && g.grad_h0 != nullptr) {
+  if (warp == 0 && rank == 0 && chunk == 0 && g.grad_h0 != nullptr) {
     float *p = g.grad_h0 + batch * g.dim + ch;
     if (on0) p[0] = back.x;
     if (on1) p[kSecond<PAIRED>] = back.y;
+  }
+}
+
+// The map of each chunk: (P, H) forward, (P, R) for the backward. Each warp scans an equal stretch of
+// the chunk, the stretches are composed at the end.
+template <typename T, bool PAIRED, bool FORWARD>
+__global__ void __launch_bounds__(kThreads, 3) recurrence_map_kernel(const RecurrenceArgs g, int64_t chunk_steps) {
+  constexpr int kRun = 8;
+  __shared__ float2 run_p[kWarps][32], run_h[kWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunk = FORWARD ? blockIdx.y : blockIdx.y + 1;  // the last (first) chunk's map is not asked for
+  const int64_t batch = blockIdx.x / g.channel_blocks;
+  const int64_t ch = int64_t(blockIdx.x % g.channel_blocks) * kChan + first_channel<PAIRED>(lane);
+  const bool on0 = ch < g.dim, on1 = ch + kSecond<PAIRED> < g.dim;
+  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + ch;
+  const T *other = FORWARD ? static_cast<const T *>(g.value) + batch * g.value_batch + ch
+                           : (g.grad != nullptr ? static_cast<const T *>(g.grad) + batch * g.steps * g.dim + ch : nullptr);
+  const int64_t other_step = FORWARD ? g.value_step : g.dim;
+  const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
+  const int64_t share = chunk_steps / kWarps;  // a whole number of runs
+  const int64_t begin = chunk * chunk_steps + warp * share, stop = min64(g.steps, begin + share);
+  const float2 zero = make_float2(0.f, 0.f);
+  float2 h = zero, p = make_float2(1.f, 1.f);
+  const int64_t runs = begin < stop ? (stop - begin + kRun - 1) / kRun : 0;
+  for (int64_t i = 0; i < runs; ++i) {
+    const int64_t t0 = begin + (FORWARD ? i : runs - 1 - i) * kRun;
+    const int n = static_cast<int>(min64(kRun, stop - t0));
+    Raw<T> rf[kRun], ro[kRun];
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const bool in = j < n;
+      rf[j] = load_raw<T, PAIRED>(gate + (t0 + j) * g.gate_step, in && on0, in && on1);
+      ro[j] = load_raw<T, PAIRED>(other + (t0 + j) * other_step, in && on0 && other != nullptr, in && on1 && other != nullptr);
+    }
+    const uint32_t cut = reset_bits(reset, t0, n);
+#pragma unroll
+    for (int i_j = 0; i_j < kRun; ++i_j) {
+      const int j = FORWARD ? i_j : kRun - 1 - i_j;
+      if (j < n) {
+        const float2 f = unpack<T>(rf[j]), o = unpack<T>(ro[j]);
+        float2 a, c;
+        gates(f.x, a.x, c.x);
+        gates(f.y, a.y, c.y);
+        const bool here = (cut >> j) & 1u;
+        if (FORWARD) {
+          if (here) h = p = zero;
+          h = fma2(a, h, mul2(c, o));
+          p = mul2(p, a);
+        } else {
+          h = mul2(a, make_float2(o.x + h.x, o.y + h.y));
+          p = mul2(p, a);
+          if (here) h = p = zero;
+        }
+      }
+    }
+  }
+  run_p[warp][lane] = p;
+  run_h[warp][lane] = h;
+  __syncthreads();
+  if (warp == 0) {
+    p = make_float2(1.f, 1.f);
+    h = zero;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const int w = FORWARD ? i : kWarps - 1 - i;
+      h = apply_run(run_p[w][lane], h, run_h[w][lane]);
+      p = mul2(p, run_p[w][lane]);
+    }
+    float2 *m = g.maps + (batch * g.chunks + chunk) * g.dim + ch;
+    if (on0) m[0] = make_float2(p.x, h.x);
+    if (on1) m[kSecond<PAIRED>] = make_float2(p.y, h.y);
   }
 }
 
@@ -374,25 +549,73 @@ int check_sizes(const char *what, int dtype, int64_t batch, int64_t steps, int64
   return TROPNN_B200_OK;
 }
 
-template <bool BACKWARD>
-int launch_recurrence(const char *what, const RecurrenceArgs &g, int dtype, int64_t batch, bool pair, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(batch * g.channel_blocks);
-#define TB_LAUNCH(T, PAIR)                                                                  \
-  do {                                                                                      \
-    if (BACKWARD)                                                                           \
-      recurrence_backward_kernel<T, PAIR><<<grid, kThreads, 0, stream>>>(g);                \
-    else                                                                                    \
-      recurrence_forward_kernel<T, PAIR><<<grid, kThreads, 0, stream>>>(g);                 \
-  } while (0)
-  if (dtype == TROPNN_B200_F32) {
-    if (pair) TB_LAUNCH(float, true); else TB_LAUNCH(float, false);
-  } else if (dtype == TROPNN_B200_F16) {
-    if (pair) TB_LAUNCH(__half, true); else TB_LAUNCH(__half, false);
-  } else {
-    if (pair) TB_LAUNCH(__nv_bfloat16, true); else TB_LAUNCH(__nv_bfloat16, false);
+// How the tiles are shared out. While CTAs are idle: more of them a cluster, as far as there are tiles.
+// With less than half the SMs busy even so and at least 4 tiles a chunk, chunks instead.
+struct Plan {
+  int ranks = 1, chunks = 1;
+  int64_t chunk_tiles = 0;
+};
+Plan plan_for(int64_t units, int64_t tiles) {
+  Plan p;
+  p.chunk_tiles = tiles;
+  while (p.ranks < kMaxCluster && units * p.ranks * 2 <= kSlots && p.ranks * 2 <= tiles) p.ranks *= 2;
+  if (p.ranks == kMaxCluster && units * p.ranks <= kSlots / 4) {
+    const int64_t each = std::max<int64_t>(4, ceil_div(tiles * units, kSlots));
+    if (ceil_div(tiles, each) >= 2 * p.ranks) {
+      p.ranks = 1;
+      p.chunk_tiles = each;
+      p.chunks = static_cast<int>(ceil_div(tiles, each));
+    }
   }
-#undef TB_LAUNCH
+  return p;
+}
+int64_t units_of(int64_t batch, int64_t dim) { return batch * ceil_div(dim, kChan); }
+int64_t forward_tile(int dtype) { return kWarps * (dtype == TROPNN_B200_F32 ? kRunFwd<float> : kRunFwd<__half>); }
+
+template <bool FORWARD, typename T, bool PAIRED>
+int launch_typed(const char *what, RecurrenceArgs g, int64_t batch, const Plan &plan, cudaStream_t stream) {
+  const unsigned units = static_cast<unsigned>(batch * g.channel_blocks);
+  if (plan.chunks > 1) {
+    constexpr int64_t tile = FORWARD ? kWarps * kRunFwd<T> : kTileBwd;
+    recurrence_map_kernel<T, PAIRED, FORWARD>
+        <<<dim3(units, static_cast<unsigned>(plan.chunks - 1)), kThreads, 0, stream>>>(g, plan.chunk_tiles * tile);
+    TB_CHECK(check_launch(what));
+  }
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(units * static_cast<unsigned>(plan.ranks), static_cast<unsigned>(plan.chunks));
+  config.blockDim = dim3(kThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(plan.ranks);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  if (FORWARD) cudaLaunchKernelEx(&config, recurrence_forward_kernel<T, PAIRED>, static_cast<const RecurrenceArgs>(g));
+  else cudaLaunchKernelEx(&config, recurrence_backward_kernel<T, PAIRED>, static_cast<const RecurrenceArgs>(g));
   return check_launch(what);
+}
+
+template <bool FORWARD>
+int launch_recurrence(const char *what, RecurrenceArgs g, int dtype, int64_t batch, bool pair, void *workspace,
+                      size_t workspace_bytes, cudaStream_t stream) {
+  const int64_t tile = FORWARD ? forward_tile(dtype) : kTileBwd;
+  const Plan plan = plan_for(batch * g.channel_blocks, ceil_div(g.steps, tile));
+  const size_t need = plan.chunks > 1 ? static_cast<size_t>(batch * plan.chunks * g.dim) * sizeof(float2) : 0;
+  TB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), TROPNN_B200_ERR_WORKSPACE,
+             "%s: %zu bytes of workspace, %zu needed", what, workspace_bytes, need);
+  g.ranks = plan.ranks;
+  g.chunks = plan.chunks;
+  g.chunk_tiles = plan.chunk_tiles;
+  g.maps = static_cast<float2 *>(workspace);
+  if (dtype == TROPNN_B200_F32)
+    return pair ? launch_typed<FORWARD, float, true>(what, g, batch, plan, stream)
+                : launch_typed<FORWARD, float, false>(what, g, batch, plan, stream);
+  if (dtype == TROPNN_B200_F16)
+    return pair ? launch_typed<FORWARD, __half, true>(what, g, batch, plan, stream)
+                : launch_typed<FORWARD, __half, false>(what, g, batch, plan, stream);
+  return pair ? launch_typed<FORWARD, __nv_bfloat16, true>(what, g, batch, plan, stream)
+              : launch_typed<FORWARD, __nv_bfloat16, false>(what, g, batch, plan, stream);
 }
 
 }  // namespace
@@ -407,10 +630,19 @@ size_t tropnn_b200_recurrence_saved_size(int64_t batch, int64_t steps, int64_t d
   return static_cast<size_t>(batch * ceil_div(steps, kTileBwd) * dim) * sizeof(float);
 }
 
+size_t tropnn_b200_recurrence_workspace_size(int64_t batch, int64_t steps, int64_t dim, int dtype) {
+  if (batch <= 0 || steps <= 0 || dim <= 0 || !is_float_dtype(dtype)) return 0;
+  const int64_t units = units_of(batch, dim);
+  const Plan f = plan_for(units, ceil_div(steps, forward_tile(dtype))), b = plan_for(units, ceil_div(steps, kTileBwd));
+  const int chunks = std::max(f.chunks, b.chunks);
+  return chunks > 1 ? static_cast<size_t>(batch * chunks * dim) * sizeof(float2) : 0;
+}
+
 int tropnn_b200_recurrence_forward(const void *gate, int64_t gate_batch_stride, int64_t gate_step_stride,
                                    const void *value, int64_t value_batch_stride, int64_t value_step_stride, int dtype,
                                    const float *h0, const uint8_t *reset, int64_t batch, int64_t steps, int64_t dim,
-                                   void *h, float *h_last, float *saved, size_t saved_bytes, void *stream) {
+                                   void *h, float *h_last, float *saved, size_t saved_bytes, void *workspace,
+                                   size_t workspace_bytes, void *stream) {
   const char *what = "recurrence_forward";
   TB_CHECK(check_sizes(what, dtype, batch, steps, dim));
   if (batch == 0 || dim == 0) return clear_error();
@@ -439,7 +671,7 @@ int tropnn_b200_recurrence_forward(const void *gate, int64_t gate_batch_stride, 
   const bool pair = dim % 2 == 0 && gate_batch_stride % 2 == 0 && gate_step_stride % 2 == 0 &&
                     value_batch_stride % 2 == 0 && value_step_stride % 2 == 0 && paired(gate, dtype) &&
                     paired(value, dtype) && paired(h, dtype);
-  TB_CHECK((launch_recurrence<false>(what, g, dtype, batch, pair, as_stream(stream))));
+  TB_CHECK((launch_recurrence<true>(what, g, dtype, batch, pair, workspace, workspace_bytes, as_stream(stream))));
   return clear_error();
 }
 
@@ -447,7 +679,8 @@ int tropnn_b200_recurrence_backward(const void *gate, int64_t gate_batch_stride,
                                     const void *value, int64_t value_batch_stride, int64_t value_step_stride, int dtype,
                                     const uint8_t *reset, int64_t batch, int64_t steps, int64_t dim, const float *saved,
                                     size_t saved_bytes, const void *grad, const float *grad_last, void *grad_gate,
-                                    void *grad_value, float *grad_h0, void *stream) {
+                                    void *grad_value, float *grad_h0, void *workspace, size_t workspace_bytes,
+                                    void *stream) {
   const char *what = "recurrence_backward";
   TB_CHECK(check_sizes(what, dtype, batch, steps, dim));
   if (batch == 0 || dim == 0) return clear_error();
@@ -478,7 +711,7 @@ int tropnn_b200_recurrence_backward(const void *gate, int64_t gate_batch_stride,
   const bool pair = dim % 2 == 0 && gate_batch_stride % 2 == 0 && gate_step_stride % 2 == 0 &&
                     value_batch_stride % 2 == 0 && value_step_stride % 2 == 0 && paired(gate, dtype) &&
                     paired(value, dtype) && paired(grad, dtype) && paired(grad_gate, dtype) && paired(grad_value, dtype);
-  TB_CHECK((launch_recurrence<true>(what, g, dtype, batch, pair, as_stream(stream))));
+  TB_CHECK((launch_recurrence<false>(what, g, dtype, batch, pair, workspace, workspace_bytes, as_stream(stream))));
   return clear_error();
 }
 

@@ -60,6 +60,11 @@ def _unit_last(t: Tensor) -> Tensor:
 # ---------------------------------------------------------------------------
 
 
+def _recurrence_workspace(lib: Any, gate: Tensor) -> tuple[Tensor | None, int]:
+    size = lib.tropnn_b200_recurrence_workspace_size(*gate.shape, nat.float_code(gate.dtype))
+    return (torch.empty(size, device=gate.device, dtype=torch.uint8), size) if size else (None, 0)
+
+
 class _GatedRecurrenceFunction(torch.autograd.Function):
     @staticmethod
     def forward(  # type: ignore[override]
@@ -72,12 +77,13 @@ class _GatedRecurrenceFunction(torch.autograd.Function):
         h_last = torch.empty((batch, dim), device=dev, dtype=torch.float32)
         saved_bytes = lib.tropnn_b200_recurrence_saved_size(batch, steps, dim) if keep else 0
         saved = torch.empty(saved_bytes // 4, device=dev, dtype=torch.float32) if keep else None
+        ws, ws_bytes = _recurrence_workspace(lib, gate)
         with _on(dev):
             _launch(
                 "recurrence_forward", lib.tropnn_b200_recurrence_forward, gate.data_ptr(), gate.stride(0),
                 gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype),
                 nat.ptr(h0), nat.ptr(reset), batch, steps, dim, h.data_ptr(), h_last.data_ptr(), nat.ptr(saved),
-                saved_bytes, nat.stream_handle(dev),
+                saved_bytes, nat.ptr(ws), ws_bytes, nat.stream_handle(dev),
             )
         if keep:
             ctx.save_for_backward(gate, value, reset, saved)
@@ -99,13 +105,14 @@ class _GatedRecurrenceFunction(torch.autograd.Function):
         grad_gate = torch.empty((batch, steps, dim), device=dev, dtype=gate.dtype)
         grad_value = torch.empty((batch, steps, dim), device=dev, dtype=gate.dtype)
         grad_h0 = torch.empty((batch, dim), device=dev, dtype=torch.float32) if ctx.needs_input_grad[2] else None
+        ws, ws_bytes = _recurrence_workspace(lib, gate)
         with _on(dev):
             _launch(
                 "recurrence_backward", lib.tropnn_b200_recurrence_backward, gate.data_ptr(), gate.stride(0),
                 gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype),
                 nat.ptr(reset), batch, steps, dim, saved.data_ptr(), ctx.saved_bytes, nat.ptr(grad_h),
                 nat.ptr(grad_last), grad_gate.data_ptr(), grad_value.data_ptr(), nat.ptr(grad_h0),
-                nat.stream_handle(dev),
+                nat.ptr(ws), ws_bytes, nat.stream_handle(dev),
             )
         return grad_gate, grad_value, grad_h0, None, None
 
