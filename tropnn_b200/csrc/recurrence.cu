@@ -102,29 +102,69 @@ __device__ __forceinline__ void store_pair(T *p, float2 v, bool on0, bool on1) {
       if (on1) p[32] = v.y;
     }
   } else {
-    const T a = from_f32<T>(v.x), b = from_f32<T>(v.y);
     if constexpr (PAIRED) {
-      const uint32_t w = uint32_t(*reinterpret_cast<const unsigned short *>(&a)) |
-                         (uint32_t(*reinterpret_cast<const unsigned short *>(&b)) << 16);
+      uint32_t w;
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 q = __float22half2_rn(v);
+        w = *reinterpret_cast<const uint32_t *>(&q);
+      } else {
+        const __nv_bfloat162 q = __float22bfloat162_rn(v);
+        w = *reinterpret_cast<const uint32_t *>(&q);
+      }
       if (on0) *reinterpret_cast<uint32_t *>(p) = w;
     } else {
-      if (on0) p[0] = a;
-      if (on1) p[32] = b;
+      if (on0) p[0] = from_f32<T>(v.x);
+      if (on1) p[32] = from_f32<T>(v.y);
     }
   }
 }
 
+// Both channels of a lane in one instruction (f32x2).
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 float2_of(uint64_t r) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(x)), "l"(bits2(y)));
+  return float2_of(r);
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(x)), "l"(bits2(y)));
+  return float2_of(r);
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(x)), "l"(bits2(y)), "l"(bits2(z)));
+  return float2_of(r);
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // a and c = 1 - a. The smaller one, m = e / (1 + e) with e = exp(-|f|), has its full relative
 // accuracy; the larger is 1 - m, the f32 next to it.
-__device__ __forceinline__ void gates(float f, float &a, float &c) {
-  const float e = __expf(-fabsf(f));
-  const float m = __fdividef(e, 1.f + e), o = 1.f - m;
-  a = f < 0.f ? m : o;
-  c = f < 0.f ? o : m;
-}
-__device__ __forceinline__ float2 mul2(float2 x, float2 y) { return make_float2(x.x * y.x, x.y * y.y); }
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-  return make_float2(fmaf(x.x, y.x, z.x), fmaf(x.y, y.y, z.y));
+__device__ __forceinline__ void gates2(float2 f, float2 &a, float2 &c) {
+  const float2 e = make_float2(exp2_approx(fabsf(f.x) * -1.4426950408889634f), exp2_approx(fabsf(f.y) * -1.4426950408889634f));
+  const float2 d = add2(e, make_float2(1.f, 1.f));
+  const float2 m = mul2(e, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+  const float2 o = fma2(m, make_float2(-1.f, -1.f), make_float2(1.f, 1.f));
+  a = make_float2(f.x < 0.f ? m.x : o.x, f.y < 0.f ? m.y : o.y);
+  c = make_float2(f.x < 0.f ? o.x : m.x, f.y < 0.f ? o.y : m.y);
 }
 
 // P h + H; a run that a reset cut (P = 0) takes nothing of h, not even an infinity's NaN.
@@ -267,11 +307,19 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
   Raw<T> rf[kRun], rx[kRun];
   auto load = [&](int64_t t0) {
     const int n = static_cast<int>(t0 >= stop ? 0 : min64(kRun, stop - t0));
+    const T *pf = gate + t0 * g.gate_step, *px = value + t0 * g.value_step;
+    if (n == kRun) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const bool in = j < n;
-      rf[j] = load_raw<T, PAIRED>(gate + (t0 + j) * g.gate_step, in && on0, in && on1);
-      rx[j] = load_raw<T, PAIRED>(value + (t0 + j) * g.value_step, in && on0, in && on1);
+      for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step) {
+        rf[j] = load_raw<T, PAIRED>(pf, on0, on1);
+        rx[j] = load_raw<T, PAIRED>(px, on0, on1);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step) {
+        rf[j] = load_raw<T, PAIRED>(pf, j < n && on0, j < n && on1);
+        rx[j] = load_raw<T, PAIRED>(px, j < n && on0, j < n && on1);
+      }
     }
   };
   load(first + rank * kTile + warp * kRun);
@@ -292,17 +340,27 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
     const float2 zero = make_float2(0.f, 0.f);
     float2 h = zero, p = make_float2(1.f, 1.f);
     float2 a[kRun], b[kRun];
+    const bool plain = n == kRun && cut == 0;  // whole runs without a reset need no tests
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-      const float2 f = unpack<T>(rf[j]), x = unpack<T>(rx[j]);
       float2 c;
-      gates(f.x, a[j].x, c.x);
-      gates(f.y, a[j].y, c.y);
-      b[j] = mul2(c, x);
-      if (j < n) {
-        if ((cut >> j) & 1u) h = p = zero;
+      gates2(unpack<T>(rf[j]), a[j], c);
+      b[j] = mul2(c, unpack<T>(rx[j]));
+    }
+    if (plain) {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
         h = fma2(a[j], h, b[j]);
         p = mul2(p, a[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (j < n) {
+          if ((cut >> j) & 1u) h = p = zero;
+          h = fma2(a[j], h, b[j]);
+          p = mul2(p, a[j]);
+        }
       }
     }
     load(t0 + int64_t(g.ranks) * kTile);
@@ -312,12 +370,21 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
       if (on0) s[0] = in.x;
       if (on1) s[kSecond<PAIRED>] = in.y;
     }
+    T *po = out + t0 * g.dim;
+    if (plain) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if (j < n) {
-        if ((cut >> j) & 1u) in = zero;
+      for (int j = 0; j < kRun; ++j, po += g.dim) {
         in = fma2(a[j], in, b[j]);
-        store_pair<T, PAIRED>(out + (t0 + j) * g.dim, in, on0, on1);
+        store_pair<T, PAIRED>(po, in, on0, on1);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j, po += g.dim) {
+        if (j < n) {
+          if ((cut >> j) & 1u) in = zero;
+          in = fma2(a[j], in, b[j]);
+          store_pair<T, PAIRED>(po, in, on0, on1);
+        }
       }
     }
   }
@@ -363,12 +430,21 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   auto load = [&](int64_t k) {
     const int64_t t0 = k * kTile + warp * kRun;
     const int n = steps_of(k);
+    const T *pf = gate + t0 * g.gate_step, *px = value + t0 * g.value_step, *pg = grad + t0 * g.dim;
+    if (n == kRun) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const bool in = j < n;
-      rf[j] = load_raw<T, PAIRED>(gate + (t0 + j) * g.gate_step, in && on0, in && on1);
-      rx[j] = load_raw<T, PAIRED>(value + (t0 + j) * g.value_step, in && on0, in && on1);
-      rg[j] = load_raw<T, PAIRED>(grad + (t0 + j) * g.dim, in && on0_g, in && on1_g);
+      for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step, pg += g.dim) {
+        rf[j] = load_raw<T, PAIRED>(pf, on0, on1);
+        rx[j] = load_raw<T, PAIRED>(px, on0, on1);
+        rg[j] = load_raw<T, PAIRED>(pg, on0_g, on1_g);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step, pg += g.dim) {
+        rf[j] = load_raw<T, PAIRED>(pf, j < n && on0, j < n && on1);
+        rx[j] = load_raw<T, PAIRED>(px, j < n && on0, j < n && on1);
+        rg[j] = load_raw<T, PAIRED>(pg, j < n && on0_g, j < n && on1_g);
+      }
     }
     before = make_float2(0.f, 0.f);
     const float *p = g.saved + (batch * g.saved_tiles + k) * g.dim + ch;
@@ -394,24 +470,36 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     const float2 zero = make_float2(0.f, 0.f);
     float2 h = zero, p = make_float2(1.f, 1.f), r = zero, h_in = before;
     float2 a[kRun], c[kRun], x[kRun], gt[kRun];
+    const bool plain = n == kRun && cut == 0;  // whole runs without a reset need no tests
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-      const float2 f = unpack<T>(rf[j]);
+      gates2(unpack<T>(rf[j]), a[j], c[j]);
       x[j] = unpack<T>(rx[j]);
       gt[j] = unpack<T>(rg[j]);
-      gates(f.x, a[j].x, c[j].x);
-      gates(f.y, a[j].y, c[j].y);
-      if (j < n) {
-        if ((cut >> j) & 1u) h = p = zero;
+    }
+    if (plain) {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
         h = fma2(a[j], h, mul2(c[j], x[j]));
         p = mul2(p, a[j]);
       }
-    }
 #pragma unroll
-    for (int j = kRun - 1; j >= 0; --j) {
-      if (j < n) {
-        r = mul2(a[j], make_float2(gt[j].x + r.x, gt[j].y + r.y));
-        if ((cut >> j) & 1u) r = zero;
+      for (int j = kRun - 1; j >= 0; --j) r = mul2(a[j], add2(gt[j], r));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (j < n) {
+          if ((cut >> j) & 1u) h = p = zero;
+          h = fma2(a[j], h, mul2(c[j], x[j]));
+          p = mul2(p, a[j]);
+        }
+      }
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) {
+        if (j < n) {
+          r = mul2(a[j], add2(gt[j], r));
+          if ((cut >> j) & 1u) r = zero;
+        }
       }
     }
     load(k - g.ranks);
@@ -421,24 +509,43 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     for (int w = 0; w < kWarps - 1; ++w) {
       if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane]);
     }
+    // x holds keep h_{t-1} - x from here on.
+    const float2 minus = make_float2(-1.f, -1.f);
+    const int64_t end = (t0 + kRun - 1) * g.dim;
+    T *pf = grad_gate + end, *px = grad_value + end;
+    if (plain) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if (j < n) {
+      for (int j = 0; j < kRun; ++j) {
         const float2 v = x[j];
-        if ((cut >> j) & 1u) h_in = zero;
-        x[j] = make_float2(h_in.x - v.x, h_in.y - v.y);  // keep h_{t-1} - x from here on
+        x[j] = fma2(v, minus, h_in);
         h_in = fma2(a[j], h_in, mul2(c[j], v));
       }
-    }
 #pragma unroll
-    for (int j = kRun - 1; j >= 0; --j) {
-      if (j < n) {
-        const float2 ds = make_float2(gt[j].x + r_in.x, gt[j].y + r_in.y);
-        const float2 gx = mul2(c[j], ds);
+      for (int j = kRun - 1; j >= 0; --j, pf -= g.dim, px -= g.dim) {
+        const float2 ds = add2(gt[j], r_in), gx = mul2(c[j], ds);
         r_in = mul2(a[j], ds);
-        store_pair<T, PAIRED>(grad_value + (t0 + j) * g.dim, gx, on0, on1);
-        store_pair<T, PAIRED>(grad_gate + (t0 + j) * g.dim, mul2(mul2(a[j], gx), x[j]), on0, on1);
-        if ((cut >> j) & 1u) r_in = zero;
+        store_pair<T, PAIRED>(px, gx, on0, on1);
+        store_pair<T, PAIRED>(pf, mul2(mul2(a[j], gx), x[j]), on0, on1);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (j < n) {
+          const float2 v = x[j];
+          if ((cut >> j) & 1u) h_in = zero;
+          x[j] = fma2(v, minus, h_in);
+          h_in = fma2(a[j], h_in, mul2(c[j], v));
+        }
+      }
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j, pf -= g.dim, px -= g.dim) {
+        if (j < n) {
+          const float2 ds = add2(gt[j], r_in), gx = mul2(c[j], ds);
+          r_in = mul2(a[j], ds);
+          store_pair<T, PAIRED>(px, gx, on0, on1);
+          store_pair<T, PAIRED>(pf, mul2(mul2(a[j], gx), x[j]), on0, on1);
+          if ((cut >> j) & 1u) r_in = zero;
+        }
       }
     }
   }
@@ -487,15 +594,14 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_map_kernel(const Recur
       if (j < n) {
         const float2 f = unpack<T>(rf[j]), o = unpack<T>(ro[j]);
         float2 a, c;
-        gates(f.x, a.x, c.x);
-        gates(f.y, a.y, c.y);
+        gates2(f, a, c);
         const bool here = (cut >> j) & 1u;
         if (FORWARD) {
           if (here) h = p = zero;
           h = fma2(a, h, mul2(c, o));
           p = mul2(p, a);
         } else {
-          h = mul2(a, make_float2(o.x + h.x, o.y + h.y));
+          h = mul2(a, add2(o, h));
           p = mul2(p, a);
           if (here) h = p = zero;
         }
@@ -531,9 +637,9 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(const T *__restric
   const int64_t row = blockIdx.y;
   if (ch >= dim) return;
   const float before = reset != nullptr && reset[row] != 0 ? 0.f : state[row * state_row + ch];
-  float a, c;
-  gates(to_f32<T>(gate[row * gate_row + ch]), a, c);
-  const float now = fmaf(a, before, c * to_f32<T>(value[row * value_row + ch]));
+  float2 a, c;
+  gates2(make_float2(to_f32<T>(gate[row * gate_row + ch]), 0.f), a, c);
+  const float now = fmaf(a.x, before, c.x * to_f32<T>(value[row * value_row + ch]));
   state[row * state_row + ch] = now;
   h[row * dim + ch] = from_f32<T>(now);
 }
