@@ -74,6 +74,8 @@ SHAPES = [
     (5, 1025, 64),
     (1, 4099, 16),  # a long one, few channels
     (40, 130, 200),
+    (2, 20011, 24),  # so few channels that the sequence is cut into chunks
+    (1, 20011, 21),
 ]
 
 

@@ -51,35 +51,47 @@ __device__ __forceinline__ int first_channel(int lane) { return PAIRED ? 2 * lan
 template <bool PAIRED>
 constexpr int kSecond = PAIRED ? 1 : 32;
 
+// `second`: distance of the lane's second channel (PAIRED: 1).
 template <typename T, bool PAIRED>
-__device__ __forceinline__ Raw<T> load_raw(const T *p, bool on0, bool on1) {
+__device__ __forceinline__ Raw<T> load_raw(const T *p, int second) {
   Raw<T> r;
   if constexpr (sizeof(T) == 4) {
-    r.a = r.b = 0.f;
     if constexpr (PAIRED) {
-      if (on0) {
-        const float2 q = __ldg(reinterpret_cast<const float2 *>(p));
-        r.a = q.x;
-        r.b = q.y;
-      }
+      const float2 q = __ldg(reinterpret_cast<const float2 *>(p));
+      r.a = q.x;
+      r.b = q.y;
     } else {
-      if (on0) r.a = __ldg(p);
-      if (on1) r.b = __ldg(p + 32);
+      r.a = __ldg(p);
+      r.b = __ldg(p + second);
     }
   } else {
-    r.v = 0u;
     if constexpr (PAIRED) {
-      if (on0) r.v = __ldg(reinterpret_cast<const unsigned int *>(p));
+      r.v = __ldg(reinterpret_cast<const unsigned int *>(p));
     } else {
       const unsigned short *u = reinterpret_cast<const unsigned short *>(p);
-      uint32_t lo = 0, hi = 0;
-      if (on0) lo = __ldg(u);
-      if (on1) hi = __ldg(u + 32);
-      r.v = lo | (hi << 16);
+      r.v = uint32_t(__ldg(u)) | (uint32_t(__ldg(u + second)) << 16);
     }
   }
   return r;
 }
+
+// A lane's two channels: where it stores, and where it loads. Lanes past the last channel load
+// channels that are there and store nothing.
+template <bool PAIRED>
+struct Lane {
+  int64_t ch;      // first channel
+  bool on0, on1;   // which of the two are there
+  int64_t from;    // loads: first channel, and the second's distance
+  int second;
+  __device__ __forceinline__ Lane(int64_t block, int64_t dim) {
+    const int lane = threadIdx.x & 31;
+    ch = block * kChan + first_channel<PAIRED>(lane);
+    on0 = ch < dim;
+    on1 = ch + kSecond<PAIRED> < dim;
+    from = on0 ? ch : (PAIRED ? dim - 2 : dim - 1);
+    second = PAIRED ? 1 : (on1 ? 32 : 0);
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ float2 unpack(Raw<T> r) {
@@ -287,6 +299,127 @@ __device__ __forceinline__ uint32_t reset_bits(const uint8_t *row, int64_t t0, i
   return bits;
 }
 
+// A run's map from its gates and c x: (p, h). `plain`: all its steps are there and none is a reset.
+template <int RUN>
+__device__ __forceinline__ void scan_run(const float2 (&a)[RUN], const float2 (&b)[RUN], int n, uint32_t cut, bool plain,
+                                         float2 &p, float2 &h) {
+  const float2 zero = make_float2(0.f, 0.f);
+  h = zero;
+  p = make_float2(1.f, 1.f);
+  if (plain) {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      h = fma2(a[j], h, b[j]);
+      p = mul2(p, a[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      if (j < n) {
+        if ((cut >> j) & 1u) h = p = zero;
+        h = fma2(a[j], h, b[j]);
+        p = mul2(p, a[j]);
+      }
+    }
+  }
+}
+// The run from the state before it: store(j, h_j).
+template <int RUN, typename Store>
+__device__ __forceinline__ void emit_run(const float2 (&a)[RUN], const float2 (&b)[RUN], int n, uint32_t cut, bool plain,
+                                         float2 in, Store store) {
+  if (plain) {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      in = fma2(a[j], in, b[j]);
+      store(j, in);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      if (j < n) {
+        if ((cut >> j) & 1u) in = make_float2(0.f, 0.f);
+        in = fma2(a[j], in, b[j]);
+        store(j, in);
+      }
+    }
+  }
+}
+// Backward: a run's maps, (p, h) forward and (p, r) from its end.
+template <int RUN>
+__device__ __forceinline__ void scan_run_back(const float2 (&a)[RUN], const float2 (&c)[RUN], const float2 (&x)[RUN],
+                                              const float2 (&gt)[RUN], int n, uint32_t cut, bool plain, float2 &p,
+                                              float2 &h, float2 &r) {
+  const float2 zero = make_float2(0.f, 0.f);
+  h = r = zero;
+  p = make_float2(1.f, 1.f);
+  if (plain) {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      h = fma2(a[j], h, mul2(c[j], x[j]));
+      p = mul2(p, a[j]);
+    }
+#pragma unroll
+    for (int j = RUN - 1; j >= 0; --j) r = mul2(a[j], add2(gt[j], r));
+  } else {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      if (j < n) {
+        if ((cut >> j) & 1u) h = p = zero;
+        h = fma2(a[j], h, mul2(c[j], x[j]));
+        p = mul2(p, a[j]);
+      }
+    }
+#pragma unroll
+    for (int j = RUN - 1; j >= 0; --j) {
+      if (j < n) {
+        r = mul2(a[j], add2(gt[j], r));
+        if ((cut >> j) & 1u) r = zero;
+      }
+    }
+  }
+}
+// The run's gradients from the state before it and r after it: store(j, grad_gate, grad_value), from
+// the last step back. x is used up.
+template <int RUN, typename Store>
+__device__ __forceinline__ void emit_run_back(const float2 (&a)[RUN], const float2 (&c)[RUN], float2 (&x)[RUN],
+                                              const float2 (&gt)[RUN], int n, uint32_t cut, bool plain, float2 h_in,
+                                              float2 r_in, Store store) {
+  const float2 zero = make_float2(0.f, 0.f), minus = make_float2(-1.f, -1.f);
+  if (plain) {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      const float2 v = x[j];
+      x[j] = fma2(v, minus, h_in);  // keep h_{t-1} - x
+      h_in = fma2(a[j], h_in, mul2(c[j], v));
+    }
+#pragma unroll
+    for (int j = RUN - 1; j >= 0; --j) {
+      const float2 ds = add2(gt[j], r_in), gx = mul2(c[j], ds);
+      r_in = mul2(a[j], ds);
+      store(j, mul2(mul2(a[j], gx), x[j]), gx);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      if (j < n) {
+        const float2 v = x[j];
+        if ((cut >> j) & 1u) h_in = zero;
+        x[j] = fma2(v, minus, h_in);
+        h_in = fma2(a[j], h_in, mul2(c[j], v));
+      }
+    }
+#pragma unroll
+    for (int j = RUN - 1; j >= 0; --j) {
+      if (j < n) {
+        const float2 ds = add2(gt[j], r_in), gx = mul2(c[j], ds);
+        r_in = mul2(a[j], ds);
+        store(j, mul2(mul2(a[j], gx), x[j]), gx);
+        if ((cut >> j) & 1u) r_in = zero;
+      }
+    }
+  }
+}
+
 template <typename T, bool PAIRED>
 __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const RecurrenceArgs g) {
   constexpr int kRun = kRunFwd<T>, kTile = kWarps * kRun;
@@ -295,10 +428,11 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
   const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
   const int unit = blockIdx.x / g.ranks;
   const int64_t batch = unit / g.channel_blocks;
-  const int64_t ch = int64_t(unit % g.channel_blocks) * kChan + first_channel<PAIRED>(lane);
-  const bool on0 = ch < g.dim, on1 = ch + kSecond<PAIRED> < g.dim;
-  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + ch;
-  const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + ch;
+  const Lane<PAIRED> at(unit % g.channel_blocks, g.dim);
+  const int64_t ch = at.ch;
+  const bool on0 = at.on0, on1 = at.on1;
+  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + at.from;
+  const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + at.from;
   T *out = static_cast<T *>(g.h) + batch * g.steps * g.dim + ch;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
   const int64_t first = chunk * g.chunk_tiles * kTile, stop = min64(g.steps, first + g.chunk_tiles * kTile);
@@ -306,19 +440,21 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
 
   Raw<T> rf[kRun], rx[kRun];
   auto load = [&](int64_t t0) {
-    const int n = static_cast<int>(t0 >= stop ? 0 : min64(kRun, stop - t0));
+    if (t0 >= stop) return;
+    // Steps past the end load the last one again.
+    const int64_t most = stop - 1 - t0;
     const T *pf = gate + t0 * g.gate_step, *px = value + t0 * g.value_step;
-    if (n == kRun) {
+    if (most >= kRun - 1) {
 #pragma unroll
       for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step) {
-        rf[j] = load_raw<T, PAIRED>(pf, on0, on1);
-        rx[j] = load_raw<T, PAIRED>(px, on0, on1);
+        rf[j] = load_raw<T, PAIRED>(pf, at.second);
+        rx[j] = load_raw<T, PAIRED>(px, at.second);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step) {
-        rf[j] = load_raw<T, PAIRED>(pf, j < n && on0, j < n && on1);
-        rx[j] = load_raw<T, PAIRED>(px, j < n && on0, j < n && on1);
+      for (int j = 0; j < kRun; ++j) {
+        rf[j] = load_raw<T, PAIRED>(pf + min64(j, most) * g.gate_step, at.second);
+        rx[j] = load_raw<T, PAIRED>(px + min64(j, most) * g.value_step, at.second);
       }
     }
   };
@@ -337,56 +473,27 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
     const int64_t t0 = tile + rank * kTile + warp * kRun;
     const int n = static_cast<int>(t0 >= stop ? 0 : min64(kRun, stop - t0));
     const uint32_t cut = reset_bits(reset, t0, n);
-    const float2 zero = make_float2(0.f, 0.f);
-    float2 h = zero, p = make_float2(1.f, 1.f);
-    float2 a[kRun], b[kRun];
-    const bool plain = n == kRun && cut == 0;  // whole runs without a reset need no tests
+    const bool plain = n == kRun && cut == 0;
+    float2 a[kRun], b[kRun], p, h;
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
       float2 c;
       gates2(unpack<T>(rf[j]), a[j], c);
       b[j] = mul2(c, unpack<T>(rx[j]));
     }
-    if (plain) {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        h = fma2(a[j], h, b[j]);
-        p = mul2(p, a[j]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        if (j < n) {
-          if ((cut >> j) & 1u) h = p = zero;
-          h = fma2(a[j], h, b[j]);
-          p = mul2(p, a[j]);
-        }
-      }
-    }
+    scan_run<kRun>(a, b, n, cut, plain, p, h);
     load(t0 + int64_t(g.ranks) * kTile);
-    float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank);
+    const float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank);
     if (g.saved != nullptr && (warp * kRun) % kTileBwd == 0 && n > 0) {
       float *s = g.saved + (batch * g.saved_tiles + t0 / kTileBwd) * g.dim + ch;
       if (on0) s[0] = in.x;
       if (on1) s[kSecond<PAIRED>] = in.y;
     }
     T *po = out + t0 * g.dim;
-    if (plain) {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j, po += g.dim) {
-        in = fma2(a[j], in, b[j]);
-        store_pair<T, PAIRED>(po, in, on0, on1);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j, po += g.dim) {
-        if (j < n) {
-          if ((cut >> j) & 1u) in = zero;
-          in = fma2(a[j], in, b[j]);
-          store_pair<T, PAIRED>(po, in, on0, on1);
-        }
-      }
-    }
+    emit_run<kRun>(a, b, n, cut, plain, in, [&](int, float2 v) {
+      store_pair<T, PAIRED>(po, v, on0, on1);
+      po += g.dim;
+    });
   }
   if (warp == 0 && rank == 0 && chunk == g.chunks - 1) {
     float *p = g.h_last + batch * g.dim + ch;
@@ -409,47 +516,47 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
   const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
   const int unit = blockIdx.x / g.ranks;
   const int64_t batch = unit / g.channel_blocks;
-  const int64_t ch = int64_t(unit % g.channel_blocks) * kChan + first_channel<PAIRED>(lane);
-  const bool on0 = ch < g.dim, on1 = ch + kSecond<PAIRED> < g.dim;
-  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + ch;
-  const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + ch;
-  const T *grad = g.grad != nullptr ? static_cast<const T *>(g.grad) + batch * g.steps * g.dim + ch : nullptr;
-  const bool on0_g = on0 && grad != nullptr, on1_g = on1 && grad != nullptr;
+  const Lane<PAIRED> at(unit % g.channel_blocks, g.dim);
+  const int64_t ch = at.ch;
+  const bool on0 = at.on0, on1 = at.on1;
+  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + at.from;
+  const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + at.from;
+  const T *grad = g.grad != nullptr ? static_cast<const T *>(g.grad) + batch * g.steps * g.dim + at.from : nullptr;
   T *grad_gate = static_cast<T *>(g.grad_gate) + batch * g.steps * g.dim + ch;
   T *grad_value = static_cast<T *>(g.grad_value) + batch * g.steps * g.dim + ch;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
   const int64_t first = chunk * g.chunk_tiles, stop = min64(g.saved_tiles, first + g.chunk_tiles);
   if (g.ranks > 1) cluster_arrive();
 
-  Raw<T> rf[kRun], rx[kRun], rg[kRun];
-  float2 before;
+  Raw<T> rf[kRun], rx[kRun], rg[kRun] = {};
+  float2 before = make_float2(0.f, 0.f);
   auto steps_of = [&](int64_t k) -> int {
     const int64_t t0 = k * kTile + warp * kRun;
     return static_cast<int>(k < first || t0 >= g.steps ? 0 : min64(kRun, g.steps - t0));
   };
   auto load = [&](int64_t k) {
-    const int64_t t0 = k * kTile + warp * kRun;
-    const int n = steps_of(k);
-    const T *pf = gate + t0 * g.gate_step, *px = value + t0 * g.value_step, *pg = grad + t0 * g.dim;
-    if (n == kRun) {
+    if (k < first) return;
+    // Steps past the end load the last one again.
+    const int64_t t0 = k * kTile + warp * kRun, from = min64(t0, g.steps - 1), most = g.steps - 1 - from;
+    const T *pf = gate + from * g.gate_step, *px = value + from * g.value_step, *pg = grad + from * g.dim;
+    if (most >= kRun - 1) {
 #pragma unroll
       for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step, pg += g.dim) {
-        rf[j] = load_raw<T, PAIRED>(pf, on0, on1);
-        rx[j] = load_raw<T, PAIRED>(px, on0, on1);
-        rg[j] = load_raw<T, PAIRED>(pg, on0_g, on1_g);
+        rf[j] = load_raw<T, PAIRED>(pf, at.second);
+        rx[j] = load_raw<T, PAIRED>(px, at.second);
+        if (grad != nullptr) rg[j] = load_raw<T, PAIRED>(pg, at.second);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step, pg += g.dim) {
-        rf[j] = load_raw<T, PAIRED>(pf, j < n && on0, j < n && on1);
-        rx[j] = load_raw<T, PAIRED>(px, j < n && on0, j < n && on1);
-        rg[j] = load_raw<T, PAIRED>(pg, j < n && on0_g, j < n && on1_g);
+      for (int j = 0; j < kRun; ++j) {
+        const int64_t d = min64(j, most);
+        rf[j] = load_raw<T, PAIRED>(pf + d * g.gate_step, at.second);
+        rx[j] = load_raw<T, PAIRED>(px + d * g.value_step, at.second);
+        if (grad != nullptr) rg[j] = load_raw<T, PAIRED>(pg + d * g.dim, at.second);
       }
     }
-    before = make_float2(0.f, 0.f);
-    const float *p = g.saved + (batch * g.saved_tiles + k) * g.dim + ch;
-    if (n > 0 && on0) before.x = __ldg(p);
-    if (n > 0 && on1) before.y = __ldg(p + kSecond<PAIRED>);
+    const float *p = g.saved + (batch * g.saved_tiles + k) * g.dim + at.from;
+    before = make_float2(__ldg(p), __ldg(p + at.second));
   };
   load(stop - 1 - rank);
   float2 back = make_float2(0.f, 0.f);  // r of the step after the cluster's tiles
@@ -467,93 +574,284 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     const int n = steps_of(k);
     const uint32_t cut = reset_bits(reset, t0, n);
 
-    const float2 zero = make_float2(0.f, 0.f);
-    float2 h = zero, p = make_float2(1.f, 1.f), r = zero, h_in = before;
-    float2 a[kRun], c[kRun], x[kRun], gt[kRun];
-    const bool plain = n == kRun && cut == 0;  // whole runs without a reset need no tests
+    const bool plain = n == kRun && cut == 0;
+    float2 a[kRun], c[kRun], x[kRun], gt[kRun], p, h, r, h_in = before;
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
       gates2(unpack<T>(rf[j]), a[j], c[j]);
       x[j] = unpack<T>(rx[j]);
       gt[j] = unpack<T>(rg[j]);
     }
-    if (plain) {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        h = fma2(a[j], h, mul2(c[j], x[j]));
-        p = mul2(p, a[j]);
-      }
-#pragma unroll
-      for (int j = kRun - 1; j >= 0; --j) r = mul2(a[j], add2(gt[j], r));
-    } else {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        if (j < n) {
-          if ((cut >> j) & 1u) h = p = zero;
-          h = fma2(a[j], h, mul2(c[j], x[j]));
-          p = mul2(p, a[j]);
-        }
-      }
-#pragma unroll
-      for (int j = kRun - 1; j >= 0; --j) {
-        if (j < n) {
-          r = mul2(a[j], add2(gt[j], r));
-          if ((cut >> j) & 1u) r = zero;
-        }
-      }
-    }
+    scan_run_back<kRun>(a, c, x, gt, n, cut, plain, p, h, r);
     load(k - g.ranks);
     run_h[buf][warp][lane] = h;
-    float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank);
+    const float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank);
 #pragma unroll
     for (int w = 0; w < kWarps - 1; ++w) {
       if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane]);
     }
-    // x holds keep h_{t-1} - x from here on.
-    const float2 minus = make_float2(-1.f, -1.f);
-    const int64_t end = (t0 + kRun - 1) * g.dim;
-    T *pf = grad_gate + end, *px = grad_value + end;
-    if (plain) {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        const float2 v = x[j];
-        x[j] = fma2(v, minus, h_in);
-        h_in = fma2(a[j], h_in, mul2(c[j], v));
-      }
-#pragma unroll
-      for (int j = kRun - 1; j >= 0; --j, pf -= g.dim, px -= g.dim) {
-        const float2 ds = add2(gt[j], r_in), gx = mul2(c[j], ds);
-        r_in = mul2(a[j], ds);
-        store_pair<T, PAIRED>(px, gx, on0, on1);
-        store_pair<T, PAIRED>(pf, mul2(mul2(a[j], gx), x[j]), on0, on1);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        if (j < n) {
-          const float2 v = x[j];
-          if ((cut >> j) & 1u) h_in = zero;
-          x[j] = fma2(v, minus, h_in);
-          h_in = fma2(a[j], h_in, mul2(c[j], v));
-        }
-      }
-#pragma unroll
-      for (int j = kRun - 1; j >= 0; --j, pf -= g.dim, px -= g.dim) {
-        if (j < n) {
-          const float2 ds = add2(gt[j], r_in), gx = mul2(c[j], ds);
-          r_in = mul2(a[j], ds);
-          store_pair<T, PAIRED>(px, gx, on0, on1);
-          store_pair<T, PAIRED>(pf, mul2(mul2(a[j], gx), x[j]), on0, on1);
-          if ((cut >> j) & 1u) r_in = zero;
-        }
-      }
-    }
+    T *pf = grad_gate + t0 * g.dim, *px = grad_value + t0 * g.dim;
+    emit_run_back<kRun>(a, c, x, gt, n, cut, plain, h_in, r_in, [&](int j, float2 gf, float2 gx) {
+      store_pair<T, PAIRED>(px + j * g.dim, gx, on0, on1);
+      store_pair<T, PAIRED>(pf + j * g.dim, gf, on0, on1);
+    });
   }
   if (warp == 0 && rank == 0 && chunk == 0 && g.grad_h0 != nullptr) {
     float *p = g.grad_h0 + batch * g.dim + ch;
     if (on0) p[0] = back.x;
     if (on1) p[kSecond<PAIRED>] = back.y;
   }
+}
+
+// The same two kernels with the data brought by TMA: each warp has its own ring of stages in shared
+// memory, loads its runs of [steps x 64 channels] into them two or three tiles ahead, writes its
+// results over the inputs of the stage and stores them from there. No registers hold data in
+// flight, no address is computed an element, rows and channels that are not there come as zeros and
+// are not written. Needs rows 16 bytes aligned (dim and strides multiples of 8 16-bit or 4 f32
+// elements); the kernels above serve all else.
+struct SequenceMaps {
+  CUtensorMap gate, value, grad, out_gate, out_value;  // out_value: h in the forward
+};
+__device__ int g_recurrence_error = 0;
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void *src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(sm100::smem_addr(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+
+template <typename T>
+__device__ __forceinline__ Raw<T> stage_raw(const T *row, int lane) {
+  Raw<T> r;
+  if constexpr (sizeof(T) == 4) {
+    const float2 q = reinterpret_cast<const float2 *>(row)[lane];
+    r.a = q.x;
+    r.b = q.y;
+  } else {
+    r.v = reinterpret_cast<const uint32_t *>(row)[lane];
+  }
+  return r;
+}
+
+// Neighbours in an f32 array that may start anywhere.
+__device__ __forceinline__ float2 two_floats(const float *p) { return make_float2(__ldg(p), __ldg(p + 1)); }
+__device__ __forceinline__ void put_two_floats(float *p, float2 v) {
+  p[0] = v.x;
+  p[1] = v.y;
+}
+
+template <typename T>
+constexpr int kStagesFwd = 3;
+template <typename T>
+constexpr int kStagesBwd = sizeof(T) == 2 ? 3 : 2;
+template <typename T, bool FORWARD>
+constexpr size_t kRingBytes = FORWARD ? size_t(kWarps) * kStagesFwd<T> * 2 * kRunFwd<T> * kChan * sizeof(T)
+                                      : size_t(kWarps) * kStagesBwd<T> * 3 * kRunBwd * kChan * sizeof(T);
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+    recurrence_forward_tma_kernel(const RecurrenceArgs g, const __grid_constant__ SequenceMaps maps) {
+  constexpr int kRun = kRunFwd<T>, kTile = kWarps * kRun, kStages = kStagesFwd<T>;
+  constexpr uint32_t kBytes = 2 * kRun * kChan * sizeof(T);
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  __shared__ Exchange ex;
+  __shared__ uint64_t full[kWarps][kStages];
+  __shared__ int abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
+  const int unit = blockIdx.x / g.ranks;
+  const int batch = unit / g.channel_blocks, ch0 = unit % g.channel_blocks * kChan;
+  const int64_t ch = ch0 + 2 * lane;
+  const bool on = ch < g.dim;
+  const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
+  const int64_t first = chunk * g.chunk_tiles * kTile, stop = min64(g.steps, first + g.chunk_tiles * kTile);
+  const int64_t stride = int64_t(g.ranks) * kTile;
+  T *ring = reinterpret_cast<T *>(dynamic) + size_t(warp) * kStages * 2 * kRun * kChan;
+  auto stage = [&](int s) -> T * { return ring + s * 2 * kRun * kChan; };
+  auto fetch = [&](int64_t t0, int s) {  // one lane
+    if (t0 >= stop) return;
+    sm100::mbar_expect_tx(&full[warp][s], kBytes);
+    sm100::tma_load_3d(stage(s), &maps.gate, &full[warp][s], ch0, static_cast<int>(t0), batch);
+    sm100::tma_load_3d(stage(s) + kRun * kChan, &maps.value, &full[warp][s], ch0, static_cast<int>(t0), batch);
+  };
+  auto flag_of = [&](int64_t t0) -> uint32_t {
+    return reset != nullptr && lane < kRun && t0 + lane < stop ? __ldg(reset + t0 + lane) : 0u;
+  };
+  if (g.ranks > 1) cluster_arrive();
+  if (threadIdx.x == 0) abort = 0;
+  const int64_t t_first = first + rank * kTile + warp * kRun;
+  if (lane == 0) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) sm100::mbar_init(&full[warp][s], 1);
+    sm100::mbar_init_fence();
+    sm100::fence_proxy_async_smem();
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) fetch(t_first + s * stride, s);
+  }
+  uint32_t flag = flag_of(t_first);
+  __syncthreads();
+
+  float2 state = make_float2(0.f, 0.f);
+  if (g.h0 != nullptr && on) state = two_floats(g.h0 + batch * g.dim + ch);
+  if (chunk > 0) state = through_chunks<true, true>(g, batch, ch, on, on, chunk, state, ex);
+  if (g.ranks > 1) cluster_wait();
+
+  int buf = 0, s = 0;
+  uint32_t parity = 0;
+  for (int64_t tile = first, t0 = t_first; tile < stop; tile += stride, t0 += stride, buf ^= 1) {
+    const int n = static_cast<int>(t0 >= stop ? 0 : min64(kRun, stop - t0));
+    const uint32_t cut = __ballot_sync(0xffffffffu, flag != 0);
+    flag = flag_of(t0 + stride);
+    const bool plain = n == kRun && cut == 0;
+    if (n > 0) sm100::mbar_wait(&full[warp][s], parity, &abort, &g_recurrence_error);
+    T *rows = stage(s);
+    float2 a[kRun], b[kRun], p, h;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      float2 c;
+      gates2(unpack<T>(stage_raw<T>(rows + j * kChan, lane)), a[j], c);
+      b[j] = mul2(c, unpack<T>(stage_raw<T>(rows + (kRun + j) * kChan, lane)));
+    }
+    scan_run<kRun>(a, b, n, cut, plain, p, h);
+    const float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank);
+    if (g.saved != nullptr && (warp * kRun) % kTileBwd == 0 && n > 0 && on)
+      put_two_floats(g.saved + (batch * g.saved_tiles + t0 / kTileBwd) * g.dim + ch, in);
+    emit_run<kRun>(a, b, n, cut, plain, in,
+                   [&](int j, float2 v) { store_pair<T, true>(rows + (kRun + j) * kChan + 2 * lane, v, true, true); });
+    sm100::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (n > 0) tma_store_3d(&maps.out_value, rows + kRun * kChan, ch0, static_cast<int>(t0), batch);
+      sm100::bulk_commit();
+      // The stage before this one has been read by its store: its next tile comes in.
+      bulk_wait_read<1>();
+      if (tile > first) fetch(t0 + (kStages - 1) * stride, s == 0 ? kStages - 1 : s - 1);
+    }
+    if (++s == kStages) {
+      s = 0;
+      parity ^= 1;
+    }
+  }
+  if (warp == 0 && rank == 0 && chunk == g.chunks - 1 && on) put_two_floats(g.h_last + batch * g.dim + ch, state);
+  if (lane == 0) sm100::bulk_wait_read_all();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+    recurrence_backward_tma_kernel(const RecurrenceArgs g, const __grid_constant__ SequenceMaps maps) {
+  constexpr int kRun = kRunBwd, kTile = kTileBwd, kStages = kStagesBwd<T>, kPart = kRun * kChan;
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  __shared__ Exchange ex;
+  __shared__ float2 run_h[2][kWarps][32];
+  __shared__ uint64_t full[kWarps][kStages];
+  __shared__ int abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
+  const int unit = blockIdx.x / g.ranks;
+  const int batch = unit / g.channel_blocks, ch0 = unit % g.channel_blocks * kChan;
+  const int64_t ch = ch0 + 2 * lane;
+  const bool on = ch < g.dim, graded = g.grad != nullptr;
+  const uint32_t bytes = (graded ? 3 : 2) * kPart * sizeof(T);
+  const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
+  const int64_t first = chunk * g.chunk_tiles, stop = min64(g.saved_tiles, first + g.chunk_tiles);
+  T *ring = reinterpret_cast<T *>(dynamic) + size_t(warp) * kStages * 3 * kPart;
+  auto stage = [&](int s) -> T * { return ring + s * 3 * kPart; };
+  auto there = [&](int64_t k) { return k >= first && k * kTile + warp * kRun < g.steps; };
+  auto fetch = [&](int64_t k, int s) {  // one lane
+    if (!there(k)) return;
+    const int t0 = static_cast<int>(k * kTile + warp * kRun);
+    sm100::mbar_expect_tx(&full[warp][s], bytes);
+    sm100::tma_load_3d(stage(s), &maps.gate, &full[warp][s], ch0, t0, batch);
+    sm100::tma_load_3d(stage(s) + kPart, &maps.value, &full[warp][s], ch0, t0, batch);
+    if (graded) sm100::tma_load_3d(stage(s) + 2 * kPart, &maps.grad, &full[warp][s], ch0, t0, batch);
+  };
+  auto flag_of = [&](int64_t k) -> uint32_t {
+    const int64_t t = k * kTile + warp * kRun + lane;
+    return reset != nullptr && k >= first && lane < kRun && t < g.steps ? __ldg(reset + t) : 0u;
+  };
+  auto before_of = [&](int64_t k) -> float2 {
+    if (!there(k) || !on) return make_float2(0.f, 0.f);
+    return two_floats(g.saved + (batch * g.saved_tiles + k) * g.dim + ch);
+  };
+  if (g.ranks > 1) cluster_arrive();
+  if (threadIdx.x == 0) abort = 0;
+  const int64_t k_first = stop - 1 - rank;
+  // Stages are filled and used in order, one a tile that this warp has steps of: only the sequence's
+  // last tile may be without.
+  const bool skip = !there(k_first) && k_first >= first;
+  const int64_t k_fill = skip ? k_first - g.ranks : k_first;
+  if (lane == 0) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) sm100::mbar_init(&full[warp][s], 1);
+    sm100::mbar_init_fence();
+    sm100::fence_proxy_async_smem();
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) fetch(k_fill - int64_t(s) * g.ranks, s);
+  }
+  uint32_t flag = flag_of(k_first);
+  float2 before = before_of(k_first);
+  __syncthreads();
+
+  float2 back = make_float2(0.f, 0.f);
+  if (g.grad_last != nullptr && on) back = two_floats(g.grad_last + batch * g.dim + ch);
+  if (chunk < g.chunks - 1) back = through_chunks<true, false>(g, batch, ch, on, on, chunk, back, ex);
+  if (g.ranks > 1) cluster_wait();
+
+  int buf = 0, s = 0, done = 0;
+  uint32_t parity = 0;
+  for (int64_t last = stop - 1, k = k_first; last >= first; last -= g.ranks, k -= g.ranks, buf ^= 1) {
+    const bool here = there(k);
+    const int n = here ? static_cast<int>(min64(kRun, g.steps - (k * kTile + warp * kRun))) : 0;
+    const uint32_t cut = __ballot_sync(0xffffffffu, flag != 0);
+    flag = flag_of(k - g.ranks);
+    float2 h_in = before;
+    before = before_of(k - g.ranks);
+    const bool plain = n == kRun && cut == 0;
+    if (here) sm100::mbar_wait(&full[warp][s], parity, &abort, &g_recurrence_error);
+    T *rows = stage(s);
+    float2 a[kRun], c[kRun], x[kRun], gt[kRun], p, h, r;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      gates2(unpack<T>(stage_raw<T>(rows + j * kChan, lane)), a[j], c[j]);
+      x[j] = unpack<T>(stage_raw<T>(rows + kPart + j * kChan, lane));
+      gt[j] = graded ? unpack<T>(stage_raw<T>(rows + 2 * kPart + j * kChan, lane)) : make_float2(0.f, 0.f);
+    }
+    scan_run_back<kRun>(a, c, x, gt, n, cut, plain, p, h, r);
+    run_h[buf][warp][lane] = h;
+    const float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank);
+#pragma unroll
+    for (int w = 0; w < kWarps - 1; ++w) {
+      if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane]);
+    }
+    emit_run_back<kRun>(a, c, x, gt, n, cut, plain, h_in, r_in, [&](int j, float2 gf, float2 gx) {
+      store_pair<T, true>(rows + j * kChan + 2 * lane, gf, true, true);
+      store_pair<T, true>(rows + kPart + j * kChan + 2 * lane, gx, true, true);
+    });
+    sm100::fence_proxy_async_smem();
+    __syncwarp();
+    if (here) {
+      if (lane == 0) {
+        const int t0 = static_cast<int>(k * kTile + warp * kRun);
+        tma_store_3d(&maps.out_gate, rows, ch0, t0, batch);
+        tma_store_3d(&maps.out_value, rows + kPart, ch0, t0, batch);
+        sm100::bulk_commit();
+        // The stage before this one has been read by its stores: its next tile comes in.
+        bulk_wait_read<1>();
+        if (done > 0) fetch(k - int64_t(kStages - 1) * g.ranks, s == 0 ? kStages - 1 : s - 1);
+      }
+      ++done;
+      if (++s == kStages) {
+        s = 0;
+        parity ^= 1;
+      }
+    }
+  }
+  if (warp == 0 && rank == 0 && chunk == 0 && g.grad_h0 != nullptr && on)
+    put_two_floats(g.grad_h0 + batch * g.dim + ch, back);
+  if (lane == 0) sm100::bulk_wait_read_all();
 }
 
 // The map of each chunk: (P, H) forward, (P, R) for the backward. Each warp scans an equal stretch of
@@ -565,11 +863,12 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_map_kernel(const Recur
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunk = FORWARD ? blockIdx.y : blockIdx.y + 1;  // the last (first) chunk's map is not asked for
   const int64_t batch = blockIdx.x / g.channel_blocks;
-  const int64_t ch = int64_t(blockIdx.x % g.channel_blocks) * kChan + first_channel<PAIRED>(lane);
-  const bool on0 = ch < g.dim, on1 = ch + kSecond<PAIRED> < g.dim;
-  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + ch;
-  const T *other = FORWARD ? static_cast<const T *>(g.value) + batch * g.value_batch + ch
-                           : (g.grad != nullptr ? static_cast<const T *>(g.grad) + batch * g.steps * g.dim + ch : nullptr);
+  const Lane<PAIRED> at(blockIdx.x % g.channel_blocks, g.dim);
+  const int64_t ch = at.ch;
+  const bool on0 = at.on0, on1 = at.on1;
+  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + at.from;
+  const T *other = FORWARD ? static_cast<const T *>(g.value) + batch * g.value_batch + at.from
+                           : (g.grad != nullptr ? static_cast<const T *>(g.grad) + batch * g.steps * g.dim + at.from : nullptr);
   const int64_t other_step = FORWARD ? g.value_step : g.dim;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
   const int64_t share = chunk_steps / kWarps;  // a whole number of runs
@@ -580,12 +879,16 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_map_kernel(const Recur
   for (int64_t i = 0; i < runs; ++i) {
     const int64_t t0 = begin + (FORWARD ? i : runs - 1 - i) * kRun;
     const int n = static_cast<int>(min64(kRun, stop - t0));
-    Raw<T> rf[kRun], ro[kRun];
+    Raw<T> rf[kRun], ro[kRun] = {};
+    const T *pf = gate + t0 * g.gate_step, *po = other + t0 * other_step;
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-      const bool in = j < n;
-      rf[j] = load_raw<T, PAIRED>(gate + (t0 + j) * g.gate_step, in && on0, in && on1);
-      ro[j] = load_raw<T, PAIRED>(other + (t0 + j) * other_step, in && on0 && other != nullptr, in && on1 && other != nullptr);
+      rf[j] = load_raw<T, PAIRED>(pf, at.second);
+      if (other != nullptr) ro[j] = load_raw<T, PAIRED>(po, at.second);
+      if (j + 1 < n) {  // steps past the end load the last one again
+        pf += g.gate_step;
+        po += other_step;
+      }
     }
     const uint32_t cut = reset_bits(reset, t0, n);
 #pragma unroll
@@ -678,8 +981,32 @@ Plan plan_for(int64_t units, int64_t tiles) {
 int64_t units_of(int64_t batch, int64_t dim) { return batch * ceil_div(dim, kChan); }
 int64_t forward_tile(int dtype) { return kWarps * (dtype == TROPNN_B200_F32 ? kRunFwd<float> : kRunFwd<__half>); }
 
+// A [batch, steps, dim] tensor (strides in elements) in boxes of `run` steps x 64 channels. False where
+// TMA cannot take it.
+bool sequence_map(CUtensorMap *map, const void *ptr, int dtype, int64_t batch, int64_t steps, int64_t dim,
+                  int64_t batch_stride, int64_t step_stride, int run) {
+  const int64_t size = dtype == TROPNN_B200_F32 ? 4 : 2;
+  // The stride of a dimension of one element is never used, but has to be a valid one.
+  if (steps == 1) step_stride = ceil_div(dim, 16) * 16;
+  if (batch == 1) batch_stride = steps * step_stride;
+  if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0 || dim > 0x7fffffffLL || steps > 0x7fffffffLL || batch > 0x7fffffffLL) return false;
+  for (int64_t stride : {step_stride, batch_stride})
+    if (stride <= 0 || stride * size % 16 != 0 || stride * size >= (1LL << 40)) return false;
+  sm100::EncodeTiledFn fn = nullptr;
+  if (sm100::encode_fn(&fn) != TROPNN_B200_OK) return false;
+  const CUtensorMapDataType type = dtype == TROPNN_B200_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == TROPNN_B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(steps), static_cast<cuuint64_t>(batch)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(step_stride * size), static_cast<cuuint64_t>(batch_stride * size)};
+  const cuuint32_t box[3] = {kChan, static_cast<cuuint32_t>(run), 1};
+  const cuuint32_t each[3] = {1, 1, 1};
+  return fn(map, type, 3, const_cast<void *>(ptr), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <bool FORWARD, typename T, bool PAIRED>
-int launch_typed(const char *what, RecurrenceArgs g, int64_t batch, const Plan &plan, cudaStream_t stream) {
+int launch_typed(const char *what, RecurrenceArgs g, int dtype, int64_t batch, const Plan &plan, cudaStream_t stream) {
   const unsigned units = static_cast<unsigned>(batch * g.channel_blocks);
   if (plan.chunks > 1) {
     constexpr int64_t tile = FORWARD ? kWarps * kRunFwd<T> : kTileBwd;
@@ -697,6 +1024,29 @@ int launch_typed(const char *what, RecurrenceArgs g, int64_t batch, const Plan &
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
+  if constexpr (PAIRED) {
+    SequenceMaps maps{};
+    constexpr int run = FORWARD ? kRunFwd<T> : kRunBwd;
+    const int64_t steps = g.steps, dim = g.dim;
+    bool fits = steps > 0 && sequence_map(&maps.gate, g.gate, dtype, batch, steps, dim, g.gate_batch, g.gate_step, run) &&
+                sequence_map(&maps.value, g.value, dtype, batch, steps, dim, g.value_batch, g.value_step, run);
+    if (FORWARD) {
+      fits = fits && sequence_map(&maps.out_value, g.h, dtype, batch, steps, dim, steps * dim, dim, run);
+    } else {
+      fits = fits && (g.grad == nullptr || sequence_map(&maps.grad, g.grad, dtype, batch, steps, dim, steps * dim, dim, run)) &&
+             sequence_map(&maps.out_gate, g.grad_gate, dtype, batch, steps, dim, steps * dim, dim, run) &&
+             sequence_map(&maps.out_value, g.grad_value, dtype, batch, steps, dim, steps * dim, dim, run);
+    }
+    if (fits) {
+      config.dynamicSmemBytes = kRingBytes<T, FORWARD>;
+      const void *kernel = FORWARD ? reinterpret_cast<const void *>(recurrence_forward_tma_kernel<T>)
+                                   : reinterpret_cast<const void *>(recurrence_backward_tma_kernel<T>);
+      TB_CHECK(ensure_dynamic_smem(kernel, config.dynamicSmemBytes, what));
+      void *args[] = {&g, &maps};
+      cudaLaunchKernelExC(&config, kernel, args);
+      return check_launch(what);
+    }
+  }
   if (FORWARD) cudaLaunchKernelEx(&config, recurrence_forward_kernel<T, PAIRED>, static_cast<const RecurrenceArgs>(g));
   else cudaLaunchKernelEx(&config, recurrence_backward_kernel<T, PAIRED>, static_cast<const RecurrenceArgs>(g));
   return check_launch(what);
@@ -715,16 +1065,30 @@ int launch_recurrence(const char *what, RecurrenceArgs g, int dtype, int64_t bat
   g.chunk_tiles = plan.chunk_tiles;
   g.maps = static_cast<float2 *>(workspace);
   if (dtype == TROPNN_B200_F32)
-    return pair ? launch_typed<FORWARD, float, true>(what, g, batch, plan, stream)
-                : launch_typed<FORWARD, float, false>(what, g, batch, plan, stream);
+    return pair ? launch_typed<FORWARD, float, true>(what, g, dtype, batch, plan, stream)
+                : launch_typed<FORWARD, float, false>(what, g, dtype, batch, plan, stream);
   if (dtype == TROPNN_B200_F16)
-    return pair ? launch_typed<FORWARD, __half, true>(what, g, batch, plan, stream)
-                : launch_typed<FORWARD, __half, false>(what, g, batch, plan, stream);
-  return pair ? launch_typed<FORWARD, __nv_bfloat16, true>(what, g, batch, plan, stream)
-              : launch_typed<FORWARD, __nv_bfloat16, false>(what, g, batch, plan, stream);
+    return pair ? launch_typed<FORWARD, __half, true>(what, g, dtype, batch, plan, stream)
+                : launch_typed<FORWARD, __half, false>(what, g, dtype, batch, plan, stream);
+  return pair ? launch_typed<FORWARD, __nv_bfloat16, true>(what, g, dtype, batch, plan, stream)
+              : launch_typed<FORWARD, __nv_bfloat16, false>(what, g, dtype, batch, plan, stream);
 }
 
 }  // namespace
+
+// Reads and clears this file's device error word (a wait for a tile that ran out).
+int read_recurrence_error(int *value) {
+  int v = 0;
+  cudaError_t err = cudaMemcpyFromSymbol(&v, g_recurrence_error, sizeof(int));
+  if (err != cudaSuccess) return set_error(TROPNN_B200_ERR_LAUNCH, "device_error: %s", cudaGetErrorString(err));
+  if (v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_recurrence_error, &zero, sizeof(int));
+  }
+  *value = v;
+  return TROPNN_B200_OK;
+}
+
 }  // namespace tropnn_b200
 
 using namespace tropnn_b200;
