@@ -170,17 +170,21 @@ __device__ __forceinline__ float rcp_approx(float x) {
 
 // a and c = 1 - a. The smaller one, m = e / (1 + e) with e = exp(-|f|), has its full relative
 // accuracy; the larger is 1 - m, the f32 next to it.
+__device__ __forceinline__ void gates1(float f, float &a, float &c) {
+  const float e = exp2_approx(fabsf(f) * -1.4426950408889634f);
+  const float m = e * rcp_approx(1.f + e), o = 1.f - m;
+  a = f < 0.f ? m : o;
+  c = f < 0.f ? o : m;
+}
 __device__ __forceinline__ void gates2(float2 f, float2 &a, float2 &c) {
-  const float2 e = make_float2(exp2_approx(fabsf(f.x) * -1.4426950408889634f), exp2_approx(fabsf(f.y) * -1.4426950408889634f));
-  const float2 d = add2(e, make_float2(1.f, 1.f));
-  const float2 m = mul2(e, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
-  const float2 o = fma2(m, make_float2(-1.f, -1.f), make_float2(1.f, 1.f));
-  a = make_float2(f.x < 0.f ? m.x : o.x, f.y < 0.f ? m.y : o.y);
-  c = make_float2(f.x < 0.f ? o.x : m.x, f.y < 0.f ? o.y : m.y);
+  gates1(f.x, a.x, c.x);
+  gates1(f.y, a.y, c.y);
 }
 
-// P h + H; a run that a reset cut (P = 0) takes nothing of h, not even an infinity's NaN.
-__device__ __forceinline__ float2 apply_run(float2 p, float2 h, float2 add) {
+// P h + H. With resets about (`cuts`), a run that one cut (P = 0) takes nothing of h, not even an
+// infinity's NaN.
+__device__ __forceinline__ float2 apply_run(float2 p, float2 h, float2 add, bool cuts) {
+  if (!cuts) return fma2(p, h, add);
   return make_float2(p.x == 0.f ? add.x : fmaf(p.x, h.x, add.x), p.y == 0.f ? add.y : fmaf(p.y, h.y, add.y));
 }
 
@@ -233,14 +237,14 @@ __device__ __forceinline__ float2 through_chunks(const RecurrenceArgs &g, int64_
     if (on0) a = __ldg(m);
     if (on1) b = __ldg(m + kSecond<PAIRED>);
     const float2 mp = make_float2(a.x, b.x);
-    h = apply_run(mp, h, make_float2(a.y, b.y));
+    h = apply_run(mp, h, make_float2(a.y, b.y), true);
     p = mul2(mp, p);
   }
   ex.p[0][warp][lane] = p;
   ex.h[0][warp][lane] = h;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) state = apply_run(ex.p[0][w][lane], state, ex.h[0][w][lane]);
+  for (int w = 0; w < kWarps; ++w) state = apply_run(ex.p[0][w][lane], state, ex.h[0][w][lane], true);
   __syncthreads();
   return state;
 }
@@ -248,7 +252,8 @@ __device__ __forceinline__ float2 through_chunks(const RecurrenceArgs &g, int64_
 // Hands this warp's (p, h) around: returns the state before its run, and moves `state` past the
 // cluster's tiles. ORDER 1: the runs follow one another by warp, -1: from the last warp back.
 template <int ORDER>
-__device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, float2 h, float2 &state, int ranks, int rank) {
+__device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, float2 h, float2 &state, int ranks, int rank,
+                                           bool cuts) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ex.p[buf][warp][lane] = p;
   ex.h[buf][warp][lane] = h;
@@ -259,7 +264,7 @@ __device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, floa
     for (int i = 0; i < kWarps; ++i) {
       const int w = ORDER > 0 ? i : kWarps - 1 - i;
       if (w == warp) in = state;
-      state = apply_run(ex.p[buf][w][lane], state, ex.h[buf][w][lane]);
+      state = apply_run(ex.p[buf][w][lane], state, ex.h[buf][w][lane], cuts);
     }
     return in;
   }
@@ -269,7 +274,7 @@ __device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, floa
     for (int i = 0; i < kWarps; ++i) {
       const int w = ORDER > 0 ? i : kWarps - 1 - i;
       const float2 pw = ex.p[buf][w][lane];
-      ch = apply_run(pw, ch, ex.h[buf][w][lane]);
+      ch = apply_run(pw, ch, ex.h[buf][w][lane], cuts);
       cp = mul2(cp, pw);
     }
     *cooperative_groups::this_cluster().map_shared_rank(&ex.rank[buf][rank][lane], warp) = make_float4(cp.x, cp.y, ch.x, ch.y);
@@ -279,12 +284,12 @@ __device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, floa
   for (int r = 0; r < ranks; ++r) {
     if (r == rank) in = state;
     const float4 m = ex.rank[buf][r][lane];
-    state = apply_run(make_float2(m.x, m.y), state, make_float2(m.z, m.w));
+    state = apply_run(make_float2(m.x, m.y), state, make_float2(m.z, m.w), cuts);
   }
 #pragma unroll
   for (int i = 0; i < kWarps - 1; ++i) {
     const int w = ORDER > 0 ? i : kWarps - 1 - i;
-    if (ORDER > 0 ? w < warp : w > warp) in = apply_run(ex.p[buf][w][lane], in, ex.h[buf][w][lane]);
+    if (ORDER > 0 ? w < warp : w > warp) in = apply_run(ex.p[buf][w][lane], in, ex.h[buf][w][lane], cuts);
   }
   return in;
 }
@@ -483,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
     }
     scan_run<kRun>(a, b, n, cut, plain, p, h);
     load(t0 + int64_t(g.ranks) * kTile);
-    const float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank);
+    const float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank, reset != nullptr);
     if (g.saved != nullptr && (warp * kRun) % kTileBwd == 0 && n > 0) {
       float *s = g.saved + (batch * g.saved_tiles + t0 / kTileBwd) * g.dim + ch;
       if (on0) s[0] = in.x;
@@ -585,10 +590,10 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const 
     scan_run_back<kRun>(a, c, x, gt, n, cut, plain, p, h, r);
     load(k - g.ranks);
     run_h[buf][warp][lane] = h;
-    const float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank);
+    const float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank, reset != nullptr);
 #pragma unroll
     for (int w = 0; w < kWarps - 1; ++w) {
-      if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane]);
+      if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane], reset != nullptr);
     }
     T *pf = grad_gate + t0 * g.dim, *px = grad_value + t0 * g.dim;
     emit_run_back<kRun>(a, c, x, gt, n, cut, plain, h_in, r_in, [&](int j, float2 gf, float2 gx) {
@@ -716,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       b[j] = mul2(c, unpack<T>(stage_raw<T>(rows + (kRun + j) * kChan, lane)));
     }
     scan_run<kRun>(a, b, n, cut, plain, p, h);
-    const float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank);
+    const float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank, reset != nullptr);
     if (g.saved != nullptr && (warp * kRun) % kTileBwd == 0 && n > 0 && on)
       put_two_floats(g.saved + (batch * g.saved_tiles + t0 / kTileBwd) * g.dim + ch, in);
     emit_run<kRun>(a, b, n, cut, plain, in,
@@ -821,10 +826,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     scan_run_back<kRun>(a, c, x, gt, n, cut, plain, p, h, r);
     run_h[buf][warp][lane] = h;
-    const float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank);
+    const float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank, reset != nullptr);
 #pragma unroll
     for (int w = 0; w < kWarps - 1; ++w) {
-      if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane]);
+      if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane], reset != nullptr);
     }
     emit_run_back<kRun>(a, c, x, gt, n, cut, plain, h_in, r_in, [&](int j, float2 gf, float2 gx) {
       store_pair<T, true>(rows + j * kChan + 2 * lane, gf, true, true);
@@ -920,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_map_kernel(const Recur
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       const int w = FORWARD ? i : kWarps - 1 - i;
-      h = apply_run(run_p[w][lane], h, run_h[w][lane]);
+      h = apply_run(run_p[w][lane], h, run_h[w][lane], true);
       p = mul2(p, run_p[w][lane]);
     }
     float2 *m = g.maps + (batch * g.chunks + chunk) * g.dim + ch;
