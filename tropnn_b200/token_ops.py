@@ -15,7 +15,6 @@ synchronisation, deterministic results.
 from __future__ import annotations
 
 import math
-from contextlib import AbstractContextManager, nullcontext
 from typing import Any
 
 import torch
@@ -37,22 +36,23 @@ MAX_TEACHER_TOP = 1024
 _REDUCTIONS = ("mean", "sum", "none")
 
 
-def _on(device: torch.device) -> AbstractContextManager[Any]:
-    """The device's context, without the cost of entering it where it is current."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _call(device: torch.device, name: str, fn: Any, *args: Any) -> None:
+    """Launches on the device's current stream, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        _launch(name, fn, *args, nat.stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            _launch(name, fn, *args, nat.stream_handle(device))
 
 
-def _same_device(device: torch.device, **tensors: Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is None:
-            continue
+def _same_device(device: torch.device, t: Tensor, name: str) -> None:
+    if t.device != device:
         _require_cuda(t, name)
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def _unit_last(t: Tensor) -> Tensor:
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 # ---------------------------------------------------------------------------
@@ -60,66 +60,69 @@ def _unit_last(t: Tensor) -> Tensor:
 # ---------------------------------------------------------------------------
 
 
-def _recurrence_workspace(lib: Any, gate: Tensor) -> tuple[Tensor | None, int]:
-    size = lib.tropnn_b200_recurrence_workspace_size(*gate.shape, nat.float_code(gate.dtype))
+def _recurrence_workspace(lib: Any, gate: Tensor, shape: tuple[int, int, int]) -> tuple[Tensor | None, int]:
+    size = lib.tropnn_b200_recurrence_workspace_size(*shape, nat.float_code(gate.dtype))
     return (torch.empty(size, device=gate.device, dtype=torch.uint8), size) if size else (None, 0)
+
+
+def _recurrence_forward(
+    gate: Tensor, value: Tensor, h0: Tensor | None, reset: Tensor | None, keep: bool
+) -> tuple[Tensor, Tensor, Tensor | None]:
+    """``(h, h_last, saved)``; ``saved`` are the states that the backward starts from."""
+    batch, steps, dim = shape = tuple(gate.shape)
+    dev = gate.device
+    lib = nat.load()
+    h = gate.new_empty(shape)
+    h_last = torch.empty((batch, dim), device=dev, dtype=torch.float32)
+    saved, saved_bytes = None, 0
+    if keep:
+        saved_bytes = lib.tropnn_b200_recurrence_saved_size(batch, steps, dim)
+        saved = h_last.new_empty(saved_bytes // 4)
+    ws, ws_bytes = _recurrence_workspace(lib, gate, shape)
+    _call(
+        dev, "recurrence_forward", lib.tropnn_b200_recurrence_forward, gate.data_ptr(), gate.stride(0), gate.stride(1),
+        value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype), nat.ptr(h0), nat.ptr(reset),
+        batch, steps, dim, h.data_ptr(), h_last.data_ptr(), nat.ptr(saved), saved_bytes, nat.ptr(ws), ws_bytes,
+    )
+    return h, h_last, saved
 
 
 class _GatedRecurrenceFunction(torch.autograd.Function):
     @staticmethod
     def forward(  # type: ignore[override]
-        ctx: Any, gate: Tensor, value: Tensor, h0: Tensor | None, reset: Tensor | None, keep: bool
+        ctx: Any, gate: Tensor, value: Tensor, h0: Tensor | None, reset: Tensor | None
     ) -> tuple[Tensor, Tensor]:
-        batch, steps, dim = gate.shape
-        dev = gate.device
-        lib = nat.load()
-        h = torch.empty((batch, steps, dim), device=dev, dtype=gate.dtype)
-        h_last = torch.empty((batch, dim), device=dev, dtype=torch.float32)
-        saved_bytes = lib.tropnn_b200_recurrence_saved_size(batch, steps, dim) if keep else 0
-        saved = torch.empty(saved_bytes // 4, device=dev, dtype=torch.float32) if keep else None
-        ws, ws_bytes = _recurrence_workspace(lib, gate)
-        with _on(dev):
-            _launch(
-                "recurrence_forward", lib.tropnn_b200_recurrence_forward, gate.data_ptr(), gate.stride(0),
-                gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype),
-                nat.ptr(h0), nat.ptr(reset), batch, steps, dim, h.data_ptr(), h_last.data_ptr(), nat.ptr(saved),
-                saved_bytes, nat.ptr(ws), ws_bytes, nat.stream_handle(dev),
-            )
-        if keep:
-            ctx.save_for_backward(gate, value, reset, saved)
-            ctx.saved_bytes = saved_bytes
-            ctx.set_materialize_grads(False)
+        h, h_last, saved = _recurrence_forward(gate, value, h0, reset, True)
+        ctx.save_for_backward(gate, value, reset, saved)
+        ctx.set_materialize_grads(False)
         return h, h_last
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad_h: Tensor | None, grad_last: Tensor | None) -> tuple[Any, ...]:
-        gate, value, reset, saved = ctx.saved_tensors
         if grad_h is None and grad_last is None:
-            return None, None, None, None, None
-        batch, steps, dim = gate.shape
-        dev = gate.device
+            return None, None, None, None
+        gate, value, reset, saved = ctx.saved_tensors
+        batch, steps, dim = shape = tuple(gate.shape)
         lib = nat.load()
         grad_h = None if grad_h is None else grad_h.contiguous()
         grad_last = None if grad_last is None else grad_last.contiguous()
-        grad_gate = torch.empty((batch, steps, dim), device=dev, dtype=gate.dtype)
-        grad_value = torch.empty((batch, steps, dim), device=dev, dtype=gate.dtype)
-        grad_h0 = torch.empty((batch, dim), device=dev, dtype=torch.float32) if ctx.needs_input_grad[2] else None
-        ws, ws_bytes = _recurrence_workspace(lib, gate)
-        with _on(dev):
-            _launch(
-                "recurrence_backward", lib.tropnn_b200_recurrence_backward, gate.data_ptr(), gate.stride(0),
-                gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype),
-                nat.ptr(reset), batch, steps, dim, saved.data_ptr(), ctx.saved_bytes, nat.ptr(grad_h),
-                nat.ptr(grad_last), grad_gate.data_ptr(), grad_value.data_ptr(), nat.ptr(grad_h0),
-                nat.ptr(ws), ws_bytes, nat.stream_handle(dev),
-            )
-        return grad_gate, grad_value, grad_h0, None, None
+        grad_gate = gate.new_empty(shape)
+        grad_value = torch.empty_like(grad_gate)
+        grad_h0 = saved.new_empty((batch, dim)) if ctx.needs_input_grad[2] else None
+        ws, ws_bytes = _recurrence_workspace(lib, gate, shape)
+        _call(
+            gate.device, "recurrence_backward", lib.tropnn_b200_recurrence_backward, gate.data_ptr(), gate.stride(0),
+            gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype),
+            nat.ptr(reset), batch, steps, dim, saved.data_ptr(), saved.numel() * 4, nat.ptr(grad_h), nat.ptr(grad_last),
+            grad_gate.data_ptr(), grad_value.data_ptr(), nat.ptr(grad_h0), nat.ptr(ws), ws_bytes,
+        )
+        return grad_gate, grad_value, grad_h0, None
 
 
 def _check_gate_value(gate: Tensor, value: Tensor, ndim: int) -> None:
     _require_cuda(gate, "gate")
-    _same_device(gate.device, value=value)
+    _same_device(gate.device, value, "value")
     if gate.ndim != ndim or value.shape != gate.shape:
         want = "[batch, steps, dim]" if ndim == 3 else "[batch, dim]"
         raise ValueError(f"gate and value must both have shape {want}, got {tuple(gate.shape)} and {tuple(value.shape)}")
@@ -128,10 +131,8 @@ def _check_gate_value(gate: Tensor, value: Tensor, ndim: int) -> None:
         raise TypeError(f"gate and value must have one dtype, got {gate.dtype} and {value.dtype}")
 
 
-def _check_reset(reset: Tensor | None, shape: tuple[int, ...], device: torch.device) -> Tensor | None:
-    if reset is None:
-        return None
-    _same_device(device, reset=reset)
+def _check_reset(reset: Tensor, shape: tuple[int, ...], device: torch.device) -> Tensor:
+    _same_device(device, reset, "reset")
     if reset.dtype not in (torch.bool, torch.uint8):
         raise TypeError(f"reset must be bool or uint8, got {reset.dtype}")
     if reset.shape != shape:
@@ -156,19 +157,20 @@ def gated_recurrence_b200(
     saved ones instead of reading ``h``.
     """
     _check_gate_value(gate, value, 3)
-    batch, steps, dim = gate.shape
     if h0 is not None:
-        _same_device(gate.device, h0=h0)
-        if h0.shape != (batch, dim):
-            raise ValueError(f"h0 must have shape {(batch, dim)}, got {tuple(h0.shape)}")
+        _same_device(gate.device, h0, "h0")
+        if h0.shape != (gate.shape[0], gate.shape[2]):
+            raise ValueError(f"h0 must have shape {(gate.shape[0], gate.shape[2])}, got {tuple(h0.shape)}")
         nat.float_code(h0.dtype)
         h0 = h0.to(torch.float32).contiguous()
-    reset = _check_reset(reset, (batch, steps), gate.device)
+    if reset is not None:
+        reset = _check_reset(reset, tuple(gate.shape[:2]), gate.device)
     gate, value = _unit_last(gate), _unit_last(value)
-    keep = torch.is_grad_enabled() and (
+    if torch.is_grad_enabled() and (
         gate.requires_grad or value.requires_grad or (h0 is not None and h0.requires_grad)
-    )
-    return _GatedRecurrenceFunction.apply(gate, value, h0, reset, keep)
+    ):
+        return _GatedRecurrenceFunction.apply(gate, value, h0, reset)
+    return _recurrence_forward(gate, value, h0, reset, False)[:2]
 
 
 def gated_recurrence_step_b200(gate: Tensor, value: Tensor, state: Tensor, *, reset: Tensor | None = None) -> Tensor:
@@ -176,25 +178,28 @@ def gated_recurrence_step_b200(gate: Tensor, value: Tensor, state: Tensor, *, re
     ``state`` f32 ``[batch, dim]``, updated in place; ``reset`` ``[batch]`` clears a row's state
     first. Returns the new state rounded to the inputs' dtype. Not differentiable."""
     _check_gate_value(gate, value, 2)
-    _same_device(gate.device, state=state)
-    if state.shape != gate.shape:
-        raise ValueError(f"state must have shape {tuple(gate.shape)}, got {tuple(state.shape)}")
+    shape = gate.shape
+    dev = gate.device
+    _same_device(dev, state, "state")
+    if state.shape != shape:
+        raise ValueError(f"state must have shape {tuple(shape)}, got {tuple(state.shape)}")
     if state.dtype != torch.float32:
         raise TypeError(f"state must be float32, got {state.dtype}")
-    batch, dim = gate.shape
-    if (dim > 1 and state.stride(1) != 1) or (batch > 1 and state.stride(0) < dim):
+    batch, dim = shape
+    state_row, unit = state.stride()
+    if (dim > 1 and unit != 1) or (batch > 1 and state_row < dim):
         raise ValueError("state must have unit stride over dim and rows of its own")
     if torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or state.requires_grad):
         raise ValueError("gated_recurrence_step_b200 is not differentiable: call it under torch.no_grad()")
-    reset = _check_reset(reset, (batch,), gate.device)
+    if reset is not None:
+        reset = _check_reset(reset, (batch,), dev)
     gate, value = _unit_last(gate), _unit_last(value)
-    h = torch.empty((batch, dim), device=gate.device, dtype=gate.dtype)
-    with _on(gate.device):
-        _launch(
-            "recurrence_step", nat.load().tropnn_b200_recurrence_step, gate.data_ptr(), gate.stride(0),
-            value.data_ptr(), value.stride(0), nat.float_code(gate.dtype), nat.ptr(reset), batch, dim,
-            state.data_ptr(), state.stride(0), h.data_ptr(), nat.stream_handle(gate.device),
-        )
+    h = gate.new_empty(shape)
+    _call(
+        dev, "recurrence_step", nat.load().tropnn_b200_recurrence_step, gate.data_ptr(), gate.stride(0),
+        value.data_ptr(), value.stride(0), nat.float_code(gate.dtype), None if reset is None else reset.data_ptr(),
+        batch, dim, state.data_ptr(), state_row, h.data_ptr(),
+    )
     return h
 
 
@@ -232,7 +237,9 @@ class _Distill:
         label_weight: float, ignore_index: int,
     ) -> None:
         _require_cuda(logits, "logits")
-        _same_device(logits.device, teacher_logits=teacher, teacher_indices=indices, labels=labels)
+        dev = logits.device
+        _same_device(dev, teacher, "teacher_logits")
+        _same_device(dev, indices, "teacher_indices")
         nat.float_code(logits.dtype)
         nat.float_code(teacher.dtype)
         if logits.ndim < 1 or logits.shape[-1] < 1:
@@ -248,6 +255,7 @@ class _Distill:
         if indices.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"teacher_indices must be int64 or int32, got {indices.dtype}")
         if labels is not None:
+            _same_device(dev, labels, "labels")
             if labels.shape != lead:
                 raise ValueError(f"labels must have shape {tuple(lead)}, got {tuple(labels.shape)}")
             if labels.dtype not in (torch.int64, torch.int32):
@@ -271,9 +279,6 @@ class _Distill:
             int(ignore_index), temperature, label_weight,
         )
 
-    def grad_like(self) -> Tensor:
-        return torch.empty(self.logits.shape, device=self.logits.device, dtype=self.logits.dtype)
-
 
 class _DistillLossFunction(torch.autograd.Function):
     @staticmethod
@@ -281,16 +286,13 @@ class _DistillLossFunction(torch.autograd.Function):
         dev = logits.device
         lib = nat.load()
         losses = torch.empty(call.lead, device=dev, dtype=torch.float32)
-        stats = torch.empty((call.rows, 4), device=dev, dtype=torch.float32)
-        with _on(dev):
-            stream = nat.stream_handle(dev)
-            _launch("distill_loss", lib.tropnn_b200_distill_loss, *call.args, losses.data_ptr(), stats.data_ptr(), stream)
-            loss, count = losses, None
-            if reduction != "none":
-                loss = torch.empty((), device=dev, dtype=torch.float32)
-                count = torch.empty((), device=dev, dtype=torch.float32)
-                _launch("distill_reduce", lib.tropnn_b200_distill_reduce, losses.data_ptr(), stats.data_ptr(),
-                        call.rows, int(reduction == "mean"), loss.data_ptr(), count.data_ptr(), stream)
+        stats = losses.new_empty((call.rows, 4))
+        _call(dev, "distill_loss", lib.tropnn_b200_distill_loss, *call.args, losses.data_ptr(), stats.data_ptr())
+        loss, count = losses, None
+        if reduction != "none":
+            loss, count = losses.new_empty(()), losses.new_empty(())
+            _call(dev, "distill_reduce", lib.tropnn_b200_distill_reduce, losses.data_ptr(), stats.data_ptr(), call.rows,
+                  int(reduction == "mean"), loss.data_ptr(), count.data_ptr())
         # The call holds its tensors' addresses; saving them finds out a change in place.
         ctx.save_for_backward(logits, stats, count, call.teacher, call.indices, call.labels)
         ctx.call = call
@@ -301,12 +303,10 @@ class _DistillLossFunction(torch.autograd.Function):
     def backward(ctx: Any, grad_loss: Tensor) -> tuple[Any, ...]:
         logits, stats, count, *_ = ctx.saved_tensors
         call = ctx.call
-        dev = logits.device
-        grad = call.grad_like()
-        scale = grad_loss.to(torch.float32).contiguous()
-        with _on(dev):
-            _launch("distill_grad", nat.load().tropnn_b200_distill_grad, *call.args, stats.data_ptr(), scale.data_ptr(),
-                    int(count is None), nat.ptr(count), grad.data_ptr(), nat.stream_handle(dev))
+        grad = logits.new_empty(logits.shape)
+        scale = grad_loss.contiguous()
+        _call(logits.device, "distill_grad", nat.load().tropnn_b200_distill_grad, *call.args, stats.data_ptr(),
+              scale.data_ptr(), int(count is None), nat.ptr(count), grad.data_ptr())
         return grad, None, None
 
 
@@ -363,7 +363,7 @@ def distill_loss_grad_b200(
     dev = logits.device
     scale: Tensor | None = None
     if isinstance(row_scale, Tensor):
-        _same_device(dev, row_scale=row_scale)
+        _same_device(dev, row_scale, "row_scale")
         if row_scale.dtype != torch.float32:
             raise TypeError(f"row_scale must be float32, got {row_scale.dtype}")
         if row_scale.numel() != 1 and row_scale.shape != call.lead:
@@ -373,10 +373,9 @@ def distill_loss_grad_b200(
         scale = torch.full((1,), float(row_scale), device=dev, dtype=torch.float32)
     per_row = scale is not None and scale.shape == call.lead
     losses = torch.empty(call.lead, device=dev, dtype=torch.float32)
-    grad = call.grad_like()
-    with _on(dev):
-        _launch("distill_loss_grad", nat.load().tropnn_b200_distill_loss_grad, *call.args, nat.ptr(scale), int(per_row),
-                losses.data_ptr(), grad.data_ptr(), nat.stream_handle(dev))
+    grad = logits.new_empty(logits.shape)
+    _call(dev, "distill_loss_grad", nat.load().tropnn_b200_distill_loss_grad, *call.args, nat.ptr(scale), int(per_row),
+          losses.data_ptr(), grad.data_ptr())
     return losses, grad
 
 
@@ -390,7 +389,7 @@ def _setting(
 ) -> tuple[Tensor | None, float]:
     """A sampling setting as (one a row, or None; the value where it is one for all)."""
     if isinstance(value, Tensor):
-        _same_device(device, **{name: value})
+        _same_device(device, value, name)
         if value.dtype != torch.float32:
             raise TypeError(f"{name} must be a number or float32, got {value.dtype}")
         if value.shape != lead:
@@ -430,7 +429,7 @@ def sample_tokens_b200(
     if logits.ndim < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must have shape [..., vocab] with vocab >= 1, got {tuple(logits.shape)}")
     lead, dev, vocab = logits.shape[:-1], logits.device, logits.shape[-1]
-    _same_device(dev, uniforms=uniforms)
+    _same_device(dev, uniforms, "uniforms")
     if uniforms.dtype != torch.float32:
         raise TypeError(f"uniforms must be float32, got {uniforms.dtype}")
     if uniforms.shape != lead:
@@ -440,7 +439,7 @@ def sample_tokens_b200(
     floor, floor_value = _setting(min_p, "min_p", lead, dev, 0.0, 1.0)
     k, k_value, k_code = None, 0, nat.I64
     if isinstance(top_k, Tensor):
-        _same_device(dev, top_k=top_k)
+        _same_device(dev, top_k, "top_k")
         if top_k.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"top_k must be a number or int32/int64, got {top_k.dtype}")
         if top_k.shape != lead:
@@ -454,10 +453,9 @@ def sample_tokens_b200(
     logits, rows, inner, outer_stride, inner_stride = _logit_rows(logits.detach())
     uniforms = uniforms.contiguous()
     tokens = torch.empty(lead, device=dev, dtype=torch.int64)
-    with _on(dev):
-        _launch(
-            "sample_tokens", nat.load().tropnn_b200_sample_tokens, logits.data_ptr(), nat.float_code(logits.dtype),
-            rows, inner, outer_stride, inner_stride, vocab, uniforms.data_ptr(), nat.ptr(t), t_value, nat.ptr(k), k_code,
-            k_value, nat.ptr(p), p_value, nat.ptr(floor), floor_value, tokens.data_ptr(), nat.stream_handle(dev),
-        )
+    _call(
+        dev, "sample_tokens", nat.load().tropnn_b200_sample_tokens, logits.data_ptr(), nat.float_code(logits.dtype),
+        rows, inner, outer_stride, inner_stride, vocab, uniforms.data_ptr(), nat.ptr(t), t_value, nat.ptr(k), k_code,
+        k_value, nat.ptr(p), p_value, nat.ptr(floor), floor_value, tokens.data_ptr(),
+    )
     return tokens
