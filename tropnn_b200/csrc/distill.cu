@@ -9,21 +9,40 @@
 // A row without teacher entries (or without a label) drops that part; a row with neither has loss
 // 0 and gradient 0 whatever its logits are.
 //
-// One pass over the row keeps a running maximum and the sums of exp((s - max) / T) and of
-// exp(s - max); a second writes the gradient. Everything is f32, rounded once on the way out.
+// The sums need the row's maximum and the gradient needs the sums, so a row is passed over twice, in
+// f32 throughout and rounded once on the way out. In one call (distill_loss_grad) a cluster of up to
+// 8 CTAs keeps the row in shared memory between the passes: bulk copies bring each CTA's slice, whose
+// running maximum and sums are formed as the chunks arrive, one exchange through distributed shared
+// memory joins them, and the gradient is written from shared memory: HBM sees one read and one write.
+// Through autograd the loss kernel reads the row and the gradient kernel reads it again with the
+// statistics known, each streaming through registers.
+// exp2 runs on the special-function unit (16 a clock and SM), two of them an element and pass where
+// T and the labels need two sums: with T = 2 the second is the square of the first.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+#include "packed.cuh"
 #include "sm100.cuh"
 
 namespace tropnn_b200 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;
 constexpr int kPerThread = kMaxTop / kThreads;
+constexpr int kMaxCluster = 8;
+constexpr int kChunks = 4;  // bulk copies of a slice
+constexpr int64_t kSliceShared = 64 * 1024 + 64;  // bytes of a row a CTA: three CTAs on an SM
+constexpr int64_t kSliceMost = 200 * 1024;        // one CTA on an SM
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.402823466e38f;
 
 enum Mode { kLoss = 0, kGrad = 1, kFused = 2 };
+// Sums an element goes into: one, two with an exponential each, two with the second the first's square.
+enum Exps { kOne = 0, kTwo = 1, kSquare = 2 };
+
+__device__ int g_distill_error = 0;
 
 struct DistillArgs {
   const void *logits;
@@ -46,13 +65,9 @@ struct DistillArgs {
   int scale_per_row;
   const float *count;
   void *grad;
+  int ranks;       // CTAs of a row
+  int slice_vecs;  // 16-byte vectors of a CTA's slice
 };
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 
 __device__ __forceinline__ float load_float(const void *p, int dtype, int64_t i) {
   if (dtype == TROPNN_B200_F32) return static_cast<const float *>(p)[i];
@@ -71,7 +86,7 @@ __device__ __forceinline__ float block_max(float v, float *shared) {
   __syncthreads();
   v = shared[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) v = fmaxf(v, shared[i]);
+  for (int i = 1; i < kWarps; ++i) v = fmaxf(v, shared[i]);
   return v;
 }
 __device__ __forceinline__ float block_sum(float v, float *shared) {
@@ -81,209 +96,450 @@ __device__ __forceinline__ float block_sum(float v, float *shared) {
   __syncthreads();
   v = shared[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) v += shared[i];
+  for (int i = 1; i < kWarps; ++i) v += shared[i];
   return v;
 }
 
-// Running maximum and sums of one thread.
-struct Online {
-  float m = kLowest, s_t = 0.f, s_1 = 0.f;
+// 16 bytes of a row as f32 pairs.
+template <typename T>
+struct Vec {
+  static constexpr int kN = 16 / sizeof(T);
+  __device__ __forceinline__ static void unpack(const uint4 &q, float2 (&v)[kN / 2]) {
+    if constexpr (std::is_same<T, float>::value) {
+      v[0] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+      v[1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
+    } else {
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) v[i] = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        else v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+      }
+    }
+  }
+  __device__ __forceinline__ static uint4 pack(const float2 (&v)[kN / 2]) {
+    if constexpr (std::is_same<T, float>::value) {
+      return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const __half2 h = __float22half2_rn(v[i]);
+          w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+          const __nv_bfloat162 h = __float22bfloat162_rn(v[i]);
+          w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __device__ __forceinline__ static float max(const uint4 &q) {
+    if constexpr (std::is_same<T, float>::value) {
+      return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 *h = reinterpret_cast<const __half2 *>(&q);
+      const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    } else {
+      const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&q);
+      const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    }
+  }
 };
-template <bool BOTH>
-__device__ __forceinline__ void raise_max(Online &o, float m, float k_t) {
-  o.s_t *= exp2_approx((o.m - m) * k_t);
-  if (BOTH) o.s_1 *= exp2_approx((o.m - m) * kLog2e);
-  o.m = m;
+template <typename T>
+__device__ __forceinline__ T lowest_logit();
+template <>
+__device__ __forceinline__ float lowest_logit<float>() { return -INFINITY; }
+template <>
+__device__ __forceinline__ __half lowest_logit<__half>() { return __ushort_as_half(0xFC00); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 lowest_logit<__nv_bfloat16>() { return __ushort_as_bfloat16(0xFF80); }
+
+// Vector v of the row's 16-byte grid, which starts at or before the row; elements outside the row are
+// -inf (which adds nothing to a sum) and never read.
+template <typename T>
+__device__ __forceinline__ uint4 load_vec(const T *grid, int64_t v, int64_t lead, int64_t end) {
+  constexpr int kN = Vec<T>::kN;
+  const int64_t p = v * kN;
+  if (p >= lead && p + kN <= end) return __ldg(reinterpret_cast<const uint4 *>(grid + p));
+  alignas(16) T e[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) e[i] = p + i >= lead && p + i < end ? grid[p + i] : lowest_logit<T>();
+  return *reinterpret_cast<const uint4 *>(e);
 }
-template <bool BOTH, int N>
-__device__ __forceinline__ void take(Online &o, const float (&v)[N], float k_t) {
-  float m = v[0];
+
+// Running maximum and sums.
+struct Online {
+  float m = kLowest;
+  float2 s_t = {0.f, 0.f}, s_1 = {0.f, 0.f};
+};
+template <int EXPS>
+__device__ __forceinline__ float second_exp(float e, float d) {
+  return EXPS == kSquare ? e * e : exp2_approx(d * kLog2e);
+}
+template <typename T, int EXPS, int COUNT>
+__device__ __forceinline__ void take(Online &o, const uint4 (&q)[COUNT], float k_t) {
+  float m = Vec<T>::max(q[0]);
 #pragma unroll
-  for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-  if (m > o.m) raise_max<BOTH>(o, m, k_t);
+  for (int i = 1; i < COUNT; ++i) m = fmaxf(m, Vec<T>::max(q[i]));
+  if (m > o.m) {
+    const float d = o.m - m, e = exp2_approx(d * k_t);
+    o.s_t = mul2(o.s_t, both(e));
+    if (EXPS != kOne) o.s_1 = mul2(o.s_1, both(second_exp<EXPS>(e, d)));
+    o.m = m;
+  }
+  const float2 minus = both(-o.m), k = both(k_t), k1 = both(kLog2e);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = v[i] - o.m;
-    o.s_t += exp2_approx(d * k_t);
-    if (BOTH) o.s_1 += exp2_approx(d * kLog2e);
+  for (int i = 0; i < COUNT; ++i) {
+    float2 v[Vec<T>::kN / 2];
+    Vec<T>::unpack(q[i], v);
+#pragma unroll
+    for (int j = 0; j < Vec<T>::kN / 2; ++j) {
+      const float2 d = add2(v[j], minus), t = mul2(d, k);
+      const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+      o.s_t = add2(o.s_t, e);
+      if (EXPS == kSquare) o.s_1 = fma2(e, e, o.s_1);
+      if (EXPS == kTwo) {
+        const float2 u = mul2(d, k1);
+        o.s_1 = add2(o.s_1, make_float2(exp2_approx(u.x), exp2_approx(u.y)));
+      }
+    }
   }
 }
 
-// Elements before the first 16-byte boundary of a row of `n`.
-template <typename T>
-__device__ __forceinline__ int64_t head_of(const T *row, int64_t n) {
-  const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(row) & 15u);
-  return min64(n, off == 0 ? 0 : (16 - off) / int64_t(sizeof(T)));
+struct RowStats {
+  float m, s_t, s_1;
+};
+template <int EXPS>
+__device__ __forceinline__ RowStats join(RowStats a, RowStats b, float k_t) {
+  const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m;
+  const float ea = exp2_approx(da * k_t), eb = exp2_approx(db * k_t);
+  RowStats r;
+  r.m = m;
+  r.s_t = a.s_t * ea + b.s_t * eb;
+  r.s_1 = EXPS == kOne ? r.s_t : a.s_1 * second_exp<EXPS>(ea, da) + b.s_1 * second_exp<EXPS>(eb, db);
+  return r;
+}
+__device__ __forceinline__ RowStats shuffled(RowStats a, int o) {
+  return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s_t, o), __shfl_xor_sync(0xffffffffu, a.s_1, o)};
 }
 
-template <typename T, int MODE, bool BOTH>
-__global__ void __launch_bounds__(kThreads, 2) distill_rows_kernel(const DistillArgs g) {
-  constexpr int kVec = 16 / sizeof(T);
-  __shared__ float red[kThreads / 32];
-  __shared__ float q_of[kMaxTop];
-  __shared__ int at_of[kMaxTop];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const T *x = static_cast<const T *>(g.logits) + (row / g.inner) * g.outer_stride + (row % g.inner) * g.inner_stride;
-
-  // The row's targets; their logits come in while the row is read.
-  int at[kPerThread];
-  float t[kPerThread], s[kPerThread];
+// A row's targets: the teacher's entries spread over the block's threads, and the label.
+struct Targets {
+  int at[kPerThread];    // -1: none
+  float t[kPerThread];   // teacher logit / T
+  int64_t label;         // -1: none
+  bool has_teacher, has_label;
+  float q_max, q_total;  // of exp(t - q_max) over the entries
+};
+__device__ __forceinline__ Targets load_targets(const DistillArgs &g, int64_t row, float *red) {
+  Targets r;
   float t_max = kLowest;
   bool found = false;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int k = tid + i * kThreads;
-    at[i] = -1;
-    t[i] = s[i] = 0.f;
+    const int k = threadIdx.x + i * kThreads;
+    r.at[i] = -1;
+    r.t[i] = 0.f;
     if (k < g.top && g.kl_weight != 0.f) {
       const int64_t v = load_index(g.indices, g.index_dtype, row * g.top + k);
       const float tv = load_float(g.teacher, g.teacher_dtype, row * g.top + k);
       if (v >= 0 && v < g.vocab && tv != -INFINITY) {
-        at[i] = static_cast<int>(v);
-        t[i] = tv * g.inv_temperature;
-        s[i] = to_f32<T>(x[v]);
-        t_max = fmaxf(t_max, t[i]);
+        r.at[i] = static_cast<int>(v);
+        r.t[i] = tv * g.inv_temperature;
+        t_max = fmaxf(t_max, r.t[i]);
         found = true;
       }
     }
   }
-  int64_t label = -1;
-  float s_label = 0.f;
+  r.label = -1;
   if (g.labels != nullptr && g.ce_weight != 0.f) {
-    label = g.labels[row];
-    if (label == g.ignore_index || label < 0 || label >= g.vocab) label = -1;
-    if (label >= 0) s_label = to_f32<T>(x[label]);
+    r.label = g.labels[row];
+    if (r.label == g.ignore_index || r.label < 0 || r.label >= g.vocab) r.label = -1;
   }
-  const bool has_teacher = __syncthreads_or(found);
-  const bool has_label = label >= 0;
-
-  float m = 0.f, inv_t = 0.f, inv_1 = 0.f;
-  if (MODE != kGrad) {
-    if (has_teacher || has_label) {
-      Online o;
-      const int64_t head = head_of(x, g.vocab), body = (g.vocab - head) / kVec;
-      if (tid < head) {
-        const float v[1] = {to_f32<T>(x[tid])};
-        take<BOTH>(o, v, g.k_t);
-      }
-      for (int64_t i = tid; i < body; i += kThreads) {
-        float v[kVec];
-        VecLoad<T, kVec>::load(x + head + i * kVec, v);
-        take<BOTH>(o, v, g.k_t);
-      }
-      const int64_t tail = head + body * kVec;
-      if (tail + tid < g.vocab) {
-        const float v[1] = {to_f32<T>(x[tail + tid])};
-        take<BOTH>(o, v, g.k_t);
-      }
-      m = block_max(o.m, red);
-      const float s_t = block_sum(o.s_t * exp2_approx((o.m - m) * g.k_t), red);
-      const float s_1 = BOTH ? block_sum(o.s_1 * exp2_approx((o.m - m) * kLog2e), red) : s_t;
-      inv_t = 1.f / s_t;
-      inv_1 = 1.f / s_1;
-      // The losses, each difference formed from the row's maximum.
-      float q_max = block_max(t_max, red), part = 0.f;
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) part += at[i] >= 0 ? expf(t[i] - q_max) : 0.f;
-      const float log_total = logf(block_sum(part, red)), log_s = logf(s_t);
-      part = 0.f;
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        if (at[i] >= 0) {
-          const float log_q = t[i] - q_max - log_total, q = expf(log_q);
-          if (q != 0.f) part += q * (log_q - ((s[i] - m) * g.inv_temperature - log_s));
-        }
-      }
-      const float kl = block_sum(part, red);
-      if (tid == 0) {
-        float loss = has_teacher ? g.kl_weight * kl : 0.f;
-        if (has_label) loss += g.ce_weight * (logf(s_1) - (s_label - m));
-        g.losses[row] = loss;
-        if (g.stats != nullptr) g.stats[row] = make_float4(m, inv_t, inv_1, 1.f);
-      }
-    } else if (tid == 0) {
-      g.losses[row] = 0.f;
-      if (g.stats != nullptr) g.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  } else {
-    const float4 st = g.stats[row];
-    m = st.x;
-    inv_t = st.y;
-    inv_1 = st.z;
-  }
-
-  if (MODE != kLoss) {
-    T *out = static_cast<T *>(g.grad) + row * g.vocab;
-    float scale = g.row_scale != nullptr ? g.row_scale[g.scale_per_row ? row : 0] : 1.f;
-    if (g.count != nullptr) scale /= fmaxf(*g.count, 1.f);
-    const float base_t = has_teacher ? scale * g.kl_grad_weight : 0.f, base_1 = has_label ? scale * g.ce_weight : 0.f;
-    const float c_t = base_t * inv_t, c_1 = base_1 * inv_1;
-    auto dense = [&](float v) -> float {
-      const float d = v - m;
-      float r = 0.f;
-      if (has_teacher) r = c_t * exp2_approx(d * g.k_t);
-      if (has_label) r = fmaf(c_1, exp2_approx(d * kLog2e), r);
-      return r;
-    };
-    const int64_t head = head_of(out, g.vocab), body = (g.vocab - head) / kVec;
-    const bool same = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
-    if (tid < head) out[tid] = from_f32<T>(dense(to_f32<T>(x[tid])));
-    for (int64_t i = tid; i < body; i += kThreads) {
-      float v[kVec];
-      if (same) {
-        VecLoad<T, kVec>::load(x + head + i * kVec, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) v[j] = to_f32<T>(x[head + i * kVec + j]);
-      }
-      alignas(16) T w[kVec];
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) w[j] = from_f32<T>(dense(v[j]));
-      *reinterpret_cast<uint4 *>(out + head + i * kVec) = *reinterpret_cast<const uint4 *>(w);
-    }
-    const int64_t tail = head + body * kVec;
-    if (tail + tid < g.vocab) out[tail + tid] = from_f32<T>(dense(to_f32<T>(x[tail + tid])));
-
-    // The targets' own entries over it: p minus all that the teacher's entries of that index and
-    // the label put there, rounded once.
-    const float q_max = block_max(t_max, red);
+  r.has_label = r.label >= 0;
+  r.has_teacher = __syncthreads_or(found);
+  r.q_max = r.q_total = 0.f;
+  if (r.has_teacher) {
+    r.q_max = block_max(t_max, red);
     float part = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) part += at[i] >= 0 ? expf(t[i] - q_max) : 0.f;
-    const float inv_total = 1.f / block_sum(part, red);
+    for (int i = 0; i < kPerThread; ++i) part += r.at[i] >= 0 ? expf(r.t[i] - r.q_max) : 0.f;
+    r.q_total = block_sum(part, red);
+  }
+  return r;
+}
+
+// The row's loss from its sums; every thread of the block takes part, thread 0 has it.
+__device__ __forceinline__ float row_loss(const DistillArgs &g, const Targets &r, const RowStats &st, const float (&s)[kPerThread],
+                                          float s_label, float *red) {
+  float loss = 0.f;
+  if (r.has_teacher) {
+    const float log_total = logf(r.q_total), log_s = logf(st.s_t);
+    float part = 0.f;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      const int k = tid + i * kThreads;
-      if (k < g.top) {
-        at_of[k] = at[i];
-        q_of[k] = at[i] >= 0 ? expf(t[i] - q_max) * inv_total : 0.f;
+      if (r.at[i] >= 0) {
+        const float log_q = r.t[i] - r.q_max - log_total, q = expf(log_q);
+        if (q != 0.f) part += q * (log_q - ((s[i] - st.m) * g.inv_temperature - log_s));
       }
     }
-    __syncthreads();
+    loss = g.kl_weight * block_sum(part, red);
+  }
+  if (r.has_label) loss += g.ce_weight * (logf(st.s_1) - (s_label - st.m));
+  return loss;
+}
+
+// The gradient of one row's elements [e0, e1), of which `source` gives any as f32 (and vectors of the
+// input grid where input and output are aligned alike): dense, then the targets' own entries over it.
+struct GradScale {
+  float base_t, base_1;  // scale (1 - w) T and scale w, 0 without such a target
+  float c_t, c_1;        // the same over the sums
+};
+__device__ __forceinline__ GradScale grad_scale(const DistillArgs &g, const Targets &r, int64_t row, float inv_t, float inv_1) {
+  float scale = g.row_scale != nullptr ? g.row_scale[g.scale_per_row ? row : 0] : 1.f;
+  if (g.count != nullptr) scale /= fmaxf(*g.count, 1.f);
+  GradScale c;
+  c.base_t = r.has_teacher ? scale * g.kl_grad_weight : 0.f;
+  c.base_1 = r.has_label ? scale * g.ce_weight : 0.f;
+  c.c_t = r.has_teacher ? c.base_t * inv_t : 0.f;
+  c.c_1 = r.has_label ? c.base_1 * inv_1 : 0.f;
+  return c;
+}
+template <int EXPS>
+__device__ __forceinline__ float2 dense2(float2 v, float m, float k_t, const GradScale &c) {
+  const float2 d = add2(v, both(-m)), t = mul2(d, both(k_t));
+  const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+  if (EXPS == kOne) return mul2(e, both(c.c_t + c.c_1));
+  if (EXPS == kSquare) return mul2(e, fma2(e, both(c.c_1), both(c.c_t)));
+  const float2 u = mul2(d, both(kLog2e));
+  return fma2(make_float2(exp2_approx(u.x), exp2_approx(u.y)), both(c.c_1), mul2(e, both(c.c_t)));
+}
+template <typename T, int EXPS, typename VecAt, typename ElementAt>
+__device__ __forceinline__ void write_dense(T *out, int64_t e0, int64_t e1, bool alike, float m, float k_t,
+                                            const GradScale &c, bool zero, VecAt vec_at, ElementAt element_at) {
+  constexpr int kN = Vec<T>::kN;
+  const int tid = threadIdx.x;
+  const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out + e0) & 15u);
+  const int64_t head = min64(e1 - e0, off == 0 ? 0 : (16 - off) / int64_t(sizeof(T)));
+  const int64_t body = (e1 - e0 - head) / kN, tail = e0 + head + body * kN;
+  auto one = [&](int64_t e) -> T {
+    return zero ? from_f32<T>(0.f) : from_f32<T>(dense2<EXPS>(both(element_at(e)), m, k_t, c).x);
+  };
+  if (tid < head) out[e0 + tid] = one(e0 + tid);
+#pragma unroll 4
+  for (int64_t i = tid; i < body; i += kThreads) {
+    const int64_t e = e0 + head + i * kN;
+    float2 v[kN / 2];
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (!zero) {
+      if (alike) {
+        Vec<T>::unpack(vec_at(e), v);
+      } else {
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      if (at[i] >= 0) {
-        float q = 0.f;
-        for (int k = 0; k < g.top; ++k) q += at_of[k] == at[i] ? q_of[k] : 0.f;
-        const float d = s[i] - m;
-        float r = base_t * (exp2_approx(d * g.k_t) * inv_t - q);
-        if (has_label) r += base_1 * (exp2_approx(d * kLog2e) * inv_1 - (at[i] == label ? 1.f : 0.f));
-        out[at[i]] = from_f32<T>(r);  // entries of one index write the same value
+        for (int j = 0; j < kN / 2; ++j) v[j] = make_float2(element_at(e + 2 * j), element_at(e + 2 * j + 1));
       }
+#pragma unroll
+      for (int j = 0; j < kN / 2; ++j) v[j] = dense2<EXPS>(v[j], m, k_t, c);
+      w = Vec<T>::pack(v);
     }
-    if (tid == 0 && has_label) {
-      bool taught = false;
-      if (has_teacher)
-        for (int k = 0; k < g.top; ++k) taught |= at_of[k] == label;
-      if (!taught) {
-        const float d = s_label - m;
-        float r = base_1 * (exp2_approx(d * kLog2e) * inv_1 - 1.f);
-        if (has_teacher) r += c_t * exp2_approx(d * g.k_t);
-        out[label] = from_f32<T>(r);
-      }
+    __stcs(reinterpret_cast<uint4 *>(out + e), w);
+  }
+  if (tail + tid < e1) out[tail + tid] = one(tail + tid);
+}
+// The targets in [e0, e1): p minus all that the teacher's entries of that index and the label put
+// there, rounded once. After write_dense; every thread takes part.
+template <typename T, int EXPS, typename ElementAt>
+__device__ __forceinline__ void write_targets(const DistillArgs &g, const Targets &r, T *out, int64_t e0, int64_t e1, float m,
+                                              const GradScale &c, float *q_of, int *at_of, ElementAt element_at) {
+  const int tid = threadIdx.x;
+  const float inv_total = r.has_teacher ? 1.f / r.q_total : 0.f;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    const int k = tid + i * kThreads;
+    if (k < g.top) {
+      at_of[k] = r.at[i];
+      q_of[k] = r.at[i] >= 0 ? expf(r.t[i] - r.q_max) * inv_total : 0.f;
     }
   }
+  __syncthreads();
+  auto put = [&](int64_t e, float q) {
+    const float p = dense2<EXPS>(both(element_at(e)), m, g.k_t, c).x;
+    out[e] = from_f32<T>(p - c.base_t * q - (e == r.label ? c.base_1 : 0.f));
+  };
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    if (r.at[i] >= e0 && r.at[i] < e1) {
+      float q = 0.f;
+      for (int k = 0; k < g.top; ++k) q += at_of[k] == r.at[i] ? q_of[k] : 0.f;
+      put(r.at[i], q);  // entries of one index write the same value
+    }
+  }
+  if (tid == 0 && r.label >= e0 && r.label < e1) {
+    bool taught = false;
+    if (r.has_teacher)
+      for (int k = 0; k < g.top; ++k) taught |= at_of[k] == r.label;
+    if (!taught) put(r.label, 0.f);
+  }
+}
+
+// Loss (MODE kLoss), or loss and gradient (kFused), of a row a cluster. RESIDENT: the slice stays in
+// shared memory for the gradient; else it is read again.
+template <typename T, int MODE, int EXPS, bool RESIDENT>
+__global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel(const DistillArgs g) {
+  constexpr int kN = Vec<T>::kN;
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  __shared__ float red[kWarps];
+  __shared__ RowStats of_warp[kWarps], of_rank[kMaxCluster];
+  __shared__ float q_of[MODE == kFused ? kMaxTop : 1];
+  __shared__ int at_of[MODE == kFused ? kMaxTop : 1];
+  __shared__ uint64_t full[kChunks];
+  __shared__ int abort;
+  uint4 *slice = reinterpret_cast<uint4 *>(dynamic);
+  const int rank = blockIdx.x % g.ranks;
+  const int64_t row = blockIdx.x / g.ranks;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const T *x = static_cast<const T *>(g.logits) + (row / g.inner) * g.outer_stride + (row % g.inner) * g.inner_stride;
+  const int64_t lead = static_cast<int64_t>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T)), end = lead + g.vocab;
+  const T *grid = x - lead;
+  const int64_t vec0 = int64_t(rank) * g.slice_vecs;
+  const int vecs = static_cast<int>(min64(g.slice_vecs, max(int64_t(0), (end + kN - 1) / kN - vec0)));
+  if (g.ranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+
+  // Whole vectors of the slice come as bulk copies; one at either end of the row may be cut.
+  const bool first_cut = vec0 == 0 && lead > 0, last_cut = vec0 + vecs == (end + kN - 1) / kN && end % kN != 0;
+  const int whole0 = first_cut ? 1 : 0, whole1 = max(vecs - (last_cut ? 1 : 0), whole0);
+  const int per_chunk = (whole1 - whole0 + kChunks - 1) / kChunks;
+  if (RESIDENT) {
+    if (tid == 0) {
+      abort = 0;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) sm100::mbar_init(&full[c], 1);
+      sm100::mbar_init_fence();
+      sm100::fence_proxy_async_smem();
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int from = min(whole0 + c * per_chunk, whole1), to = min(from + per_chunk, whole1);
+        if (to > from) {
+          sm100::mbar_expect_tx(&full[c], (to - from) * 16);
+          sm100::bulk_load_1d(slice + from, grid + (vec0 + from) * kN, (to - from) * 16, &full[c]);
+        }
+      }
+    }
+    if (tid == 32 && first_cut && vecs > 0) slice[0] = load_vec<T>(grid, vec0, lead, end);
+    if (tid == 64 && last_cut && vecs > whole0) slice[vecs - 1] = load_vec<T>(grid, vec0 + vecs - 1, lead, end);
+  }
+  const Targets r = load_targets(g, row, red);
+  const bool wanted = r.has_teacher || r.has_label;
+  float s[kPerThread] = {}, s_label = 0.f;
+  if (rank == 0) {  // the targets' logits for the loss
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i)
+      if (r.at[i] >= 0) s[i] = to_f32<T>(x[r.at[i]]);
+    if (r.has_label) s_label = to_f32<T>(x[r.label]);
+  }
+
+  // One order of summation for all three kernels: cut vectors first, then chunk by chunk. (load_targets'
+  // barriers put the setup of the copies and the cut vectors before this.)
+  auto at = [&](int v) -> uint4 {
+    if constexpr (RESIDENT) return slice[v];
+    else return load_vec<T>(grid, vec0 + v, lead, end);
+  };
+  Online o;
+  if (wanted && tid == 0) {
+    if (first_cut && vecs > 0) {
+      const uint4 q[1] = {at(0)};
+      take<T, EXPS>(o, q, g.k_t);
+    }
+    if (last_cut && vecs > whole0) {
+      const uint4 q[1] = {at(vecs - 1)};
+      take<T, EXPS>(o, q, g.k_t);
+    }
+  }
+  for (int c = 0; c < kChunks; ++c) {
+    const int from = min(whole0 + c * per_chunk, whole1), to = min(from + per_chunk, whole1);
+    if (to <= from) break;
+    if (RESIDENT) sm100::mbar_wait(&full[c], 0, &abort, &g_distill_error);
+    if (!wanted) continue;
+    int v = from + tid;
+    for (; v + 3 * kThreads < to; v += 4 * kThreads) {
+      uint4 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = RESIDENT ? slice[v + i * kThreads] : __ldg(reinterpret_cast<const uint4 *>(grid + (vec0 + v + i * kThreads) * kN));
+      take<T, EXPS>(o, q, g.k_t);
+    }
+    for (; v < to; v += kThreads) {
+      const uint4 q[1] = {at(v)};
+      take<T, EXPS>(o, q, g.k_t);
+    }
+  }
+  RowStats st = {o.m, o.s_t.x + o.s_t.y, o.s_1.x + o.s_1.y};
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) st = join<EXPS>(st, shuffled(st, d), g.k_t);
+  if (lane == 0) of_warp[warp] = st;
+  __syncthreads();
+  st = of_warp[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) st = join<EXPS>(st, of_warp[w], g.k_t);
+  if (g.ranks > 1) {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // all have started
+    if (tid < g.ranks) *cooperative_groups::this_cluster().map_shared_rank(&of_rank[rank], tid) = st;
+    cooperative_groups::this_cluster().sync();
+    st = of_rank[0];
+    for (int i = 1; i < g.ranks; ++i) st = join<EXPS>(st, of_rank[i], g.k_t);
+  }
+  const float inv_t = 1.f / st.s_t, inv_1 = 1.f / st.s_1;
+  if (rank == 0) {
+    const float loss = wanted ? row_loss(g, r, st, s, s_label, red) : 0.f;
+    if (tid == 0) {
+      g.losses[row] = loss;
+      if (MODE == kLoss && g.stats != nullptr) g.stats[row] = wanted ? make_float4(st.m, inv_t, inv_1, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+
+  if constexpr (MODE == kFused) {
+    T *out = static_cast<T *>(g.grad) + row * g.vocab;
+    const int64_t e0 = max(int64_t(0), vec0 * kN - lead), e1 = min64(g.vocab, (vec0 + vecs) * kN - lead);
+    const GradScale c = grad_scale(g, r, row, inv_t, inv_1);
+    const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
+    auto vec_at = [&](int64_t e) -> uint4 {
+      if constexpr (RESIDENT) return slice[(e + lead) / kN - vec0];
+      else return __ldg(reinterpret_cast<const uint4 *>(x + e));
+    };
+    auto element_at = [&](int64_t e) -> float {
+      if constexpr (RESIDENT) return to_f32<T>(reinterpret_cast<const T *>(slice)[e + lead - vec0 * kN]);
+      else return ldg_f32(x + e);
+    };
+    if (e1 > e0) write_dense<T, EXPS>(out, e0, e1, alike, st.m, g.k_t, c, !wanted, vec_at, element_at);
+    if (wanted) write_targets<T, EXPS>(g, r, out, e0, e1, st.m, c, q_of, at_of, element_at);
+  }
+}
+
+// The gradient from the loss's statistics: each CTA a part of a row.
+template <typename T, int EXPS>
+__global__ void __launch_bounds__(kThreads, 4) distill_grad_kernel(const DistillArgs g) {
+  constexpr int kN = Vec<T>::kN;
+  __shared__ float red[kWarps];
+  __shared__ float q_of[kMaxTop];
+  __shared__ int at_of[kMaxTop];
+  const int64_t row = blockIdx.x / g.ranks, part = blockIdx.x % g.ranks;
+  const T *x = static_cast<const T *>(g.logits) + (row / g.inner) * g.outer_stride + (row % g.inner) * g.inner_stride;
+  T *out = static_cast<T *>(g.grad) + row * g.vocab;
+  const Targets r = load_targets(g, row, red);
+  const float4 st = g.stats[row];
+  const GradScale c = grad_scale(g, r, row, st.y, st.z);
+  // Parts end on the output's 16-byte grid.
+  const int64_t lead = static_cast<int64_t>((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T));
+  const int64_t e0 = max(int64_t(0), part * g.slice_vecs * kN - lead), e1 = min64(g.vocab, (part + 1) * g.slice_vecs * kN - lead);
+  const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
+  auto vec_at = [&](int64_t e) -> uint4 { return __ldg(reinterpret_cast<const uint4 *>(x + e)); };
+  auto element_at = [&](int64_t e) -> float { return ldg_f32(x + e); };
+  const bool wanted = r.has_teacher || r.has_label;
+  if (e1 > e0) write_dense<T, EXPS>(out, e0, e1, alike, st.x, g.k_t, c, !wanted, vec_at, element_at);
+  if (wanted) write_targets<T, EXPS>(g, r, out, e0, e1, st.x, c, q_of, at_of, element_at);
 }
 
 // losses summed in a fixed order; *count = rows with a target; *loss = sum, or sum / max(count, 1).
@@ -312,12 +568,53 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float *losse
   }
 }
 
+template <typename T, int MODE, int EXPS>
+int launch_rows(const char *what, DistillArgs g, int64_t rows, cudaStream_t stream) {
+  int sms = 0;
+  TB_CHECK(sm100::sm_count(&sms));
+  // The fewest CTAs a row that keep its slices at three CTAs an SM, more while SMs are idle.
+  const int64_t row_bytes = g.vocab * int64_t(sizeof(T)) + 32;
+  int ranks = 1;
+  while (ranks < kMaxCluster && (row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 8192)))
+    ranks *= 2;
+  if (MODE == kGrad) ranks = static_cast<int>(std::max<int64_t>(ranks, ceil_div(row_bytes, kSliceShared)));
+  const int64_t slice = ceil_div(row_bytes / 16, ranks);
+  TB_REQUIRE(rows * ranks <= 0x7fffffffLL && slice <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: too many rows", what);
+  g.ranks = ranks;
+  g.slice_vecs = static_cast<int>(slice);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(rows * ranks));
+  config.blockDim = dim3(kThreads);
+  config.stream = stream;
+  const void *kernel = nullptr;
+  cudaLaunchAttribute attr{};
+  if constexpr (MODE == kGrad) {
+    kernel = reinterpret_cast<const void *>(distill_grad_kernel<T, EXPS>);
+  } else {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(ranks);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    kernel = reinterpret_cast<const void *>(distill_row_kernel<T, MODE, EXPS, false>);
+    if constexpr (MODE == kFused) {
+      if (slice * 16 <= kSliceMost) {
+        kernel = reinterpret_cast<const void *>(distill_row_kernel<T, MODE, EXPS, true>);
+        config.dynamicSmemBytes = static_cast<size_t>(slice) * 16;
+        // The static tables count too: above 48 KB in all the kernel has to be told.
+        TB_CHECK(ensure_dynamic_smem(kernel, std::max<size_t>(config.dynamicSmemBytes, 49 * 1024), what));
+      }
+    }
+  }
+  void *args[] = {&g};
+  cudaLaunchKernelExC(&config, kernel, args);
+  return check_launch(what);
+}
 template <typename T, int MODE>
-void launch_rows(const DistillArgs &g, int64_t rows, bool both, cudaStream_t stream) {
-  if (both)
-    distill_rows_kernel<T, MODE, true><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(g);
-  else
-    distill_rows_kernel<T, MODE, false><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(g);
+int launch_exps(const char *what, const DistillArgs &g, int64_t rows, int exps, cudaStream_t stream) {
+  if (exps == kOne) return launch_rows<T, MODE, kOne>(what, g, rows, stream);
+  if (exps == kTwo) return launch_rows<T, MODE, kTwo>(what, g, rows, stream);
+  return launch_rows<T, MODE, kSquare>(what, g, rows, stream);
 }
 
 template <int MODE>
@@ -350,11 +647,10 @@ int run_rows(const char *what, DistillArgs g, int dtype, int64_t rows, int64_t v
   g.kl_weight = (1.f - label_weight) * t * t;
   g.kl_grad_weight = (1.f - label_weight) * t;
   g.ce_weight = label_weight;
-  const bool both = t != 1.f && label_weight != 0.f;
-  if (dtype == TROPNN_B200_F32) launch_rows<float, MODE>(g, rows, both, stream);
-  else if (dtype == TROPNN_B200_F16) launch_rows<__half, MODE>(g, rows, both, stream);
-  else launch_rows<__nv_bfloat16, MODE>(g, rows, both, stream);
-  return check_launch(what);
+  const int exps = t == 1.f || label_weight == 0.f ? kOne : t == 2.f ? kSquare : kTwo;
+  if (dtype == TROPNN_B200_F32) return launch_exps<float, MODE>(what, g, rows, exps, stream);
+  if (dtype == TROPNN_B200_F16) return launch_exps<__half, MODE>(what, g, rows, exps, stream);
+  return launch_exps<__nv_bfloat16, MODE>(what, g, rows, exps, stream);
 }
 
 DistillArgs make_args(const void *logits, int64_t inner, int64_t outer_stride, int64_t inner_stride, const void *teacher,
@@ -376,6 +672,21 @@ DistillArgs make_args(const void *logits, int64_t inner, int64_t outer_stride, i
 }
 
 }  // namespace
+
+// Reads and clears this file's device error word (a wait for a bulk copy that ran out).
+int read_distill_error(int *value) {
+  int v = 0;
+  cudaError_t err = cudaMemcpyFromSymbol(&v, g_distill_error, sizeof(int));
+  if (err != cudaSuccess)
+    return set_error(TROPNN_B200_ERR_LAUNCH, "reading the device error word: %s", cudaGetErrorString(err));
+  if (v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_distill_error, &zero, sizeof(int));
+  }
+  *value = v;
+  return TROPNN_B200_OK;
+}
+
 }  // namespace tropnn_b200
 
 using namespace tropnn_b200;

@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "packed.cuh"
 #include "sm100.cuh"
 
 namespace tropnn_b200 {
@@ -129,43 +130,6 @@ __device__ __forceinline__ void store_pair(T *p, float2 v, bool on0, bool on1) {
       if (on1) p[32] = from_f32<T>(v.y);
     }
   }
-}
-
-// Both channels of a lane in one instruction (f32x2).
-__device__ __forceinline__ uint64_t bits2(float2 v) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
-  return r;
-}
-__device__ __forceinline__ float2 float2_of(uint64_t r) {
-  float2 v;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-  return v;
-}
-__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(x)), "l"(bits2(y)));
-  return float2_of(r);
-}
-__device__ __forceinline__ float2 add2(float2 x, float2 y) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(x)), "l"(bits2(y)));
-  return float2_of(r);
-}
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(x)), "l"(bits2(y)), "l"(bits2(z)));
-  return float2_of(r);
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
 }
 
 // a and c = 1 - a. The smaller one, m = e / (1 + e) with e = exp(-|f|), has its full relative
@@ -1085,7 +1049,7 @@ int launch_recurrence(const char *what, RecurrenceArgs g, int dtype, int64_t bat
 int read_recurrence_error(int *value) {
   int v = 0;
   cudaError_t err = cudaMemcpyFromSymbol(&v, g_recurrence_error, sizeof(int));
-  if (err != cudaSuccess) return set_error(TROPNN_B200_ERR_LAUNCH, "device_error: %s", cudaGetErrorString(err));
+  if (err != cudaSuccess) return set_error(TROPNN_B200_ERR_LAUNCH, "reading the device error word: %s", cudaGetErrorString(err));
   if (v != 0) {
     const int zero = 0;
     cudaMemcpyToSymbol(g_recurrence_error, &zero, sizeof(int));

@@ -55,6 +55,7 @@ int read_lut_grad_error(int *value);
 int read_proj_error(int *value);
 int read_gemm_tf32_error(int *value);
 int read_recurrence_error(int *value);
+int read_distill_error(int *value);
 int trop_gm_sm100_impl(const void *g_split, int64_t rows, int64_t code_dim, const void *code, int dtype, int64_t heads,
                        int64_t cells, const uint8_t *winner, const uint8_t *runner, const float *margins,
                        float code_scale, float *gm, const uint32_t *absmax, cudaStream_t stream);
@@ -943,7 +944,7 @@ int tropnn_b200_transpose_to_half(const void *x, int x_dtype, int64_t rows, int6
 
 int tropnn_b200_device_error(int *value) {
   TB_CHECK(tropnn_b200::check_current_device());
-  int score = 0, hidden = 0, gemm = 0, peer = 0, pgrad = 0, lgrad = 0, lutg = 0, proj = 0, gtf32 = 0, pair = 0, rec = 0;
+  int score = 0, hidden = 0, gemm = 0, peer = 0, pgrad = 0, lgrad = 0, lutg = 0, proj = 0, gtf32 = 0, pair = 0, rec = 0, dist = 0;
   TB_CHECK(tropnn_b200::read_score_error(&score));
   TB_CHECK(tropnn_b200::read_hidden_error(&hidden));
   TB_CHECK(tropnn_b200::read_gemm_error(&gemm));
@@ -955,7 +956,8 @@ int tropnn_b200_device_error(int *value) {
   TB_CHECK(tropnn_b200::read_gemm_tf32_error(&gtf32));
   TB_CHECK(tropnn_b200::read_pairwise_error(&pair));
   TB_CHECK(tropnn_b200::read_recurrence_error(&rec));
-  *value = score | hidden | gemm | peer | pgrad | lgrad | lutg | proj | gtf32 | pair | rec;
+  TB_CHECK(tropnn_b200::read_distill_error(&dist));
+  *value = score | hidden | gemm | peer | pgrad | lgrad | lutg | proj | gtf32 | pair | rec | dist;
   return tropnn_b200::clear_error();
 }
 
