@@ -213,18 +213,26 @@ __device__ __forceinline__ void take(Online &o, const uint4 (&q)[COUNT], float k
 struct RowStats {
   float m, s_t, s_1;
 };
+// `a`'s sums relative to a larger maximum.
 template <int EXPS>
-__device__ __forceinline__ RowStats join(RowStats a, RowStats b, float k_t) {
-  const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m;
-  const float ea = exp2_approx(da * k_t), eb = exp2_approx(db * k_t);
-  RowStats r;
-  r.m = m;
-  r.s_t = a.s_t * ea + b.s_t * eb;
-  r.s_1 = EXPS == kOne ? r.s_t : a.s_1 * second_exp<EXPS>(ea, da) + b.s_1 * second_exp<EXPS>(eb, db);
-  return r;
+__device__ __forceinline__ RowStats raised(RowStats a, float m, float k_t) {
+  const float d = a.m - m, e = exp2_approx(d * k_t);
+  return {m, a.s_t * e, EXPS == kOne ? 0.f : a.s_1 * second_exp<EXPS>(e, d)};
 }
-__device__ __forceinline__ RowStats shuffled(RowStats a, int o) {
-  return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s_t, o), __shfl_xor_sync(0xffffffffu, a.s_1, o)};
+// All of the lanes' (of the first WIDTH lanes', in each group of WIDTH) statistics together.
+template <int EXPS, int WIDTH>
+__device__ __forceinline__ RowStats joined(RowStats a, float k_t) {
+  float m = a.m;
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  a = raised<EXPS>(a, m, k_t);
+#pragma unroll
+  for (int o = WIDTH / 2; o > 0; o >>= 1) {
+    a.s_t += __shfl_xor_sync(0xffffffffu, a.s_t, o);
+    if (EXPS != kOne) a.s_1 += __shfl_xor_sync(0xffffffffu, a.s_1, o);
+  }
+  if (EXPS == kOne) a.s_1 = a.s_t;
+  return a;
 }
 
 // A row's targets: the teacher's entries spread over the block's threads, and the label.
@@ -350,39 +358,59 @@ __device__ __forceinline__ void write_dense(T *out, int64_t e0, int64_t e1, bool
   }
   if (tail + tid < e1) out[tail + tid] = one(tail + tid);
 }
+// The teacher's entries of a row, and those of them in a CTA's part.
+struct EntryTable {
+  alignas(16) int at[kMaxTop];
+  alignas(16) float q[kMaxTop];
+  uint16_t mine[kMaxTop];  // entry numbers
+  int count;
+};
 // The targets in [e0, e1): p minus all that the teacher's entries of that index and the label put
 // there, rounded once. After write_dense; every thread takes part.
 template <typename T, int EXPS, typename ElementAt>
 __device__ __forceinline__ void write_targets(const DistillArgs &g, const Targets &r, T *out, int64_t e0, int64_t e1, float m,
-                                              const GradScale &c, float *q_of, int *at_of, ElementAt element_at) {
+                                              const GradScale &c, EntryTable &table, ElementAt element_at) {
   const int tid = threadIdx.x;
   const float inv_total = r.has_teacher ? 1.f / r.q_total : 0.f;
+  const int padded = r.has_teacher ? (g.top + 3) & ~3 : 0;
+  if (tid == 0) table.count = 0;
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     const int k = tid + i * kThreads;
-    if (k < g.top) {
-      at_of[k] = r.at[i];
-      q_of[k] = r.at[i] >= 0 ? expf(r.t[i] - r.q_max) * inv_total : 0.f;
+    if (k < padded) {
+      table.at[k] = r.at[i];
+      table.q[k] = r.at[i] >= 0 ? expf(r.t[i] - r.q_max) * inv_total : 0.f;
+      if (r.at[i] >= e0 && r.at[i] < e1) table.mine[atomicAdd(&table.count, 1)] = static_cast<uint16_t>(k);
     }
   }
   __syncthreads();
+  auto sum_at = [&](int e, bool &found) -> float {  // in the entries' order
+    float q = 0.f;
+    for (int k = 0; k < padded; k += 4) {
+      const int4 a = *reinterpret_cast<const int4 *>(&table.at[k]);
+      const float4 v = *reinterpret_cast<const float4 *>(&table.q[k]);
+      q += a.x == e ? v.x : 0.f;
+      q += a.y == e ? v.y : 0.f;
+      q += a.z == e ? v.z : 0.f;
+      q += a.w == e ? v.w : 0.f;
+      found |= a.x == e || a.y == e || a.z == e || a.w == e;
+    }
+    return q;
+  };
   auto put = [&](int64_t e, float q) {
     const float p = dense2<EXPS>(both(element_at(e)), m, g.k_t, c).x;
     out[e] = from_f32<T>(p - c.base_t * q - (e == r.label ? c.base_1 : 0.f));
   };
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    if (r.at[i] >= e0 && r.at[i] < e1) {
-      float q = 0.f;
-      for (int k = 0; k < g.top; ++k) q += at_of[k] == r.at[i] ? q_of[k] : 0.f;
-      put(r.at[i], q);  // entries of one index write the same value
-    }
+  bool found = false;
+  for (int i = tid; i < table.count; i += kThreads) {
+    const int e = table.at[table.mine[i]];
+    put(e, sum_at(e, found));  // entries of one index write the same value
   }
-  if (tid == 0 && r.label >= e0 && r.label < e1) {
-    bool taught = false;
-    if (r.has_teacher)
-      for (int k = 0; k < g.top; ++k) taught |= at_of[k] == r.label;
-    if (!taught) put(r.label, 0.f);
+  if (tid == kThreads - 1 && r.label >= e0 && r.label < e1) {
+    found = false;
+    const float q = sum_at(static_cast<int>(r.label), found);
+    if (!found) put(r.label, q);
   }
 }
 
@@ -394,8 +422,7 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ float red[kWarps];
   __shared__ RowStats of_warp[kWarps], of_rank[kMaxCluster];
-  __shared__ float q_of[MODE == kFused ? kMaxTop : 1];
-  __shared__ int at_of[MODE == kFused ? kMaxTop : 1];
+  __shared__ EntryTable table;
   __shared__ uint64_t full[kChunks];
   __shared__ int abort;
   uint4 *slice = reinterpret_cast<uint4 *>(dynamic);
@@ -477,29 +504,18 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
     }
   }
   RowStats st = {o.m, o.s_t.x + o.s_t.y, o.s_1.x + o.s_1.y};
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) st = join<EXPS>(st, shuffled(st, d), g.k_t);
+  st = joined<EXPS, 32>(st, g.k_t);
   if (lane == 0) of_warp[warp] = st;
   __syncthreads();
-  st = of_warp[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) st = join<EXPS>(st, of_warp[w], g.k_t);
+  st = joined<EXPS, kWarps>(of_warp[lane % kWarps], g.k_t);
   if (g.ranks > 1) {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // all have started
     if (tid < g.ranks) *cooperative_groups::this_cluster().map_shared_rank(&of_rank[rank], tid) = st;
     cooperative_groups::this_cluster().sync();
-    st = of_rank[0];
-    for (int i = 1; i < g.ranks; ++i) st = join<EXPS>(st, of_rank[i], g.k_t);
+    const RowStats none = {kLowest, 0.f, 0.f};
+    st = joined<EXPS, kMaxCluster>(lane % kMaxCluster < g.ranks ? of_rank[lane % kMaxCluster] : none, g.k_t);
   }
   const float inv_t = 1.f / st.s_t, inv_1 = 1.f / st.s_1;
-  if (rank == 0) {
-    const float loss = wanted ? row_loss(g, r, st, s, s_label, red) : 0.f;
-    if (tid == 0) {
-      g.losses[row] = loss;
-      if (MODE == kLoss && g.stats != nullptr) g.stats[row] = wanted ? make_float4(st.m, inv_t, inv_1, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  }
-
   if constexpr (MODE == kFused) {
     T *out = static_cast<T *>(g.grad) + row * g.vocab;
     const int64_t e0 = max(int64_t(0), vec0 * kN - lead), e1 = min64(g.vocab, (vec0 + vecs) * kN - lead);
@@ -514,7 +530,14 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
       else return ldg_f32(x + e);
     };
     if (e1 > e0) write_dense<T, EXPS>(out, e0, e1, alike, st.m, g.k_t, c, !wanted, vec_at, element_at);
-    if (wanted) write_targets<T, EXPS>(g, r, out, e0, e1, st.m, c, q_of, at_of, element_at);
+    if (wanted) write_targets<T, EXPS>(g, r, out, e0, e1, st.m, c, table, element_at);
+  }
+  if (rank == 0) {
+    const float loss = wanted ? row_loss(g, r, st, s, s_label, red) : 0.f;
+    if (tid == 0) {
+      g.losses[row] = loss;
+      if (MODE == kLoss && g.stats != nullptr) g.stats[row] = wanted ? make_float4(st.m, inv_t, inv_1, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
   }
 }
 
@@ -523,8 +546,7 @@ template <typename T, int EXPS>
 __global__ void __launch_bounds__(kThreads, 4) distill_grad_kernel(const DistillArgs g) {
   constexpr int kN = Vec<T>::kN;
   __shared__ float red[kWarps];
-  __shared__ float q_of[kMaxTop];
-  __shared__ int at_of[kMaxTop];
+  __shared__ EntryTable table;
   const int64_t row = blockIdx.x / g.ranks, part = blockIdx.x % g.ranks;
   const T *x = static_cast<const T *>(g.logits) + (row / g.inner) * g.outer_stride + (row % g.inner) * g.inner_stride;
   T *out = static_cast<T *>(g.grad) + row * g.vocab;
@@ -539,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_grad_kernel(const Distill
   auto element_at = [&](int64_t e) -> float { return ldg_f32(x + e); };
   const bool wanted = r.has_teacher || r.has_label;
   if (e1 > e0) write_dense<T, EXPS>(out, e0, e1, alike, st.x, g.k_t, c, !wanted, vec_at, element_at);
-  if (wanted) write_targets<T, EXPS>(g, r, out, e0, e1, st.x, c, q_of, at_of, element_at);
+  if (wanted) write_targets<T, EXPS>(g, r, out, e0, e1, st.x, c, table, element_at);
 }
 
 // losses summed in a fixed order; *count = rows with a target; *loss = sum, or sum / max(count, 1).
@@ -568,16 +590,21 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float *losse
   }
 }
 
+// CTAs an SM up to which a row is split further.
+template <int MODE>
+constexpr int kIdle = MODE == kGrad ? 4 : 1;
+
 template <typename T, int MODE, int EXPS>
 int launch_rows(const char *what, DistillArgs g, int64_t rows, cudaStream_t stream) {
   int sms = 0;
   TB_CHECK(sm100::sm_count(&sms));
-  // The fewest CTAs a row that keep its slices at three CTAs an SM, more while SMs are idle.
+  // In one call: the fewest CTAs a row that keep its slices at three CTAs an SM. Loss or gradient alone:
+  // a CTA a row. More of them while SMs are idle.
   const int64_t row_bytes = g.vocab * int64_t(sizeof(T)) + 32;
+  const int64_t most = MODE == kFused ? kSliceShared : int64_t(1) << 40;
   int ranks = 1;
-  while (ranks < kMaxCluster && (row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 8192)))
+  while (ranks < kMaxCluster && (row_bytes > ranks * most || (rows * ranks * 2 <= kIdle<MODE> * sms && row_bytes > ranks * 8192)))
     ranks *= 2;
-  if (MODE == kGrad) ranks = static_cast<int>(std::max<int64_t>(ranks, ceil_div(row_bytes, kSliceShared)));
   const int64_t slice = ceil_div(row_bytes / 16, ranks);
   TB_REQUIRE(rows * ranks <= 0x7fffffffLL && slice <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: too many rows", what);
   g.ranks = ranks;
