@@ -30,7 +30,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;
-constexpr int kPerThread = kMaxTop / kThreads;
 constexpr int kMaxCluster = 8;
 constexpr int kChunks = 4;  // bulk copies of a slice
 constexpr int64_t kSliceShared = 64 * 1024 + 64;  // bytes of a row a CTA: three CTAs on an SM
@@ -59,7 +58,7 @@ struct DistillArgs {
   float k_t;                                                    // log2(e) / T
   // kLoss, kFused
   float *losses;
-  float4 *stats;  // max, 1 / sum at T, 1 / sum at 1, 1 where the row has a target
+  float4 *stats;  // max, 1 / sum at T, 1 / sum at 1, 1 for teacher entries + 2 for a label
   // kGrad, kFused: scale of row n's gradient = row_scale[n or 0] / max(count, 1)
   const float *row_scale;
   int scale_per_row;
@@ -76,28 +75,6 @@ __device__ __forceinline__ float load_float(const void *p, int dtype, int64_t i)
 }
 __device__ __forceinline__ int64_t load_index(const void *p, int dtype, int64_t i) {
   return dtype == TROPNN_B200_I64 ? static_cast<const int64_t *>(p)[i] : static_cast<const int32_t *>(p)[i];
-}
-
-__device__ __forceinline__ float block_max(float v, float *shared) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = shared[0];
-#pragma unroll
-  for (int i = 1; i < kWarps; ++i) v = fmaxf(v, shared[i]);
-  return v;
-}
-__device__ __forceinline__ float block_sum(float v, float *shared) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = shared[0];
-#pragma unroll
-  for (int i = 1; i < kWarps; ++i) v += shared[i];
-  return v;
 }
 
 // 16 bytes of a row as f32 pairs.
@@ -235,86 +212,113 @@ __device__ __forceinline__ RowStats joined(RowStats a, float k_t) {
   return a;
 }
 
-// A row's targets: the teacher's entries spread over the block's threads, and the label.
-struct Targets {
-  int at[kPerThread];    // -1: none
-  float t[kPerThread];   // teacher logit / T
-  int64_t label;         // -1: none
-  bool has_teacher, has_label;
-  float q_max, q_total;  // of exp(t - q_max) over the entries
+// The teacher's entries of a row with their shares, and those of them in a CTA's part of the row.
+struct EntryTable {
+  alignas(16) int at[kMaxTop];  // -1: none
+  alignas(16) float q[kMaxTop];
+  uint16_t mine[kMaxTop];  // entry numbers
+  int count;               // of mine
+  int padded;              // entries, up to a multiple of four; 0: no teacher
+  int label;               // -1: none
 };
-__device__ __forceinline__ Targets load_targets(const DistillArgs &g, int64_t row, float *red) {
-  Targets r;
+// What the loss needs of the targets beside the row's sums.
+struct LossParts {
+  float entropy, cross, from, s_label;  // sum q log q, sum q (s - from) / T
+};
+
+// One warp reads the row's targets and fills the table, while the others are at the row itself.
+template <typename T>
+__device__ __forceinline__ LossParts load_targets(const DistillArgs &g, int64_t row, const T *x, int64_t e0, int64_t e1,
+                                                  bool for_loss, EntryTable &table) {
+  const int lane = threadIdx.x & 31;
+  LossParts parts = {0.f, 0.f, 0.f, 0.f};
+  int64_t label = -1;
+  if (g.labels != nullptr && g.ce_weight != 0.f) {
+    label = g.labels[row];
+    if (label == g.ignore_index || label < 0 || label >= g.vocab) label = -1;
+    if (for_loss && label >= 0) parts.s_label = to_f32<T>(x[label]);
+  }
+  const int top = g.kl_weight != 0.f ? g.top : 0, padded = (top + 31) & ~31;
   float t_max = kLowest;
   bool found = false;
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    const int k = threadIdx.x + i * kThreads;
-    r.at[i] = -1;
-    r.t[i] = 0.f;
-    if (k < g.top && g.kl_weight != 0.f) {
+#pragma unroll 4
+  for (int k = lane; k < padded; k += 32) {
+    int at = -1;
+    float t = 0.f;
+    if (k < top) {
       const int64_t v = load_index(g.indices, g.index_dtype, row * g.top + k);
       const float tv = load_float(g.teacher, g.teacher_dtype, row * g.top + k);
       if (v >= 0 && v < g.vocab && tv != -INFINITY) {
-        r.at[i] = static_cast<int>(v);
-        r.t[i] = tv * g.inv_temperature;
-        t_max = fmaxf(t_max, r.t[i]);
+        at = static_cast<int>(v);
+        t = tv * g.inv_temperature;
+        t_max = fmaxf(t_max, t);
         found = true;
       }
     }
+    table.at[k] = at;
+    table.q[k] = t;
   }
-  r.label = -1;
-  if (g.labels != nullptr && g.ce_weight != 0.f) {
-    r.label = g.labels[row];
-    if (r.label == g.ignore_index || r.label < 0 || r.label >= g.vocab) r.label = -1;
-  }
-  r.has_label = r.label >= 0;
-  r.has_teacher = __syncthreads_or(found);
-  r.q_max = r.q_total = 0.f;
-  if (r.has_teacher) {
-    r.q_max = block_max(t_max, red);
-    float part = 0.f;
+  int mine = 0;
+  found = __any_sync(0xffffffffu, found);
+  if (found) {
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) part += r.at[i] >= 0 ? expf(r.t[i] - r.q_max) : 0.f;
-    r.q_total = block_sum(part, red);
-  }
-  return r;
-}
-
-// The row's loss from its sums; every thread of the block takes part, thread 0 has it.
-__device__ __forceinline__ float row_loss(const DistillArgs &g, const Targets &r, const RowStats &st, const float (&s)[kPerThread],
-                                          float s_label, float *red) {
-  float loss = 0.f;
-  if (r.has_teacher) {
-    const float log_total = logf(r.q_total), log_s = logf(st.s_t);
-    float part = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      if (r.at[i] >= 0) {
-        const float log_q = r.t[i] - r.q_max - log_total, q = expf(log_q);
-        if (q != 0.f) part += q * (log_q - ((s[i] - st.m) * g.inv_temperature - log_s));
+    for (int o = 16; o > 0; o >>= 1) t_max = fmaxf(t_max, __shfl_xor_sync(0xffffffffu, t_max, o));
+    float total = 0.f, from = -INFINITY;
+    for (int k = lane; k < padded; k += 32) {
+      if (table.at[k] >= 0) {
+        total += expf(table.q[k] - t_max);
+        if (for_loss) from = fmaxf(from, to_f32<T>(x[table.at[k]]));
       }
     }
-    loss = g.kl_weight * block_sum(part, red);
+    total = warp_sum(total);
+    if (for_loss) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) from = fmaxf(from, __shfl_xor_sync(0xffffffffu, from, o));
+      if (from == -INFINITY) from = 0.f;
+    }
+    const float log_total = logf(total);
+    for (int k = lane; k < padded; k += 32) {
+      const int at = table.at[k];
+      float q = 0.f;
+      if (at >= 0) {
+        const float log_q = table.q[k] - t_max - log_total;
+        q = expf(log_q);
+        if (for_loss && q != 0.f) {
+          parts.entropy += q * log_q;
+          parts.cross += q * ((to_f32<T>(x[at]) - from) * g.inv_temperature);
+        }
+      }
+      table.q[k] = q;
+      const bool here = at >= e0 && at < e1;
+      const uint32_t all = __ballot_sync(0xffffffffu, here);
+      if (here) table.mine[mine + __popc(all & ((1u << lane) - 1u))] = static_cast<uint16_t>(k);
+      mine += __popc(all);
+    }
+    parts.entropy = warp_sum(parts.entropy);
+    parts.cross = warp_sum(parts.cross);
+    parts.from = from;
   }
-  if (r.has_label) loss += g.ce_weight * (logf(st.s_1) - (s_label - st.m));
-  return loss;
+  if (lane == 0) {
+    table.count = mine;
+    table.padded = found ? padded : 0;
+    table.label = static_cast<int>(label);
+  }
+  return parts;
 }
 
-// The gradient of one row's elements [e0, e1), of which `source` gives any as f32 (and vectors of the
-// input grid where input and output are aligned alike): dense, then the targets' own entries over it.
 struct GradScale {
   float base_t, base_1;  // scale (1 - w) T and scale w, 0 without such a target
   float c_t, c_1;        // the same over the sums
 };
-__device__ __forceinline__ GradScale grad_scale(const DistillArgs &g, const Targets &r, int64_t row, float inv_t, float inv_1) {
+__device__ __forceinline__ GradScale grad_scale(const DistillArgs &g, bool has_teacher, bool has_label, int64_t row,
+                                                float inv_t, float inv_1) {
   float scale = g.row_scale != nullptr ? g.row_scale[g.scale_per_row ? row : 0] : 1.f;
   if (g.count != nullptr) scale /= fmaxf(*g.count, 1.f);
   GradScale c;
-  c.base_t = r.has_teacher ? scale * g.kl_grad_weight : 0.f;
-  c.base_1 = r.has_label ? scale * g.ce_weight : 0.f;
-  c.c_t = r.has_teacher ? c.base_t * inv_t : 0.f;
-  c.c_1 = r.has_label ? c.base_1 * inv_1 : 0.f;
+  c.base_t = has_teacher ? scale * g.kl_grad_weight : 0.f;
+  c.base_1 = has_label ? scale * g.ce_weight : 0.f;
+  c.c_t = has_teacher ? c.base_t * inv_t : 0.f;
+  c.c_1 = has_label ? c.base_1 * inv_1 : 0.f;
   return c;
 }
 template <int EXPS>
@@ -326,65 +330,71 @@ __device__ __forceinline__ float2 dense2(float2 v, float m, float k_t, const Gra
   const float2 u = mul2(d, both(kLog2e));
   return fma2(make_float2(exp2_approx(u.x), exp2_approx(u.y)), both(c.c_1), mul2(e, both(c.c_t)));
 }
+// The dense part of the gradient of a row's elements [e0, e1). vec_at gives vectors of the input where
+// it is aligned as the output, element_at any element.
 template <typename T, int EXPS, typename VecAt, typename ElementAt>
 __device__ __forceinline__ void write_dense(T *out, int64_t e0, int64_t e1, bool alike, float m, float k_t,
-                                            const GradScale &c, bool zero, VecAt vec_at, ElementAt element_at) {
-  constexpr int kN = Vec<T>::kN;
+                                            const GradScale &c, VecAt vec_at, ElementAt element_at) {
+  constexpr int kN = Vec<T>::kN, kAhead = 4;
   const int tid = threadIdx.x;
   const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out + e0) & 15u);
   const int64_t head = min64(e1 - e0, off == 0 ? 0 : (16 - off) / int64_t(sizeof(T)));
-  const int64_t body = (e1 - e0 - head) / kN, tail = e0 + head + body * kN;
-  auto one = [&](int64_t e) -> T {
-    return zero ? from_f32<T>(0.f) : from_f32<T>(dense2<EXPS>(both(element_at(e)), m, k_t, c).x);
+  const int64_t start = e0 + head, tail = start + (e1 - start) / kN * kN;
+  const int body = static_cast<int>((tail - start) / kN);
+  auto one = [&](int64_t e) { out[e] = from_f32<T>(dense2<EXPS>(both(element_at(e)), m, k_t, c).x); };
+  auto put = [&](int i, float2 (&v)[kN / 2]) {
+#pragma unroll
+    for (int j = 0; j < kN / 2; ++j) v[j] = dense2<EXPS>(v[j], m, k_t, c);
+    __stcs(reinterpret_cast<uint4 *>(out + start) + i, Vec<T>::pack(v));
   };
-  if (tid < head) out[e0 + tid] = one(e0 + tid);
-#pragma unroll 4
-  for (int64_t i = tid; i < body; i += kThreads) {
-    const int64_t e = e0 + head + i * kN;
-    float2 v[kN / 2];
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (!zero) {
-      if (alike) {
-        Vec<T>::unpack(vec_at(e), v);
-      } else {
+  if (tid < head) one(e0 + tid);
+  if (alike) {
+    int i = tid;
+    for (; i + (kAhead - 1) * kThreads < body; i += kAhead * kThreads) {
+      uint4 q[kAhead];
 #pragma unroll
-        for (int j = 0; j < kN / 2; ++j) v[j] = make_float2(element_at(e + 2 * j), element_at(e + 2 * j + 1));
+      for (int n = 0; n < kAhead; ++n) q[n] = vec_at(start, i + n * kThreads);
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        float2 v[kN / 2];
+        Vec<T>::unpack(q[n], v);
+        put(i + n * kThreads, v);
       }
-#pragma unroll
-      for (int j = 0; j < kN / 2; ++j) v[j] = dense2<EXPS>(v[j], m, k_t, c);
-      w = Vec<T>::pack(v);
     }
-    __stcs(reinterpret_cast<uint4 *>(out + e), w);
+    for (; i < body; i += kThreads) {
+      float2 v[kN / 2];
+      Vec<T>::unpack(vec_at(start, i), v);
+      put(i, v);
+    }
+  } else {
+    for (int i = tid; i < body; i += kThreads) {
+      float2 v[kN / 2];
+#pragma unroll
+      for (int j = 0; j < kN / 2; ++j) {
+        const int64_t e = start + int64_t(i) * kN + 2 * j;
+        v[j] = make_float2(element_at(e), element_at(e + 1));
+      }
+      put(i, v);
+    }
   }
-  if (tail + tid < e1) out[tail + tid] = one(tail + tid);
+  if (tail + tid < e1) one(tail + tid);
 }
-// The teacher's entries of a row, and those of them in a CTA's part.
-struct EntryTable {
-  alignas(16) int at[kMaxTop];
-  alignas(16) float q[kMaxTop];
-  uint16_t mine[kMaxTop];  // entry numbers
-  int count;
-};
-// The targets in [e0, e1): p minus all that the teacher's entries of that index and the label put
-// there, rounded once. After write_dense; every thread takes part.
+template <typename T>
+__device__ __forceinline__ void write_zeros(T *out, int64_t e0, int64_t e1) {
+  constexpr int kN = Vec<T>::kN;
+  const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out + e0) & 15u);
+  const int64_t head = min64(e1 - e0, off == 0 ? 0 : (16 - off) / int64_t(sizeof(T)));
+  const int64_t start = e0 + head, tail = start + (e1 - start) / kN * kN;
+  if (int64_t(threadIdx.x) < head) out[e0 + threadIdx.x] = from_f32<T>(0.f);
+  for (int64_t e = start + threadIdx.x * kN; e < tail; e += kThreads * kN) __stcs(reinterpret_cast<uint4 *>(out + e), make_uint4(0, 0, 0, 0));
+  if (tail + threadIdx.x < e1) out[tail + threadIdx.x] = from_f32<T>(0.f);
+}
+// The targets of the part over it: p minus all that the teacher's entries of that index and the label
+// put there, rounded once. After a barrier that follows write_dense; every thread takes part.
 template <typename T, int EXPS, typename ElementAt>
-__device__ __forceinline__ void write_targets(const DistillArgs &g, const Targets &r, T *out, int64_t e0, int64_t e1, float m,
-                                              const GradScale &c, EntryTable &table, ElementAt element_at) {
-  const int tid = threadIdx.x;
-  const float inv_total = r.has_teacher ? 1.f / r.q_total : 0.f;
-  const int padded = r.has_teacher ? (g.top + 3) & ~3 : 0;
-  if (tid == 0) table.count = 0;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    const int k = tid + i * kThreads;
-    if (k < padded) {
-      table.at[k] = r.at[i];
-      table.q[k] = r.at[i] >= 0 ? expf(r.t[i] - r.q_max) * inv_total : 0.f;
-      if (r.at[i] >= e0 && r.at[i] < e1) table.mine[atomicAdd(&table.count, 1)] = static_cast<uint16_t>(k);
-    }
-  }
-  __syncthreads();
+__device__ __forceinline__ void write_targets(T *out, int64_t e0, int64_t e1, float m, float k_t, const GradScale &c,
+                                              const EntryTable &table, ElementAt element_at) {
+  const int tid = threadIdx.x, padded = table.padded, label = table.label;
   auto sum_at = [&](int e, bool &found) -> float {  // in the entries' order
     float q = 0.f;
     for (int k = 0; k < padded; k += 4) {
@@ -398,19 +408,19 @@ __device__ __forceinline__ void write_targets(const DistillArgs &g, const Target
     }
     return q;
   };
-  auto put = [&](int64_t e, float q) {
-    const float p = dense2<EXPS>(both(element_at(e)), m, g.k_t, c).x;
-    out[e] = from_f32<T>(p - c.base_t * q - (e == r.label ? c.base_1 : 0.f));
+  auto put = [&](int e, float q) {
+    const float p = dense2<EXPS>(both(element_at(e)), m, k_t, c).x;
+    out[e] = from_f32<T>(p - c.base_t * q - (e == label ? c.base_1 : 0.f));
   };
   bool found = false;
   for (int i = tid; i < table.count; i += kThreads) {
     const int e = table.at[table.mine[i]];
     put(e, sum_at(e, found));  // entries of one index write the same value
   }
-  if (tid == kThreads - 1 && r.label >= e0 && r.label < e1) {
+  if (tid == kThreads - 1 && label >= e0 && label < e1) {
     found = false;
-    const float q = sum_at(static_cast<int>(r.label), found);
-    if (!found) put(r.label, q);
+    const float q = sum_at(label, found);
+    if (!found) put(label, q);
   }
 }
 
@@ -420,7 +430,6 @@ template <typename T, int MODE, int EXPS, bool RESIDENT>
 __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel(const DistillArgs g) {
   constexpr int kN = Vec<T>::kN;
   extern __shared__ __align__(128) uint8_t dynamic[];
-  __shared__ float red[kWarps];
   __shared__ RowStats of_warp[kWarps], of_rank[kMaxCluster];
   __shared__ EntryTable table;
   __shared__ uint64_t full[kChunks];
@@ -434,6 +443,7 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
   const T *grid = x - lead;
   const int64_t vec0 = int64_t(rank) * g.slice_vecs;
   const int vecs = static_cast<int>(min64(g.slice_vecs, max(int64_t(0), (end + kN - 1) / kN - vec0)));
+  const int64_t e0 = max(int64_t(0), vec0 * kN - lead), e1 = max(e0, min64(g.vocab, (vec0 + vecs) * kN - lead));
   if (g.ranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
   // Whole vectors of the slice come as bulk copies; one at either end of the row may be cut.
@@ -456,33 +466,27 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
         }
       }
     }
-    if (tid == 32 && first_cut && vecs > 0) slice[0] = load_vec<T>(grid, vec0, lead, end);
-    if (tid == 64 && last_cut && vecs > whole0) slice[vecs - 1] = load_vec<T>(grid, vec0 + vecs - 1, lead, end);
+    __syncthreads();  // the barriers are set up
   }
-  const Targets r = load_targets(g, row, red);
-  const bool wanted = r.has_teacher || r.has_label;
-  float s[kPerThread] = {}, s_label = 0.f;
-  if (rank == 0) {  // the targets' logits for the loss
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i)
-      if (r.at[i] >= 0) s[i] = to_f32<T>(x[r.at[i]]);
-    if (r.has_label) s_label = to_f32<T>(x[r.label]);
-  }
+  LossParts parts = {};
+  if (warp == 0) parts = load_targets<T>(g, row, x, e0, e1, rank == 0, table);
 
-  // One order of summation for all three kernels: cut vectors first, then chunk by chunk. (load_targets'
-  // barriers put the setup of the copies and the cut vectors before this.)
+  // One order of summation for all kernels: cut vectors first, then chunk by chunk. A row without a
+  // target is summed up too, and nothing made of it.
   auto at = [&](int v) -> uint4 {
     if constexpr (RESIDENT) return slice[v];
     else return load_vec<T>(grid, vec0 + v, lead, end);
   };
   Online o;
-  if (wanted && tid == 0) {
+  if (tid == kThreads - 1) {
     if (first_cut && vecs > 0) {
-      const uint4 q[1] = {at(0)};
+      const uint4 q[1] = {load_vec<T>(grid, vec0, lead, end)};
+      if (RESIDENT) slice[0] = q[0];
       take<T, EXPS>(o, q, g.k_t);
     }
     if (last_cut && vecs > whole0) {
-      const uint4 q[1] = {at(vecs - 1)};
+      const uint4 q[1] = {load_vec<T>(grid, vec0 + vecs - 1, lead, end)};
+      if (RESIDENT) slice[vecs - 1] = q[0];
       take<T, EXPS>(o, q, g.k_t);
     }
   }
@@ -490,7 +494,6 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
     const int from = min(whole0 + c * per_chunk, whole1), to = min(from + per_chunk, whole1);
     if (to <= from) break;
     if (RESIDENT) sm100::mbar_wait(&full[c], 0, &abort, &g_distill_error);
-    if (!wanted) continue;
     int v = from + tid;
     for (; v + 3 * kThreads < to; v += 4 * kThreads) {
       uint4 q[4];
@@ -516,28 +519,35 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
     st = joined<EXPS, kMaxCluster>(lane % kMaxCluster < g.ranks ? of_rank[lane % kMaxCluster] : none, g.k_t);
   }
   const float inv_t = 1.f / st.s_t, inv_1 = 1.f / st.s_1;
+  const bool has_teacher = table.padded > 0, has_label = table.label >= 0;
   if constexpr (MODE == kFused) {
     T *out = static_cast<T *>(g.grad) + row * g.vocab;
-    const int64_t e0 = max(int64_t(0), vec0 * kN - lead), e1 = min64(g.vocab, (vec0 + vecs) * kN - lead);
-    const GradScale c = grad_scale(g, r, row, inv_t, inv_1);
-    const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
-    auto vec_at = [&](int64_t e) -> uint4 {
-      if constexpr (RESIDENT) return slice[(e + lead) / kN - vec0];
-      else return __ldg(reinterpret_cast<const uint4 *>(x + e));
-    };
-    auto element_at = [&](int64_t e) -> float {
-      if constexpr (RESIDENT) return to_f32<T>(reinterpret_cast<const T *>(slice)[e + lead - vec0 * kN]);
-      else return ldg_f32(x + e);
-    };
-    if (e1 > e0) write_dense<T, EXPS>(out, e0, e1, alike, st.m, g.k_t, c, !wanted, vec_at, element_at);
-    if (wanted) write_targets<T, EXPS>(g, r, out, e0, e1, st.m, c, table, element_at);
-  }
-  if (rank == 0) {
-    const float loss = wanted ? row_loss(g, r, st, s, s_label, red) : 0.f;
-    if (tid == 0) {
-      g.losses[row] = loss;
-      if (MODE == kLoss && g.stats != nullptr) g.stats[row] = wanted ? make_float4(st.m, inv_t, inv_1, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (has_teacher || has_label) {
+      const GradScale c = grad_scale(g, has_teacher, has_label, row, inv_t, inv_1);
+      const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
+      auto vec_at = [&](int64_t start, int i) -> uint4 {
+        if constexpr (RESIDENT) return slice[static_cast<int>((start + lead) / kN - vec0) + i];
+        else return __ldg(reinterpret_cast<const uint4 *>(x + start) + i);
+      };
+      auto element_at = [&](int64_t e) -> float {
+        if constexpr (RESIDENT) return to_f32<T>(reinterpret_cast<const T *>(slice)[e + lead - vec0 * kN]);
+        else return ldg_f32(x + e);
+      };
+      write_dense<T, EXPS>(out, e0, e1, alike, st.m, g.k_t, c, vec_at, element_at);
+      __syncthreads();
+      write_targets<T, EXPS>(out, e0, e1, st.m, g.k_t, c, table, element_at);
+    } else {
+      write_zeros<T>(out, e0, e1);
     }
+  }
+  if (rank == 0 && tid == 0) {
+    float loss = 0.f;
+    if (has_teacher)
+      loss = g.kl_weight * (parts.entropy - parts.cross - ((parts.from - st.m) * g.inv_temperature - logf(st.s_t)));
+    if (has_label) loss += g.ce_weight * (logf(st.s_1) - (parts.s_label - st.m));
+    g.losses[row] = loss;
+    if (MODE == kLoss && g.stats != nullptr)
+      g.stats[row] = make_float4(st.m, inv_t, inv_1, static_cast<float>((has_teacher ? 1 : 0) + (has_label ? 2 : 0)));
   }
 }
 
@@ -545,23 +555,28 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
 template <typename T, int EXPS>
 __global__ void __launch_bounds__(kThreads, 4) distill_grad_kernel(const DistillArgs g) {
   constexpr int kN = Vec<T>::kN;
-  __shared__ float red[kWarps];
   __shared__ EntryTable table;
   const int64_t row = blockIdx.x / g.ranks, part = blockIdx.x % g.ranks;
   const T *x = static_cast<const T *>(g.logits) + (row / g.inner) * g.outer_stride + (row % g.inner) * g.inner_stride;
   T *out = static_cast<T *>(g.grad) + row * g.vocab;
-  const Targets r = load_targets(g, row, red);
   const float4 st = g.stats[row];
-  const GradScale c = grad_scale(g, r, row, st.y, st.z);
+  const int has = static_cast<int>(st.w);
   // Parts end on the output's 16-byte grid.
   const int64_t lead = static_cast<int64_t>((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T));
-  const int64_t e0 = max(int64_t(0), part * g.slice_vecs * kN - lead), e1 = min64(g.vocab, (part + 1) * g.slice_vecs * kN - lead);
+  const int64_t e0 = max(int64_t(0), part * g.slice_vecs * kN - lead);
+  const int64_t e1 = max(e0, min64(g.vocab, (part + 1) * g.slice_vecs * kN - lead));
+  if (has == 0) {
+    write_zeros<T>(out, e0, e1);
+    return;
+  }
+  if (threadIdx.x < 32) load_targets<T>(g, row, x, e0, e1, false, table);
+  const GradScale c = grad_scale(g, (has & 1) != 0, (has & 2) != 0, row, st.y, st.z);
   const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
-  auto vec_at = [&](int64_t e) -> uint4 { return __ldg(reinterpret_cast<const uint4 *>(x + e)); };
+  auto vec_at = [&](int64_t start, int i) -> uint4 { return __ldg(reinterpret_cast<const uint4 *>(x + start) + i); };
   auto element_at = [&](int64_t e) -> float { return ldg_f32(x + e); };
-  const bool wanted = r.has_teacher || r.has_label;
-  if (e1 > e0) write_dense<T, EXPS>(out, e0, e1, alike, st.x, g.k_t, c, !wanted, vec_at, element_at);
-  if (wanted) write_targets<T, EXPS>(g, r, out, e0, e1, st.x, c, table, element_at);
+  write_dense<T, EXPS>(out, e0, e1, alike, st.x, g.k_t, c, vec_at, element_at);
+  __syncthreads();
+  write_targets<T, EXPS>(out, e0, e1, st.x, g.k_t, c, table, element_at);
 }
 
 // losses summed in a fixed order; *count = rows with a target; *loss = sum, or sum / max(count, 1).
@@ -571,7 +586,7 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float *losse
   float s = 0.f, c = 0.f;
   for (int64_t i = threadIdx.x; i < rows; i += 1024) {
     s += losses[i];
-    c += stats[i].w;  // whole numbers: exact below 2^24 rows a thread
+    c += stats[i].w > 0.f ? 1.f : 0.f;  // whole numbers: exact below 2^24 rows a thread
   }
   s = warp_sum(s);
   c = warp_sum(c);
