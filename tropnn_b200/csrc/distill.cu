@@ -32,6 +32,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
 constexpr int kChunks = 4;  // bulk copies of a slice
+constexpr int kBatch = 4 * kThreads;  // vectors that the block takes at once
 constexpr int64_t kSliceShared = 64 * 1024 + 64;  // bytes of a row a CTA: three CTAs on an SM
 constexpr int64_t kSliceMost = 200 * 1024;        // one CTA on an SM
 constexpr float kLog2e = 1.4426950408889634f;
@@ -135,6 +136,12 @@ __device__ __forceinline__ __half lowest_logit<__half>() { return __ushort_as_ha
 template <>
 __device__ __forceinline__ __nv_bfloat16 lowest_logit<__nv_bfloat16>() { return __ushort_as_bfloat16(0xFF80); }
 
+template <typename T>
+__device__ __forceinline__ uint4 nothing_vec() {  // -inf throughout
+  const uint32_t w = std::is_same<T, float>::value ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+  return make_uint4(w, w, w, w);
+}
+
 // Vector v of the row's 16-byte grid, which starts at or before the row; elements outside the row are
 // -inf (which adds nothing to a sum) and never read.
 template <typename T>
@@ -212,98 +219,129 @@ __device__ __forceinline__ RowStats joined(RowStats a, float k_t) {
   return a;
 }
 
-// The teacher's entries of a row with their shares, and those of them in a CTA's part of the row.
-struct EntryTable {
-  alignas(16) int at[kMaxTop];  // -1: none
-  alignas(16) float q[kMaxTop];
-  uint16_t mine[kMaxTop];  // entry numbers
-  int count;               // of mine
-  int padded;              // entries, up to a multiple of four; 0: no teacher
-  int label;               // -1: none
+// A row's targets. Warp w reads the teacher's entries [128 w, 128 w + 128) while other warps are at the
+// row itself; after the barrier that the row's sums take anyway, each thread has the parts at hand.
+constexpr int kEntriesPerWarp = kMaxTop / kWarps, kEntriesPerLane = kEntriesPerWarp / 32;
+struct TeacherPart {
+  float t_max, total;         // sum of e = exp(t - t_max), t = teacher logit / T
+  float entropy, cross, from; // sums of e (t - t_max) and of e (s - from) / T
+  int count;                  // of its entries in the CTA's part of the row
 };
-// What the loss needs of the targets beside the row's sums.
-struct LossParts {
-  float entropy, cross, from, s_label;  // sum q log q, sum q (s - from) / T
+struct EntryTable {
+  alignas(16) int at[kMaxTop];   // -1: none
+  alignas(16) float q[kMaxTop];  // t, later its share exp(t - t_max) / total
+  uint16_t mine[kMaxTop];        // numbers of the entries in the CTA's part, a stretch a warp
+  TeacherPart part[kWarps];
+  int label;  // -1: none
+  float s_label;
 };
 
-// One warp reads the row's targets and fills the table, while the others are at the row itself.
 template <typename T>
-__device__ __forceinline__ LossParts load_targets(const DistillArgs &g, int64_t row, const T *x, int64_t e0, int64_t e1,
-                                                  bool for_loss, EntryTable &table) {
-  const int lane = threadIdx.x & 31;
-  LossParts parts = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ void load_targets(const DistillArgs &g, int64_t row, const T *x, int64_t e0, int64_t e1,
+                                             bool for_loss, EntryTable &table) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int top = g.kl_weight != 0.f ? g.top : 0, base = warp * kEntriesPerWarp;
+  if (base >= max(top, 1)) return;
   int64_t label = -1;
-  if (g.labels != nullptr && g.ce_weight != 0.f) {
-    label = g.labels[row];
-    if (label == g.ignore_index || label < 0 || label >= g.vocab) label = -1;
-    if (for_loss && label >= 0) parts.s_label = to_f32<T>(x[label]);
-  }
-  const int top = g.kl_weight != 0.f ? g.top : 0, padded = (top + 31) & ~31;
-  float t_max = kLowest;
-  bool found = false;
-#pragma unroll 4
-  for (int k = lane; k < padded; k += 32) {
-    int at = -1;
-    float t = 0.f;
+  if (warp == 0 && g.labels != nullptr && g.ce_weight != 0.f) label = g.labels[row];
+  int64_t at[kEntriesPerLane];
+  float t[kEntriesPerLane], s[kEntriesPerLane];
+#pragma unroll
+  for (int i = 0; i < kEntriesPerLane; ++i) {
+    const int k = base + i * 32 + lane;
+    at[i] = -1;
+    t[i] = 0.f;
     if (k < top) {
-      const int64_t v = load_index(g.indices, g.index_dtype, row * g.top + k);
-      const float tv = load_float(g.teacher, g.teacher_dtype, row * g.top + k);
-      if (v >= 0 && v < g.vocab && tv != -INFINITY) {
-        at = static_cast<int>(v);
-        t = tv * g.inv_temperature;
-        t_max = fmaxf(t_max, t);
-        found = true;
-      }
+      at[i] = load_index(g.indices, g.index_dtype, row * g.top + k);
+      t[i] = load_float(g.teacher, g.teacher_dtype, row * g.top + k);
     }
-    table.at[k] = at;
-    table.q[k] = t;
   }
-  int mine = 0;
-  found = __any_sync(0xffffffffu, found);
-  if (found) {
+  if (label == g.ignore_index || label < 0 || label >= g.vocab) label = -1;
+  float s_label = 0.f;
+  if (for_loss && label >= 0) s_label = to_f32<T>(x[label]);
+  TeacherPart p = {kLowest, 0.f, 0.f, 0.f, -INFINITY, 0};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t_max = fmaxf(t_max, __shfl_xor_sync(0xffffffffu, t_max, o));
-    float total = 0.f, from = -INFINITY;
-    for (int k = lane; k < padded; k += 32) {
-      if (table.at[k] >= 0) {
-        total += expf(table.q[k] - t_max);
-        if (for_loss) from = fmaxf(from, to_f32<T>(x[table.at[k]]));
-      }
+  for (int i = 0; i < kEntriesPerLane; ++i) {
+    s[i] = -INFINITY;
+    if (at[i] < 0 || at[i] >= g.vocab || t[i] == -INFINITY) at[i] = -1;
+    if (at[i] >= 0) {
+      t[i] *= g.inv_temperature;
+      p.t_max = fmaxf(p.t_max, t[i]);
+      if (for_loss) s[i] = to_f32<T>(x[at[i]]);
     }
-    total = warp_sum(total);
-    if (for_loss) {
+  }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) from = fmaxf(from, __shfl_xor_sync(0xffffffffu, from, o));
-      if (from == -INFINITY) from = 0.f;
-    }
-    const float log_total = logf(total);
-    for (int k = lane; k < padded; k += 32) {
-      const int at = table.at[k];
-      float q = 0.f;
-      if (at >= 0) {
-        const float log_q = table.q[k] - t_max - log_total;
-        q = expf(log_q);
-        if (for_loss && q != 0.f) {
-          parts.entropy += q * log_q;
-          parts.cross += q * ((to_f32<T>(x[at]) - from) * g.inv_temperature);
-        }
-      }
-      table.q[k] = q;
-      const bool here = at >= e0 && at < e1;
+  for (int i = 0; i < kEntriesPerLane; ++i) {
+    const int k = base + i * 32 + lane;
+    if (base + i * 32 < top) {
+      table.at[k] = static_cast<int>(at[i]);
+      table.q[k] = t[i];
+      const bool here = at[i] >= e0 && at[i] < e1;
       const uint32_t all = __ballot_sync(0xffffffffu, here);
-      if (here) table.mine[mine + __popc(all & ((1u << lane) - 1u))] = static_cast<uint16_t>(k);
-      mine += __popc(all);
+      if (here) table.mine[base + p.count + __popc(all & ((1u << lane) - 1u))] = static_cast<uint16_t>(k);
+      p.count += __popc(all);
     }
-    parts.entropy = warp_sum(parts.entropy);
-    parts.cross = warp_sum(parts.cross);
-    parts.from = from;
+    p.from = fmaxf(p.from, s[i]);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    p.t_max = fmaxf(p.t_max, __shfl_xor_sync(0xffffffffu, p.t_max, o));
+    p.from = fmaxf(p.from, __shfl_xor_sync(0xffffffffu, p.from, o));
+  }
+  if (p.from == -INFINITY) p.from = 0.f;
+#pragma unroll
+  for (int i = 0; i < kEntriesPerLane; ++i) {
+    if (at[i] >= 0) {
+      const float d = t[i] - p.t_max, e = expf(d);
+      p.total += e;
+      if (e != 0.f) {
+        p.entropy += e * d;
+        p.cross += e * ((s[i] - p.from) * g.inv_temperature);
+      }
+    }
+  }
+  p.total = warp_sum(p.total);
+  p.entropy = warp_sum(p.entropy);
+  p.cross = warp_sum(p.cross);
   if (lane == 0) {
-    table.count = mine;
-    table.padded = found ? padded : 0;
-    table.label = static_cast<int>(label);
+    table.part[warp] = p;
+    if (warp == 0) {
+      table.label = static_cast<int>(label);
+      table.s_label = s_label;
+    }
   }
-  return parts;
+}
+// The parts together, after a barrier.
+struct Teacher {
+  int parts;  // 0: no entries
+  float t_max, total;
+  __device__ __forceinline__ Teacher(const DistillArgs &g, const EntryTable &table) {
+    parts = g.kl_weight != 0.f ? (g.top + kEntriesPerWarp - 1) / kEntriesPerWarp : 0;
+    t_max = kLowest;
+    total = 0.f;
+    for (int w = 0; w < parts; ++w) t_max = fmaxf(t_max, table.part[w].t_max);
+    for (int w = 0; w < parts; ++w) total += table.part[w].total * expf(table.part[w].t_max - t_max);
+    if (total == 0.f) parts = 0;  // NaN stays
+  }
+};
+__device__ __forceinline__ float teacher_loss(const DistillArgs &g, const EntryTable &table, const Teacher &teacher, float m,
+                                              float s_t) {
+  float entropy = 0.f, cross = 0.f;
+  for (int w = 0; w < teacher.parts; ++w) {
+    const TeacherPart &p = table.part[w];
+    const float f = expf(p.t_max - teacher.t_max);
+    if (p.total == 0.f) continue;
+    entropy += f * (p.entropy + p.total * (p.t_max - teacher.t_max));
+    cross += f * (p.cross + p.total * ((p.from - m) * g.inv_temperature));
+  }
+  return (entropy - cross) / teacher.total - logf(teacher.total) + logf(s_t);
+}
+// Entries become shares, all threads; a barrier has to follow.
+__device__ __forceinline__ void form_shares(const DistillArgs &g, const Teacher &teacher, EntryTable &table) {
+  if (teacher.parts == 0) return;
+  const float inv_total = 1.f / teacher.total;
+  for (int k = threadIdx.x; k < (g.top + 31 & ~31); k += kThreads)
+    table.q[k] = table.at[k] >= 0 ? expf(table.q[k] - teacher.t_max) * inv_total : 0.f;
 }
 
 struct GradScale {
@@ -390,11 +428,12 @@ __device__ __forceinline__ void write_zeros(T *out, int64_t e0, int64_t e1) {
   if (tail + threadIdx.x < e1) out[tail + threadIdx.x] = from_f32<T>(0.f);
 }
 // The targets of the part over it: p minus all that the teacher's entries of that index and the label
-// put there, rounded once. After a barrier that follows write_dense; every thread takes part.
+// put there, rounded once. After a barrier that follows write_dense and form_shares; every thread takes
+// part.
 template <typename T, int EXPS, typename ElementAt>
-__device__ __forceinline__ void write_targets(T *out, int64_t e0, int64_t e1, float m, float k_t, const GradScale &c,
-                                              const EntryTable &table, ElementAt element_at) {
-  const int tid = threadIdx.x, padded = table.padded, label = table.label;
+__device__ __forceinline__ void write_targets(const DistillArgs &g, T *out, int64_t e0, int64_t e1, float m, const GradScale &c,
+                                              const EntryTable &table, int parts, ElementAt element_at) {
+  const int tid = threadIdx.x, padded = parts > 0 ? g.top + 3 & ~3 : 0, label = table.label;
   auto sum_at = [&](int e, bool &found) -> float {  // in the entries' order
     float q = 0.f;
     for (int k = 0; k < padded; k += 4) {
@@ -409,13 +448,19 @@ __device__ __forceinline__ void write_targets(T *out, int64_t e0, int64_t e1, fl
     return q;
   };
   auto put = [&](int e, float q) {
-    const float p = dense2<EXPS>(both(element_at(e)), m, k_t, c).x;
+    const float p = dense2<EXPS>(both(element_at(e)), m, g.k_t, c).x;
     out[e] = from_f32<T>(p - c.base_t * q - (e == label ? c.base_1 : 0.f));
   };
   bool found = false;
-  for (int i = tid; i < table.count; i += kThreads) {
-    const int e = table.at[table.mine[i]];
-    put(e, sum_at(e, found));  // entries of one index write the same value
+  // The warps' stretches of entries are spread over the block one after the other.
+  int before = 0;
+  for (int w = 0; w < parts; ++w) {
+    const int count = table.part[w].count;
+    for (int i = (tid - before) & (kThreads - 1); i < count; i += kThreads) {
+      const int e = table.at[table.mine[w * kEntriesPerWarp + i]];
+      put(e, sum_at(e, found));  // entries of one index write the same value
+    }
+    before += count;
   }
   if (tid == kThreads - 1 && label >= e0 && label < e1) {
     found = false;
@@ -449,7 +494,8 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
   // Whole vectors of the slice come as bulk copies; one at either end of the row may be cut.
   const bool first_cut = vec0 == 0 && lead > 0, last_cut = vec0 + vecs == (end + kN - 1) / kN && end % kN != 0;
   const int whole0 = first_cut ? 1 : 0, whole1 = max(vecs - (last_cut ? 1 : 0), whole0);
-  const int per_chunk = (whole1 - whole0 + kChunks - 1) / kChunks;
+  // Chunks are whole batches of the block, so that kernels with and without them sum up alike.
+  const int per_chunk = (whole1 - whole0 + kChunks * kBatch - 1) / (kChunks * kBatch) * kBatch;
   if (RESIDENT) {
     if (tid == 0) {
       abort = 0;
@@ -468,15 +514,10 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
     }
     __syncthreads();  // the barriers are set up
   }
-  LossParts parts = {};
-  if (warp == 0) parts = load_targets<T>(g, row, x, e0, e1, rank == 0, table);
+  load_targets<T>(g, row, x, e0, e1, rank == 0, table);
 
-  // One order of summation for all kernels: cut vectors first, then chunk by chunk. A row without a
+  // One order of summation for all kernels: cut vectors first, then batch by batch. A row without a
   // target is summed up too, and nothing made of it.
-  auto at = [&](int v) -> uint4 {
-    if constexpr (RESIDENT) return slice[v];
-    else return load_vec<T>(grid, vec0 + v, lead, end);
-  };
   Online o;
   if (tid == kThreads - 1) {
     if (first_cut && vecs > 0) {
@@ -490,19 +531,18 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
       take<T, EXPS>(o, q, g.k_t);
     }
   }
-  for (int c = 0; c < kChunks; ++c) {
-    const int from = min(whole0 + c * per_chunk, whole1), to = min(from + per_chunk, whole1);
-    if (to <= from) break;
+  const uint4 *whole = RESIDENT ? slice : reinterpret_cast<const uint4 *>(grid) + vec0;
+  const uint4 nothing = nothing_vec<T>();
+  for (int from = whole0, c = 0; from < whole1; from += per_chunk, ++c) {
+    const int to = min(from + per_chunk, whole1);
     if (RESIDENT) sm100::mbar_wait(&full[c], 0, &abort, &g_distill_error);
-    int v = from + tid;
-    for (; v + 3 * kThreads < to; v += 4 * kThreads) {
+    for (int v = from + tid; v < to; v += kBatch) {
       uint4 q[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = RESIDENT ? slice[v + i * kThreads] : __ldg(reinterpret_cast<const uint4 *>(grid + (vec0 + v + i * kThreads) * kN));
-      take<T, EXPS>(o, q, g.k_t);
-    }
-    for (; v < to; v += kThreads) {
-      const uint4 q[1] = {at(v)};
+      for (int i = 0; i < 4; ++i) {
+        q[i] = nothing;
+        if (v + i * kThreads < to) q[i] = RESIDENT ? whole[v + i * kThreads] : __ldg(whole + v + i * kThreads);
+      }
       take<T, EXPS>(o, q, g.k_t);
     }
   }
@@ -519,7 +559,8 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
     st = joined<EXPS, kMaxCluster>(lane % kMaxCluster < g.ranks ? of_rank[lane % kMaxCluster] : none, g.k_t);
   }
   const float inv_t = 1.f / st.s_t, inv_1 = 1.f / st.s_1;
-  const bool has_teacher = table.padded > 0, has_label = table.label >= 0;
+  const Teacher teacher(g, table);
+  const bool has_teacher = teacher.parts > 0, has_label = table.label >= 0;
   if constexpr (MODE == kFused) {
     T *out = static_cast<T *>(g.grad) + row * g.vocab;
     if (has_teacher || has_label) {
@@ -533,18 +574,18 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
         if constexpr (RESIDENT) return to_f32<T>(reinterpret_cast<const T *>(slice)[e + lead - vec0 * kN]);
         else return ldg_f32(x + e);
       };
+      form_shares(g, teacher, table);
       write_dense<T, EXPS>(out, e0, e1, alike, st.m, g.k_t, c, vec_at, element_at);
       __syncthreads();
-      write_targets<T, EXPS>(out, e0, e1, st.m, g.k_t, c, table, element_at);
+      write_targets<T, EXPS>(g, out, e0, e1, st.m, c, table, teacher.parts, element_at);
     } else {
       write_zeros<T>(out, e0, e1);
     }
   }
   if (rank == 0 && tid == 0) {
     float loss = 0.f;
-    if (has_teacher)
-      loss = g.kl_weight * (parts.entropy - parts.cross - ((parts.from - st.m) * g.inv_temperature - logf(st.s_t)));
-    if (has_label) loss += g.ce_weight * (logf(st.s_1) - (parts.s_label - st.m));
+    if (has_teacher) loss = g.kl_weight * teacher_loss(g, table, teacher, st.m, st.s_t);
+    if (has_label) loss += g.ce_weight * (logf(st.s_1) - (table.s_label - st.m));
     g.losses[row] = loss;
     if (MODE == kLoss && g.stats != nullptr)
       g.stats[row] = make_float4(st.m, inv_t, inv_1, static_cast<float>((has_teacher ? 1 : 0) + (has_label ? 2 : 0)));
@@ -569,14 +610,17 @@ __global__ void __launch_bounds__(kThreads, 4) distill_grad_kernel(const Distill
     write_zeros<T>(out, e0, e1);
     return;
   }
-  if (threadIdx.x < 32) load_targets<T>(g, row, x, e0, e1, false, table);
+  load_targets<T>(g, row, x, e0, e1, false, table);
   const GradScale c = grad_scale(g, (has & 1) != 0, (has & 2) != 0, row, st.y, st.z);
   const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
   auto vec_at = [&](int64_t start, int i) -> uint4 { return __ldg(reinterpret_cast<const uint4 *>(x + start) + i); };
   auto element_at = [&](int64_t e) -> float { return ldg_f32(x + e); };
   write_dense<T, EXPS>(out, e0, e1, alike, st.x, g.k_t, c, vec_at, element_at);
   __syncthreads();
-  write_targets<T, EXPS>(out, e0, e1, st.x, g.k_t, c, table, element_at);
+  const Teacher teacher(g, table);
+  form_shares(g, teacher, table);
+  __syncthreads();
+  write_targets<T, EXPS>(g, out, e0, e1, st.x, c, table, teacher.parts, element_at);
 }
 
 // losses summed in a fixed order; *count = rows with a target; *loss = sum, or sum / max(count, 1).
