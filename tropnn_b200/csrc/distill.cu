@@ -27,7 +27,8 @@
 namespace tropnn_b200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // at the row; one more warp is at the targets
+constexpr int kBlock = kThreads + 32;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
@@ -68,6 +69,14 @@ struct DistillArgs {
   int ranks;       // CTAs of a row
   int slice_vecs;  // 16-byte vectors of a CTA's slice
 };
+
+// Rows and `inner` are below 2^31.
+template <typename T>
+__device__ __forceinline__ const T *row_of(const DistillArgs &g, uint32_t row) {
+  if (g.inner == 1) return static_cast<const T *>(g.logits) + row * g.outer_stride;
+  const uint32_t outer = row / static_cast<uint32_t>(g.inner), rest = row - outer * static_cast<uint32_t>(g.inner);
+  return static_cast<const T *>(g.logits) + outer * g.outer_stride + rest * g.inner_stride;
+}
 
 __device__ __forceinline__ float load_float(const void *p, int dtype, int64_t i) {
   if (dtype == TROPNN_B200_F32) return static_cast<const float *>(p)[i];
@@ -219,8 +228,9 @@ __device__ __forceinline__ RowStats joined(RowStats a, float k_t) {
   return a;
 }
 
-// A row's targets. Warp w reads the teacher's entries [128 w, 128 w + 128) while other warps are at the
-// row itself; after the barrier that the row's sums take anyway, each thread has the parts at hand.
+// A row's targets. Up to 128 entries of the teacher are read by a warp of its own while the others are at
+// the row; of more, warp w reads [128 w, 128 w + 128) before its share of the row. After the barrier
+// that the row's sums take anyway, each thread has the parts at hand.
 constexpr int kEntriesPerWarp = kMaxTop / kWarps, kEntriesPerLane = kEntriesPerWarp / 32;
 struct TeacherPart {
   float t_max, total;         // sum of e = exp(t - t_max), t = teacher logit / T
@@ -239,9 +249,11 @@ struct EntryTable {
 template <typename T>
 __device__ __forceinline__ void load_targets(const DistillArgs &g, int64_t row, const T *x, int64_t e0, int64_t e1,
                                              bool for_loss, EntryTable &table) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int top = g.kl_weight != 0.f ? g.top : 0, base = warp * kEntriesPerWarp;
-  if (base >= max(top, 1)) return;
+  const int lane = threadIdx.x & 31;
+  const int top = g.kl_weight != 0.f ? g.top : 0;
+  const int warp = static_cast<int>(threadIdx.x >> 5) - (top <= kEntriesPerWarp ? kWarps : 0);
+  const int base = warp * kEntriesPerWarp;
+  if (warp < 0 || base >= max(top, 1)) return;
   int64_t label = -1;
   if (warp == 0 && g.labels != nullptr && g.ce_weight != 0.f) label = g.labels[row];
   int64_t at[kEntriesPerLane];
@@ -340,7 +352,7 @@ __device__ __forceinline__ float teacher_loss(const DistillArgs &g, const EntryT
 __device__ __forceinline__ void form_shares(const DistillArgs &g, const Teacher &teacher, EntryTable &table) {
   if (teacher.parts == 0) return;
   const float inv_total = 1.f / teacher.total;
-  for (int k = threadIdx.x; k < (g.top + 31 & ~31); k += kThreads)
+  for (int k = threadIdx.x; k < (g.top + 31 & ~31); k += kBlock)
     table.q[k] = table.at[k] >= 0 ? expf(table.q[k] - teacher.t_max) * inv_total : 0.f;
 }
 
@@ -348,10 +360,13 @@ struct GradScale {
   float base_t, base_1;  // scale (1 - w) T and scale w, 0 without such a target
   float c_t, c_1;        // the same over the sums
 };
-__device__ __forceinline__ GradScale grad_scale(const DistillArgs &g, bool has_teacher, bool has_label, int64_t row,
-                                                float inv_t, float inv_1) {
+__device__ __forceinline__ float scale_of(const DistillArgs &g, int64_t row) {
   float scale = g.row_scale != nullptr ? g.row_scale[g.scale_per_row ? row : 0] : 1.f;
   if (g.count != nullptr) scale /= fmaxf(*g.count, 1.f);
+  return scale;
+}
+__device__ __forceinline__ GradScale grad_scale(const DistillArgs &g, bool has_teacher, bool has_label, float scale,
+                                                float inv_t, float inv_1) {
   GradScale c;
   c.base_t = has_teacher ? scale * g.kl_grad_weight : 0.f;
   c.base_1 = has_label ? scale * g.ce_weight : 0.f;
@@ -375,6 +390,7 @@ __device__ __forceinline__ void write_dense(T *out, int64_t e0, int64_t e1, bool
                                             const GradScale &c, VecAt vec_at, ElementAt element_at) {
   constexpr int kN = Vec<T>::kN, kAhead = 4;
   const int tid = threadIdx.x;
+  if (tid >= kThreads) return;
   const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out + e0) & 15u);
   const int64_t head = min64(e1 - e0, off == 0 ? 0 : (16 - off) / int64_t(sizeof(T)));
   const int64_t start = e0 + head, tail = start + (e1 - start) / kN * kN;
@@ -424,7 +440,7 @@ __device__ __forceinline__ void write_zeros(T *out, int64_t e0, int64_t e1) {
   const int64_t head = min64(e1 - e0, off == 0 ? 0 : (16 - off) / int64_t(sizeof(T)));
   const int64_t start = e0 + head, tail = start + (e1 - start) / kN * kN;
   if (int64_t(threadIdx.x) < head) out[e0 + threadIdx.x] = from_f32<T>(0.f);
-  for (int64_t e = start + threadIdx.x * kN; e < tail; e += kThreads * kN) __stcs(reinterpret_cast<uint4 *>(out + e), make_uint4(0, 0, 0, 0));
+  for (int64_t e = start + threadIdx.x * kN; e < tail; e += kBlock * kN) __stcs(reinterpret_cast<uint4 *>(out + e), make_uint4(0, 0, 0, 0));
   if (tail + threadIdx.x < e1) out[tail + threadIdx.x] = from_f32<T>(0.f);
 }
 // The targets of the part over it: p minus all that the teacher's entries of that index and the label
@@ -451,6 +467,7 @@ __device__ __forceinline__ void write_targets(const DistillArgs &g, T *out, int6
     const float p = dense2<EXPS>(both(element_at(e)), m, g.k_t, c).x;
     out[e] = from_f32<T>(p - c.base_t * q - (e == label ? c.base_1 : 0.f));
   };
+  if (tid >= kThreads) return;
   bool found = false;
   // The warps' stretches of entries are spread over the block one after the other.
   int before = 0;
@@ -472,7 +489,7 @@ __device__ __forceinline__ void write_targets(const DistillArgs &g, T *out, int6
 // Loss (MODE kLoss), or loss and gradient (kFused), of a row a cluster. RESIDENT: the slice stays in
 // shared memory for the gradient; else it is read again.
 template <typename T, int MODE, int EXPS, bool RESIDENT>
-__global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel(const DistillArgs g) {
+__global__ void __launch_bounds__(kBlock, RESIDENT ? 3 : 4) distill_row_kernel(const DistillArgs g) {
   constexpr int kN = Vec<T>::kN;
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ RowStats of_warp[kWarps], of_rank[kMaxCluster];
@@ -480,10 +497,11 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
   __shared__ uint64_t full[kChunks];
   __shared__ int abort;
   uint4 *slice = reinterpret_cast<uint4 *>(dynamic);
-  const int rank = blockIdx.x % g.ranks;
-  const int64_t row = blockIdx.x / g.ranks;
+  const uint32_t row32 = blockIdx.x / static_cast<uint32_t>(g.ranks);
+  const int rank = static_cast<int>(blockIdx.x - row32 * g.ranks);
+  const int64_t row = row32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const T *x = static_cast<const T *>(g.logits) + (row / g.inner) * g.outer_stride + (row % g.inner) * g.inner_stride;
+  const T *x = row_of<T>(g, row32);
   const int64_t lead = static_cast<int64_t>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T)), end = lead + g.vocab;
   const T *grid = x - lead;
   const int64_t vec0 = int64_t(rank) * g.slice_vecs;
@@ -514,6 +532,7 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
     }
     __syncthreads();  // the barriers are set up
   }
+  const float scale = MODE == kFused ? scale_of(g, row) : 1.f;
   load_targets<T>(g, row, x, e0, e1, rank == 0, table);
 
   // One order of summation for all kernels: cut vectors first, then batch by batch. A row without a
@@ -533,23 +552,25 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
   }
   const uint4 *whole = RESIDENT ? slice : reinterpret_cast<const uint4 *>(grid) + vec0;
   const uint4 nothing = nothing_vec<T>();
-  for (int from = whole0, c = 0; from < whole1; from += per_chunk, ++c) {
-    const int to = min(from + per_chunk, whole1);
-    if (RESIDENT) sm100::mbar_wait(&full[c], 0, &abort, &g_distill_error);
-    for (int v = from + tid; v < to; v += kBatch) {
-      uint4 q[4];
+  if (warp < kWarps) {
+    for (int from = whole0, c = 0; from < whole1; from += per_chunk, ++c) {
+      const int to = min(from + per_chunk, whole1);
+      if (RESIDENT) sm100::mbar_wait(&full[c], 0, &abort, &g_distill_error);
+      for (int v = from + tid; v < to; v += kBatch) {
+        uint4 q[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        q[i] = nothing;
-        if (v + i * kThreads < to) q[i] = RESIDENT ? whole[v + i * kThreads] : __ldg(whole + v + i * kThreads);
+        for (int i = 0; i < 4; ++i) {
+          q[i] = nothing;
+          if (v + i * kThreads < to) q[i] = RESIDENT ? whole[v + i * kThreads] : __ldg(whole + v + i * kThreads);
+        }
+        take<T, EXPS>(o, q, g.k_t);
       }
-      take<T, EXPS>(o, q, g.k_t);
     }
+    const RowStats mine = joined<EXPS, 32>({o.m, o.s_t.x + o.s_t.y, o.s_1.x + o.s_1.y}, g.k_t);
+    if (lane == 0) of_warp[warp] = mine;
   }
-  RowStats st = {o.m, o.s_t.x + o.s_t.y, o.s_1.x + o.s_1.y};
-  st = joined<EXPS, 32>(st, g.k_t);
-  if (lane == 0) of_warp[warp] = st;
   __syncthreads();
+  RowStats st;
   st = joined<EXPS, kWarps>(of_warp[lane % kWarps], g.k_t);
   if (g.ranks > 1) {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // all have started
@@ -564,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
   if constexpr (MODE == kFused) {
     T *out = static_cast<T *>(g.grad) + row * g.vocab;
     if (has_teacher || has_label) {
-      const GradScale c = grad_scale(g, has_teacher, has_label, row, inv_t, inv_1);
+      const GradScale c = grad_scale(g, has_teacher, has_label, scale, inv_t, inv_1);
       const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
       auto vec_at = [&](int64_t start, int i) -> uint4 {
         if constexpr (RESIDENT) return slice[static_cast<int>((start + lead) / kN - vec0) + i];
@@ -594,11 +615,12 @@ __global__ void __launch_bounds__(kThreads, RESIDENT ? 3 : 4) distill_row_kernel
 
 // The gradient from the loss's statistics: each CTA a part of a row.
 template <typename T, int EXPS>
-__global__ void __launch_bounds__(kThreads, 4) distill_grad_kernel(const DistillArgs g) {
+__global__ void __launch_bounds__(kBlock, 4) distill_grad_kernel(const DistillArgs g) {
   constexpr int kN = Vec<T>::kN;
   __shared__ EntryTable table;
-  const int64_t row = blockIdx.x / g.ranks, part = blockIdx.x % g.ranks;
-  const T *x = static_cast<const T *>(g.logits) + (row / g.inner) * g.outer_stride + (row % g.inner) * g.inner_stride;
+  const uint32_t row32 = blockIdx.x / static_cast<uint32_t>(g.ranks);
+  const int64_t row = row32, part = blockIdx.x - row32 * g.ranks;
+  const T *x = row_of<T>(g, row32);
   T *out = static_cast<T *>(g.grad) + row * g.vocab;
   const float4 st = g.stats[row];
   const int has = static_cast<int>(st.w);
@@ -611,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_grad_kernel(const Distill
     return;
   }
   load_targets<T>(g, row, x, e0, e1, false, table);
-  const GradScale c = grad_scale(g, (has & 1) != 0, (has & 2) != 0, row, st.y, st.z);
+  const GradScale c = grad_scale(g, (has & 1) != 0, (has & 2) != 0, scale_of(g, row), st.y, st.z);
   const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
   auto vec_at = [&](int64_t start, int i) -> uint4 { return __ldg(reinterpret_cast<const uint4 *>(x + start) + i); };
   auto element_at = [&](int64_t e) -> float { return ldg_f32(x + e); };
@@ -670,7 +692,7 @@ int launch_rows(const char *what, DistillArgs g, int64_t rows, cudaStream_t stre
   g.slice_vecs = static_cast<int>(slice);
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(rows * ranks));
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3(kBlock);
   config.stream = stream;
   const void *kernel = nullptr;
   cudaLaunchAttribute attr{};
@@ -711,7 +733,7 @@ int run_rows(const char *what, DistillArgs g, int dtype, int64_t rows, int64_t v
              g.teacher_dtype);
   TB_REQUIRE(g.index_dtype == TROPNN_B200_I64 || g.index_dtype == TROPNN_B200_I32, TROPNN_B200_ERR_DTYPE,
              "%s: index dtype %d is not i32/i64", what, g.index_dtype);
-  TB_REQUIRE(rows >= 0 && rows <= 0x7fffffffLL && vocab >= 1 && vocab <= 0x7fffffffLL && g.inner >= 1,
+  TB_REQUIRE(rows >= 0 && rows <= 0x7fffffffLL && vocab >= 1 && vocab <= 0x7fffffffLL && g.inner >= 1 && g.inner <= 0x7fffffffLL,
              TROPNN_B200_ERR_INVALID, "%s: bad sizes (rows %lld, vocab %lld)", what, (long long)rows, (long long)vocab);
   TB_REQUIRE(g.top >= 0 && g.top <= kMaxTop, TROPNN_B200_ERR_INVALID, "%s: 0 to %d teacher entries a row, got %d", what,
              kMaxTop, g.top);
