@@ -18,7 +18,9 @@
 // that bin's tokens name the logit; how many tokens of that logit stay is arithmetic, and which ones
 // a running count in index order, taken together with the final sums. Where a top-k leaves at most
 // 256 tokens, they go to the cluster's first CTA, which does the rest. Passes after the first skip
-// vectors whose largest logit lies below what they look for.
+// vectors whose largest logit lies below what they look for. With no top-k or top-p about and many
+// rows, a row is one CTA's or two's, which stream it and keep the maxima of batches of four vectors
+// alone: the second pass reads again, from L2, the batches that can hold kept tokens.
 #include <cfloat>
 
 #include <cooperative_groups.h>
@@ -54,7 +56,8 @@ struct SampleArgs {
   float temperature_value, top_p_value, min_p_value;
   int64_t top_k_value;
   int64_t *tokens;
-  int slice_vecs;  // 16-byte vectors of a CTA's slice
+  int slice_vecs;   // 16-byte vectors of a CTA's slice
+  int maxima_rows;  // batches a thread whose maxima are kept; 0: none
 };
 
 // Larger for larger logits; -0 as +0.
@@ -184,6 +187,12 @@ __device__ __forceinline__ __half lowest_logit<__half>() { return __ushort_as_ha
 template <>
 __device__ __forceinline__ __nv_bfloat16 lowest_logit<__nv_bfloat16>() { return __ushort_as_bfloat16(0xFF80); }
 
+template <typename T>
+__device__ __forceinline__ uint4 nothing_vec() {  // -inf throughout
+  const uint32_t w = std::is_same<T, float>::value ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+  return make_uint4(w, w, w, w);
+}
+
 // Vector v of the row's 16-byte grid, which starts at or before the row: elements outside the row
 // are -inf and never read.
 template <typename T>
@@ -258,9 +267,10 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
 
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int64_t row = blockIdx.x / ranks;
+  const uint32_t row = blockIdx.x / static_cast<uint32_t>(ranks);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const T *x = static_cast<const T *>(g.logits) + (row / g.inner) * g.outer_stride + (row % g.inner) * g.inner_stride;
+  const uint32_t outer = g.inner == 1 ? row : row / static_cast<uint32_t>(g.inner);  // both below 2^31
+  const T *x = static_cast<const T *>(g.logits) + outer * g.outer_stride + (row - outer * g.inner) * g.inner_stride;
   const int64_t lead = static_cast<int64_t>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T)), end = lead + g.vocab;
   const T *grid = x - lead;
   const int64_t vec0 = int64_t(rank) * g.slice_vecs;
@@ -283,21 +293,38 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
   const bool by_weight = SEARCH && !(top_p >= 1.f);
   if (ranks > 1) cluster_arrive();
 
-  // The slice, and the row's maximum (NaN where a logit is).
+  // The slice, and the row's maximum (NaN where a logit is). Each warp has a stretch of the slice.
+  const int per_warp = (vecs + kThreads - 1) / kThreads * 32;
+  const int begin = min(warp * per_warp, vecs), stop = min(begin + per_warp, vecs);
   float m = -INFINITY;
-  constexpr int kAhead = SEARCH ? 8 : 4;
-  for (int v0 = tid; v0 < vecs; v0 += kThreads * kAhead) {
-    uint4 q[kAhead];
+  constexpr int kAhead = 4;
+  constexpr bool kMaxima = !RESIDENT && !SEARCH;
+  float *maxima = reinterpret_cast<float *>(dynamic) + tid;  // kMaxima: [batch][thread]
+  auto load4 = [&](int v, uint4 (&q)[kAhead]) {  // v and every 32nd vector after it, -inf past the stretch
+    const int64_t p = (vec0 + v) * kN;
+    if (p >= lead && v + 32 * (kAhead - 1) < stop && p + (32 * (kAhead - 1) + 1) * kN <= end) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (v0 + i * kThreads < vecs) q[i] = load_vec<T>(grid, vec0 + v0 + i * kThreads, lead, end);
+      for (int i = 0; i < kAhead; ++i) q[i] = __ldg(reinterpret_cast<const uint4 *>(grid + p) + 32 * i);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (v0 + i * kThreads < vecs) {
-        if constexpr (RESIDENT) kept_slice[v0 + i * kThreads] = q[i];
-        m = max_nan(m, vec_max<T, true>(q[i]));
+      for (int i = 0; i < kAhead; ++i) {
+        q[i] = nothing_vec<T>();
+        if (v + 32 * i < stop) q[i] = load_vec<T>(grid, vec0 + v + 32 * i, lead, end);
       }
     }
+  };
+  for (int v = begin + lane, n = 0; v < stop; v += 32 * kAhead, ++n) {
+    uint4 q[kAhead];
+    load4(v, q);
+    float batch = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if constexpr (RESIDENT)
+        if (v + 32 * i < stop) kept_slice[v + 32 * i] = q[i];
+      batch = max_nan(batch, vec_max<T, true>(q[i]));
+    }
+    if (kMaxima && g.maxima_rows > 0) maxima[n * kThreads] = batch;
+    m = max_nan(m, batch);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -596,13 +623,10 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
       if (cutting) at_cut |= in && f[j] <= cut_high ? 1u << j : 0u;
     }
   };
-  const int per_warp = (vecs + kThreads - 1) / kThreads * 32;
-  const int begin = min(warp * per_warp, vecs), stop = min(begin + per_warp, vecs);
   uint64_t sum = 0;
   uint32_t tied = 0, tie_weight = 0;
-  for (int v = begin + lane; v < stop; v += 32) {
-    const uint4 q = at(v);
-    if (vec_max<T, false>(q) < floor_x) continue;
+  auto add = [&](const uint4 &q) {
+    if (vec_max<T, false>(q) < floor_x) return;
     uint32_t w[kN], at_cut;
     kept(q, w, at_cut);
     if (at_cut != 0) {
@@ -617,6 +641,17 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
     }
 #pragma unroll
     for (int j = 0; j < kN; ++j) sum += w[j];
+  };
+  if (kMaxima) {
+    for (int v = begin + lane, n = 0; v < stop; v += 32 * kAhead, ++n) {
+      if (g.maxima_rows > 0 && maxima[n * kThreads] < floor_x) continue;
+      uint4 q[kAhead];
+      load4(v, q);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) add(q[i]);
+    }
+  } else {
+    for (int v = begin + lane; v < stop; v += 32) add(at(v));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -717,19 +752,35 @@ template <typename T>
 int launch_sample(const char *what, SampleArgs g, int64_t rows, cudaStream_t stream) {
   int sms = 0;
   TB_CHECK(sm100::sm_count(&sms));
-  // The fewest CTAs a row that keep its slices at two CTAs an SM, more while SMs are idle.
-  const int64_t row_bytes = g.vocab * int64_t(sizeof(T)) + 32;
-  int ranks = 1;
-  while (ranks < kMaxCluster && (row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 4096)))
-    ranks *= 2;
-  const int64_t vecs = row_bytes / 16;
-  const int64_t slice = ceil_div(vecs, ranks);
-  const bool resident = slice * 16 <= kSliceMost;
   const bool search = g.top_k != nullptr || g.top_k_value > 0 || g.top_p != nullptr || g.top_p_value < 1.f || g.min_p != nullptr ||
                       !(g.min_p_value <= 1.f);
+  const int64_t row_bytes = g.vocab * int64_t(sizeof(T)) + 32;
+  // Streamed: no search, and rows for six CTAs an SM at no more than two a row. Else in shared memory:
+  // the fewest CTAs a row that keep its slices at two or three CTAs an SM, more while SMs are idle.
+  const bool stream_rows = !search && rows * 2 >= 6 * sms;
+  int ranks = 1;
+  if (stream_rows) {
+    if (rows < 6 * sms) ranks = 2;
+  } else {
+    while (ranks < kMaxCluster && (row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 4096)))
+      ranks *= 2;
+  }
+  const int64_t vecs = row_bytes / 16;
+  const int64_t slice = ceil_div(vecs, ranks);
+  const bool resident = !stream_rows && slice * 16 <= kSliceMost;
   TB_REQUIRE(rows * ranks <= 0x7fffffffLL && slice <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: too many rows", what);
   g.slice_vecs = static_cast<int>(slice);
-  const size_t smem = (search ? sizeof(Histogram) : 0) + 16 + (resident ? static_cast<size_t>(slice) * 16 : 0);
+  size_t smem = 16;
+  if (search) smem += sizeof(Histogram);
+  if (resident) smem += static_cast<size_t>(slice) * 16;
+  g.maxima_rows = 0;
+  if (!resident && !search) {
+    const int64_t batches = ceil_div(ceil_div(slice, kThreads), 4);
+    if (batches * kThreads * 4 <= 64 * 1024) {
+      g.maxima_rows = static_cast<int>(batches);
+      smem += static_cast<size_t>(batches) * kThreads * 4;
+    }
+  }
   const void *kernel = resident ? (search ? reinterpret_cast<const void *>(sample_kernel<T, true, true>)
                                           : reinterpret_cast<const void *>(sample_kernel<T, true, false>))
                                 : (search ? reinterpret_cast<const void *>(sample_kernel<T, false, true>)
@@ -765,7 +816,7 @@ extern "C" int tropnn_b200_sample_tokens(const void *logits, int dtype, int64_t 
   TB_REQUIRE(is_float_dtype(dtype), TROPNN_B200_ERR_DTYPE, "%s: logits dtype %d is not f32/f16/bf16", what, dtype);
   TB_REQUIRE(top_k == nullptr || top_k_dtype == TROPNN_B200_I64 || top_k_dtype == TROPNN_B200_I32, TROPNN_B200_ERR_DTYPE,
              "%s: top_k dtype %d is not i32/i64", what, top_k_dtype);
-  TB_REQUIRE(rows >= 0 && rows <= 0x7fffffffLL && vocab >= 1 && vocab <= 0x7fffffffLL && inner >= 1,
+  TB_REQUIRE(rows >= 0 && rows <= 0x7fffffffLL && vocab >= 1 && vocab <= 0x7fffffffLL && inner >= 1 && inner <= 0x7fffffffLL,
              TROPNN_B200_ERR_INVALID, "%s: bad sizes (rows %lld, vocab %lld)", what, (long long)rows, (long long)vocab);
   if (rows == 0) return clear_error();
   TB_REQUIRE(logits != nullptr && uniforms != nullptr && tokens != nullptr, TROPNN_B200_ERR_INVALID, "%s: null pointer", what);
