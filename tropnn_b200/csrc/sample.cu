@@ -214,6 +214,49 @@ __device__ __forceinline__ void cluster_sync(int ranks) {
   else __syncthreads();
 }
 
+template <typename T>
+__device__ __forceinline__ float lowest_finite() {
+  return std::is_same<T, float>::value ? -3.4028234663852886e38f : std::is_same<T, __half>::value ? -65504.f : -3.3895313892515355e38f;
+}
+// Which elements of a lane's four vectors lie in [lo, hi] (as T, the bounds widened to it): bit n for the
+// n-th 32-bit word's (low) element, 16 + n for its high one. Never one that is -inf: those fill the
+// vectors past the slice and outside the row, which are not to be read.
+template <typename T, bool BELOW>
+__device__ __forceinline__ uint32_t mask_of(const uint4 (&q)[4], float lo, float hi) {
+  lo = fmaxf(lo, lowest_finite<T>());
+  uint32_t mask = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int n = 4 * i + k;
+      if constexpr (std::is_same<T, float>::value) {
+        const float f = __uint_as_float(w[k]);
+        if (f >= lo && (!BELOW || f <= hi)) mask |= 1u << n;
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 f = *reinterpret_cast<const __half2 *>(&w[k]);
+        uint32_t in = __hge2_mask(f, __half2half2(__float2half_rd(lo)));
+        if (BELOW) in &= __hle2_mask(f, __half2half2(__float2half_ru(hi)));
+        mask |= in & (0x00010001u << n);
+      } else {
+        const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162 *>(&w[k]);
+        uint32_t in = __hge2_mask(f, __bfloat162bfloat162(__float2bfloat16_rd(lo)));
+        if (BELOW) in &= __hle2_mask(f, __bfloat162bfloat162(__float2bfloat16_ru(hi)));
+        mask |= in & (0x00010001u << n);
+      }
+    }
+  }
+  return mask;
+}
+// Element (vector of the four, position in it) of a mask's bit.
+template <typename T>
+__device__ __forceinline__ void place_of(int bit, int &vector, int &element) {
+  const int n = bit & 15;
+  vector = n >> 2;
+  element = sizeof(T) == 4 ? n & 3 : 2 * (n & 3) + (bit >> 4);
+}
+
 // Inclusive prefix sums of a count and a weight over the block's threads, and their totals.
 __device__ __forceinline__ void block_scan(uint32_t &count, uint64_t &weight, uint32_t &all_count, uint64_t &all_weight,
                                            Shared &sh) {
@@ -279,6 +322,10 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
     if constexpr (RESIDENT) return kept_slice[v];
     else return load_vec<T>(grid, vec0 + v, lead, end);
   };
+  auto element = [&](int v, int j) -> float {
+    if constexpr (RESIDENT) return to_f32<T>(reinterpret_cast<const T *>(kept_slice)[v * kN + j]);
+    else return ldg_f32(grid + (vec0 + v) * kN + j);
+  };
   auto index0 = [&](int v) -> uint32_t { return static_cast<uint32_t>((vec0 + v) * kN - lead); };  // may wrap: unused then
 
   const float temperature = g.temperature != nullptr ? g.temperature[row] : g.temperature_value;
@@ -311,6 +358,33 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
         q[i] = nothing_vec<T>();
         if (v + 32 * i < stop) q[i] = load_vec<T>(grid, vec0 + v + 32 * i, lead, end);
       }
+    }
+  };
+  auto again4 = [&](int v, uint4 (&q)[kAhead]) {  // the same in later passes
+    if constexpr (RESIDENT) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        q[i] = nothing_vec<T>();
+        if (v + 32 * i < stop) q[i] = kept_slice[v + 32 * i];
+      }
+    } else {
+      load4(v, q);
+    }
+  };
+  // Calls visit(x, index) for the logits of the warp's stretch that `mask` (of a batch) has a bit for,
+  // with all lanes together: lanes without one bring -inf.
+  auto each = [&](int v, uint32_t mask, auto visit) {
+    while (__any_sync(0xffffffffu, mask != 0)) {
+      float x = -INFINITY;
+      uint32_t i = 0;
+      if (mask != 0) {
+        int vector, j;
+        place_of<T>(__ffs(mask) - 1, vector, j);
+        mask &= mask - 1;
+        x = element(v + 32 * vector, j);
+        i = index0(v + 32 * vector) + j;
+      }
+      visit(x, i);
     }
   };
   for (int v = begin + lane, n = 0; v < stop; v += 32 * kAhead, ++n) {
@@ -401,13 +475,13 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
       const int shift = max(0, 32 - __clz(range) - kDigitBits);
       for (int i = tid; i < kBins; i += kThreads) hist.count[i] = hist.low[i] = hist.high[i] = 0;
       __syncthreads();
-      const float floor_x = fresh ? scale.below(kLowestZ) : logit_of(o.key_low);
-      for (int v = tid; v < vecs; v += kThreads) {
-        const uint4 q = at(v);
-        if (vec_max<T, false>(q) < floor_x) continue;
-        float f[kN];
-        Vec<T>::unpack(q, f);
-        if (fresh) {
+      if (fresh) {
+        const float floor_x = scale.below(kLowestZ);
+        for (int v = begin + lane; v < stop; v += 32) {
+          const uint4 q = at(v);
+          if (vec_max<T, false>(q) < floor_x) continue;
+          float f[kN];
+          Vec<T>::unpack(q, f);
           if (by_weight) {
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
@@ -427,18 +501,22 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
               if (b < kBins) atomicAdd(&hist.count[b], 1u);
             }
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kN; ++j) {
-            const uint32_t down = o.key_high - key_of(f[j]);  // larger keys first
-            const float z = scale.z(f[j]);
+        }
+      } else {
+        const float low = logit_of(o.key_low), high = logit_of(o.key_high);
+        for (int v0 = begin; v0 < stop; v0 += 32 * kAhead) {
+          uint4 q[kAhead];
+          again4(v0 + lane, q);
+          each(v0 + lane, mask_of<T, true>(q, low, high), [&](float x, uint32_t) {
+            const uint32_t down = o.key_high - key_of(x);  // larger keys first
+            const float z = scale.z(x);
             if (down <= range && Scale::bin(z) == o.bin) {
               const uint32_t w = Scale::weight(expf(z));
               const uint32_t old = atomicAdd(&hist.low[down >> shift], w);
               if (old + w < old) atomicAdd(&hist.high[down >> shift], 1u);
               atomicAdd(&hist.count[down >> shift], 1u);
             }
-          }
+          });
         }
       }
       cluster_sync(ranks);
@@ -544,18 +622,15 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
       if (o.command == kFinish) {
         Few *to = cluster.map_shared_rank(&few, 0);
         uint32_t *listed = cluster.map_shared_rank(&sh.listed, 0);
-        const float floor_bin = scale.bin_low(o.bin);
-        for (int v = tid; v < vecs; v += kThreads) {
-          const uint4 q = at(v);
-          if (vec_max<T, false>(q) < floor_bin) continue;
-          float f[kN];
-          Vec<T>::unpack(q, f);
-#pragma unroll
-          for (int j = 0; j < kN; ++j) {
-            if (Scale::bin(scale.z(f[j])) > o.bin) continue;
+        const float low = scale.bin_low(o.bin);
+        for (int v0 = begin; v0 < stop; v0 += 32 * kAhead) {
+          uint4 q[kAhead];
+          again4(v0 + lane, q);
+          each(v0 + lane, mask_of<T, false>(q, low, 0.f), [&](float x, uint32_t i) {
+            if (x == -INFINITY || Scale::bin(scale.z(x)) > o.bin) return;
             const uint32_t place = atomicAdd(listed, 1u);
-            if (place < kFew) to->key[place] = (uint64_t(key_of(f[j])) << 32) | (0xFFFFFFFFu - (index0(v) + j));
-          }
+            if (place < kFew) to->key[place] = (uint64_t(key_of(x)) << 32) | (0xFFFFFFFFu - i);
+          });
         }
         cluster_sync(ranks);
         if (rank != 0) return;
@@ -620,38 +695,49 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
       const float e = expf(scale.z(f[j]));
       const bool in = e >= min_p && (!cutting || f[j] >= cut_low);
       w[j] = in ? Scale::weight(e) : 0u;
-      if (cutting) at_cut |= in && f[j] <= cut_high ? 1u << j : 0u;
+      if (cutting) at_cut |= w[j] != 0 && f[j] <= cut_high ? 1u << j : 0u;
     }
   };
   uint64_t sum = 0;
   uint32_t tied = 0, tie_weight = 0;
-  auto add = [&](const uint4 &q) {
-    if (vec_max<T, false>(q) < floor_x) return;
-    uint32_t w[kN], at_cut;
-    kept(q, w, at_cut);
-    if (at_cut != 0) {
-      tied += __popc(at_cut);
-#pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        if ((at_cut >> j) & 1u) {
-          tie_weight = w[j];  // the same for all
-          w[j] = 0;
+  for (int v0 = begin, n = 0; v0 < stop; v0 += 32 * kAhead, ++n) {
+    const int v = v0 + lane;
+    uint4 q[kAhead];
+    bool some = v < stop;
+    if (kMaxima && g.maxima_rows > 0 && some) some = maxima[n * kThreads] >= floor_x;
+    if (!__any_sync(0xffffffffu, some)) continue;
+    again4(some ? v : stop, q);
+    const uint32_t mask = mask_of<T, false>(q, floor_x, 0.f);
+    if (__reduce_max_sync(0xffffffffu, __popc(mask)) <= kN) {  // few: one at a time
+      each(v, mask, [&](float x, uint32_t) {
+        const float e = expf(scale.z(x));
+        const uint32_t w = e >= min_p && (!cutting || x >= cut_low) ? Scale::weight(e) : 0u;
+        if (cutting && w != 0 && x <= cut_high) {
+          ++tied;
+          tie_weight = w;  // the same for all
+        } else {
+          sum += w;
         }
+      });
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        uint32_t w[kN], at_cut;
+        kept(q[i], w, at_cut);
+        if (at_cut != 0) {
+          tied += __popc(at_cut);
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            if ((at_cut >> j) & 1u) {
+              tie_weight = w[j];
+              w[j] = 0;
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kN; ++j) sum += w[j];
       }
     }
-#pragma unroll
-    for (int j = 0; j < kN; ++j) sum += w[j];
-  };
-  if (kMaxima) {
-    for (int v = begin + lane, n = 0; v < stop; v += 32 * kAhead, ++n) {
-      if (g.maxima_rows > 0 && maxima[n * kThreads] < floor_x) continue;
-      uint4 q[kAhead];
-      load4(v, q);
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) add(q[i]);
-    }
-  } else {
-    for (int v = begin + lane; v < stop; v += 32) add(at(v));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -666,9 +752,9 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
   __syncthreads();
   if (lane == 0 && tie_weight != 0) atomicMax(&sh.tied, tie_weight);
   uint64_t all = sh.warp_sum[lane % kWarps], before = lane < warp ? all : 0;
-  const uint32_t each = sh.warp_count[lane % kWarps];
-  uint32_t ties_before = __reduce_add_sync(0xffffffffu, lane < warp ? each : 0u);
-  const uint32_t all_ties = __reduce_add_sync(0xffffffffu, lane < kWarps ? each : 0u);
+  const uint32_t warp_ties = sh.warp_count[lane % kWarps];
+  uint32_t ties_before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_ties : 0u);
+  const uint32_t all_ties = __reduce_add_sync(0xffffffffu, lane < kWarps ? warp_ties : 0u);
 #pragma unroll
   for (int o = kWarps / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
 #pragma unroll
