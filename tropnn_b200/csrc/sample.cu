@@ -18,9 +18,9 @@
 // that bin's tokens name the logit; how many tokens of that logit stay is arithmetic, and which ones
 // a running count in index order, taken together with the final sums. Where a top-k leaves at most
 // 256 tokens, they go to the cluster's first CTA, which does the rest. Passes after the first skip
-// vectors whose largest logit lies below what they look for. With no top-k or top-p about and many
-// rows, a row is one CTA's or two's, which stream it and keep the maxima of batches of four vectors
-// alone: the second pass reads again, from L2, the batches that can hold kept tokens.
+// vectors whose largest logit lies below what they look for. With no top-k or top-p about a row is
+// streamed and the maxima of batches of four vectors alone are kept: the second pass reads again, from
+// L2, the batches that can hold kept tokens.
 #include <cfloat>
 
 #include <cooperative_groups.h>
@@ -43,7 +43,7 @@ constexpr int kFew = 256;
 // W >= 1 needs z >= ln(0.5 / 2^31) = -22.18: the bins cover the tokens that weigh anything.
 constexpr float kLowestZ = -22.25f;
 constexpr float kBinScale = kBins / -kLowestZ;
-constexpr int64_t kSliceShared = 64 * 1024 + 64;  // bytes of logits a CTA, two (without a search three) on an SM
+constexpr int64_t kSliceShared = 64 * 1024 + 64;  // bytes of logits a CTA, two on an SM
 constexpr int64_t kSliceMost = 168 * 1024;        // one CTA on an SM
 
 struct SampleArgs {
@@ -109,8 +109,8 @@ struct Order {
 };
 
 struct Shared {
-  uint64_t warp_sum[kWarps];
-  uint32_t warp_count[kWarps];
+  uint64_t warp_sum[kWarps], slot_sum[kWarps][32];
+  uint32_t warp_count[kWarps], slot_ties[kWarps][32];
   uint64_t sums[kMaxCluster];
   uint32_t ties[kMaxCluster], tie_weight[kMaxCluster];
   float maxima[kMaxCluster];
@@ -257,6 +257,15 @@ __device__ __forceinline__ void place_of(int bit, int &vector, int &element) {
   element = sizeof(T) == 4 ? n & 3 : 2 * (n & 3) + (bit >> 4);
 }
 
+// The sum over a warp, in every lane.
+__device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
+  const uint32_t a = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v) & 0xFFFFu);
+  const uint32_t b = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 16) & 0xFFFFu);
+  const uint32_t c = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 32) & 0xFFFFu);
+  const uint32_t d = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 48));
+  return a + (uint64_t(b) << 16) + (uint64_t(c) << 32) + (uint64_t(d) << 48);
+}
+
 // Inclusive prefix sums of a count and a weight over the block's threads, and their totals.
 __device__ __forceinline__ void block_scan(uint32_t &count, uint64_t &weight, uint32_t &all_count, uint64_t &all_weight,
                                            Shared &sh) {
@@ -297,10 +306,14 @@ __device__ __forceinline__ void block_scan(uint32_t &count, uint64_t &weight, ui
   }
 }
 
-// RESIDENT: the slice stays in shared memory; else every pass reads global memory (L2) again.
-// SEARCH: some row may have a top-k or a top-p.
+// SEARCH: some row may have a top-k or a top-p. Then with RESIDENT the slice stays in shared memory, else
+// every pass reads global memory (L2) again. Without a search half as many threads a CTA stream the
+// slice, RESIDENT false.
+template <bool SEARCH>
+constexpr int kBlock = SEARCH ? kThreads : kThreads / 2;
 template <typename T, bool RESIDENT, bool SEARCH>
-__global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const SampleArgs g) {
+__global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(const SampleArgs g) {
+  constexpr int kThreads = kBlock<SEARCH>, kWarps = kThreads / 32;
   constexpr int kN = Vec<T>::kN;
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared sh;
@@ -387,9 +400,7 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
       visit(x, i);
     }
   };
-  for (int v = begin + lane, n = 0; v < stop; v += 32 * kAhead, ++n) {
-    uint4 q[kAhead];
-    load4(v, q);
+  auto take = [&](int v, int n, const uint4 (&q)[kAhead]) {
     float batch = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -399,6 +410,13 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
     }
     if (kMaxima && g.maxima_rows > 0) maxima[n * kThreads] = batch;
     m = max_nan(m, batch);
+  };
+  for (int v = begin + lane, n = 0; v < stop; v += 64 * kAhead, n += 2) {  // two batches on their way
+    uint4 q[kAhead], r[kAhead];
+    load4(v, q);
+    load4(v + 32 * kAhead, r);
+    take(v, n, q);
+    if (v + 32 * kAhead < stop) take(v + 32 * kAhead, n + 1, r);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -698,50 +716,61 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
       if (cutting) at_cut |= w[j] != 0 && f[j] <= cut_high ? 1u << j : 0u;
     }
   };
+  // The sums are also kept for 32 slots of consecutive batches a warp, so that the token is found by them.
   uint64_t sum = 0;
   uint32_t tied = 0, tie_weight = 0;
-  for (int v0 = begin, n = 0; v0 < stop; v0 += 32 * kAhead, ++n) {
-    const int v = v0 + lane;
-    uint4 q[kAhead];
-    bool some = v < stop;
-    if (kMaxima && g.maxima_rows > 0 && some) some = maxima[n * kThreads] >= floor_x;
-    if (!__any_sync(0xffffffffu, some)) continue;
-    again4(some ? v : stop, q);
-    const uint32_t mask = mask_of<T, false>(q, floor_x, 0.f);
-    if (__reduce_max_sync(0xffffffffu, __popc(mask)) <= kN) {  // few: one at a time
-      each(v, mask, [&](float x, uint32_t) {
-        const float e = expf(scale.z(x));
-        const uint32_t w = e >= min_p && (!cutting || x >= cut_low) ? Scale::weight(e) : 0u;
-        if (cutting && w != 0 && x <= cut_high) {
-          ++tied;
-          tie_weight = w;  // the same for all
-        } else {
-          sum += w;
-        }
-      });
-    } else {
+  const int batches = (stop - begin + 32 * kAhead - 1) / (32 * kAhead), per_slot = (batches + 31) / 32;
+  for (int slot = 0, n = 0; n < batches; ++slot) {
+    uint64_t lane_sum = 0;
+    uint32_t lane_tied = 0;
+    for (const int last = min(n + per_slot, batches); n < last; ++n) {
+      const int v = begin + n * 32 * kAhead + lane;
+      uint4 q[kAhead];
+      bool some = v < stop;
+      if (kMaxima && g.maxima_rows > 0 && some) some = maxima[n * kThreads] >= floor_x;
+      if (!__any_sync(0xffffffffu, some)) continue;
+      again4(some ? v : stop, q);
+      const uint32_t mask = mask_of<T, false>(q, floor_x, 0.f);
+      if (__reduce_max_sync(0xffffffffu, __popc(mask)) <= kN) {  // few: one at a time
+        each(v, mask, [&](float x, uint32_t) {
+          const float e = expf(scale.z(x));
+          const uint32_t w = e >= min_p && (!cutting || x >= cut_low) ? Scale::weight(e) : 0u;
+          if (cutting && w != 0 && x <= cut_high) {
+            ++lane_tied;
+            tie_weight = w;  // the same for all
+          } else {
+            lane_sum += w;
+          }
+        });
+      } else {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        uint32_t w[kN], at_cut;
-        kept(q[i], w, at_cut);
-        if (at_cut != 0) {
-          tied += __popc(at_cut);
+        for (int i = 0; i < kAhead; ++i) {
+          uint32_t w[kN], at_cut;
+          kept(q[i], w, at_cut);
+          if (at_cut != 0) {
+            lane_tied += __popc(at_cut);
 #pragma unroll
-          for (int j = 0; j < kN; ++j) {
-            if ((at_cut >> j) & 1u) {
-              tie_weight = w[j];
-              w[j] = 0;
+            for (int j = 0; j < kN; ++j) {
+              if ((at_cut >> j) & 1u) {
+                tie_weight = w[j];
+                w[j] = 0;
+              }
             }
           }
-        }
 #pragma unroll
-        for (int j = 0; j < kN; ++j) sum += w[j];
+          for (int j = 0; j < kN; ++j) lane_sum += w[j];
+        }
       }
     }
+    lane_sum = warp_sum64(lane_sum);
+    lane_tied = __reduce_add_sync(0xffffffffu, lane_tied);
+    if (lane == 0) {
+      sh.slot_sum[warp][slot] = lane_sum;
+      sh.slot_ties[warp][slot] = lane_tied;
+    }
+    sum += lane_sum;
+    tied += lane_tied;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  tied = __reduce_add_sync(0xffffffffu, tied);
   tie_weight = __reduce_max_sync(0xffffffffu, tie_weight);
   __syncthreads();
   if (tid == 0) sh.tied = 0;
@@ -783,54 +812,73 @@ __global__ void __launch_bounds__(kThreads, SEARCH ? 2 : 3) sample_kernel(const 
   sum += uint64_t(min(ties_before + tied, ties) - min(ties_before, ties)) * tie_weight;
   const uint64_t target = target_of(total);
   if (target < before || target >= before + sum) return;  // one warp of the cluster goes on
-  for (int v0 = begin; v0 < stop; v0 += 32) {
-    const int v = v0 + lane;
-    uint32_t w[kN], at_cut = 0;
-    if (v < stop) {
-      kept(at(v), w, at_cut);
-    } else {
+  const int slots = (batches + per_slot - 1) / per_slot;
+  uint64_t slot_sum = lane < slots ? sh.slot_sum[warp][lane] : 0;
+  uint32_t slot_ties = lane < slots ? sh.slot_ties[warp][lane] : 0, upto_ties = slot_ties;
 #pragma unroll
-      for (int j = 0; j < kN; ++j) w[j] = 0;
-    }
-    uint32_t rank_in = __popc(at_cut);  // of the lane's first token at the cut
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t below = __shfl_up_sync(0xffffffffu, upto_ties, o);
+    if (lane >= o) upto_ties += below;
+  }
+  const uint32_t first_tie = ties_before + upto_ties - slot_ties;
+  slot_sum += uint64_t(min(first_tie + slot_ties, ties) - min(first_tie, ties)) * tie_weight;
+  uint64_t upto_sum = slot_sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t below = __shfl_up_sync(0xffffffffu, rank_in, o);
-      if (lane >= o) rank_in += below;
-    }
-    const uint32_t passed = __shfl_sync(0xffffffffu, rank_in, 31);
-    rank_in += ties_before - __popc(at_cut);
-    uint64_t mine = 0;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t below = __shfl_up_sync(0xffffffffu, upto_sum, o);
+    if (lane >= o) upto_sum += below;
+  }
+  const int slot = __ffs(__ballot_sync(0xffffffffu, before + upto_sum > target)) - 1;
+  before += __shfl_sync(0xffffffffu, upto_sum - slot_sum, slot);
+  ties_before = __shfl_sync(0xffffffffu, first_tie, slot);
+  for (int n = slot * per_slot; n < batches; ++n) {
+    const int v0 = begin + n * 32 * kAhead + lane;
+    uint4 q[kAhead];
+    again4(v0, q);
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      if ((at_cut >> j) & 1u) {
-        if (rank_in >= ties) w[j] = 0;
-        ++rank_in;
+    for (int i = 0; i < kAhead; ++i) {
+      uint32_t w[kN], at_cut;
+      kept(q[i], w, at_cut);
+      uint32_t rank_in = __popc(at_cut);  // of the lane's first token at the cut
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t below = __shfl_up_sync(0xffffffffu, rank_in, o);
+        if (lane >= o) rank_in += below;
       }
-      mine += w[j];
-    }
-    ties_before += passed;
-    uint64_t upto = mine;
+      const uint32_t passed = __shfl_sync(0xffffffffu, rank_in, 31);
+      rank_in += ties_before - __popc(at_cut);
+      uint64_t mine = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t below = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += below;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, before + upto > target);
-    if (past != 0) {
-      if (lane == __ffs(past) - 1) {
-        uint64_t run = before + upto - mine;
-        int found = -1;
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          run += w[j];
-          if (found < 0 && run > target) found = j;
+      for (int j = 0; j < kN; ++j) {
+        if ((at_cut >> j) & 1u) {
+          if (rank_in >= ties) w[j] = 0;
+          ++rank_in;
         }
-        g.tokens[row] = index0(v) + found;
+        mine += w[j];
       }
-      return;
+      ties_before += passed;
+      uint64_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t below = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += below;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, before + upto > target);
+      if (past != 0) {
+        if (lane == __ffs(past) - 1) {
+          uint64_t run = before + upto - mine;
+          int found = -1;
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            run += w[j];
+            if (found < 0 && run > target) found = j;
+          }
+          g.tokens[row] = index0(v0 + 32 * i) + found;
+        }
+        return;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    before += __shfl_sync(0xffffffffu, upto, 31);
   }
 }
 
@@ -841,40 +889,35 @@ int launch_sample(const char *what, SampleArgs g, int64_t rows, cudaStream_t str
   const bool search = g.top_k != nullptr || g.top_k_value > 0 || g.top_p != nullptr || g.top_p_value < 1.f || g.min_p != nullptr ||
                       !(g.min_p_value <= 1.f);
   const int64_t row_bytes = g.vocab * int64_t(sizeof(T)) + 32;
-  // Streamed: no search, and rows for six CTAs an SM at no more than two a row. Else in shared memory:
-  // the fewest CTAs a row that keep its slices at two or three CTAs an SM, more while SMs are idle.
-  const bool stream_rows = !search && rows * 2 >= 6 * sms;
+  // With a search: the fewest CTAs a row that keep its slices at two CTAs an SM, more while SMs are idle.
+  // Without: as many as fit on the SMs at once, so that there is one wave of them.
   int ranks = 1;
-  if (stream_rows) {
-    if (rows < 6 * sms) ranks = 2;
-  } else {
-    while (ranks < kMaxCluster && (row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 4096)))
-      ranks *= 2;
-  }
+  while (ranks < kMaxCluster && (search ? row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 4096)
+                                        : rows * ranks * 2 <= 4 * sms && row_bytes > ranks * 4096))
+    ranks *= 2;
   const int64_t vecs = row_bytes / 16;
   const int64_t slice = ceil_div(vecs, ranks);
-  const bool resident = !stream_rows && slice * 16 <= kSliceMost;
+  const bool resident = search && slice * 16 <= kSliceMost;
   TB_REQUIRE(rows * ranks <= 0x7fffffffLL && slice <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: too many rows", what);
   g.slice_vecs = static_cast<int>(slice);
   size_t smem = 16;
   if (search) smem += sizeof(Histogram);
   if (resident) smem += static_cast<size_t>(slice) * 16;
   g.maxima_rows = 0;
-  if (!resident && !search) {
-    const int64_t batches = ceil_div(ceil_div(slice, kThreads), 4);
-    if (batches * kThreads * 4 <= 64 * 1024) {
+  if (!search) {
+    const int64_t batches = ceil_div(ceil_div(slice, kBlock<false>), 4);
+    if (batches * kBlock<false> * 4 <= 48 * 1024) {
       g.maxima_rows = static_cast<int>(batches);
-      smem += static_cast<size_t>(batches) * kThreads * 4;
+      smem += static_cast<size_t>(batches) * kBlock<false> * 4;
     }
   }
-  const void *kernel = resident ? (search ? reinterpret_cast<const void *>(sample_kernel<T, true, true>)
-                                          : reinterpret_cast<const void *>(sample_kernel<T, true, false>))
-                                : (search ? reinterpret_cast<const void *>(sample_kernel<T, false, true>)
-                                          : reinterpret_cast<const void *>(sample_kernel<T, false, false>));
+  const void *kernel = !search    ? reinterpret_cast<const void *>(sample_kernel<T, false, false>)
+                       : resident ? reinterpret_cast<const void *>(sample_kernel<T, true, true>)
+                                  : reinterpret_cast<const void *>(sample_kernel<T, false, true>);
   TB_CHECK(ensure_dynamic_smem(kernel, smem, what));
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(rows * ranks));
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3(search ? kBlock<true> : kBlock<false>);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attr{};
