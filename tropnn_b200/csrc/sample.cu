@@ -58,6 +58,7 @@ struct SampleArgs {
   int64_t *tokens;
   int slice_vecs;   // 16-byte vectors of a CTA's slice
   int maxima_rows;  // batches a thread whose maxima are kept; 0: none
+  int maxima_offset;
 };
 
 // Larger for larger logits; -0 as +0.
@@ -358,8 +359,10 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
   const int begin = min(warp * per_warp, vecs), stop = min(begin + per_warp, vecs);
   float m = -INFINITY;
   constexpr int kAhead = 4;
-  constexpr bool kMaxima = !RESIDENT && !SEARCH;
-  float *maxima = reinterpret_cast<float *>(dynamic) + tid;  // kMaxima: [batch][thread]
+  const int batches = (stop - begin + 32 * kAhead - 1) / (32 * kAhead);  // of the warp
+  // The batches' maxima, [batch][thread], where there is room for them.
+  float *maxima = reinterpret_cast<float *>(dynamic + g.maxima_offset) + tid;
+  const bool has_maxima = g.maxima_rows > 0;
   auto load4 = [&](int v, uint4 (&q)[kAhead]) {  // v and every 32nd vector after it, -inf past the stretch
     const int64_t p = (vec0 + v) * kN;
     if (p >= lead && v + 32 * (kAhead - 1) < stop && p + (32 * (kAhead - 1) + 1) * kN <= end) {
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
         if (v + 32 * i < stop) kept_slice[v + 32 * i] = q[i];
       batch = max_nan(batch, vec_max<T, true>(q[i]));
     }
-    if (kMaxima && g.maxima_rows > 0) maxima[n * kThreads] = batch;
+    if (has_maxima) maxima[n * kThreads] = batch;
     m = max_nan(m, batch);
   };
   for (int v = begin + lane, n = 0; v < stop; v += 64 * kAhead, n += 2) {  // two batches on their way
@@ -439,14 +442,15 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
   }
   if (!(temperature > 0.f)) {
     uint32_t first = 0xFFFFFFFFu;
-    for (int v = tid; v < vecs; v += kThreads) {
-      const uint4 q = at(v);
-      if (vec_max<T, false>(q) < scale.best) continue;
-      float f[kN];
-      Vec<T>::unpack(q, f);
-#pragma unroll
-      for (int j = kN - 1; j >= 0; --j)
-        if (f[j] == scale.best) first = min(first, index0(v) + j);
+    for (int n = 0; n < batches; ++n) {
+      const int v = begin + n * 32 * kAhead + lane;
+      const bool some = v < stop && (!has_maxima || maxima[n * kThreads] >= scale.best);
+      if (!__any_sync(0xffffffffu, some)) continue;
+      uint4 q[kAhead];
+      again4(some ? v : stop, q);
+      each(v, mask_of<T, false>(q, scale.best, 0.f), [&](float x, uint32_t i) {
+        if (x == scale.best) first = min(first, i);
+      });
     }
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) sh.warp_count[warp] = first;
@@ -482,6 +486,31 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
     double limit_weight = -1.0;  // not known yet
     auto limit_of = [&](uint64_t all) { return fmax(static_cast<double>(top_p) * static_cast<double>(all), 0.5); };
     uint64_t base_count = 0, base_weight = 0;  // before the keys in question
+    // Of a top-k, nothing below the k-th largest of this slice's batch maxima: k tokens are above.
+    float floor_x = scale.below(kLowestZ);
+    bool few_above = false;
+    if (by_count && has_maxima && g.maxima_rows >= 2) {
+      for (int i = tid; i < kBins; i += kThreads) hist.count[i] = 0;
+      if (tid == 0) sh.found = -1;
+      __syncthreads();
+      for (int n = 0; n < batches; ++n) {
+        if (begin + n * 32 * kAhead + lane < stop) {
+          const int b = Scale::bin(scale.z(maxima[n * kThreads]));
+          if (b < kBins) atomicAdd(&hist.count[b], 1u);
+        }
+      }
+      __syncthreads();
+      const uint4 c = reinterpret_cast<const uint4 *>(hist.count)[tid];
+      uint32_t upto = c.x + c.y + c.z + c.w, all;
+      uint64_t none = 0, all_none;
+      const uint32_t own = upto;
+      block_scan(upto, none, all, all_none, sh);
+      if (upto >= limit_count && upto - own < limit_count) sh.found = tid * 4 + 3;  // within four bins
+      __syncthreads();
+      few_above = sh.found >= 0;
+      if (few_above) floor_x = scale.bin_low(sh.found);
+      __syncthreads();
+    }
     Order o;
     o.command = kFresh;
     o.bin = 0;
@@ -494,29 +523,40 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
       for (int i = tid; i < kBins; i += kThreads) hist.count[i] = hist.low[i] = hist.high[i] = 0;
       __syncthreads();
       if (fresh) {
-        const float floor_x = scale.below(kLowestZ);
-        for (int v = begin + lane; v < stop; v += 32) {
-          const uint4 q = at(v);
-          if (vec_max<T, false>(q) < floor_x) continue;
-          float f[kN];
-          Vec<T>::unpack(q, f);
+        auto enter = [&](float x) {
+          const float z = scale.z(x);
+          const int b = Scale::bin(z);
           if (by_weight) {
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-              const float z = scale.z(f[j]);
-              const int b = Scale::bin(z);
-              const uint32_t w = Scale::weight(expf(z));
-              if (b < kBins) {
-                const uint32_t old = atomicAdd(&hist.low[b], w);
-                if (old + w < old) atomicAdd(&hist.high[b], 1u);
-                if (by_count) atomicAdd(&hist.count[b], 1u);
-              }
+            const uint32_t w = Scale::weight(expf(z));
+            if (b < kBins) {
+              const uint32_t old = atomicAdd(&hist.low[b], w);
+              if (old + w < old) atomicAdd(&hist.high[b], 1u);
+              if (by_count) atomicAdd(&hist.count[b], 1u);
             }
-          } else {
+          } else if (b < kBins) {
+            atomicAdd(&hist.count[b], 1u);
+          }
+        };
+        if (few_above) {
+          for (int n = 0; n < batches; ++n) {
+            const int v = begin + n * 32 * kAhead + lane;
+            const bool some = v < stop && maxima[n * kThreads] >= floor_x;
+            if (!__any_sync(0xffffffffu, some)) continue;
+            uint4 q[kAhead];
+            again4(some ? v : stop, q);
+            each(v, mask_of<T, false>(q, floor_x, 0.f), [&](float x, uint32_t) { enter(x); });
+          }
+        } else {
+          for (int n = 0; n < batches; ++n) {
+            uint4 q[kAhead];
+            again4(begin + n * 32 * kAhead + lane, q);
 #pragma unroll
-            for (int j = 0; j < kN; ++j) {
-              const int b = Scale::bin(scale.z(f[j]));
-              if (b < kBins) atomicAdd(&hist.count[b], 1u);
+            for (int i = 0; i < kAhead; ++i) {
+              if (vec_max<T, false>(q[i]) < floor_x) continue;
+              float f[kN];
+              Vec<T>::unpack(q[i], f);
+#pragma unroll
+              for (int j = 0; j < kN; ++j) enter(f[j]);
             }
           }
         }
@@ -529,9 +569,11 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
             const uint32_t down = o.key_high - key_of(x);  // larger keys first
             const float z = scale.z(x);
             if (down <= range && Scale::bin(z) == o.bin) {
-              const uint32_t w = Scale::weight(expf(z));
-              const uint32_t old = atomicAdd(&hist.low[down >> shift], w);
-              if (old + w < old) atomicAdd(&hist.high[down >> shift], 1u);
+              if (by_weight) {
+                const uint32_t w = Scale::weight(expf(z));
+                const uint32_t old = atomicAdd(&hist.low[down >> shift], w);
+                if (old + w < old) atomicAdd(&hist.high[down >> shift], 1u);
+              }
               atomicAdd(&hist.count[down >> shift], 1u);
             }
           });
@@ -547,16 +589,20 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
         for (int r = 0; r < kMaxCluster; ++r) {
           if (r < ranks) {
             const Histogram *h = cluster.map_shared_rank(&hist, r);
-            const uint4 hc = reinterpret_cast<const uint4 *>(h->count)[tid], hl = reinterpret_cast<const uint4 *>(h->low)[tid],
-                        hh = reinterpret_cast<const uint4 *>(h->high)[tid];
-            c[0] += hc.x;
-            c[1] += hc.y;
-            c[2] += hc.z;
-            c[3] += hc.w;
-            w[0] += (uint64_t(hh.x) << 32) + hl.x;
-            w[1] += (uint64_t(hh.y) << 32) + hl.y;
-            w[2] += (uint64_t(hh.z) << 32) + hl.z;
-            w[3] += (uint64_t(hh.w) << 32) + hl.w;
+            if (by_count || !fresh) {
+              const uint4 hc = reinterpret_cast<const uint4 *>(h->count)[tid];
+              c[0] += hc.x;
+              c[1] += hc.y;
+              c[2] += hc.z;
+              c[3] += hc.w;
+            }
+            if (by_weight) {
+              const uint4 hl = reinterpret_cast<const uint4 *>(h->low)[tid], hh = reinterpret_cast<const uint4 *>(h->high)[tid];
+              w[0] += (uint64_t(hh.x) << 32) + hl.x;
+              w[1] += (uint64_t(hh.y) << 32) + hl.y;
+              w[2] += (uint64_t(hh.z) << 32) + hl.z;
+              w[3] += (uint64_t(hh.w) << 32) + hl.w;
+            }
           }
         }
         const uint32_t cs = c[0] + c[1] + c[2] + c[3];
@@ -719,7 +765,7 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
   // The sums are also kept for 32 slots of consecutive batches a warp, so that the token is found by them.
   uint64_t sum = 0;
   uint32_t tied = 0, tie_weight = 0;
-  const int batches = (stop - begin + 32 * kAhead - 1) / (32 * kAhead), per_slot = (batches + 31) / 32;
+  const int per_slot = (batches + 31) / 32;
   for (int slot = 0, n = 0; n < batches; ++slot) {
     uint64_t lane_sum = 0;
     uint32_t lane_tied = 0;
@@ -727,7 +773,7 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
       const int v = begin + n * 32 * kAhead + lane;
       uint4 q[kAhead];
       bool some = v < stop;
-      if (kMaxima && g.maxima_rows > 0 && some) some = maxima[n * kThreads] >= floor_x;
+      if (has_maxima && some) some = maxima[n * kThreads] >= floor_x;
       if (!__any_sync(0xffffffffu, some)) continue;
       again4(some ? v : stop, q);
       const uint32_t mask = mask_of<T, false>(q, floor_x, 0.f);
@@ -889,35 +935,41 @@ int launch_sample(const char *what, SampleArgs g, int64_t rows, cudaStream_t str
   const bool search = g.top_k != nullptr || g.top_k_value > 0 || g.top_p != nullptr || g.top_p_value < 1.f || g.min_p != nullptr ||
                       !(g.min_p_value <= 1.f);
   const int64_t row_bytes = g.vocab * int64_t(sizeof(T)) + 32;
-  // With a search: the fewest CTAs a row that keep its slices at two CTAs an SM, more while SMs are idle.
-  // Without: as many as fit on the SMs at once, so that there is one wave of them.
+  // With a search: a row's slices in shared memory, the fewest CTAs a row that keep two of them on an SM
+  // and more while SMs are idle, as long as all the rows' CTAs are there at once. Else, and without a
+  // search: streamed by as many CTAs a row as are there at once.
+  const int64_t slots = (search ? 2 : 4) * sms;
   int ranks = 1;
-  while (ranks < kMaxCluster && (search ? row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 4096)
-                                        : rows * ranks * 2 <= 4 * sms && row_bytes > ranks * 4096))
+  while (ranks < kMaxCluster && (row_bytes > ranks * kSliceShared || (rows * ranks * 2 <= sms && row_bytes > ranks * 4096)))
     ranks *= 2;
+  const bool resident = search && rows * ranks <= slots && ceil_div(row_bytes, ranks) <= kSliceMost;
+  if (!resident) {
+    ranks = 1;
+    while (ranks < kMaxCluster && rows * ranks * 2 <= slots && row_bytes > ranks * 4096) ranks *= 2;
+  }
   const int64_t vecs = row_bytes / 16;
   const int64_t slice = ceil_div(vecs, ranks);
-  const bool resident = search && slice * 16 <= kSliceMost;
   TB_REQUIRE(rows * ranks <= 0x7fffffffLL && slice <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: too many rows", what);
   g.slice_vecs = static_cast<int>(slice);
   size_t smem = 16;
   if (search) smem += sizeof(Histogram);
   if (resident) smem += static_cast<size_t>(slice) * 16;
+  const int threads = search ? kBlock<true> : kBlock<false>;
+  const int64_t batches = ceil_div(ceil_div(slice, threads), 4), room = resident ? 8 * 1024 : search ? 64 * 1024 : 48 * 1024;
   g.maxima_rows = 0;
-  if (!search) {
-    const int64_t batches = ceil_div(ceil_div(slice, kBlock<false>), 4);
-    if (batches * kBlock<false> * 4 <= 48 * 1024) {
-      g.maxima_rows = static_cast<int>(batches);
-      smem += static_cast<size_t>(batches) * kBlock<false> * 4;
-    }
+  g.maxima_offset = static_cast<int>(smem);
+  if (batches * threads * 4 <= room) {
+    g.maxima_rows = static_cast<int>(batches);
+    smem += static_cast<size_t>(batches) * threads * 4;
   }
   const void *kernel = !search    ? reinterpret_cast<const void *>(sample_kernel<T, false, false>)
                        : resident ? reinterpret_cast<const void *>(sample_kernel<T, true, true>)
                                   : reinterpret_cast<const void *>(sample_kernel<T, false, true>);
-  TB_CHECK(ensure_dynamic_smem(kernel, smem, what));
+  // The static part counts too: above 48 KB in all the kernel has to be told.
+  TB_CHECK(ensure_dynamic_smem(kernel, std::max<size_t>(smem, 49 * 1024), what));
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(rows * ranks));
-  config.blockDim = dim3(search ? kBlock<true> : kBlock<false>);
+  config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attr{};
