@@ -1010,7 +1010,8 @@ int launch_typed(const char *what, RecurrenceArgs g, int dtype, int64_t batch, c
       config.dynamicSmemBytes = kRingBytes<T, FORWARD>;
       const void *kernel = FORWARD ? reinterpret_cast<const void *>(recurrence_forward_tma_kernel<T>)
                                    : reinterpret_cast<const void *>(recurrence_backward_tma_kernel<T>);
-      TB_CHECK(ensure_dynamic_smem(kernel, config.dynamicSmemBytes, what));
+      // The static part counts too: above 48 KB in all the kernel has to be told.
+      TB_CHECK(ensure_dynamic_smem(kernel, std::max<size_t>(config.dynamicSmemBytes, 49 * 1024), what));
       void *args[] = {&g, &maps};
       cudaLaunchKernelExC(&config, kernel, args);
       return check_launch(what);
