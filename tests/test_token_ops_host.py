@@ -29,10 +29,10 @@ def test_cpu_tensors_are_refused() -> None:
             call()
 
 
-def test_saved_states_are_one_in_64(lib) -> None:
+def test_saved_states_are_one_in_8(lib) -> None:
     size = lib.tropnn_b200_recurrence_saved_size
-    assert size(2, 64, 10) == 2 * 1 * 10 * 4
-    assert size(2, 65, 10) == 2 * 2 * 10 * 4
+    assert size(2, 8, 10) == 2 * 1 * 10 * 4
+    assert size(2, 9, 10) == 2 * 2 * 10 * 4
     assert size(0, 64, 10) == size(2, 0, 10) == size(2, 64, 0) == size(-1, 64, 10) == 0
 
 

@@ -3,17 +3,20 @@
 //   a_t = sigmoid(f_t), c_t = 1 - a_t = sigmoid(-f_t)          (per channel)
 //   h_t = keep_t a_t h_{t-1} + c_t x_t                          (keep_t = 0 at a reset, else 1)
 //
-// The recurrence is linear, so a run of steps maps the state before it to P h + H with P the
-// product of its keep_t a_t. A warp owns a run of consecutive steps of 64 channels (two a lane): it
-// scans them in registers from h = 0 for (P, H), hands those to the other warps through shared
-// memory, composes the runs before its own into its incoming state and scans again from there.
-// A CTA's 8 warps take a tile of 8 runs. One read of gate and value, one write of h: the kernels are
-// bound by HBM traffic where enough CTAs are at work:
-//  - a cluster of up to 8 CTAs takes as many consecutive tiles at once and exchanges their maps
-//    through distributed shared memory, while the next tiles' loads are under way;
-//  - with too few channels for that (a long sequence of a small batch) the sequence is cut into
-//    chunks: a first launch computes each chunk's map, and every chunk composes those before its own.
-//    The inputs are then read twice, the second time largely from L2.
+// The recurrence is linear, so a stretch of steps maps the state before it to P h + H with P the
+// product of its keep_t a_t. A lane has two neighbouring channels, a warp 64; both are computed in f32x2
+// instructions. Two schemes, each bound by issue slots and latencies before HBM:
+//  - tiles (the forward where the channels fill the GPU: 28 blocks of 64 and more, rows of the batch counted): a warp scans a run
+//    of steps in registers, the runs' maps are exchanged, and the run is scanned again from the state
+//    before it. Gate and value are read and turned into gates once; every tile waits for a barrier.
+//  - segments (the backward, and the forward of few channels): each warp has a stretch of the sequence
+//    of its own and goes over it twice without waiting for any other, first for the stretch's map, then,
+//    with the state before it composed, for the results. The second pass finds its inputs in L2 as far
+//    as they fit (126 MB). The one exchange goes through the shared memory of a cluster of up to 8 CTAs,
+//    or through global memory between two launches.
+// Measured at 8 x 2048 x 1024 bf16: forward 29 us by tiles (3.5 TB/s of reads and writes), 41 us by
+// segments; backward 44 us by segments (3.8 TB/s), 58 us by tiles. At 1 x 65536 x 256 f16: forward 37 us
+// by segments, 46 us by tiles of chunks.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -26,14 +29,9 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kChan = 64;                    // channels of a CTA, two a lane
-// Steps of a warp's run: what leaves room for the next tile's values in 128 registers a thread.
-template <typename T>
-constexpr int kRunFwd = sizeof(T) == 2 ? 16 : 8;
-constexpr int kRunBwd = 8;
-constexpr int kTileBwd = kWarps * kRunBwd;  // 64: also the distance of the saved states
-static_assert(kTileBwd % kRunFwd<float> == 0 && kTileBwd % kRunFwd<__half> == 0, "saved states start at a run");
+constexpr int kRun = 8;  // steps that a warp takes at once, and the distance of the saved states
 constexpr int kMaxCluster = 8;
-constexpr int kSlots = 2 * 148;  // CTAs at once
+constexpr int kMapSlots = kWarps + 1;  // maps of a chunk in global memory: its segments', and its own
 
 // Two channels of one step as they lie in memory.
 template <typename T>
@@ -157,16 +155,14 @@ struct RecurrenceArgs {
   int64_t gate_batch, gate_step, value_batch, value_step;
   const float *h0;
   const uint8_t *reset;
-  int64_t steps, dim;
+  int64_t steps, dim, runs;  // runs: ceil(steps / kRun)
   int channel_blocks;
-  int ranks;            // CTAs of a cluster
-  int chunks;           // of the sequence, each a launch-grid row
-  int64_t chunk_tiles;  // tiles of a chunk
-  float2 *maps;         // chunks > 1: (P, H) or (P, R) of [batch, chunk, dim]
+  int chunks;            // of the sequence, a CTA each
+  int64_t segment_runs;  // of a warp; a chunk is kWarps segments
+  float2 *maps;          // two launches: (P, H) or (P, R) of [batch, chunk, kMapSlots, dim]
   void *h;
   float *h_last;
-  float *saved;  // [batch, saved_tiles, dim]: the state before each 64-step tile; NULL: not kept
-  int64_t saved_tiles;
+  float *saved;  // [batch, runs, dim]: the state before each run; NULL: not kept
   // backward
   const void *grad;
   const float *grad_last;
@@ -174,49 +170,405 @@ struct RecurrenceArgs {
   float *grad_h0;
 };
 
+// What a launch does: both passes with a cluster's exchange between them, or one of the two.
+enum Pass { kBoth = 0, kMaps = 1, kApply = 2 };
+
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// Exchange of run maps: (P, H) of the CTA's warps and of the cluster's CTAs, two lane channels each.
+// Neighbours in an f32 array that may start anywhere.
+__device__ __forceinline__ float2 two_floats(const float *p, int second) { return make_float2(__ldg(p), __ldg(p + second)); }
+
+// Maps of the CTA's segments and of the cluster's chunks, two lane channels each.
 struct Exchange {
+  float2 p[kWarps][32], h[kWarps][32];
+  float4 rank[kMaxCluster][32];
+};
+
+// Hands this warp's (p, h) around and returns the state before its segment, from the state before the
+// sequence. FORWARD: segments follow one another by warp and chunk, else from the last back.
+template <bool FORWARD, bool PAIRED, int PASS>
+__device__ __forceinline__ float2 exchange(const RecurrenceArgs &g, int64_t batch, const Lane<PAIRED> &at, int chunk, float2 p,
+                                           float2 h, float2 state, Exchange &ex) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool cuts = g.reset != nullptr;
+  const int place = FORWARD ? chunk : g.chunks - 1 - chunk;  // chunks before this one
+  const int order = FORWARD ? warp : kWarps - 1 - warp;      // segments of the chunk before this one
+  if (PASS != kApply) {
+    ex.p[order][lane] = p;
+    ex.h[order][lane] = h;
+    __syncthreads();
+    if (PASS == kMaps ? order == kWarps - 1 : warp < g.chunks) {  // the chunk's map
+      float2 cp = make_float2(1.f, 1.f), ch = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        ch = apply_run(ex.p[w][lane], ch, ex.h[w][lane], cuts);
+        cp = mul2(cp, ex.p[w][lane]);
+      }
+      if (PASS == kBoth) {
+        if (g.chunks > 1)
+          *cooperative_groups::this_cluster().map_shared_rank(&ex.rank[place][lane], warp) = make_float4(cp.x, cp.y, ch.x, ch.y);
+      } else {
+        float2 *m = g.maps + ((batch * g.chunks + chunk) * kMapSlots + kWarps) * g.dim + at.ch;
+        if (at.on0) m[0] = make_float2(cp.x, ch.x);
+        if (at.on1) m[kSecond<PAIRED>] = make_float2(cp.y, ch.y);
+      }
+    }
+    if (PASS == kMaps) {
+      float2 *m = g.maps + ((batch * g.chunks + chunk) * kMapSlots + order) * g.dim + at.ch;
+      if (at.on0) m[0] = make_float2(p.x, h.x);
+      if (at.on1) m[kSecond<PAIRED>] = make_float2(p.y, h.y);
+      return state;
+    }
+    if (g.chunks > 1) {
+      cluster_arrive();
+      cluster_wait();
+      for (int r = 0; r < place; ++r) {
+        const float4 m = ex.rank[r][lane];
+        state = apply_run(make_float2(m.x, m.y), state, make_float2(m.z, m.w), cuts);
+      }
+    }
+    for (int w = 0; w < order; ++w) state = apply_run(ex.p[w][lane], state, ex.h[w][lane], cuts);
+    return state;
+  }
+  // From global memory: the chunks before this one, a share a warp, then this one's segments.
+  auto map_at = [&](int c, int slot, float2 &mp, float2 &mh) {
+    const float2 *m = g.maps + ((batch * g.chunks + (FORWARD ? c : g.chunks - 1 - c)) * kMapSlots + slot) * g.dim + at.from;
+    const float2 a = __ldg(m), b = __ldg(m + at.second);
+    mp = make_float2(a.x, b.x);
+    mh = make_float2(a.y, b.y);
+  };
+  const int share = (place + kWarps - 1) / kWarps, first = min(warp * share, place), stop = min(first + share, place);
+  p = make_float2(1.f, 1.f);
+  h = make_float2(0.f, 0.f);
+#pragma unroll 8
+  for (int c = first; c < stop; ++c) {
+    float2 mp, mh;
+    map_at(c, kWarps, mp, mh);
+    h = apply_run(mp, h, mh, cuts);
+    p = mul2(mp, p);
+  }
+  ex.p[warp][lane] = p;
+  ex.h[warp][lane] = h;
+  float2 own_p[kWarps - 1], own_h[kWarps - 1];
+#pragma unroll
+  for (int w = 0; w < kWarps - 1; ++w)
+    if (w < order) map_at(place, w, own_p[w], own_h[w]);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) state = apply_run(ex.p[w][lane], state, ex.h[w][lane], cuts);
+#pragma unroll
+  for (int w = 0; w < kWarps - 1; ++w)
+    if (w < order) state = apply_run(own_p[w], state, own_h[w], cuts);
+  return state;
+}
+
+// The reset flags of a run as bits, from the byte that each lane loaded ahead.
+__device__ __forceinline__ uint32_t flag_of(const uint8_t *reset, int t0, int steps) {
+  const int t = t0 + static_cast<int>(threadIdx.x & 31);
+  return reset != nullptr && (threadIdx.x & 31) < kRun && t < steps ? __ldg(reset + t) : 0u;
+}
+
+// Tensor maps of the TMA form.
+struct SequenceMaps {
+  CUtensorMap gate, value, grad, out_gate, out_value;  // out_value: h in the forward
+};
+__device__ int g_recurrence_error = 0;
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void *src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(sm100::smem_addr(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+
+template <typename T>
+__device__ __forceinline__ float2 stage_pair(const T *row, int lane) {
+  Raw<T> r;
+  if constexpr (sizeof(T) == 4) {
+    const float2 q = reinterpret_cast<const float2 *>(row)[lane];
+    r.a = q.x;
+    r.b = q.y;
+  } else {
+    r.v = reinterpret_cast<const uint32_t *>(row)[lane];
+  }
+  return unpack<T>(r);
+}
+
+// How a warp's runs of up to three tensors come in and its results go out. TMA: a ring of stages in
+// shared memory a warp, filled two or three runs ahead across both passes; results are written over a
+// stage's inputs and stored from there, rows and channels that are not there come as zeros and are not
+// written. Needs rows 16 bytes aligned (dim and strides multiples of 8 16-bit or 4 f32 elements). Else
+// plain loads, a run ahead in registers, by pairs of channels where alignment allows.
+template <typename T, int TENSORS>
+constexpr int kStages = TENSORS == 3 && sizeof(T) == 4 ? 2 : 3;
+template <typename T, int TENSORS>
+constexpr size_t kRingBytes = size_t(kWarps) * kStages<T, TENSORS> * TENSORS * kRun * kChan * sizeof(T);
+
+template <typename T, int TENSORS, bool TMA, bool PAIRED>
+struct Stream {
+  static constexpr int kDeep = kStages<T, TENSORS>;
+  // TMA
+  T *ring;
+  uint64_t *full;
+  int *abort;
+  const CUtensorMap *maps[TENSORS];
+  int ch0, batch, s = 0;
+  uint32_t parity = 0;
+  bool stored = false;
+  // plain
+  const T *from[TENSORS];
+  int64_t stride[TENSORS];
+  int steps, second;
+  Raw<T> raw[TMA ? 1 : TENSORS][TMA ? 1 : kRun];
+
+  __device__ __forceinline__ T *rows(int tensor) { return ring + (s * TENSORS + tensor) * kRun * kChan; }
+  // Starts the loads of the tensors in `which` (a bit each) of the run at t0, `ahead` stages on.
+  __device__ __forceinline__ void fetch(int t0, uint32_t which, int ahead) {
+    if constexpr (TMA) {
+      if ((threadIdx.x & 31) == 0) {
+        int at = s + ahead;
+        if (at >= kDeep) at -= kDeep;
+        sm100::mbar_expect_tx(&full[at], __popc(which) * kRun * kChan * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < TENSORS; ++i)
+          if ((which >> i) & 1u)
+            sm100::tma_load_3d(ring + (at * TENSORS + i) * kRun * kChan, maps[i], &full[at], ch0, t0, batch);
+      }
+    } else {
+      // Steps past the end load the last one again.
+      const int most = steps - 1 - t0;
+#pragma unroll
+      for (int i = 0; i < TENSORS; ++i) {
+        if (!((which >> i) & 1u)) continue;
+        const T *p = from[i] + t0 * stride[i];
+        if (most >= kRun - 1) {
+#pragma unroll
+          for (int j = 0; j < kRun; ++j, p += stride[i]) raw[i][j] = load_raw<T, PAIRED>(p, second);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) raw[i][j] = load_raw<T, PAIRED>(p + min(j, most) * stride[i], second);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void wait() {
+    if constexpr (TMA) sm100::mbar_wait(&full[s], parity, abort, &g_recurrence_error);
+  }
+  __device__ __forceinline__ float2 get(int tensor, int j) {
+    if constexpr (TMA) return stage_pair<T>(rows(tensor) + j * kChan, threadIdx.x & 31);
+    else return unpack<T>(raw[tensor][j]);
+  }
+  // The stage has been read.
+  __device__ __forceinline__ void next() {
+    if constexpr (TMA) {
+      if (++s == kDeep) {
+        s = 0;
+        parity ^= 1;
+      }
+    }
+  }
+};
+
+// Items of a warp: its segment's runs for the maps, then again for the results, in one order. Steps are
+// below 2^31.
+template <bool FORWARD, int PASS>
+struct Items {
+  int first, count, total;  // runs, items
+  __device__ __forceinline__ Items(const RecurrenceArgs &g, int chunk, int warp) {
+    const int64_t runs = g.runs, at = min64((int64_t(chunk) * kWarps + warp) * g.segment_runs, runs);
+    first = static_cast<int>(at);
+    count = static_cast<int>(min64(g.segment_runs, runs - at));
+    total = PASS == kBoth ? 2 * count : count;
+  }
+  __device__ __forceinline__ int start(int i) const {  // first step of item i
+    const int n = PASS == kBoth && i >= count ? i - count : i;
+    return (FORWARD ? first + n : first + count - 1 - n) * kRun;
+  }
+};
+
+template <typename T, bool TMA, bool PAIRED, int PASS>
+__global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
+    recurrence_forward_kernel(const RecurrenceArgs g, const __grid_constant__ SequenceMaps maps) {
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  __shared__ Exchange ex;
+  __shared__ uint64_t full[kWarps][4];
+  __shared__ int abort;
+  using In = Stream<T, 2, TMA, PAIRED>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit = blockIdx.x / g.chunks, chunk = blockIdx.x - unit * g.chunks;
+  const int64_t batch = unit / g.channel_blocks;
+  const int block = unit - static_cast<int>(batch) * g.channel_blocks;
+  const Lane<PAIRED> at(block, g.dim);
+  const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
+  const Items<true, PASS> items(g, chunk, warp);
+  const int total = items.total, steps = static_cast<int>(g.steps);
+
+  In in;
+  if constexpr (TMA) {
+    in.ring = reinterpret_cast<T *>(dynamic) + size_t(warp) * In::kDeep * 2 * kRun * kChan;
+    in.full = full[warp];
+    in.abort = &abort;
+    in.maps[0] = &maps.gate;
+    in.maps[1] = &maps.value;
+    in.ch0 = block * kChan;
+    in.batch = static_cast<int>(batch);
+    if (threadIdx.x == 0) abort = 0;
+    if (lane == 0) {
+#pragma unroll
+      for (int s = 0; s < In::kDeep; ++s) sm100::mbar_init(&full[warp][s], 1);
+      sm100::mbar_init_fence();
+      sm100::fence_proxy_async_smem();
+    }
+    __syncthreads();
+  } else {
+    in.from[0] = static_cast<const T *>(g.gate) + batch * g.gate_batch + at.from;
+    in.from[1] = static_cast<const T *>(g.value) + batch * g.value_batch + at.from;
+    in.stride[0] = g.gate_step;
+    in.stride[1] = g.value_step;
+    in.steps = steps;
+    in.second = at.second;
+  }
+  const int ahead = TMA ? In::kDeep : 1;
+  for (int i = 0; i < ahead; ++i)
+    if (i < total) in.fetch(items.start(i), 3, i);
+  uint32_t flag = total > 0 ? flag_of(reset, items.start(0), steps) : 0;
+
+  float2 h = make_float2(0.f, 0.f), p = make_float2(1.f, 1.f);
+  int item = 0;
+  // One run: step(j, a, c x) for each of its steps, then the loads of a later one.
+  auto gates_of = [&](float2 (&a)[kRun], float2 (&b)[kRun]) {
+    in.wait();
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      float2 c;
+      gates2(in.get(0, j), a[j], c);
+      b[j] = mul2(c, in.get(1, j));
+    }
+  };
+  auto flags = [&]() -> uint32_t {
+    if (reset == nullptr) return 0;
+    const uint32_t cut = __ballot_sync(0xffffffffu, flag != 0);
+    flag = item + 1 < total ? flag_of(reset, items.start(item + 1), steps) : 0;
+    return cut;
+  };
+  if (PASS != kApply) {
+    for (; item < items.count; ++item) {
+      const int t0 = items.start(item);
+      const int n = min(kRun, steps - t0);
+      const uint32_t cut = flags();
+      float2 a[kRun], b[kRun];
+      gates_of(a, b);
+      if constexpr (TMA) __syncwarp();  // all lanes have read the stage
+      if (item + ahead < total) in.fetch(items.start(item + ahead), 3, 0);
+      in.next();
+      if (n == kRun && cut == 0) {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          h = fma2(a[j], h, b[j]);
+          p = mul2(p, a[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          if (j < n) {
+            if ((cut >> j) & 1u) h = p = make_float2(0.f, 0.f);
+            h = fma2(a[j], h, b[j]);
+            p = mul2(p, a[j]);
+          }
+        }
+      }
+    }
+  }
+  float2 state = make_float2(0.f, 0.f);
+  if (g.h0 != nullptr) state = two_floats(g.h0 + batch * g.dim + at.from, at.second);
+  state = exchange<true, PAIRED, PASS>(g, batch, at, chunk, p, h, state, ex);
+  if (PASS == kMaps) return;
+
+  T *out = static_cast<T *>(g.h) + batch * g.steps * g.dim + at.ch;
+  for (; item < total; ++item) {
+    const int t0 = items.start(item);
+    const int n = min(kRun, steps - t0);
+    const uint32_t cut = flags();
+    float2 a[kRun], b[kRun];
+    gates_of(a, b);
+    if constexpr (!TMA)
+      if (item + 1 < total) in.fetch(items.start(item + 1), 3, 0);
+    if (g.saved != nullptr) {
+      float *s = g.saved + (batch * g.runs + t0 / kRun) * g.dim + at.ch;
+      if (at.on0) s[0] = state.x;
+      if (at.on1) s[kSecond<PAIRED>] = state.y;
+    }
+    auto put = [&](int j) {
+      if constexpr (TMA) store_pair<T, true>(in.rows(1) + j * kChan + 2 * lane, state, true, true);
+      else store_pair<T, PAIRED>(out + int64_t(t0 + j) * g.dim, state, at.on0, at.on1);
+    };
+    if (n == kRun && cut == 0) {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        state = fma2(a[j], state, b[j]);
+        put(j);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (j < n) {
+          if ((cut >> j) & 1u) state = make_float2(0.f, 0.f);
+          state = fma2(a[j], state, b[j]);
+          put(j);
+        }
+      }
+    }
+    if constexpr (TMA) {
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(&maps.out_value, in.rows(1), in.ch0, t0, in.batch);
+        sm100::bulk_commit();
+        bulk_wait_read<1>();  // the stage before this one has been read by its store
+      }
+      // That stage's next run comes in; the first run's stage has no store before it.
+      if (in.stored && item - 1 + In::kDeep < total) in.fetch(items.start(item - 1 + In::kDeep), 3, In::kDeep - 1);
+      in.stored = true;
+    }
+    in.next();
+  }
+  if (warp == kWarps - 1 && chunk == g.chunks - 1) {
+    float *last = g.h_last + batch * g.dim + at.ch;
+    if (at.on0) last[0] = state.x;
+    if (at.on1) last[kSecond<PAIRED>] = state.y;
+  }
+  if (TMA && lane == 0) sm100::bulk_wait_read_all();
+}
+
+// Forward with channels enough to fill the GPU: tiles in the order of the sequence. A CTA's 8 warps take a
+// tile of 8 runs of a warp each, scan them in registers for their maps, exchange those and scan again
+// from the state before each run: gate and value are read and turned into gates once, at the price of a
+// barrier a tile. A cluster of up to 8 CTAs takes as many consecutive tiles at once and exchanges their
+// maps through distributed shared memory; the next tiles' loads are under way meanwhile.
+// Steps of a warp's run: what leaves room for the next tile's values in 128 registers a thread.
+template <typename T>
+constexpr int kTileRun = sizeof(T) == 2 ? 16 : 8;
+constexpr int kTileStages = 3;
+template <typename T>
+constexpr size_t kTileRingBytes = size_t(kWarps) * kTileStages * 2 * kTileRun<T> * kChan * sizeof(T);
+
+__device__ __forceinline__ void put_two_floats(float *p, float2 v) {
+  p[0] = v.x;
+  p[1] = v.y;
+}
+
+// Exchange of a tile: (P, H) of the CTA's warps and of the cluster's CTAs, two lane channels each.
+struct TileExchange {
   float2 p[2][kWarps][32], h[2][kWarps][32];
   float4 rank[2][kMaxCluster][32];
 };
 
-// The chunks' maps before (FORWARD) or after this one, composed onto `state`: the warps take a share
-// each, in order.
-template <bool PAIRED, bool FORWARD>
-__device__ __forceinline__ float2 through_chunks(const RecurrenceArgs &g, int64_t batch, int64_t ch, bool on0, bool on1,
-                                                 int chunk, float2 state, Exchange &ex) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int count = FORWARD ? chunk : g.chunks - 1 - chunk;
-  const int share = (count + kWarps - 1) / kWarps;
-  const int first = min(warp * share, count), stop = min(first + share, count);
-  float2 p = make_float2(1.f, 1.f), h = make_float2(0.f, 0.f);
-#pragma unroll 4
-  for (int i = first; i < stop; ++i) {
-    const int q = FORWARD ? i : g.chunks - 1 - i;
-    const float2 *m = g.maps + (batch * g.chunks + q) * g.dim + ch;
-    float2 a = make_float2(1.f, 0.f), b = make_float2(1.f, 0.f);
-    if (on0) a = __ldg(m);
-    if (on1) b = __ldg(m + kSecond<PAIRED>);
-    const float2 mp = make_float2(a.x, b.x);
-    h = apply_run(mp, h, make_float2(a.y, b.y), true);
-    p = mul2(mp, p);
-  }
-  ex.p[0][warp][lane] = p;
-  ex.h[0][warp][lane] = h;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) state = apply_run(ex.p[0][w][lane], state, ex.h[0][w][lane], true);
-  __syncthreads();
-  return state;
-}
-
-// Hands this warp's (p, h) around: returns the state before its run, and moves `state` past the
-// cluster's tiles. ORDER 1: the runs follow one another by warp, -1: from the last warp back.
-template <int ORDER>
-__device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, float2 h, float2 &state, int ranks, int rank,
+// Hands this warp's (p, h) around: returns the state before its run, and moves `state` past the cluster's
+// tiles.
+__device__ __forceinline__ float2 tile_exchange(TileExchange &ex, int buf, float2 p, float2 h, float2 &state, int ranks, int rank,
                                            bool cuts) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ex.p[buf][warp][lane] = p;
@@ -226,7 +578,7 @@ __device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, floa
   if (ranks == 1) {
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      const int w = ORDER > 0 ? i : kWarps - 1 - i;
+      const int w = i;
       if (w == warp) in = state;
       state = apply_run(ex.p[buf][w][lane], state, ex.h[buf][w][lane], cuts);
     }
@@ -236,7 +588,7 @@ __device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, floa
     float2 cp = make_float2(1.f, 1.f), ch = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      const int w = ORDER > 0 ? i : kWarps - 1 - i;
+      const int w = i;
       const float2 pw = ex.p[buf][w][lane];
       ch = apply_run(pw, ch, ex.h[buf][w][lane], cuts);
       cp = mul2(cp, pw);
@@ -252,8 +604,8 @@ __device__ __forceinline__ float2 exchange(Exchange &ex, int buf, float2 p, floa
   }
 #pragma unroll
   for (int i = 0; i < kWarps - 1; ++i) {
-    const int w = ORDER > 0 ? i : kWarps - 1 - i;
-    if (ORDER > 0 ? w < warp : w > warp) in = apply_run(ex.p[buf][w][lane], in, ex.h[buf][w][lane], cuts);
+    const int w = i;
+    if (w < warp) in = apply_run(ex.p[buf][w][lane], in, ex.h[buf][w][lane], cuts);
   }
   return in;
 }
@@ -292,13 +644,14 @@ __device__ __forceinline__ void scan_run(const float2 (&a)[RUN], const float2 (&
     }
   }
 }
-// The run from the state before it: store(j, h_j).
-template <int RUN, typename Store>
+// The run from the state before it: save(j, h_{j-1}) at every kRun-th step, store(j, h_j).
+template <int RUN, typename Save, typename Store>
 __device__ __forceinline__ void emit_run(const float2 (&a)[RUN], const float2 (&b)[RUN], int n, uint32_t cut, bool plain,
-                                         float2 in, Store store) {
+                                         float2 in, Save save, Store store) {
   if (plain) {
 #pragma unroll
     for (int j = 0; j < RUN; ++j) {
+      if (j % kRun == 0) save(j, in);
       in = fma2(a[j], in, b[j]);
       store(j, in);
     }
@@ -306,6 +659,7 @@ __device__ __forceinline__ void emit_run(const float2 (&a)[RUN], const float2 (&
 #pragma unroll
     for (int j = 0; j < RUN; ++j) {
       if (j < n) {
+        if (j % kRun == 0) save(j, in);
         if ((cut >> j) & 1u) in = make_float2(0.f, 0.f);
         in = fma2(a[j], in, b[j]);
         store(j, in);
@@ -313,89 +667,13 @@ __device__ __forceinline__ void emit_run(const float2 (&a)[RUN], const float2 (&
     }
   }
 }
-// Backward: a run's maps, (p, h) forward and (p, r) from its end.
-template <int RUN>
-__device__ __forceinline__ void scan_run_back(const float2 (&a)[RUN], const float2 (&c)[RUN], const float2 (&x)[RUN],
-                                              const float2 (&gt)[RUN], int n, uint32_t cut, bool plain, float2 &p,
-                                              float2 &h, float2 &r) {
-  const float2 zero = make_float2(0.f, 0.f);
-  h = r = zero;
-  p = make_float2(1.f, 1.f);
-  if (plain) {
-#pragma unroll
-    for (int j = 0; j < RUN; ++j) {
-      h = fma2(a[j], h, mul2(c[j], x[j]));
-      p = mul2(p, a[j]);
-    }
-#pragma unroll
-    for (int j = RUN - 1; j >= 0; --j) r = mul2(a[j], add2(gt[j], r));
-  } else {
-#pragma unroll
-    for (int j = 0; j < RUN; ++j) {
-      if (j < n) {
-        if ((cut >> j) & 1u) h = p = zero;
-        h = fma2(a[j], h, mul2(c[j], x[j]));
-        p = mul2(p, a[j]);
-      }
-    }
-#pragma unroll
-    for (int j = RUN - 1; j >= 0; --j) {
-      if (j < n) {
-        r = mul2(a[j], add2(gt[j], r));
-        if ((cut >> j) & 1u) r = zero;
-      }
-    }
-  }
-}
-// The run's gradients from the state before it and r after it: store(j, grad_gate, grad_value), from
-// the last step back. x is used up.
-template <int RUN, typename Store>
-__device__ __forceinline__ void emit_run_back(const float2 (&a)[RUN], const float2 (&c)[RUN], float2 (&x)[RUN],
-                                              const float2 (&gt)[RUN], int n, uint32_t cut, bool plain, float2 h_in,
-                                              float2 r_in, Store store) {
-  const float2 zero = make_float2(0.f, 0.f), minus = make_float2(-1.f, -1.f);
-  if (plain) {
-#pragma unroll
-    for (int j = 0; j < RUN; ++j) {
-      const float2 v = x[j];
-      x[j] = fma2(v, minus, h_in);  // keep h_{t-1} - x
-      h_in = fma2(a[j], h_in, mul2(c[j], v));
-    }
-#pragma unroll
-    for (int j = RUN - 1; j >= 0; --j) {
-      const float2 ds = add2(gt[j], r_in), gx = mul2(c[j], ds);
-      r_in = mul2(a[j], ds);
-      store(j, mul2(mul2(a[j], gx), x[j]), gx);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < RUN; ++j) {
-      if (j < n) {
-        const float2 v = x[j];
-        if ((cut >> j) & 1u) h_in = zero;
-        x[j] = fma2(v, minus, h_in);
-        h_in = fma2(a[j], h_in, mul2(c[j], v));
-      }
-    }
-#pragma unroll
-    for (int j = RUN - 1; j >= 0; --j) {
-      if (j < n) {
-        const float2 ds = add2(gt[j], r_in), gx = mul2(c[j], ds);
-        r_in = mul2(a[j], ds);
-        store(j, mul2(mul2(a[j], gx), x[j]), gx);
-        if ((cut >> j) & 1u) r_in = zero;
-      }
-    }
-  }
-}
-
 template <typename T, bool PAIRED>
-__global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const RecurrenceArgs g) {
-  constexpr int kRun = kRunFwd<T>, kTile = kWarps * kRun;
-  __shared__ Exchange ex;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
-  const int unit = blockIdx.x / g.ranks;
+__global__ void __launch_bounds__(kThreads, 2) recurrence_tiles_kernel(const RecurrenceArgs g) {
+  constexpr int kLong = kTileRun<T>, kTile = kWarps * kLong;
+  __shared__ TileExchange ex;
+  const int warp = threadIdx.x >> 5;
+  const int rank = blockIdx.x % g.chunks;
+  const int unit = blockIdx.x / g.chunks;
   const int64_t batch = unit / g.channel_blocks;
   const Lane<PAIRED> at(unit % g.channel_blocks, g.dim);
   const int64_t ch = at.ch;
@@ -404,254 +682,106 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_forward_kernel(const R
   const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + at.from;
   T *out = static_cast<T *>(g.h) + batch * g.steps * g.dim + ch;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
-  const int64_t first = chunk * g.chunk_tiles * kTile, stop = min64(g.steps, first + g.chunk_tiles * kTile);
-  if (g.ranks > 1) cluster_arrive();
+  const int64_t first = 0, stop = g.steps;
+  if (g.chunks > 1) cluster_arrive();
 
-  Raw<T> rf[kRun], rx[kRun];
+  Raw<T> rf[kLong], rx[kLong];
   auto load = [&](int64_t t0) {
     if (t0 >= stop) return;
     // Steps past the end load the last one again.
     const int64_t most = stop - 1 - t0;
     const T *pf = gate + t0 * g.gate_step, *px = value + t0 * g.value_step;
-    if (most >= kRun - 1) {
+    if (most >= kLong - 1) {
 #pragma unroll
-      for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step) {
+      for (int j = 0; j < kLong; ++j, pf += g.gate_step, px += g.value_step) {
         rf[j] = load_raw<T, PAIRED>(pf, at.second);
         rx[j] = load_raw<T, PAIRED>(px, at.second);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) {
+      for (int j = 0; j < kLong; ++j) {
         rf[j] = load_raw<T, PAIRED>(pf + min64(j, most) * g.gate_step, at.second);
         rx[j] = load_raw<T, PAIRED>(px + min64(j, most) * g.value_step, at.second);
       }
     }
   };
-  load(first + rank * kTile + warp * kRun);
+  load(first + rank * kTile + warp * kLong);
   float2 state = make_float2(0.f, 0.f);  // the state before the cluster's tiles, the same in every warp
   if (g.h0 != nullptr) {
     const float *p = g.h0 + batch * g.dim + ch;
     if (on0) state.x = p[0];
     if (on1) state.y = p[kSecond<PAIRED>];
   }
-  if (chunk > 0) state = through_chunks<PAIRED, true>(g, batch, ch, on0, on1, chunk, state, ex);
-  if (g.ranks > 1) cluster_wait();
+  if (g.chunks > 1) cluster_wait();
 
   int buf = 0;
-  for (int64_t tile = first; tile < stop; tile += int64_t(g.ranks) * kTile, buf ^= 1) {
-    const int64_t t0 = tile + rank * kTile + warp * kRun;
-    const int n = static_cast<int>(t0 >= stop ? 0 : min64(kRun, stop - t0));
+  for (int64_t tile = first; tile < stop; tile += int64_t(g.chunks) * kTile, buf ^= 1) {
+    const int64_t t0 = tile + rank * kTile + warp * kLong;
+    const int n = static_cast<int>(t0 >= stop ? 0 : min64(kLong, stop - t0));
     const uint32_t cut = reset_bits(reset, t0, n);
-    const bool plain = n == kRun && cut == 0;
-    float2 a[kRun], b[kRun], p, h;
+    const bool plain = n == kLong && cut == 0;
+    float2 a[kLong], b[kLong], p, h;
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
+    for (int j = 0; j < kLong; ++j) {
       float2 c;
       gates2(unpack<T>(rf[j]), a[j], c);
       b[j] = mul2(c, unpack<T>(rx[j]));
     }
-    scan_run<kRun>(a, b, n, cut, plain, p, h);
-    load(t0 + int64_t(g.ranks) * kTile);
-    const float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank, reset != nullptr);
-    if (g.saved != nullptr && (warp * kRun) % kTileBwd == 0 && n > 0) {
-      float *s = g.saved + (batch * g.saved_tiles + t0 / kTileBwd) * g.dim + ch;
-      if (on0) s[0] = in.x;
-      if (on1) s[kSecond<PAIRED>] = in.y;
-    }
+    scan_run<kLong>(a, b, n, cut, plain, p, h);
+    load(t0 + int64_t(g.chunks) * kTile);
+    const float2 in = tile_exchange(ex, buf, p, h, state, g.chunks, rank, reset != nullptr);
     T *po = out + t0 * g.dim;
-    emit_run<kRun>(a, b, n, cut, plain, in, [&](int, float2 v) {
+    auto save = [&](int j, float2 v) {
+      if (g.saved == nullptr) return;
+      float *s = g.saved + (batch * g.runs + (t0 + j) / kRun) * g.dim + ch;
+      if (on0) s[0] = v.x;
+      if (on1) s[kSecond<PAIRED>] = v.y;
+    };
+    emit_run<kLong>(a, b, n, cut, plain, in, save, [&](int, float2 v) {
       store_pair<T, PAIRED>(po, v, on0, on1);
       po += g.dim;
     });
   }
-  if (warp == 0 && rank == 0 && chunk == g.chunks - 1) {
+  if (warp == 0 && rank == 0) {
     float *p = g.h_last + batch * g.dim + ch;
     if (on0) p[0] = state.x;
     if (on1) p[kSecond<PAIRED>] = state.y;
   }
 }
 
-// Backward. With r_t = keep_t a_t ds_t the part of step t's gradient that reaches h_{t-1}:
-//   ds_t = grad_t + r_{t+1},  grad_value = c ds,  grad_gate = a c (keep h_{t-1} - x) ds
-// h_{t-1} is scanned again from the state saved before the tile (in 32 bits; h itself is not
-// read), the same way as forward within the tile; r comes from the sequence's end, across the
-// cluster's tiles. Both have the same P.
-template <typename T, bool PAIRED>
-__global__ void __launch_bounds__(kThreads, 2) recurrence_backward_kernel(const RecurrenceArgs g) {
-  constexpr int kRun = kRunBwd, kTile = kTileBwd;
-  __shared__ Exchange ex;
-  __shared__ float2 run_h[2][kWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
-  const int unit = blockIdx.x / g.ranks;
-  const int64_t batch = unit / g.channel_blocks;
-  const Lane<PAIRED> at(unit % g.channel_blocks, g.dim);
-  const int64_t ch = at.ch;
-  const bool on0 = at.on0, on1 = at.on1;
-  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + at.from;
-  const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + at.from;
-  const T *grad = g.grad != nullptr ? static_cast<const T *>(g.grad) + batch * g.steps * g.dim + at.from : nullptr;
-  T *grad_gate = static_cast<T *>(g.grad_gate) + batch * g.steps * g.dim + ch;
-  T *grad_value = static_cast<T *>(g.grad_value) + batch * g.steps * g.dim + ch;
-  const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
-  const int64_t first = chunk * g.chunk_tiles, stop = min64(g.saved_tiles, first + g.chunk_tiles);
-  if (g.ranks > 1) cluster_arrive();
-
-  Raw<T> rf[kRun], rx[kRun], rg[kRun] = {};
-  float2 before = make_float2(0.f, 0.f);
-  auto steps_of = [&](int64_t k) -> int {
-    const int64_t t0 = k * kTile + warp * kRun;
-    return static_cast<int>(k < first || t0 >= g.steps ? 0 : min64(kRun, g.steps - t0));
-  };
-  auto load = [&](int64_t k) {
-    if (k < first) return;
-    // Steps past the end load the last one again.
-    const int64_t t0 = k * kTile + warp * kRun, from = min64(t0, g.steps - 1), most = g.steps - 1 - from;
-    const T *pf = gate + from * g.gate_step, *px = value + from * g.value_step, *pg = grad + from * g.dim;
-    if (most >= kRun - 1) {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j, pf += g.gate_step, px += g.value_step, pg += g.dim) {
-        rf[j] = load_raw<T, PAIRED>(pf, at.second);
-        rx[j] = load_raw<T, PAIRED>(px, at.second);
-        if (grad != nullptr) rg[j] = load_raw<T, PAIRED>(pg, at.second);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        const int64_t d = min64(j, most);
-        rf[j] = load_raw<T, PAIRED>(pf + d * g.gate_step, at.second);
-        rx[j] = load_raw<T, PAIRED>(px + d * g.value_step, at.second);
-        if (grad != nullptr) rg[j] = load_raw<T, PAIRED>(pg + d * g.dim, at.second);
-      }
-    }
-    const float *p = g.saved + (batch * g.saved_tiles + k) * g.dim + at.from;
-    before = make_float2(__ldg(p), __ldg(p + at.second));
-  };
-  load(stop - 1 - rank);
-  float2 back = make_float2(0.f, 0.f);  // r of the step after the cluster's tiles
-  if (g.grad_last != nullptr) {
-    const float *p = g.grad_last + batch * g.dim + ch;
-    if (on0) back.x = p[0];
-    if (on1) back.y = p[kSecond<PAIRED>];
-  }
-  if (chunk < g.chunks - 1) back = through_chunks<PAIRED, false>(g, batch, ch, on0, on1, chunk, back, ex);
-  if (g.ranks > 1) cluster_wait();
-
-  int buf = 0;
-  for (int64_t last = stop - 1; last >= first; last -= g.ranks, buf ^= 1) {
-    const int64_t k = last - rank, t0 = k * kTile + warp * kRun;
-    const int n = steps_of(k);
-    const uint32_t cut = reset_bits(reset, t0, n);
-
-    const bool plain = n == kRun && cut == 0;
-    float2 a[kRun], c[kRun], x[kRun], gt[kRun], p, h, r, h_in = before;
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      gates2(unpack<T>(rf[j]), a[j], c[j]);
-      x[j] = unpack<T>(rx[j]);
-      gt[j] = unpack<T>(rg[j]);
-    }
-    scan_run_back<kRun>(a, c, x, gt, n, cut, plain, p, h, r);
-    load(k - g.ranks);
-    run_h[buf][warp][lane] = h;
-    const float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank, reset != nullptr);
-#pragma unroll
-    for (int w = 0; w < kWarps - 1; ++w) {
-      if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane], reset != nullptr);
-    }
-    T *pf = grad_gate + t0 * g.dim, *px = grad_value + t0 * g.dim;
-    emit_run_back<kRun>(a, c, x, gt, n, cut, plain, h_in, r_in, [&](int j, float2 gf, float2 gx) {
-      store_pair<T, PAIRED>(px + j * g.dim, gx, on0, on1);
-      store_pair<T, PAIRED>(pf + j * g.dim, gf, on0, on1);
-    });
-  }
-  if (warp == 0 && rank == 0 && chunk == 0 && g.grad_h0 != nullptr) {
-    float *p = g.grad_h0 + batch * g.dim + ch;
-    if (on0) p[0] = back.x;
-    if (on1) p[kSecond<PAIRED>] = back.y;
-  }
-}
-
-// The same two kernels with the data brought by TMA: each warp has its own ring of stages in shared
-// memory, loads its runs of [steps x 64 channels] into them two or three tiles ahead, writes its
-// results over the inputs of the stage and stores them from there. No registers hold data in
-// flight, no address is computed an element, rows and channels that are not there come as zeros and
-// are not written. Needs rows 16 bytes aligned (dim and strides multiples of 8 16-bit or 4 f32
-// elements); the kernels above serve all else.
-struct SequenceMaps {
-  CUtensorMap gate, value, grad, out_gate, out_value;  // out_value: h in the forward
-};
-__device__ int g_recurrence_error = 0;
-
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void *src, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(sm100::smem_addr(src)), "r"(x), "r"(y), "r"(z)
-               : "memory");
-}
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
-
-template <typename T>
-__device__ __forceinline__ Raw<T> stage_raw(const T *row, int lane) {
-  Raw<T> r;
-  if constexpr (sizeof(T) == 4) {
-    const float2 q = reinterpret_cast<const float2 *>(row)[lane];
-    r.a = q.x;
-    r.b = q.y;
-  } else {
-    r.v = reinterpret_cast<const uint32_t *>(row)[lane];
-  }
-  return r;
-}
-
-// Neighbours in an f32 array that may start anywhere.
-__device__ __forceinline__ float2 two_floats(const float *p) { return make_float2(__ldg(p), __ldg(p + 1)); }
-__device__ __forceinline__ void put_two_floats(float *p, float2 v) {
-  p[0] = v.x;
-  p[1] = v.y;
-}
-
-template <typename T>
-constexpr int kStagesFwd = 3;
-template <typename T>
-constexpr int kStagesBwd = sizeof(T) == 2 ? 3 : 2;
-template <typename T, bool FORWARD>
-constexpr size_t kRingBytes = FORWARD ? size_t(kWarps) * kStagesFwd<T> * 2 * kRunFwd<T> * kChan * sizeof(T)
-                                      : size_t(kWarps) * kStagesBwd<T> * 3 * kRunBwd * kChan * sizeof(T);
-
+// The same with TMA: each warp has a ring of its own.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
-    recurrence_forward_tma_kernel(const RecurrenceArgs g, const __grid_constant__ SequenceMaps maps) {
-  constexpr int kRun = kRunFwd<T>, kTile = kWarps * kRun, kStages = kStagesFwd<T>;
-  constexpr uint32_t kBytes = 2 * kRun * kChan * sizeof(T);
+    recurrence_tiles_tma_kernel(const RecurrenceArgs g, const __grid_constant__ SequenceMaps maps) {
+  constexpr int kLong = kTileRun<T>, kTile = kWarps * kLong, kStages = kTileStages;
+  constexpr uint32_t kBytes = 2 * kLong * kChan * sizeof(T);
   extern __shared__ __align__(128) uint8_t dynamic[];
-  __shared__ Exchange ex;
+  __shared__ TileExchange ex;
   __shared__ uint64_t full[kWarps][kStages];
   __shared__ int abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
-  const int unit = blockIdx.x / g.ranks;
+  const int rank = blockIdx.x % g.chunks;
+  const int unit = blockIdx.x / g.chunks;
   const int batch = unit / g.channel_blocks, ch0 = unit % g.channel_blocks * kChan;
   const int64_t ch = ch0 + 2 * lane;
   const bool on = ch < g.dim;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
-  const int64_t first = chunk * g.chunk_tiles * kTile, stop = min64(g.steps, first + g.chunk_tiles * kTile);
-  const int64_t stride = int64_t(g.ranks) * kTile;
-  T *ring = reinterpret_cast<T *>(dynamic) + size_t(warp) * kStages * 2 * kRun * kChan;
-  auto stage = [&](int s) -> T * { return ring + s * 2 * kRun * kChan; };
+  const int64_t first = 0, stop = g.steps;
+  const int64_t stride = int64_t(g.chunks) * kTile;
+  T *ring = reinterpret_cast<T *>(dynamic) + size_t(warp) * kStages * 2 * kLong * kChan;
+  auto stage = [&](int s) -> T * { return ring + s * 2 * kLong * kChan; };
   auto fetch = [&](int64_t t0, int s) {  // one lane
     if (t0 >= stop) return;
     sm100::mbar_expect_tx(&full[warp][s], kBytes);
     sm100::tma_load_3d(stage(s), &maps.gate, &full[warp][s], ch0, static_cast<int>(t0), batch);
-    sm100::tma_load_3d(stage(s) + kRun * kChan, &maps.value, &full[warp][s], ch0, static_cast<int>(t0), batch);
+    sm100::tma_load_3d(stage(s) + kLong * kChan, &maps.value, &full[warp][s], ch0, static_cast<int>(t0), batch);
   };
   auto flag_of = [&](int64_t t0) -> uint32_t {
-    return reset != nullptr && lane < kRun && t0 + lane < stop ? __ldg(reset + t0 + lane) : 0u;
+    return reset != nullptr && lane < kLong && t0 + lane < stop ? __ldg(reset + t0 + lane) : 0u;
   };
-  if (g.ranks > 1) cluster_arrive();
+  if (g.chunks > 1) cluster_arrive();
   if (threadIdx.x == 0) abort = 0;
-  const int64_t t_first = first + rank * kTile + warp * kRun;
+  const int64_t t_first = first + rank * kTile + warp * kLong;
   if (lane == 0) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) sm100::mbar_init(&full[warp][s], 1);
@@ -664,36 +794,36 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
 
   float2 state = make_float2(0.f, 0.f);
-  if (g.h0 != nullptr && on) state = two_floats(g.h0 + batch * g.dim + ch);
-  if (chunk > 0) state = through_chunks<true, true>(g, batch, ch, on, on, chunk, state, ex);
-  if (g.ranks > 1) cluster_wait();
+  if (g.h0 != nullptr && on) state = two_floats(g.h0 + batch * g.dim + ch, 1);
+  if (g.chunks > 1) cluster_wait();
 
   int buf = 0, s = 0;
   uint32_t parity = 0;
   for (int64_t tile = first, t0 = t_first; tile < stop; tile += stride, t0 += stride, buf ^= 1) {
-    const int n = static_cast<int>(t0 >= stop ? 0 : min64(kRun, stop - t0));
+    const int n = static_cast<int>(t0 >= stop ? 0 : min64(kLong, stop - t0));
     const uint32_t cut = __ballot_sync(0xffffffffu, flag != 0);
     flag = flag_of(t0 + stride);
-    const bool plain = n == kRun && cut == 0;
+    const bool plain = n == kLong && cut == 0;
     if (n > 0) sm100::mbar_wait(&full[warp][s], parity, &abort, &g_recurrence_error);
     T *rows = stage(s);
-    float2 a[kRun], b[kRun], p, h;
+    float2 a[kLong], b[kLong], p, h;
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
+    for (int j = 0; j < kLong; ++j) {
       float2 c;
-      gates2(unpack<T>(stage_raw<T>(rows + j * kChan, lane)), a[j], c);
-      b[j] = mul2(c, unpack<T>(stage_raw<T>(rows + (kRun + j) * kChan, lane)));
+      gates2(stage_pair<T>(rows + j * kChan, lane), a[j], c);
+      b[j] = mul2(c, stage_pair<T>(rows + (kLong + j) * kChan, lane));
     }
-    scan_run<kRun>(a, b, n, cut, plain, p, h);
-    const float2 in = exchange<1>(ex, buf, p, h, state, g.ranks, rank, reset != nullptr);
-    if (g.saved != nullptr && (warp * kRun) % kTileBwd == 0 && n > 0 && on)
-      put_two_floats(g.saved + (batch * g.saved_tiles + t0 / kTileBwd) * g.dim + ch, in);
-    emit_run<kRun>(a, b, n, cut, plain, in,
-                   [&](int j, float2 v) { store_pair<T, true>(rows + (kRun + j) * kChan + 2 * lane, v, true, true); });
+    scan_run<kLong>(a, b, n, cut, plain, p, h);
+    const float2 in = tile_exchange(ex, buf, p, h, state, g.chunks, rank, reset != nullptr);
+    auto save = [&](int j, float2 v) {
+      if (g.saved != nullptr && on) put_two_floats(g.saved + (batch * g.runs + (t0 + j) / kRun) * g.dim + ch, v);
+    };
+    emit_run<kLong>(a, b, n, cut, plain, in, save,
+                   [&](int j, float2 v) { store_pair<T, true>(rows + (kLong + j) * kChan + 2 * lane, v, true, true); });
     sm100::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      if (n > 0) tma_store_3d(&maps.out_value, rows + kRun * kChan, ch0, static_cast<int>(t0), batch);
+      if (n > 0) tma_store_3d(&maps.out_value, rows + kLong * kChan, ch0, static_cast<int>(t0), batch);
       sm100::bulk_commit();
       // The stage before this one has been read by its store: its next tile comes in.
       bulk_wait_read<1>();
@@ -704,198 +834,209 @@ __global__ void __launch_bounds__(kThreads, 2)
       parity ^= 1;
     }
   }
-  if (warp == 0 && rank == 0 && chunk == g.chunks - 1 && on) put_two_floats(g.h_last + batch * g.dim + ch, state);
+  if (warp == 0 && rank == 0 && on) put_two_floats(g.h_last + batch * g.dim + ch, state);
   if (lane == 0) sm100::bulk_wait_read_all();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2)
-    recurrence_backward_tma_kernel(const RecurrenceArgs g, const __grid_constant__ SequenceMaps maps) {
-  constexpr int kRun = kRunBwd, kTile = kTileBwd, kStages = kStagesBwd<T>, kPart = kRun * kChan;
+// Backward. With r_t = keep_t a_t ds_t the part of step t's gradient that reaches h_{t-1}:
+//   ds_t = grad_t + r_{t+1},  grad_value = c ds,  grad_gate = a c (keep h_{t-1} - x) ds
+// r is the forward's recurrence from the sequence's end, with the same P: a first pass over gate and
+// grad for the segments' maps, then a second over all three with r coming in. h_{t-1} is scanned from
+// the state saved before the run, in 32 bits; h itself is not read.
+template <typename T, bool TMA, bool PAIRED, int PASS>
+__global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
+    recurrence_backward_kernel(const RecurrenceArgs g, const __grid_constant__ SequenceMaps maps) {
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ Exchange ex;
-  __shared__ float2 run_h[2][kWarps][32];
-  __shared__ uint64_t full[kWarps][kStages];
+  __shared__ uint64_t full[kWarps][4];
   __shared__ int abort;
+  using In = Stream<T, 3, TMA, PAIRED>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % g.ranks, chunk = blockIdx.y;
-  const int unit = blockIdx.x / g.ranks;
-  const int batch = unit / g.channel_blocks, ch0 = unit % g.channel_blocks * kChan;
-  const int64_t ch = ch0 + 2 * lane;
-  const bool on = ch < g.dim, graded = g.grad != nullptr;
-  const uint32_t bytes = (graded ? 3 : 2) * kPart * sizeof(T);
+  const int unit = blockIdx.x / g.chunks, chunk = blockIdx.x - unit * g.chunks;
+  const int64_t batch = unit / g.channel_blocks;
+  const int block = unit - static_cast<int>(batch) * g.channel_blocks;
+  const Lane<PAIRED> at(block, g.dim);
+  const bool graded = g.grad != nullptr;
+  const uint32_t for_maps = graded ? 5u : 1u, for_all = graded ? 7u : 3u;  // gate, value, grad
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
-  const int64_t first = chunk * g.chunk_tiles, stop = min64(g.saved_tiles, first + g.chunk_tiles);
-  T *ring = reinterpret_cast<T *>(dynamic) + size_t(warp) * kStages * 3 * kPart;
-  auto stage = [&](int s) -> T * { return ring + s * 3 * kPart; };
-  auto there = [&](int64_t k) { return k >= first && k * kTile + warp * kRun < g.steps; };
-  auto fetch = [&](int64_t k, int s) {  // one lane
-    if (!there(k)) return;
-    const int t0 = static_cast<int>(k * kTile + warp * kRun);
-    sm100::mbar_expect_tx(&full[warp][s], bytes);
-    sm100::tma_load_3d(stage(s), &maps.gate, &full[warp][s], ch0, t0, batch);
-    sm100::tma_load_3d(stage(s) + kPart, &maps.value, &full[warp][s], ch0, t0, batch);
-    if (graded) sm100::tma_load_3d(stage(s) + 2 * kPart, &maps.grad, &full[warp][s], ch0, t0, batch);
-  };
-  auto flag_of = [&](int64_t k) -> uint32_t {
-    const int64_t t = k * kTile + warp * kRun + lane;
-    return reset != nullptr && k >= first && lane < kRun && t < g.steps ? __ldg(reset + t) : 0u;
-  };
-  auto before_of = [&](int64_t k) -> float2 {
-    if (!there(k) || !on) return make_float2(0.f, 0.f);
-    return two_floats(g.saved + (batch * g.saved_tiles + k) * g.dim + ch);
-  };
-  if (g.ranks > 1) cluster_arrive();
-  if (threadIdx.x == 0) abort = 0;
-  const int64_t k_first = stop - 1 - rank;
-  // Stages are filled and used in order, one a tile that this warp has steps of: only the sequence's
-  // last tile may be without.
-  const bool skip = !there(k_first) && k_first >= first;
-  const int64_t k_fill = skip ? k_first - g.ranks : k_first;
-  if (lane == 0) {
+  const Items<false, PASS> items(g, chunk, warp);
+  const int total = items.total, steps = static_cast<int>(g.steps);
+  if (PASS == kBoth && g.chunks > 1) cluster_arrive();
+
+  In in;
+  if constexpr (TMA) {
+    in.ring = reinterpret_cast<T *>(dynamic) + size_t(warp) * In::kDeep * 3 * kRun * kChan;
+    in.full = full[warp];
+    in.abort = &abort;
+    in.maps[0] = &maps.gate;
+    in.maps[1] = &maps.value;
+    in.maps[2] = &maps.grad;
+    in.ch0 = block * kChan;
+    in.batch = static_cast<int>(batch);
+    if (threadIdx.x == 0) abort = 0;
+    if (lane == 0) {
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) sm100::mbar_init(&full[warp][s], 1);
-    sm100::mbar_init_fence();
-    sm100::fence_proxy_async_smem();
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) fetch(k_fill - int64_t(s) * g.ranks, s);
+      for (int s = 0; s < In::kDeep; ++s) sm100::mbar_init(&full[warp][s], 1);
+      sm100::mbar_init_fence();
+      sm100::fence_proxy_async_smem();
+    }
+    __syncthreads();
+  } else {
+    in.from[0] = static_cast<const T *>(g.gate) + batch * g.gate_batch + at.from;
+    in.from[1] = static_cast<const T *>(g.value) + batch * g.value_batch + at.from;
+    in.from[2] = static_cast<const T *>(g.grad) + (graded ? batch * g.steps * g.dim + at.from : 0);
+    in.stride[0] = g.gate_step;
+    in.stride[1] = g.value_step;
+    in.stride[2] = g.dim;
+    in.steps = steps;
+    in.second = at.second;
   }
-  uint32_t flag = flag_of(k_first);
-  float2 before = before_of(k_first);
-  __syncthreads();
-
-  float2 back = make_float2(0.f, 0.f);
-  if (g.grad_last != nullptr && on) back = two_floats(g.grad_last + batch * g.dim + ch);
-  if (chunk < g.chunks - 1) back = through_chunks<true, false>(g, batch, ch, on, on, chunk, back, ex);
-  if (g.ranks > 1) cluster_wait();
-
-  int buf = 0, s = 0, done = 0;
-  uint32_t parity = 0;
-  for (int64_t last = stop - 1, k = k_first; last >= first; last -= g.ranks, k -= g.ranks, buf ^= 1) {
-    const bool here = there(k);
-    const int n = here ? static_cast<int>(min64(kRun, g.steps - (k * kTile + warp * kRun))) : 0;
+  auto which_of = [&](int i) { return PASS != kApply && i < items.count ? for_maps : for_all; };
+  const int ahead = TMA ? In::kDeep : 1;
+  for (int i = 0; i < ahead; ++i)
+    if (i < total) in.fetch(items.start(i), which_of(i), i);
+  uint32_t flag = total > 0 ? flag_of(reset, items.start(0), steps) : 0;
+  int item = 0;
+  auto flags = [&]() -> uint32_t {
+    if (reset == nullptr) return 0;
     const uint32_t cut = __ballot_sync(0xffffffffu, flag != 0);
-    flag = flag_of(k - g.ranks);
-    float2 h_in = before;
-    before = before_of(k - g.ranks);
-    const bool plain = n == kRun && cut == 0;
-    if (here) sm100::mbar_wait(&full[warp][s], parity, &abort, &g_recurrence_error);
-    T *rows = stage(s);
-    float2 a[kRun], c[kRun], x[kRun], gt[kRun], p, h, r;
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      gates2(unpack<T>(stage_raw<T>(rows + j * kChan, lane)), a[j], c[j]);
-      x[j] = unpack<T>(stage_raw<T>(rows + kPart + j * kChan, lane));
-      gt[j] = graded ? unpack<T>(stage_raw<T>(rows + 2 * kPart + j * kChan, lane)) : make_float2(0.f, 0.f);
-    }
-    scan_run_back<kRun>(a, c, x, gt, n, cut, plain, p, h, r);
-    run_h[buf][warp][lane] = h;
-    const float2 r_in = exchange<-1>(ex, buf, p, r, back, g.ranks, rank, reset != nullptr);
-#pragma unroll
-    for (int w = 0; w < kWarps - 1; ++w) {
-      if (w < warp) h_in = apply_run(ex.p[buf][w][lane], h_in, run_h[buf][w][lane], reset != nullptr);
-    }
-    emit_run_back<kRun>(a, c, x, gt, n, cut, plain, h_in, r_in, [&](int j, float2 gf, float2 gx) {
-      store_pair<T, true>(rows + j * kChan + 2 * lane, gf, true, true);
-      store_pair<T, true>(rows + kPart + j * kChan + 2 * lane, gx, true, true);
-    });
-    sm100::fence_proxy_async_smem();
-    __syncwarp();
-    if (here) {
-      if (lane == 0) {
-        const int t0 = static_cast<int>(k * kTile + warp * kRun);
-        tma_store_3d(&maps.out_gate, rows, ch0, t0, batch);
-        tma_store_3d(&maps.out_value, rows + kPart, ch0, t0, batch);
-        sm100::bulk_commit();
-        // The stage before this one has been read by its stores: its next tile comes in.
-        bulk_wait_read<1>();
-        if (done > 0) fetch(k - int64_t(kStages - 1) * g.ranks, s == 0 ? kStages - 1 : s - 1);
-      }
-      ++done;
-      if (++s == kStages) {
-        s = 0;
-        parity ^= 1;
-      }
-    }
-  }
-  if (warp == 0 && rank == 0 && chunk == 0 && g.grad_h0 != nullptr && on)
-    put_two_floats(g.grad_h0 + batch * g.dim + ch, back);
-  if (lane == 0) sm100::bulk_wait_read_all();
-}
-
-// The map of each chunk: (P, H) forward, (P, R) for the backward. Each warp scans an equal stretch of
-// the chunk, the stretches are composed at the end.
-template <typename T, bool PAIRED, bool FORWARD>
-__global__ void __launch_bounds__(kThreads, 3) recurrence_map_kernel(const RecurrenceArgs g, int64_t chunk_steps) {
-  constexpr int kRun = 8;
-  __shared__ float2 run_p[kWarps][32], run_h[kWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int chunk = FORWARD ? blockIdx.y : blockIdx.y + 1;  // the last (first) chunk's map is not asked for
-  const int64_t batch = blockIdx.x / g.channel_blocks;
-  const Lane<PAIRED> at(blockIdx.x % g.channel_blocks, g.dim);
-  const int64_t ch = at.ch;
-  const bool on0 = at.on0, on1 = at.on1;
-  const T *gate = static_cast<const T *>(g.gate) + batch * g.gate_batch + at.from;
-  const T *other = FORWARD ? static_cast<const T *>(g.value) + batch * g.value_batch + at.from
-                           : (g.grad != nullptr ? static_cast<const T *>(g.grad) + batch * g.steps * g.dim + at.from : nullptr);
-  const int64_t other_step = FORWARD ? g.value_step : g.dim;
-  const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
-  const int64_t share = chunk_steps / kWarps;  // a whole number of runs
-  const int64_t begin = chunk * chunk_steps + warp * share, stop = min64(g.steps, begin + share);
+    flag = item + 1 < total ? flag_of(reset, items.start(item + 1), steps) : 0;
+    return cut;
+  };
   const float2 zero = make_float2(0.f, 0.f);
-  float2 h = zero, p = make_float2(1.f, 1.f);
-  const int64_t runs = begin < stop ? (stop - begin + kRun - 1) / kRun : 0;
-  for (int64_t i = 0; i < runs; ++i) {
-    const int64_t t0 = begin + (FORWARD ? i : runs - 1 - i) * kRun;
-    const int n = static_cast<int>(min64(kRun, stop - t0));
-    Raw<T> rf[kRun], ro[kRun] = {};
-    const T *pf = gate + t0 * g.gate_step, *po = other + t0 * other_step;
+  float2 r = zero, p = make_float2(1.f, 1.f);
+  if (PASS != kApply) {
+    for (; item < items.count; ++item) {
+      const int t0 = items.start(item);
+      const int n = min(kRun, steps - t0);
+      const uint32_t cut = flags();
+      in.wait();
+      float2 a[kRun], gt[kRun];
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      rf[j] = load_raw<T, PAIRED>(pf, at.second);
-      if (other != nullptr) ro[j] = load_raw<T, PAIRED>(po, at.second);
-      if (j + 1 < n) {  // steps past the end load the last one again
-        pf += g.gate_step;
-        po += other_step;
+      for (int j = 0; j < kRun; ++j) {
+        float2 c;
+        gates2(in.get(0, j), a[j], c);
+        gt[j] = graded ? in.get(2, j) : zero;
       }
-    }
-    const uint32_t cut = reset_bits(reset, t0, n);
+      if constexpr (TMA) __syncwarp();  // all lanes have read the stage
+      if (item + ahead < total) in.fetch(items.start(item + ahead), which_of(item + ahead), 0);
+      in.next();
+      if (n == kRun && cut == 0) {
 #pragma unroll
-    for (int i_j = 0; i_j < kRun; ++i_j) {
-      const int j = FORWARD ? i_j : kRun - 1 - i_j;
-      if (j < n) {
-        const float2 f = unpack<T>(rf[j]), o = unpack<T>(ro[j]);
-        float2 a, c;
-        gates2(f, a, c);
-        const bool here = (cut >> j) & 1u;
-        if (FORWARD) {
-          if (here) h = p = zero;
-          h = fma2(a, h, mul2(c, o));
-          p = mul2(p, a);
-        } else {
-          h = mul2(a, add2(o, h));
-          p = mul2(p, a);
-          if (here) h = p = zero;
+        for (int j = kRun - 1; j >= 0; --j) {
+          r = mul2(a[j], add2(gt[j], r));
+          p = mul2(p, a[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = kRun - 1; j >= 0; --j) {
+          if (j < n) {
+            r = mul2(a[j], add2(gt[j], r));
+            p = mul2(p, a[j]);
+            if ((cut >> j) & 1u) r = p = zero;
+          }
         }
       }
     }
   }
-  run_p[warp][lane] = p;
-  run_h[warp][lane] = h;
-  __syncthreads();
-  if (warp == 0) {
-    p = make_float2(1.f, 1.f);
-    h = zero;
+  float2 back = zero;  // r of the step after the sequence
+  if (g.grad_last != nullptr) back = two_floats(g.grad_last + batch * g.dim + at.from, at.second);
+  if (PASS == kBoth && g.chunks > 1) cluster_wait();  // all have started
+  back = exchange<false, PAIRED, PASS>(g, batch, at, chunk, p, r, back, ex);
+  if (PASS == kMaps) return;
+
+  T *grad_gate = static_cast<T *>(g.grad_gate) + batch * g.steps * g.dim + at.ch;
+  T *grad_value = static_cast<T *>(g.grad_value) + batch * g.steps * g.dim + at.ch;
+  auto before_of = [&](int i) -> float2 {
+    if (i >= total) return zero;
+    return two_floats(g.saved + (batch * g.runs + items.start(i) / kRun) * g.dim + at.from, at.second);
+  };
+  float2 before = before_of(item);
+  for (; item < total; ++item) {
+    const int t0 = items.start(item);
+    const int n = min(kRun, steps - t0);
+    const uint32_t cut = flags();
+    float2 h = before;
+    before = before_of(item + 1);
+    in.wait();
+    float2 a[kRun], c[kRun], u[kRun], gt[kRun];
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const int w = FORWARD ? i : kWarps - 1 - i;
-      h = apply_run(run_p[w][lane], h, run_h[w][lane], true);
-      p = mul2(p, run_p[w][lane]);
+    for (int j = 0; j < kRun; ++j) {
+      gates2(in.get(0, j), a[j], c[j]);
+      u[j] = in.get(1, j);
+      if constexpr (!TMA) gt[j] = graded ? in.get(2, j) : zero;
     }
-    float2 *m = g.maps + (batch * g.chunks + chunk) * g.dim + ch;
-    if (on0) m[0] = make_float2(p.x, h.x);
-    if (on1) m[kSecond<PAIRED>] = make_float2(p.y, h.y);
+    if constexpr (!TMA)
+      if (item + 1 < total) in.fetch(items.start(item + 1), for_all, 0);
+    auto grad_at = [&](int j) -> float2 {
+      if constexpr (TMA) return graded ? in.get(2, j) : zero;
+      else return gt[j];
+    };
+    auto put = [&](int j, float2 ds) {
+      const float2 gx = mul2(c[j], ds), gf = mul2(mul2(a[j], gx), u[j]);
+      if constexpr (TMA) {
+        store_pair<T, true>(in.rows(0) + j * kChan + 2 * lane, gf, true, true);
+        store_pair<T, true>(in.rows(1) + j * kChan + 2 * lane, gx, true, true);
+      } else {
+        store_pair<T, PAIRED>(grad_gate + int64_t(t0 + j) * g.dim, gf, at.on0, at.on1);
+        store_pair<T, PAIRED>(grad_value + int64_t(t0 + j) * g.dim, gx, at.on0, at.on1);
+      }
+    };
+    const float2 minus = make_float2(-1.f, -1.f);
+    if (n == kRun && cut == 0) {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const float2 x = u[j];
+        u[j] = fma2(x, minus, h);  // keep h_{t-1} - x
+        h = fma2(a[j], h, mul2(c[j], x));
+      }
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) {
+        const float2 ds = add2(grad_at(j), back);
+        back = mul2(a[j], ds);
+        put(j, ds);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (j < n) {
+          const float2 x = u[j];
+          if ((cut >> j) & 1u) h = zero;
+          u[j] = fma2(x, minus, h);
+          h = fma2(a[j], h, mul2(c[j], x));
+        }
+      }
+#pragma unroll
+      for (int j = kRun - 1; j >= 0; --j) {
+        if (j < n) {
+          const float2 ds = add2(grad_at(j), back);
+          back = mul2(a[j], ds);
+          put(j, ds);
+          if ((cut >> j) & 1u) back = zero;
+        }
+      }
+    }
+    if constexpr (TMA) {
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(&maps.out_gate, in.rows(0), in.ch0, t0, in.batch);
+        tma_store_3d(&maps.out_value, in.rows(1), in.ch0, t0, in.batch);
+        sm100::bulk_commit();
+        bulk_wait_read<1>();  // the stage before this one has been read by its stores
+      }
+      // That stage's next run comes in; the first run's stage has no store before it.
+      if (in.stored && item - 1 + In::kDeep < total) in.fetch(items.start(item - 1 + In::kDeep), for_all, In::kDeep - 1);
+      in.stored = true;
+    }
+    in.next();
   }
+  if (warp == 0 && chunk == 0 && g.grad_h0 != nullptr) {
+    float *out = g.grad_h0 + batch * g.dim + at.ch;
+    if (at.on0) out[0] = back.x;
+    if (at.on1) out[kSecond<PAIRED>] = back.y;
+  }
+  if (TMA && lane == 0) sm100::bulk_wait_read_all();
 }
 
 // One token of every row: state (f32, updated in place) and h. A few KB to a few MB: launch
@@ -923,32 +1064,38 @@ int check_sizes(const char *what, int dtype, int64_t batch, int64_t steps, int64
   TB_REQUIRE(is_float_dtype(dtype), TROPNN_B200_ERR_DTYPE, "%s: dtype %d is not f32/f16/bf16", what, dtype);
   TB_REQUIRE(batch >= 0 && steps >= 0 && dim >= 0, TROPNN_B200_ERR_INVALID, "%s: bad sizes (batch %lld, steps %lld, dim %lld)",
              what, (long long)batch, (long long)steps, (long long)dim);
-  TB_REQUIRE(batch * ceil_div(dim, kChan) <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: batch x dim too large", what);
+  TB_REQUIRE(batch * ceil_div(dim, kChan) * kMaxCluster <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: batch x dim too large", what);
+  TB_REQUIRE(steps <= 0x7fffffffLL - kRun, TROPNN_B200_ERR_INVALID, "%s: %lld steps are too many", what, (long long)steps);
   return TROPNN_B200_OK;
 }
 
-// How the tiles are shared out. While CTAs are idle: more of them a cluster, as far as there are tiles.
-// With less than half the SMs busy even so and at least 4 tiles a chunk, chunks instead.
+// How a sequence is shared out: chunks of kWarps segments, a CTA each, as many as are on the GPU at once.
+// Up to 8 chunks are a cluster. Where 8 are less than half of that, and at least 4 runs a segment are
+// left, there are more chunks and two launches; a forward pass not cut so goes by tiles.
 struct Plan {
-  int ranks = 1, chunks = 1;
-  int64_t chunk_tiles = 0;
+  int chunks = 1;
+  bool two_launches = false;
+  int64_t segment_runs = 0;
 };
-Plan plan_for(int64_t units, int64_t tiles) {
+Plan plan_for(int64_t units, int64_t runs, int64_t slots) {
   Plan p;
-  p.chunk_tiles = tiles;
-  while (p.ranks < kMaxCluster && units * p.ranks * 2 <= kSlots && p.ranks * 2 <= tiles) p.ranks *= 2;
-  if (p.ranks == kMaxCluster && units * p.ranks <= kSlots / 4) {
-    const int64_t each = std::max<int64_t>(4, ceil_div(tiles * units, kSlots));
-    if (ceil_div(tiles, each) >= 2 * p.ranks) {
-      p.ranks = 1;
-      p.chunk_tiles = each;
-      p.chunks = static_cast<int>(ceil_div(tiles, each));
+  p.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxCluster, slots / units, runs / kWarps})));
+  if (p.chunks == kMaxCluster && units * p.chunks * 2 <= slots) {
+    const int64_t many = min64(slots / units, runs / (4 * kWarps));
+    if (many >= 2 * kMaxCluster) {
+      p.chunks = static_cast<int>(many);
+      p.two_launches = true;
     }
   }
+  p.segment_runs = std::max<int64_t>(1, ceil_div(runs, int64_t(p.chunks) * kWarps));
+  if (p.two_launches) p.chunks = static_cast<int>(ceil_div(runs, p.segment_runs * kWarps));
   return p;
 }
 int64_t units_of(int64_t batch, int64_t dim) { return batch * ceil_div(dim, kChan); }
-int64_t forward_tile(int dtype) { return kWarps * (dtype == TROPNN_B200_F32 ? kRunFwd<float> : kRunFwd<__half>); }
+int64_t slots_of(bool forward, int dtype) { return 148 * (dtype == TROPNN_B200_F32 || !forward ? 2 : 3); }
+size_t maps_bytes(const Plan &p, int64_t batch, int64_t dim) {
+  return p.two_launches ? static_cast<size_t>(batch * p.chunks * kMapSlots * dim) * sizeof(float2) : 0;
+}
 
 // A [batch, steps, dim] tensor (strides in elements) in boxes of `run` steps x 64 channels. False where
 // TMA cannot take it.
@@ -974,74 +1121,83 @@ bool sequence_map(CUtensorMap *map, const void *ptr, int dtype, int64_t batch, i
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool FORWARD, typename T, bool PAIRED>
-int launch_typed(const char *what, RecurrenceArgs g, int dtype, int64_t batch, const Plan &plan, cudaStream_t stream) {
-  const unsigned units = static_cast<unsigned>(batch * g.channel_blocks);
-  if (plan.chunks > 1) {
-    constexpr int64_t tile = FORWARD ? kWarps * kRunFwd<T> : kTileBwd;
-    recurrence_map_kernel<T, PAIRED, FORWARD>
-        <<<dim3(units, static_cast<unsigned>(plan.chunks - 1)), kThreads, 0, stream>>>(g, plan.chunk_tiles * tile);
-    TB_CHECK(check_launch(what));
-  }
+int launch_clusters(const char *what, const void *kernel, size_t smem, int64_t ctas, int cluster, RecurrenceArgs &g,
+                    SequenceMaps &maps, cudaStream_t stream) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(units * static_cast<unsigned>(plan.ranks), static_cast<unsigned>(plan.chunks));
+  config.gridDim = dim3(static_cast<unsigned>(ctas));
   config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(plan.ranks);
+  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  if constexpr (PAIRED) {
-    SequenceMaps maps{};
-    constexpr int run = FORWARD ? kRunFwd<T> : kRunBwd;
-    const int64_t steps = g.steps, dim = g.dim;
-    bool fits = steps > 0 && sequence_map(&maps.gate, g.gate, dtype, batch, steps, dim, g.gate_batch, g.gate_step, run) &&
-                sequence_map(&maps.value, g.value, dtype, batch, steps, dim, g.value_batch, g.value_step, run);
-    if (FORWARD) {
-      fits = fits && sequence_map(&maps.out_value, g.h, dtype, batch, steps, dim, steps * dim, dim, run);
-    } else {
-      fits = fits && (g.grad == nullptr || sequence_map(&maps.grad, g.grad, dtype, batch, steps, dim, steps * dim, dim, run)) &&
-             sequence_map(&maps.out_gate, g.grad_gate, dtype, batch, steps, dim, steps * dim, dim, run) &&
-             sequence_map(&maps.out_value, g.grad_value, dtype, batch, steps, dim, steps * dim, dim, run);
-    }
-    if (fits) {
-      config.dynamicSmemBytes = kRingBytes<T, FORWARD>;
-      const void *kernel = FORWARD ? reinterpret_cast<const void *>(recurrence_forward_tma_kernel<T>)
-                                   : reinterpret_cast<const void *>(recurrence_backward_tma_kernel<T>);
-      // The static part counts too: above 48 KB in all the kernel has to be told.
-      TB_CHECK(ensure_dynamic_smem(kernel, std::max<size_t>(config.dynamicSmemBytes, 49 * 1024), what));
-      void *args[] = {&g, &maps};
-      cudaLaunchKernelExC(&config, kernel, args);
-      return check_launch(what);
-    }
-  }
-  if (FORWARD) cudaLaunchKernelEx(&config, recurrence_forward_kernel<T, PAIRED>, static_cast<const RecurrenceArgs>(g));
-  else cudaLaunchKernelEx(&config, recurrence_backward_kernel<T, PAIRED>, static_cast<const RecurrenceArgs>(g));
+  // The static part counts too: above 48 KB in all the kernel has to be told.
+  if (smem > 0) TB_CHECK(ensure_dynamic_smem(kernel, std::max<size_t>(smem, 49 * 1024), what));
+  void *args[] = {&g, &maps};
+  cudaLaunchKernelExC(&config, kernel, args);
   return check_launch(what);
+}
+template <bool FORWARD, typename T, bool TMA, bool PAIRED, int PASS>
+int launch_pass(const char *what, RecurrenceArgs g, SequenceMaps &maps, int64_t units, cudaStream_t stream) {
+  const void *kernel;
+  if constexpr (FORWARD) kernel = reinterpret_cast<const void *>(recurrence_forward_kernel<T, TMA, PAIRED, PASS>);
+  else kernel = reinterpret_cast<const void *>(recurrence_backward_kernel<T, TMA, PAIRED, PASS>);
+  return launch_clusters(what, kernel, TMA ? kRingBytes<T, FORWARD ? 2 : 3> : 0, units * g.chunks, PASS == kBoth ? g.chunks : 1, g,
+                         maps, stream);
+}
+template <typename T, bool TMA, bool PAIRED>
+int launch_tiles(const char *what, RecurrenceArgs g, SequenceMaps &maps, int64_t units, cudaStream_t stream) {
+  const int64_t tiles = ceil_div(g.steps, kWarps * kTileRun<T>);
+  g.chunks = 1;  // CTAs of a cluster, two of them an SM in all
+  while (g.chunks < kMaxCluster && units * g.chunks * 2 <= 2 * 148 && g.chunks * 2 <= tiles) g.chunks *= 2;
+  const void *kernel = TMA ? reinterpret_cast<const void *>(recurrence_tiles_tma_kernel<T>)
+                           : reinterpret_cast<const void *>(recurrence_tiles_kernel<T, PAIRED>);
+  return launch_clusters(what, kernel, TMA ? kTileRingBytes<T> : 0, units * g.chunks, g.chunks, g, maps, stream);
+}
+template <bool FORWARD, typename T, bool TMA, bool PAIRED>
+int launch_form(const char *what, const RecurrenceArgs &g, SequenceMaps &maps, int64_t units, bool two_launches, cudaStream_t stream) {
+  if (!two_launches) {
+    if constexpr (FORWARD) return launch_tiles<T, TMA, PAIRED>(what, g, maps, units, stream);
+    else return launch_pass<FORWARD, T, TMA, PAIRED, kBoth>(what, g, maps, units, stream);
+  }
+  TB_CHECK((launch_pass<FORWARD, T, TMA, PAIRED, kMaps>(what, g, maps, units, stream)));
+  return launch_pass<FORWARD, T, TMA, PAIRED, kApply>(what, g, maps, units, stream);
+}
+template <bool FORWARD, typename T>
+int launch_typed(const char *what, const RecurrenceArgs &g, int dtype, int64_t batch, bool pair, bool two_launches, cudaStream_t stream) {
+  const int64_t units = batch * g.channel_blocks, steps = g.steps, dim = g.dim;
+  const int run = FORWARD && !two_launches ? kTileRun<T> : kRun;
+  SequenceMaps maps{};
+  bool fits = pair && steps > 0 && sequence_map(&maps.gate, g.gate, dtype, batch, steps, dim, g.gate_batch, g.gate_step, run) &&
+              sequence_map(&maps.value, g.value, dtype, batch, steps, dim, g.value_batch, g.value_step, run);
+  if (FORWARD) {
+    fits = fits && sequence_map(&maps.out_value, g.h, dtype, batch, steps, dim, steps * dim, dim, run);
+  } else {
+    fits = fits && (g.grad == nullptr || sequence_map(&maps.grad, g.grad, dtype, batch, steps, dim, steps * dim, dim, run)) &&
+           sequence_map(&maps.out_gate, g.grad_gate, dtype, batch, steps, dim, steps * dim, dim, run) &&
+           sequence_map(&maps.out_value, g.grad_value, dtype, batch, steps, dim, steps * dim, dim, run);
+  }
+  if (fits) return launch_form<FORWARD, T, true, true>(what, g, maps, units, two_launches, stream);
+  if (pair) return launch_form<FORWARD, T, false, true>(what, g, maps, units, two_launches, stream);
+  return launch_form<FORWARD, T, false, false>(what, g, maps, units, two_launches, stream);
 }
 
 template <bool FORWARD>
 int launch_recurrence(const char *what, RecurrenceArgs g, int dtype, int64_t batch, bool pair, void *workspace,
                       size_t workspace_bytes, cudaStream_t stream) {
-  const int64_t tile = FORWARD ? forward_tile(dtype) : kTileBwd;
-  const Plan plan = plan_for(batch * g.channel_blocks, ceil_div(g.steps, tile));
-  const size_t need = plan.chunks > 1 ? static_cast<size_t>(batch * plan.chunks * g.dim) * sizeof(float2) : 0;
+  const Plan plan = plan_for(batch * g.channel_blocks, g.runs, slots_of(FORWARD, dtype));
+  const size_t need = maps_bytes(plan, batch, g.dim);
   TB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), TROPNN_B200_ERR_WORKSPACE,
              "%s: %zu bytes of workspace, %zu needed", what, workspace_bytes, need);
-  g.ranks = plan.ranks;
   g.chunks = plan.chunks;
-  g.chunk_tiles = plan.chunk_tiles;
+  g.segment_runs = plan.segment_runs;
   g.maps = static_cast<float2 *>(workspace);
-  if (dtype == TROPNN_B200_F32)
-    return pair ? launch_typed<FORWARD, float, true>(what, g, dtype, batch, plan, stream)
-                : launch_typed<FORWARD, float, false>(what, g, dtype, batch, plan, stream);
-  if (dtype == TROPNN_B200_F16)
-    return pair ? launch_typed<FORWARD, __half, true>(what, g, dtype, batch, plan, stream)
-                : launch_typed<FORWARD, __half, false>(what, g, dtype, batch, plan, stream);
-  return pair ? launch_typed<FORWARD, __nv_bfloat16, true>(what, g, dtype, batch, plan, stream)
-              : launch_typed<FORWARD, __nv_bfloat16, false>(what, g, dtype, batch, plan, stream);
+  if (dtype == TROPNN_B200_F32) return launch_typed<FORWARD, float>(what, g, dtype, batch, pair, plan.two_launches, stream);
+  if (dtype == TROPNN_B200_F16) return launch_typed<FORWARD, __half>(what, g, dtype, batch, pair, plan.two_launches, stream);
+  return launch_typed<FORWARD, __nv_bfloat16>(what, g, dtype, batch, pair, plan.two_launches, stream);
 }
 
 }  // namespace
@@ -1067,15 +1223,14 @@ extern "C" {
 
 size_t tropnn_b200_recurrence_saved_size(int64_t batch, int64_t steps, int64_t dim) {
   if (batch <= 0 || steps <= 0 || dim <= 0) return 0;
-  return static_cast<size_t>(batch * ceil_div(steps, kTileBwd) * dim) * sizeof(float);
+  return static_cast<size_t>(batch * ceil_div(steps, kRun) * dim) * sizeof(float);
 }
 
 size_t tropnn_b200_recurrence_workspace_size(int64_t batch, int64_t steps, int64_t dim, int dtype) {
   if (batch <= 0 || steps <= 0 || dim <= 0 || !is_float_dtype(dtype)) return 0;
-  const int64_t units = units_of(batch, dim);
-  const Plan f = plan_for(units, ceil_div(steps, forward_tile(dtype))), b = plan_for(units, ceil_div(steps, kTileBwd));
-  const int chunks = std::max(f.chunks, b.chunks);
-  return chunks > 1 ? static_cast<size_t>(batch * chunks * dim) * sizeof(float2) : 0;
+  const int64_t units = units_of(batch, dim), runs = ceil_div(steps, kRun);
+  return std::max(maps_bytes(plan_for(units, runs, slots_of(true, dtype)), batch, dim),
+                  maps_bytes(plan_for(units, runs, slots_of(false, dtype)), batch, dim));
 }
 
 int tropnn_b200_recurrence_forward(const void *gate, int64_t gate_batch_stride, int64_t gate_step_stride,
@@ -1107,7 +1262,7 @@ int tropnn_b200_recurrence_forward(const void *gate, int64_t gate_batch_stride, 
   g.h = h;
   g.h_last = h_last;
   g.saved = saved;
-  g.saved_tiles = ceil_div(steps, kTileBwd);
+  g.runs = ceil_div(steps, kRun);
   const bool pair = dim % 2 == 0 && gate_batch_stride % 2 == 0 && gate_step_stride % 2 == 0 &&
                     value_batch_stride % 2 == 0 && value_step_stride % 2 == 0 && paired(gate, dtype) &&
                     paired(value, dtype) && paired(h, dtype);
@@ -1142,7 +1297,7 @@ int tropnn_b200_recurrence_backward(const void *gate, int64_t gate_batch_stride,
   g.dim = dim;
   g.channel_blocks = static_cast<int>(ceil_div(dim, kChan));
   g.saved = const_cast<float *>(saved);
-  g.saved_tiles = ceil_div(steps, kTileBwd);
+  g.runs = ceil_div(steps, kRun);
   g.grad = grad;
   g.grad_last = grad_last;
   g.grad_gate = grad_gate;

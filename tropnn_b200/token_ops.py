@@ -153,8 +153,8 @@ def gated_recurrence_b200(
     tokens that start a document: nothing of the state before them is kept. Returns ``(h, h_last)``:
     ``h`` in the inputs' dtype and the last state in f32, which continues a sequence as ``h0`` of
     the next call or as the state of ``gated_recurrence_step_b200``. The state is f32 throughout.
-    Differentiable in gate, value and h0 (once); the backward scans the states again from one in 64
-    saved ones instead of reading ``h``.
+    Differentiable in gate, value and h0 (once); the backward scans the states again from every
+    eighth, saved in f32, instead of reading ``h``.
     """
     _check_gate_value(gate, value, 3)
     if h0 is not None:
