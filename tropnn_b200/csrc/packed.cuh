@@ -45,4 +45,22 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
+// 2^x for x <= 0 on the FMA and integer pipes, to 2.2e-7 of it (0 below 2^-126.5): x = n + f with n whole
+// and |f| <= 1/2, 2^f by the polynomial of degree 5 that is closest to it in relative error (7.5e-8,
+// fitted by iteratively reweighted least squares on Chebyshev nodes), times 2^n put together from its
+// bits. Adding 1.5 * 2^23 rounds x to n and leaves n in the sum's low bits.
+__device__ __forceinline__ float2 exp2_poly2(float2 x) {
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x.x) : "f"(x.x), "f"(-127.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x.y) : "f"(x.y), "f"(-127.f));
+  const float2 t = add2(x, both(12582912.f)), n = add2(t, both(-12582912.f)), f = fma2(n, both(-1.f), x);
+  float2 p = fma2(f, both(0.001327647129073739f), both(0.009675540961325169f));
+  p = fma2(p, f, both(0.05550713092088699f));
+  p = fma2(p, f, both(0.24022120237350464f));
+  p = fma2(p, f, both(0.6931469440460205f));
+  p = fma2(p, f, both(1.0000001192092896f));
+  const float2 scale = make_float2(__int_as_float(__float_as_int(t.x) * (1 << 23) + 0x3F800000),
+                                   __int_as_float(__float_as_int(t.y) * (1 << 23) + 0x3F800000));
+  return mul2(p, scale);
+}
+
 }  // namespace tropnn_b200
