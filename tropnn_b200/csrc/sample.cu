@@ -59,6 +59,7 @@ struct SampleArgs {
   int slice_vecs;   // 16-byte vectors of a CTA's slice
   int maxima_rows;  // batches a thread whose maxima are kept; 0: none
   int maxima_offset;
+  bool halves;  // how the histogram holds weights
 };
 
 // Larger for larger logits; -0 as +0.
@@ -522,6 +523,17 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
       const int shift = max(0, 32 - __clz(range) - kDigitBits);
       for (int i = tid; i < kBins; i += kThreads) hist.count[i] = hist.low[i] = hist.high[i] = 0;
       __syncthreads();
+      // A weight in two words: its halves, where no more than 2^16 tokens are a CTA's, so that neither
+      // sum passes 32 bits; else the sum's low word and its carries.
+      auto add_weight = [&](int b, uint32_t w) {
+        if (g.halves) {
+          atomicAdd(&hist.low[b], w & 0xFFFFu);
+          atomicAdd(&hist.high[b], w >> 16);
+        } else {
+          const uint32_t old = atomicAdd(&hist.low[b], w);
+          if (old + w < old) atomicAdd(&hist.high[b], 1u);
+        }
+      };
       if (fresh) {
         auto enter = [&](float x) {
           const float z = scale.z(x);
@@ -529,8 +541,7 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
           if (by_weight) {
             const uint32_t w = Scale::weight(expf(z));
             if (b < kBins) {
-              const uint32_t old = atomicAdd(&hist.low[b], w);
-              if (old + w < old) atomicAdd(&hist.high[b], 1u);
+              add_weight(b, w);
               if (by_count) atomicAdd(&hist.count[b], 1u);
             }
           } else if (b < kBins) {
@@ -570,9 +581,7 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
             const float z = scale.z(x);
             if (down <= range && Scale::bin(z) == o.bin) {
               if (by_weight) {
-                const uint32_t w = Scale::weight(expf(z));
-                const uint32_t old = atomicAdd(&hist.low[down >> shift], w);
-                if (old + w < old) atomicAdd(&hist.high[down >> shift], 1u);
+                add_weight(down >> shift, Scale::weight(expf(z)));
               }
               atomicAdd(&hist.count[down >> shift], 1u);
             }
@@ -598,10 +607,11 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
             }
             if (by_weight) {
               const uint4 hl = reinterpret_cast<const uint4 *>(h->low)[tid], hh = reinterpret_cast<const uint4 *>(h->high)[tid];
-              w[0] += (uint64_t(hh.x) << 32) + hl.x;
-              w[1] += (uint64_t(hh.y) << 32) + hl.y;
-              w[2] += (uint64_t(hh.z) << 32) + hl.z;
-              w[3] += (uint64_t(hh.w) << 32) + hl.w;
+              const int up = g.halves ? 16 : 32;
+              w[0] += (uint64_t(hh.x) << up) + hl.x;
+              w[1] += (uint64_t(hh.y) << up) + hl.y;
+              w[2] += (uint64_t(hh.z) << up) + hl.z;
+              w[3] += (uint64_t(hh.w) << up) + hl.w;
             }
           }
         }
@@ -951,6 +961,7 @@ int launch_sample(const char *what, SampleArgs g, int64_t rows, cudaStream_t str
   const int64_t slice = ceil_div(vecs, ranks);
   TB_REQUIRE(rows * ranks <= 0x7fffffffLL && slice <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: too many rows", what);
   g.slice_vecs = static_cast<int>(slice);
+  g.halves = slice * (16 / int64_t(sizeof(T))) <= 65536;
   size_t smem = 16;
   if (search) smem += sizeof(Histogram);
   if (resident) smem += static_cast<size_t>(slice) * 16;
