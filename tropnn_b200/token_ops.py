@@ -212,16 +212,16 @@ def _logit_rows(logits: Tensor) -> tuple[Tensor, int, int, int, int]:
     """``(logits, rows, inner, outer_stride, inner_stride)``: row n of ``logits[..., vocab]`` starts
     at element ``(n // inner) * outer_stride + (n % inner) * inner_stride``. A slice such as
     ``logits[:, :-1]`` of a batch of sequences is read in place; other layouts are copied."""
-    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
-        logits = logits.contiguous()
-    shape, stride = logits.shape[:-1], logits.stride()[:-1]
+    stride = logits.stride()
+    if stride[-1] != 1 and logits.shape[-1] > 1:
+        logits = logits.detach().contiguous()
+        stride = logits.stride()
+    shape = logits.shape
     if len(shape) == 2:
-        return logits, shape[0] * shape[1], max(1, shape[1]), stride[0], stride[1]
-    if len(shape) == 1:
         return logits, shape[0], 1, stride[0], 0
-    logits = logits.contiguous()
-    rows = math.prod(shape)
-    return logits, rows, 1, logits.shape[-1], 0
+    if len(shape) == 3:
+        return logits, shape[0] * shape[1], max(1, shape[1]), stride[0], stride[1]
+    return logits.detach().contiguous(), math.prod(shape[:-1]), 1, shape[-1], 0
 
 
 # ---------------------------------------------------------------------------
@@ -268,10 +268,12 @@ class _Distill:
         if label_weight > 0.0 and labels is None:
             raise ValueError("label_weight > 0 needs labels")
         self.lead = lead
-        self.logits, self.rows, inner, outer_stride, inner_stride = _logit_rows(logits.detach())
-        self.teacher = teacher.detach().contiguous()
+        self.logits, self.rows, inner, outer_stride, inner_stride = _logit_rows(logits)
+        self.teacher = teacher if teacher.is_contiguous() else teacher.detach().contiguous()
         self.indices = indices.contiguous()
-        self.labels = None if labels is None else labels.to(torch.int64).contiguous()
+        self.labels = labels
+        if labels is not None and not (labels.dtype == torch.int64 and labels.is_contiguous()):
+            self.labels = labels.to(torch.int64).contiguous()
         self.args = (
             self.logits.data_ptr(), nat.float_code(logits.dtype), self.rows, inner, outer_stride, inner_stride,
             logits.shape[-1], self.teacher.data_ptr(), nat.float_code(teacher.dtype), self.indices.data_ptr(),
@@ -280,19 +282,26 @@ class _Distill:
         )
 
 
+def _distill_loss(call: _Distill, reduction: str) -> tuple[Tensor, Tensor, Tensor | None]:
+    """``(loss, stats, count)``: the statistics that the gradient needs, and the divisor of a mean or
+    sum."""
+    lib = nat.load()
+    dev = call.logits.device
+    losses = torch.empty(call.lead, device=dev, dtype=torch.float32)
+    stats = losses.new_empty((call.rows, 4))
+    _call(dev, "distill_loss", lib.tropnn_b200_distill_loss, *call.args, losses.data_ptr(), stats.data_ptr())
+    if reduction == "none":
+        return losses, stats, None
+    loss, count = losses.new_empty(()), losses.new_empty(())
+    _call(dev, "distill_reduce", lib.tropnn_b200_distill_reduce, losses.data_ptr(), stats.data_ptr(), call.rows,
+          int(reduction == "mean"), loss.data_ptr(), count.data_ptr())
+    return loss, stats, count
+
+
 class _DistillLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, logits: Tensor, call: _Distill, reduction: str) -> Tensor:  # type: ignore[override]
-        dev = logits.device
-        lib = nat.load()
-        losses = torch.empty(call.lead, device=dev, dtype=torch.float32)
-        stats = losses.new_empty((call.rows, 4))
-        _call(dev, "distill_loss", lib.tropnn_b200_distill_loss, *call.args, losses.data_ptr(), stats.data_ptr())
-        loss, count = losses, None
-        if reduction != "none":
-            loss, count = losses.new_empty(()), losses.new_empty(())
-            _call(dev, "distill_reduce", lib.tropnn_b200_distill_reduce, losses.data_ptr(), stats.data_ptr(), call.rows,
-                  int(reduction == "mean"), loss.data_ptr(), count.data_ptr())
+        loss, stats, count = _distill_loss(call, reduction)
         # The call holds its tensors' addresses; saving them finds out a change in place.
         ctx.save_for_backward(logits, stats, count, call.teacher, call.indices, call.labels)
         ctx.call = call
@@ -340,7 +349,9 @@ def distill_loss_b200(
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     call = _Distill(logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
-    return _DistillLossFunction.apply(logits, call, reduction)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _DistillLossFunction.apply(logits, call, reduction)
+    return _distill_loss(call, reduction)[0]
 
 
 def distill_loss_grad_b200(
@@ -450,7 +461,7 @@ def sample_tokens_b200(
         if k_value < 0:
             raise ValueError(f"top_k must be >= 0, got {k_value}")
         k_value = min(k_value, vocab)
-    logits, rows, inner, outer_stride, inner_stride = _logit_rows(logits.detach())
+    logits, rows, inner, outer_stride, inner_stride = _logit_rows(logits)
     uniforms = uniforms.contiguous()
     tokens = torch.empty(lead, device=dev, dtype=torch.int64)
     _call(
