@@ -116,6 +116,11 @@ __device__ __forceinline__ void bulk_load_1d(void *dst, const void *src, uint32_
                : "memory");
 }
 
+// Brings `bytes` (a multiple of 16, from a 16-byte aligned address) of global memory into L2.
+__device__ __forceinline__ void bulk_prefetch(const void *src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
 // 2-D tiled TMA load into this CTA's shared memory, completion counted on `bar`.
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y) {
   asm volatile(
