@@ -68,6 +68,8 @@ struct DistillArgs {
   void *grad;
   int ranks;       // CTAs of a row
   int slice_vecs;  // 16-byte vectors of a CTA's slice
+  int64_t rows;
+  int rows_at_once;  // that the GPU holds
 };
 
 // Rows and `inner` are below 2^31.
@@ -164,10 +166,14 @@ __device__ __forceinline__ uint4 load_vec(const T *grid, int64_t v, int64_t lead
   return *reinterpret_cast<const uint4 *>(e);
 }
 
-// The gradient's CTA asks for the beginning of its part before it has the statistics: 4096 x 32000 bf16
-// 104 us without, 98 with 32 KB, 89 with 64 KB; at 8192 x 131072 702 us with 64 KB and 737 with 128 KB,
-// as the CTAs there hold more than L2 does. (The loss has no such wait: 58 -> 55 us at the one, but 34 ->
-// 35 at 1000 x 50001 f16, so it does without.)
+// The whole vectors of x's elements [e0, e1), the first 64 KB of them, on their way to L2.
+//  - The gradient's CTA asks for its part before it has the statistics: 4096 x 32000 bf16 104 us without,
+//    98 with 32 KB, 89 with 64 KB; at 8192 x 131072 705, 705 and 702, but 737 with 128 KB, as the CTAs there
+//    ask for more than L2 holds.
+//  - With a row in shared memory a CTA asks, as it begins to write, for the slice of the row that follows
+//    when all rows now on the GPU are done: 8192 x 131072 bf16 918 us without, 874 with it.
+//  - The loss, which is at its rows at once, does without: 58 -> 55 us at 4096 x 32000, but 34 -> 35 at
+//    1000 x 50001 f16, and 64 with the row that follows.
 constexpr int64_t kPrefetch = 64 * 1024;
 template <typename T>
 __device__ __forceinline__ void prefetch(const T *x, int64_t e0, int64_t e1) {
@@ -604,6 +610,8 @@ __global__ void __launch_bounds__(kBlock, RESIDENT ? 3 : 4) distill_row_kernel(c
   const bool has_teacher = teacher.parts > 0, has_label = table.label >= 0;
   if constexpr (MODE == kFused) {
     T *out = static_cast<T *>(g.grad) + row * g.vocab;
+    if (RESIDENT && tid == kThreads && row + g.rows_at_once < g.rows)
+      prefetch<T>(row_of<T>(g, row32 + g.rows_at_once), e0, e1);
     if (has_teacher || has_label) {
       const GradScale c = grad_scale(g, has_teacher, has_label, scale, inv_t, inv_1);
       const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
@@ -729,6 +737,8 @@ int launch_rows(const char *what, DistillArgs g, int64_t rows, cudaStream_t stre
     if constexpr (MODE == kFused) {
       if (slice * 16 <= kSliceMost) {
         kernel = reinterpret_cast<const void *>(distill_row_kernel<T, MODE, EXPS, true>);
+        g.rows = rows;
+        g.rows_at_once = std::max(1, (slice * 16 <= kSliceShared ? 3 : 1) * sms / ranks);
         config.dynamicSmemBytes = static_cast<size_t>(slice) * 16;
         // The static tables count too: above 48 KB in all the kernel has to be told.
         TB_CHECK(ensure_dynamic_smem(kernel, std::max<size_t>(config.dynamicSmemBytes, 49 * 1024), what));

@@ -333,10 +333,6 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
   const T *grid = x - lead;
   const int64_t vec0 = int64_t(rank) * g.slice_vecs;
   const int vecs = static_cast<int>(min64(g.slice_vecs, max(int64_t(0), (end + kN - 1) / kN - vec0)));
-  auto at = [&](int v) -> uint4 {
-    if constexpr (RESIDENT) return kept_slice[v];
-    else return load_vec<T>(grid, vec0 + v, lead, end);
-  };
   auto element = [&](int v, int j) -> float {
     if constexpr (RESIDENT) return to_f32<T>(reinterpret_cast<const T *>(kept_slice)[v * kN + j]);
     else return ldg_f32(grid + (vec0 + v) * kN + j);
