@@ -240,6 +240,31 @@ def test_steps_continue_a_prefill(batch, dim, dtype) -> None:
     assert bool(room[:, dim:].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_steps_do_not_depend_on_alignment(dtype) -> None:
+    """The same rows where four channels lie on one boundary and where a row or a pointer does not."""
+    gate, value, h0 = _inputs(70, 1, 260, dtype, 15)
+    gate, value = gate[:, 0], value[:, 0]
+    reset = (torch.rand(70, generator=torch.Generator().manual_seed(3)) < 0.3).cuda()
+    want, want_state = _reference(gate[:, None], value[:, None], h0, reset[:, None])
+
+    def placed(t, pad, offset):
+        room = torch.full((t.shape[0] * (t.shape[1] + pad) + offset,), float("nan"), device="cuda", dtype=t.dtype)
+        view = room[offset:].view(t.shape[0], -1)[:, : t.shape[1]]
+        return view.copy_(t)
+
+    results = []
+    for pads in ((0, 0, 0), (4, 8, 12), (1, 0, 0), (0, 3, 0), (0, 0, 2)):
+        for offsets in ((0, 0, 0), (4, 4, 4), (1, 0, 0), (0, 2, 0), (0, 0, 3)):
+            g, x, s = (placed(t, pad, offset) for t, pad, offset in zip((gate, value, h0), pads, offsets))
+            h = tropnn_b200.gated_recurrence_step_b200(g, x, s, reset=reset)
+            _close(h, want[:, 0], dtype)
+            _close(s, want_state, torch.float32)
+            results.append((h, s.clone()))
+    for h, s in results[1:]:
+        assert torch.equal(h, results[0][0]) and torch.equal(s, results[0][1])
+
+
 def test_runs_are_bitwise_equal_and_do_not_depend_on_the_batch() -> None:
     gate, value, h0 = _inputs(5, 777, 130, torch.bfloat16, 12)
     runs = []

@@ -18,6 +18,12 @@
 // statistics known, each streaming through registers.
 // exp2 runs on the special-function unit (16 a clock and SM), two of them an element and pass where
 // T and the labels need two sums: with T = 2 the second is the square of the first.
+//
+// Measured (bf16): the loss of 8192 x 131072 335 us (6.4 TB/s, 98 % of a copy's rate), the gradient 683 us
+// (6.3 TB/s), both HBM-bound; in one call 877 us (4.9 TB/s), bound by how the three CTAs of an SM overlap
+// their loads, exponentials (476 us of that unit) and stores. 4096 x 32000 with labels at T = 2: 56 us,
+// 84 us and 106 us. In one call four CTAs an SM with six slices a row take 975 us, eight slices 1141; with
+// the row read again instead of kept 2048 x 131072 takes 247 us and not 227, 1 x 131072 7.4 and not 6.6.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -707,7 +713,8 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float *losse
   }
 }
 
-// CTAs an SM up to which a row is split further.
+// CTAs an SM up to which a row is split further. 16 x 131072 bf16, split and not: loss 6.9 and 13.6 us,
+// gradient 4.9 and 12.1 us (148 rows 17 and 23 us), in one call 8.0 and 9.0 us.
 template <int MODE>
 constexpr int kIdle = MODE == kGrad ? 4 : 1;
 

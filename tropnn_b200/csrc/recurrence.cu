@@ -16,7 +16,8 @@
 //    or through global memory between two launches.
 // Measured at 8 x 2048 x 1024 bf16: forward 29 us by tiles (3.5 TB/s of reads and writes), 41 us by
 // segments; backward 44 us by segments (3.8 TB/s), 58 us by tiles. At 1 x 65536 x 256 f16: forward 37 us
-// by segments, 46 us by tiles of chunks.
+// and backward 45 us by segments in two launches, 169 and 231 us by tiles and segments of one cluster.
+// At 3 x 1531 x 777 f32, whose rows allow neither pairs nor TMA: 19 and 43 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -1039,22 +1040,42 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
   if (TMA && lane == 0) sm100::bulk_wait_read_all();
 }
 
-// One token of every row: state (f32, updated in place) and h. A few KB to a few MB: launch
-// latency, then one read and one write of each operand.
-template <typename T>
+// One token of every row: state (f32, updated in place) and h. One read and one write of each operand:
+// launch latency up to some hundred rows (8 x 1024 bf16 1.2 us), then HBM. N channels a thread: 4 where
+// addresses and strides allow it, else 1 (4096 x 4096 bf16: 36 us, 6.6 TB/s, and 61 us).
+template <typename T, int N>
 __global__ void __launch_bounds__(256) recurrence_step_kernel(const T *__restrict__ gate, int64_t gate_row,
                                                               const T *__restrict__ value, int64_t value_row,
                                                               const uint8_t *__restrict__ reset, int64_t dim,
                                                               float *state, int64_t state_row, T *__restrict__ h) {
-  const int64_t ch = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  struct alignas(N * sizeof(T)) Values {
+    T v[N];
+  };
+  struct alignas(N * sizeof(float)) States {
+    float v[N];
+  };
+  const int64_t ch = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) * N;
   const int64_t row = blockIdx.y;
   if (ch >= dim) return;
-  const float before = reset != nullptr && reset[row] != 0 ? 0.f : state[row * state_row + ch];
-  float2 a, c;
-  gates2(make_float2(to_f32<T>(gate[row * gate_row + ch]), 0.f), a, c);
-  const float now = fmaf(a.x, before, c.x * to_f32<T>(value[row * value_row + ch]));
-  state[row * state_row + ch] = now;
-  h[row * dim + ch] = from_f32<T>(now);
+  const Values f = *reinterpret_cast<const Values *>(gate + row * gate_row + ch);
+  const Values x = *reinterpret_cast<const Values *>(value + row * value_row + ch);
+  States s = *reinterpret_cast<const States *>(state + row * state_row + ch);
+  const bool fresh = reset != nullptr && reset[row] != 0;
+  Values out;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const int j = N > 1 ? i + 1 : i;
+    float2 a, c;
+    gates2(make_float2(to_f32<T>(f.v[i]), N > 1 ? to_f32<T>(f.v[j]) : 0.f), a, c);
+    s.v[i] = fmaf(a.x, fresh ? 0.f : s.v[i], c.x * to_f32<T>(x.v[i]));
+    out.v[i] = from_f32<T>(s.v[i]);
+    if (N > 1) {
+      s.v[j] = fmaf(a.y, fresh ? 0.f : s.v[j], c.y * to_f32<T>(x.v[j]));
+      out.v[j] = from_f32<T>(s.v[j]);
+    }
+  }
+  *reinterpret_cast<States *>(state + row * state_row + ch) = s;
+  *reinterpret_cast<Values *>(h + row * dim + ch) = out;
 }
 
 inline size_t elem_bytes(int dtype) { return dtype == TROPNN_B200_F32 ? 4 : 2; }
@@ -1071,7 +1092,8 @@ int check_sizes(const char *what, int dtype, int64_t batch, int64_t steps, int64
 
 // How a sequence is shared out: chunks of kWarps segments, a CTA each, as many as are on the GPU at once.
 // Up to 8 chunks are a cluster. Where 8 are less than half of that, and at least 4 runs a segment are
-// left, there are more chunks and two launches; a forward pass not cut so goes by tiles.
+// left, there are more chunks and two launches; a forward pass not cut so goes by tiles. 1 x 16384 x 1024
+// bf16, cut and not: forward 39 and 58 us, backward 45 and 82 us.
 struct Plan {
   int chunks = 1;
   bool two_launches = false;
@@ -1097,6 +1119,9 @@ size_t maps_bytes(const Plan &p, int64_t batch, int64_t dim) {
   return p.two_launches ? static_cast<size_t>(batch * p.chunks * kMapSlots * dim) * sizeof(float2) : 0;
 }
 
+// Sequences come by TMA where they can, else by loads of pairs of channels, else of single ones. 8 x 2048 x
+// 1024 bf16 by TMA and by pairs: forward 29.0 and 30.5 us, backward 44 and 59; 1 x 65536 x 256 f16 37 and
+// 54, 45 and 56.
 // A [batch, steps, dim] tensor (strides in elements) in boxes of `run` steps x 64 channels. False where
 // TMA cannot take it.
 bool sequence_map(CUtensorMap *map, const void *ptr, int dtype, int64_t batch, int64_t steps, int64_t dim,
@@ -1322,20 +1347,26 @@ int tropnn_b200_recurrence_step(const void *gate, int64_t gate_stride, const voi
   int64_t done = 0;
   while (done < batch) {  // a launch takes 65535 rows (the grid's y extent)
     const int64_t rows = min64(batch - done, 65535);
-    const dim3 grid(static_cast<unsigned>(ceil_div(dim, 256)), static_cast<unsigned>(rows));
     const size_t eb = elem_bytes(dtype);
     const char *gp = static_cast<const char *>(gate) + done * gate_stride * int64_t(eb);
     const char *vp = static_cast<const char *>(value) + done * value_stride * int64_t(eb);
     char *hp = static_cast<char *>(h) + done * dim * int64_t(eb);
     const uint8_t *rp = reset != nullptr ? reset + done : nullptr;
     float *sp = state + done * state_stride;
-#define TB_STEP(T)                                                                                              \
-  recurrence_step_kernel<T><<<grid, 256, 0, as_stream(stream)>>>(reinterpret_cast<const T *>(gp), gate_stride,   \
-                                                                 reinterpret_cast<const T *>(vp), value_stride, rp, \
-                                                                 dim, sp, state_stride, reinterpret_cast<T *>(hp))
+    const bool wide = (dim | gate_stride | value_stride | state_stride) % 4 == 0 &&
+                      (reinterpret_cast<uintptr_t>(gp) | reinterpret_cast<uintptr_t>(vp) | reinterpret_cast<uintptr_t>(hp)) % (4 * eb) == 0 &&
+                      reinterpret_cast<uintptr_t>(sp) % 16 == 0;
+    const int64_t threads = wide ? dim / 4 : dim;
+    const dim3 grid(static_cast<unsigned>(ceil_div(threads, 256)), static_cast<unsigned>(rows));
+#define TB_STEP_N(T, N)                                                                                          \
+  recurrence_step_kernel<T, N><<<grid, 256, 0, as_stream(stream)>>>(reinterpret_cast<const T *>(gp), gate_stride, \
+                                                                    reinterpret_cast<const T *>(vp), value_stride, rp, \
+                                                                    dim, sp, state_stride, reinterpret_cast<T *>(hp))
+#define TB_STEP(T) wide ? (TB_STEP_N(T, 4)) : (TB_STEP_N(T, 1))
     if (dtype == TROPNN_B200_F32) TB_STEP(float);
     else if (dtype == TROPNN_B200_F16) TB_STEP(__half);
     else TB_STEP(__nv_bfloat16);
+#undef TB_STEP_N
 #undef TB_STEP
     TB_CHECK(check_launch(what));
     done += rows;
