@@ -275,6 +275,32 @@ def test_side_stream_two_backwards_and_in_place_changes() -> None:
         torch.autograd.grad(loss, leaf)
 
 
+@pytest.mark.parametrize("view", [False, True])
+def test_saved_tensors_are_released_and_may_be_moved(view) -> None:
+    """A loss that outlives its backward holds no logits, and saved tensors may come back elsewhere."""
+    logits, teacher, at, labels = _inputs(64, 5000, 8, torch.bfloat16, 16)
+    if view:
+        logits = torch.cat([logits, logits], dim=1)[:, :5000]
+    kw = dict(temperature=2.0, label_weight=0.25)
+    leaf = logits.detach().requires_grad_()
+    (want,) = torch.autograd.grad(tropnn_b200.distill_loss_b200(leaf, teacher, at, labels, **kw), leaf)
+    with torch.autograd.graph.save_on_cpu():
+        loss = tropnn_b200.distill_loss_b200(leaf, teacher, at, labels, **kw)
+    junk = [torch.full_like(t, 1) for t in (logits, teacher, at, labels)]
+    (got,) = torch.autograd.grad(loss, leaf)
+    assert torch.equal(got, want)
+    del junk, loss
+
+    before = torch.cuda.memory_allocated()
+    student = leaf * 1.0
+    loss = tropnn_b200.distill_loss_b200(student, teacher, at, labels, **kw)
+    del student
+    loss.backward()
+    leaf.grad = None
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - before <= 4096  # the loss itself
+
+
 def test_offsets_past_32_bits() -> None:
     far = (1 << 31) + 8
     store = torch.zeros(far + 4096, dtype=torch.float16, device="cuda")

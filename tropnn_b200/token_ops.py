@@ -229,94 +229,102 @@ def _logit_rows(logits: Tensor) -> tuple[Tensor, int, int, int, int]:
 # ---------------------------------------------------------------------------
 
 
-class _Distill:
-    """Checked arguments of one call, in the order of the C entry points."""
-
-    def __init__(
-        self, logits: Tensor, teacher: Tensor, indices: Tensor, labels: Tensor | None, temperature: float,
-        label_weight: float, ignore_index: int,
-    ) -> None:
-        _require_cuda(logits, "logits")
-        dev = logits.device
-        _same_device(dev, teacher, "teacher_logits")
-        _same_device(dev, indices, "teacher_indices")
-        nat.float_code(logits.dtype)
-        nat.float_code(teacher.dtype)
-        if logits.ndim < 1 or logits.shape[-1] < 1:
-            raise ValueError(f"logits must have shape [..., vocab] with vocab >= 1, got {tuple(logits.shape)}")
-        lead = logits.shape[:-1]
-        if teacher.ndim != logits.ndim or teacher.shape[:-1] != lead or indices.shape != teacher.shape:
-            raise ValueError(
-                f"teacher_logits and teacher_indices must both have shape {(*lead, 'top')}, got {tuple(teacher.shape)} "
-                f"and {tuple(indices.shape)}"
-            )
-        if teacher.shape[-1] > MAX_TEACHER_TOP:
-            raise ValueError(f"at most {MAX_TEACHER_TOP} teacher entries a row, got {teacher.shape[-1]}")
-        if indices.dtype not in (torch.int64, torch.int32):
-            raise TypeError(f"teacher_indices must be int64 or int32, got {indices.dtype}")
-        if labels is not None:
-            _same_device(dev, labels, "labels")
-            if labels.shape != lead:
-                raise ValueError(f"labels must have shape {tuple(lead)}, got {tuple(labels.shape)}")
-            if labels.dtype not in (torch.int64, torch.int32):
-                raise TypeError(f"labels must be int64 or int32, got {labels.dtype}")
-        temperature, label_weight = float(temperature), float(label_weight)
-        if not (0.0 < temperature < math.inf):
-            raise ValueError(f"temperature must be positive and finite, got {temperature}")
-        if not (0.0 <= label_weight <= 1.0):
-            raise ValueError(f"label_weight must be in [0, 1], got {label_weight}")
-        if label_weight > 0.0 and labels is None:
-            raise ValueError("label_weight > 0 needs labels")
-        self.lead = lead
-        self.logits, self.rows, inner, outer_stride, inner_stride = _logit_rows(logits)
-        self.teacher = teacher if teacher.is_contiguous() else teacher.detach().contiguous()
-        self.indices = indices.contiguous()
-        self.labels = labels
-        if labels is not None and not (labels.dtype == torch.int64 and labels.is_contiguous()):
-            self.labels = labels.to(torch.int64).contiguous()
-        self.args = (
-            self.logits.data_ptr(), nat.float_code(logits.dtype), self.rows, inner, outer_stride, inner_stride,
-            logits.shape[-1], self.teacher.data_ptr(), nat.float_code(teacher.dtype), self.indices.data_ptr(),
-            nat.I64 if indices.dtype == torch.int64 else nat.I32, teacher.shape[-1], nat.ptr(self.labels),
-            int(ignore_index), temperature, label_weight,
+def _distill_check(
+    logits: Tensor, teacher: Tensor, indices: Tensor, labels: Tensor | None, temperature: float, label_weight: float,
+    ignore_index: int,
+) -> tuple[Tensor, Tensor, Tensor | None, tuple[int, float, float]]:
+    """The teacher's entries and the labels as the kernels take them, and the settings."""
+    _require_cuda(logits, "logits")
+    dev = logits.device
+    _same_device(dev, teacher, "teacher_logits")
+    _same_device(dev, indices, "teacher_indices")
+    nat.float_code(logits.dtype)
+    nat.float_code(teacher.dtype)
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must have shape [..., vocab] with vocab >= 1, got {tuple(logits.shape)}")
+    lead = logits.shape[:-1]
+    if teacher.ndim != logits.ndim or teacher.shape[:-1] != lead or indices.shape != teacher.shape:
+        raise ValueError(
+            f"teacher_logits and teacher_indices must both have shape {(*lead, 'top')}, got {tuple(teacher.shape)} "
+            f"and {tuple(indices.shape)}"
         )
+    if teacher.shape[-1] > MAX_TEACHER_TOP:
+        raise ValueError(f"at most {MAX_TEACHER_TOP} teacher entries a row, got {teacher.shape[-1]}")
+    if indices.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"teacher_indices must be int64 or int32, got {indices.dtype}")
+    if labels is not None:
+        _same_device(dev, labels, "labels")
+        if labels.shape != lead:
+            raise ValueError(f"labels must have shape {tuple(lead)}, got {tuple(labels.shape)}")
+        if labels.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"labels must be int64 or int32, got {labels.dtype}")
+        if labels.dtype != torch.int64 or not labels.is_contiguous():
+            labels = labels.to(torch.int64).contiguous()
+    temperature, label_weight = float(temperature), float(label_weight)
+    if not (0.0 < temperature < math.inf):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not (0.0 <= label_weight <= 1.0):
+        raise ValueError(f"label_weight must be in [0, 1], got {label_weight}")
+    if label_weight > 0.0 and labels is None:
+        raise ValueError("label_weight > 0 needs labels")
+    if teacher.requires_grad or not teacher.is_contiguous():
+        teacher = teacher.detach().contiguous()
+    return teacher, indices.contiguous(), labels, (int(ignore_index), temperature, label_weight)
 
 
-def _distill_loss(call: _Distill, reduction: str) -> tuple[Tensor, Tensor, Tensor | None]:
+def _distill_args(
+    logits: Tensor, teacher: Tensor, indices: Tensor, labels: Tensor | None, settings: tuple[int, float, float]
+) -> tuple[Tensor, int, tuple[Any, ...]]:
+    """``(logits as read, rows, the C entry points' common arguments)``."""
+    read, rows, inner, outer_stride, inner_stride = _logit_rows(logits)
+    return read, rows, (
+        read.data_ptr(), nat.float_code(read.dtype), rows, inner, outer_stride, inner_stride, read.shape[-1],
+        teacher.data_ptr(), nat.float_code(teacher.dtype), indices.data_ptr(),
+        nat.I64 if indices.dtype == torch.int64 else nat.I32, teacher.shape[-1], nat.ptr(labels), *settings,
+    )
+
+
+def _distill_loss(
+    logits: Tensor, teacher: Tensor, indices: Tensor, labels: Tensor | None, settings: tuple[int, float, float],
+    reduction: str,
+) -> tuple[Tensor, Tensor, Tensor | None]:
     """``(loss, stats, count)``: the statistics that the gradient needs, and the divisor of a mean or
     sum."""
     lib = nat.load()
-    dev = call.logits.device
-    losses = torch.empty(call.lead, device=dev, dtype=torch.float32)
-    stats = losses.new_empty((call.rows, 4))
-    _call(dev, "distill_loss", lib.tropnn_b200_distill_loss, *call.args, losses.data_ptr(), stats.data_ptr())
+    dev = logits.device
+    read, rows, args = _distill_args(logits, teacher, indices, labels, settings)
+    losses = torch.empty(logits.shape[:-1], device=dev, dtype=torch.float32)
+    stats = losses.new_empty((rows, 4))
+    _call(dev, "distill_loss", lib.tropnn_b200_distill_loss, *args, losses.data_ptr(), stats.data_ptr())
     if reduction == "none":
         return losses, stats, None
     loss, count = losses.new_empty(()), losses.new_empty(())
-    _call(dev, "distill_reduce", lib.tropnn_b200_distill_reduce, losses.data_ptr(), stats.data_ptr(), call.rows,
+    _call(dev, "distill_reduce", lib.tropnn_b200_distill_reduce, losses.data_ptr(), stats.data_ptr(), rows,
           int(reduction == "mean"), loss.data_ptr(), count.data_ptr())
     return loss, stats, count
 
 
 class _DistillLossFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, logits: Tensor, call: _Distill, reduction: str) -> Tensor:  # type: ignore[override]
-        loss, stats, count = _distill_loss(call, reduction)
-        # The call holds its tensors' addresses; saving them finds out a change in place.
-        ctx.save_for_backward(logits, stats, count, call.teacher, call.indices, call.labels)
-        ctx.call = call
+    def forward(  # type: ignore[override]
+        ctx: Any, logits: Tensor, teacher: Tensor, indices: Tensor, labels: Tensor | None,
+        settings: tuple[int, float, float], reduction: str,
+    ) -> Tensor:
+        loss, stats, count = _distill_loss(logits, teacher, indices, labels, settings, reduction)
+        ctx.save_for_backward(logits, stats, count, teacher, indices, labels)
+        ctx.settings = settings
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad_loss: Tensor) -> tuple[Any, ...]:
-        logits, stats, count, *_ = ctx.saved_tensors
-        call = ctx.call
-        grad = logits.new_empty(logits.shape)
+        logits, stats, count, teacher, indices, labels = ctx.saved_tensors
+        read, _, args = _distill_args(logits, teacher, indices, labels, ctx.settings)
+        grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
         scale = grad_loss.contiguous()
-        _call(logits.device, "distill_grad", nat.load().tropnn_b200_distill_grad, *call.args, stats.data_ptr(),
+        _call(logits.device, "distill_grad", nat.load().tropnn_b200_distill_grad, *args, stats.data_ptr(),
               scale.data_ptr(), int(count is None), nat.ptr(count), grad.data_ptr())
-        return grad, None, None
+        return grad, None, None, None, None, None
 
 
 def distill_loss_b200(
@@ -348,10 +356,11 @@ def distill_loss_b200(
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
-    call = _Distill(logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
+    teacher, indices, labels, settings = _distill_check(
+        logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _DistillLossFunction.apply(logits, call, reduction)
-    return _distill_loss(call, reduction)[0]
+        return _DistillLossFunction.apply(logits, teacher, indices, labels, settings, reduction)
+    return _distill_loss(logits, teacher, indices, labels, settings, reduction)[0]
 
 
 def distill_loss_grad_b200(
@@ -370,22 +379,24 @@ def distill_loss_grad_b200(
     one-element f32 tensor, or f32 ``[...]``: the upstream gradient with the divisor of a mean and
     a loss scale in it, so that a gradient in f16 is scaled before it is rounded. For training
     loops that call the head's backward themselves, such as a head in chunks of rows."""
-    call = _Distill(logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
-    dev = logits.device
+    teacher, indices, labels, settings = _distill_check(
+        logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
+    dev, lead = logits.device, logits.shape[:-1]
     scale: Tensor | None = None
     if isinstance(row_scale, Tensor):
         _same_device(dev, row_scale, "row_scale")
         if row_scale.dtype != torch.float32:
             raise TypeError(f"row_scale must be float32, got {row_scale.dtype}")
-        if row_scale.numel() != 1 and row_scale.shape != call.lead:
-            raise ValueError(f"row_scale must have one element or shape {tuple(call.lead)}, got {tuple(row_scale.shape)}")
+        if row_scale.numel() != 1 and row_scale.shape != lead:
+            raise ValueError(f"row_scale must have one element or shape {tuple(lead)}, got {tuple(row_scale.shape)}")
         scale = row_scale.detach().contiguous()
     elif row_scale is not None:
         scale = torch.full((1,), float(row_scale), device=dev, dtype=torch.float32)
-    per_row = scale is not None and scale.shape == call.lead
-    losses = torch.empty(call.lead, device=dev, dtype=torch.float32)
+    per_row = scale is not None and scale.shape == lead
+    read, _, args = _distill_args(logits, teacher, indices, labels, settings)
+    losses = torch.empty(lead, device=dev, dtype=torch.float32)
     grad = logits.new_empty(logits.shape)
-    _call(dev, "distill_loss_grad", nat.load().tropnn_b200_distill_loss_grad, *call.args, nat.ptr(scale), int(per_row),
+    _call(dev, "distill_loss_grad", nat.load().tropnn_b200_distill_loss_grad, *args, nat.ptr(scale), int(per_row),
           losses.data_ptr(), grad.data_ptr())
     return losses, grad
 
