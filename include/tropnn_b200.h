@@ -620,7 +620,8 @@ TROPNN_B200_API int tropnn_b200_trop_backward(const float *grad_hidden, const fl
  * gate and value in `dtype` (F32/F16/BF16) with strides in elements over batch and steps and unit
  * stride over dim; h0 f32 [batch, dim] (NULL: zeros), reset u8 [batch, steps] (NULL: none). h
  * [batch, steps, dim] contiguous in `dtype`, h_last f32 [batch, dim] (h0 when steps is 0). The
- * state is f32 throughout. `saved` (NULL: not kept) receives the f32 states that the backward
+ * state is f32 throughout; one that is not finite stays so until a reset (an infinity may become a
+ * NaN). `saved` (NULL: not kept) receives the f32 states that the backward
  * starts from, tropnn_b200_recurrence_saved_size bytes. The workspace (that of the forward or of the
  * backward call alone, 0 bytes unless a long sequence is cut into chunks) is
  * tropnn_b200_recurrence_workspace_size bytes, 8-byte aligned. Deterministic.

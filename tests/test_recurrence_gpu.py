@@ -210,6 +210,65 @@ def test_reset_drops_whatever_came_before(start, poison) -> None:
     _close(last, tail_last, torch.float32)
 
 
+STRETCHES = [  # one tile a CTA and clusters of tiles, segments in a cluster and in two launches; TMA, pairs, single channels
+    (1, 400, 66, torch.float32),
+    (2, 1100, 128, torch.bfloat16),
+    (40, 300, 256, torch.float16),
+    (3, 700, 51, torch.float16),
+    (1, 6000, 96, torch.float32),
+    (2, 20011, 24, torch.float16),
+    (1, 20011, 21, torch.float32),
+]
+
+
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize(("batch", "steps", "dim", "dtype"), STRETCHES)
+def test_resets_that_are_all_false_hide_nothing(batch, steps, dim, dtype, poison) -> None:
+    """A value that is not finite stays one for all later tokens, and a gradient for all earlier ones, also
+    where the gates between multiply to less than f32 holds: reset false throughout is no reset."""
+    gen = torch.Generator().manual_seed(steps)
+    gate = torch.randn(batch, steps, dim, generator=gen).to(dtype).cuda()
+    value = torch.randn(batch, steps, dim, generator=gen).to(dtype).cuda()
+    grad = torch.randn(batch, steps, dim, generator=gen).to(dtype).cuda()
+    value[:, 0] = poison
+    grad[:, -1, ::2] = poison
+    runs = []
+    for reset in (None, torch.zeros(batch, steps, dtype=torch.bool, device="cuda")):
+        leaves = [t.detach().requires_grad_() for t in (gate, value)]
+        h, last = tropnn_b200.gated_recurrence_b200(*leaves, reset=reset)
+        runs.append((h, last, *torch.autograd.grad(h, leaves, grad)))
+    assert not bool(runs[0][1].isfinite().any()) and not bool(runs[0][3][:, 0, ::2].isfinite().any())
+    for got, want in zip(runs[1], runs[0]):
+        assert torch.equal(got.isfinite(), want.isfinite())
+        assert torch.equal(got[want.isfinite()], want[want.isfinite()])
+
+
+@pytest.mark.parametrize(("batch", "steps", "dim", "dtype"), STRETCHES)
+@pytest.mark.parametrize("part", [0.1, 0.5, 0.97])
+def test_reset_drops_a_nan_of_a_gate(batch, steps, dim, dtype, part) -> None:
+    """Gates that are NaN on one side of a reset leave states and gradients of the other side alone."""
+    gate, value, h0 = _inputs(batch, steps, dim, dtype, 9)
+    start = int(part * steps)
+    reset = torch.zeros(batch, steps, dtype=torch.bool, device="cuda")
+    reset[:, start] = True
+    grad = torch.randn(batch, steps, dim, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    none = torch.zeros(batch, dim, device="cuda")
+    for bad, good in ((slice(0, start), slice(start, steps)), (slice(start, steps), slice(0, start))):
+        poisoned = gate.clone()
+        poisoned[:, bad] = float("nan")
+        leaves = [t.detach().requires_grad_() for t in (poisoned, value, h0)]
+        h, last = tropnn_b200.gated_recurrence_b200(*leaves, reset=reset)
+        got = (h, *torch.autograd.grad([h, last], leaves, [grad, none]))
+        first = h0 if good.start == 0 else None
+        want = _reference(gate[:, good], value[:, good], first, None, grad[:, good])
+        for mine, ref in zip(got[:3], (want[0], want[2], want[3])):
+            _close(mine[:, good], ref, dtype)
+        if good.start == 0:
+            _close(got[3], want[4], torch.float32)
+        else:
+            _close(last, want[1], torch.float32)
+
+
 def test_reset_at_the_first_and_last_token_and_everywhere() -> None:
     gate, value, h0 = _inputs(3, 70, 64, torch.float32, 8)
     reset = torch.zeros(3, 70, dtype=torch.uint8, device="cuda")

@@ -4,7 +4,7 @@
 //   h_t = keep_t a_t h_{t-1} + c_t x_t                          (keep_t = 0 at a reset, else 1)
 //
 // The recurrence is linear, so a stretch of steps maps the state before it to P h + H with P the
-// product of its keep_t a_t. A lane has two neighbouring channels, a warp 64; both are computed in f32x2
+// product of its gates (marked where a reset cuts it). A lane has two neighbouring channels, a warp 64; both are computed in f32x2
 // instructions. Two schemes, each bound by issue slots and latencies before HBM:
 //  - tiles (the forward where the channels fill the GPU: 28 blocks of 64 and more, rows of the batch counted): a warp scans a run
 //    of steps in registers, the runs' maps are exchanged, and the run is scanned again from the state
@@ -144,11 +144,18 @@ __device__ __forceinline__ void gates2(float2 f, float2 &a, float2 &c) {
   gates1(f.y, a.y, c.y);
 }
 
-// P h + H. With resets about (`cuts`), a run that one cut (P = 0) takes nothing of h, not even an
-// infinity's NaN.
+// P h + H. A stretch that a reset cuts takes nothing of h, whatever h or its own P is: it says so by P =
+// kCut. A product of gates is never negative, but is 0 where it underflows (128 gates of an untrained
+// layer often do), and then a NaN in h stays one. `cuts`: resets are given.
+constexpr float kCut = -1.f;
 __device__ __forceinline__ float2 apply_run(float2 p, float2 h, float2 add, bool cuts) {
   if (!cuts) return fma2(p, h, add);
-  return make_float2(p.x == 0.f ? add.x : fmaf(p.x, h.x, add.x), p.y == 0.f ? add.y : fmaf(p.y, h.y, add.y));
+  return make_float2(p.x < 0.f ? add.x : fmaf(p.x, h.x, add.x), p.y < 0.f ? add.y : fmaf(p.y, h.y, add.y));
+}
+// P of two stretches, one after the other.
+__device__ __forceinline__ float2 join_runs(float2 p, float2 q, bool cuts) {
+  if (!cuts) return mul2(p, q);
+  return make_float2(p.x < 0.f || q.x < 0.f ? kCut : p.x * q.x, p.y < 0.f || q.y < 0.f ? kCut : p.y * q.y);
 }
 
 struct RecurrenceArgs {
@@ -204,7 +211,7 @@ __device__ __forceinline__ float2 exchange(const RecurrenceArgs &g, int64_t batc
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         ch = apply_run(ex.p[w][lane], ch, ex.h[w][lane], cuts);
-        cp = mul2(cp, ex.p[w][lane]);
+        cp = join_runs(cp, ex.p[w][lane], cuts);
       }
       if (PASS == kBoth) {
         if (g.chunks > 1)
@@ -247,7 +254,7 @@ __device__ __forceinline__ float2 exchange(const RecurrenceArgs &g, int64_t batc
     float2 mp, mh;
     map_at(c, kWarps, mp, mh);
     h = apply_run(mp, h, mh, cuts);
-    p = mul2(mp, p);
+    p = join_runs(mp, p, cuts);
   }
   ex.p[warp][lane] = p;
   ex.h[warp][lane] = h;
@@ -438,6 +445,7 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
   uint32_t flag = total > 0 ? flag_of(reset, items.start(0), steps) : 0;
 
   float2 h = make_float2(0.f, 0.f), p = make_float2(1.f, 1.f);
+  uint32_t was_cut = 0;
   int item = 0;
   // One run: step(j, a, c x) for each of its steps, then the loads of a later one.
   auto gates_of = [&](float2 (&a)[kRun], float2 (&b)[kRun]) {
@@ -475,13 +483,15 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
 #pragma unroll
         for (int j = 0; j < kRun; ++j) {
           if (j < n) {
-            if ((cut >> j) & 1u) h = p = make_float2(0.f, 0.f);
+            if ((cut >> j) & 1u) h = make_float2(0.f, 0.f);
             h = fma2(a[j], h, b[j]);
             p = mul2(p, a[j]);
           }
         }
+        was_cut |= cut;
       }
     }
+    if (was_cut != 0) p = both(kCut);
   }
   float2 state = make_float2(0.f, 0.f);
   if (g.h0 != nullptr) state = two_floats(g.h0 + batch * g.dim + at.from, at.second);
@@ -592,7 +602,7 @@ __device__ __forceinline__ float2 tile_exchange(TileExchange &ex, int buf, float
       const int w = i;
       const float2 pw = ex.p[buf][w][lane];
       ch = apply_run(pw, ch, ex.h[buf][w][lane], cuts);
-      cp = mul2(cp, pw);
+      cp = join_runs(cp, pw, cuts);
     }
     *cooperative_groups::this_cluster().map_shared_rank(&ex.rank[buf][rank][lane], warp) = make_float4(cp.x, cp.y, ch.x, ch.y);
   }
@@ -638,11 +648,12 @@ __device__ __forceinline__ void scan_run(const float2 (&a)[RUN], const float2 (&
 #pragma unroll
     for (int j = 0; j < RUN; ++j) {
       if (j < n) {
-        if ((cut >> j) & 1u) h = p = zero;
+        if ((cut >> j) & 1u) h = zero;
         h = fma2(a[j], h, b[j]);
         p = mul2(p, a[j]);
       }
     }
+    if (cut != 0) p = both(kCut);
   }
 }
 // The run from the state before it: save(j, h_{j-1}) at every kRun-th step, store(j, h_j).
@@ -906,6 +917,7 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
   };
   const float2 zero = make_float2(0.f, 0.f);
   float2 r = zero, p = make_float2(1.f, 1.f);
+  uint32_t was_cut = 0;
   if (PASS != kApply) {
     for (; item < items.count; ++item) {
       const int t0 = items.start(item);
@@ -934,11 +946,13 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
           if (j < n) {
             r = mul2(a[j], add2(gt[j], r));
             p = mul2(p, a[j]);
-            if ((cut >> j) & 1u) r = p = zero;
+            if ((cut >> j) & 1u) r = zero;
           }
         }
+        was_cut |= cut;
       }
     }
+    if (was_cut != 0) p = both(kCut);
   }
   float2 back = zero;  // r of the step after the sequence
   if (g.grad_last != nullptr) back = two_floats(g.grad_last + batch * g.dim + at.from, at.second);

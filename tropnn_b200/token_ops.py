@@ -152,7 +152,9 @@ def gated_recurrence_b200(
     is the state before the first token (zeros by default), ``reset`` ``[batch, steps]`` marks the
     tokens that start a document: nothing of the state before them is kept. Returns ``(h, h_last)``:
     ``h`` in the inputs' dtype and the last state in f32, which continues a sequence as ``h0`` of
-    the next call or as the state of ``gated_recurrence_step_b200``. The state is f32 throughout.
+    the next call or as the state of ``gated_recurrence_step_b200``. The state is f32 throughout. One
+    that is not finite stays so until a reset, but an infinity may become a NaN on the way (0 times it,
+    where the gates of a stretch multiply to less than f32 holds).
     Differentiable in gate, value and h0 (once); the backward scans the states again from every
     eighth, saved in f32, instead of reading ``h``.
     """
