@@ -363,6 +363,22 @@ def test_offsets_past_32_bits() -> None:
     _close(last, want[1], torch.float32)
 
 
+def test_a_step_tells_autograd_that_it_changed_the_state() -> None:
+    gate, value, h0 = _inputs(3, 4, 16, torch.float32, 16)
+    _, state = tropnn_b200.gated_recurrence_b200(gate, value, h0)
+    weight = torch.ones(16, device="cuda", requires_grad=True)
+    loss = (weight * state).sum()  # keeps the state for the weight's gradient
+    with torch.no_grad():
+        tropnn_b200.gated_recurrence_step_b200(gate[:, 0], value[:, 0], state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        _, state = tropnn_b200.gated_recurrence_b200(gate, value, h0)
+        tropnn_b200.gated_recurrence_step_b200(gate[:, 0], value[:, 0], state)
+    with torch.no_grad():
+        tropnn_b200.gated_recurrence_step_b200(gate[:, 0], value[:, 0], state)  # of inference mode: as before
+
+
 def test_refusals() -> None:
     op, step = tropnn_b200.gated_recurrence_b200, tropnn_b200.gated_recurrence_step_b200
     t = torch.zeros(2, 3, 4, device="cuda")

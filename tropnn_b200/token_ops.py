@@ -202,6 +202,7 @@ def gated_recurrence_step_b200(gate: Tensor, value: Tensor, state: Tensor, *, re
         value.data_ptr(), value.stride(0), nat.float_code(gate.dtype), None if reset is None else reset.data_ptr(),
         batch, dim, state.data_ptr(), state_row, h.data_ptr(),
     )
+    torch.autograd.graph.increment_version(state)  # autograd is told, as of torch's in-place operations
     return h
 
 
