@@ -320,6 +320,26 @@ def test_no_rows() -> None:
     assert torch.autograd.grad(loss, logits)[0].shape == (0, 10)
 
 
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_is_refused(grad_mode) -> None:
+    """A tangent is not lost, which would be a derivative of 0."""
+    logits, teacher, at, _ = _inputs(2, 50, 3, torch.float32, 36)
+    scale = torch.ones(2, device="cuda")
+    make = torch.autograd.forward_ad.make_dual
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        tropnn_b200.distill_loss_b200(logits, teacher, at)
+        moved, moved_teacher = make(logits, torch.ones_like(logits)), make(teacher, torch.ones_like(teacher))
+        for call in (
+            lambda: tropnn_b200.distill_loss_b200(moved, teacher, at),
+            lambda: tropnn_b200.distill_loss_b200(logits, moved_teacher, at),
+            lambda: tropnn_b200.distill_loss_grad_b200(moved, teacher, at),
+            lambda: tropnn_b200.distill_loss_grad_b200(logits, moved_teacher, at),
+            lambda: tropnn_b200.distill_loss_grad_b200(logits, teacher, at, row_scale=make(scale, scale)),
+        ):
+            with pytest.raises(NotImplementedError):
+                call()
+
+
 def test_refusals() -> None:
     op = tropnn_b200.distill_loss_b200
     x, t = torch.zeros(2, 9, device="cuda"), torch.zeros(2, 3, device="cuda")

@@ -379,6 +379,22 @@ def test_a_step_tells_autograd_that_it_changed_the_state() -> None:
         tropnn_b200.gated_recurrence_step_b200(gate[:, 0], value[:, 0], state)  # of inference mode: as before
 
 
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_is_refused(grad_mode) -> None:
+    """A tangent is not lost, which would be a derivative of 0."""
+    gate, value, h0 = _inputs(2, 5, 16, torch.float32, 17)
+    for place in range(3):
+        with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+            args = [gate, value, h0]
+            tropnn_b200.gated_recurrence_b200(*args)
+            args[place] = torch.autograd.forward_ad.make_dual(args[place], torch.ones_like(args[place]))
+            with pytest.raises(NotImplementedError):
+                tropnn_b200.gated_recurrence_b200(*args)
+            row = [args[0][:, 0], args[1][:, 0], args[2]]
+            with pytest.raises(NotImplementedError):
+                tropnn_b200.gated_recurrence_step_b200(*row)
+
+
 def test_refusals() -> None:
     op, step = tropnn_b200.gated_recurrence_b200, tropnn_b200.gated_recurrence_step_b200
     t = torch.zeros(2, 3, 4, device="cuda")

@@ -19,6 +19,7 @@ from typing import Any
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
@@ -49,6 +50,15 @@ def _same_device(device: torch.device, t: Tensor, name: str) -> None:
     if t.device != device:
         _require_cuda(t, name)
         raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _no_tangent(name: str, *tensors: Any) -> None:
+    """Refuses forward-mode derivatives, which a call past autograd would give as 0."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual tensors about (unpacking takes 0.3 us each)
+        return
+    for t in tensors:
+        if isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _unit_last(t: Tensor) -> Tensor:
@@ -155,10 +165,11 @@ def gated_recurrence_b200(
     the next call or as the state of ``gated_recurrence_step_b200``. The state is f32 throughout. One
     that is not finite stays so until a reset, but an infinity may become a NaN on the way (0 times it,
     where the gates of a stretch multiply to less than f32 holds).
-    Differentiable in gate, value and h0 (once); the backward scans the states again from every
-    eighth, saved in f32, instead of reading ``h``.
+    Differentiable in gate, value and h0 (once, in reverse mode); the backward scans the states again
+    from every eighth, saved in f32, instead of reading ``h``.
     """
     _check_gate_value(gate, value, 3)
+    _no_tangent("gated_recurrence_b200", gate, value, h0)
     if h0 is not None:
         _same_device(gate.device, h0, "h0")
         if h0.shape != (gate.shape[0], gate.shape[2]):
@@ -180,6 +191,7 @@ def gated_recurrence_step_b200(gate: Tensor, value: Tensor, state: Tensor, *, re
     ``state`` f32 ``[batch, dim]``, updated in place; ``reset`` ``[batch]`` clears a row's state
     first. Returns the new state rounded to the inputs' dtype. Not differentiable."""
     _check_gate_value(gate, value, 2)
+    _no_tangent("gated_recurrence_step_b200", gate, value, state)
     shape = gate.shape
     dev = gate.device
     _same_device(dev, state, "state")
@@ -354,13 +366,14 @@ def distill_loss_b200(
     vocab)`` gives no label term; a row with neither has loss 0 and gradient 0 and does not count in
     the "mean" (which is 0 where no row counts). ``reduction`` is "mean", "sum" or "none" (a loss a
     row). Everything is computed in f32 and the loss is f32; logits of f32/f16/bf16, sliced rows and
-    steps in place. Differentiable (once) in the logits; the teacher gets no gradient. The backward
-    reads the logits again: ``distill_loss_grad_b200`` does both in one pass.
+    steps in place. Differentiable (once, in reverse mode) in the logits; the teacher gets no gradient.
+    The backward reads the logits again: ``distill_loss_grad_b200`` does both in one pass.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     teacher, indices, labels, settings = _distill_check(
         logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
+    _no_tangent("distill_loss_b200", logits, teacher_logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillLossFunction.apply(logits, teacher, indices, labels, settings, reduction)
     return _distill_loss(logits, teacher, indices, labels, settings, reduction)[0]
@@ -384,6 +397,7 @@ def distill_loss_grad_b200(
     loops that call the head's backward themselves, such as a head in chunks of rows."""
     teacher, indices, labels, settings = _distill_check(
         logits, teacher_logits, teacher_indices, labels, temperature, label_weight, ignore_index)
+    _no_tangent("distill_loss_grad_b200", logits, teacher_logits, row_scale)
     dev, lead = logits.device, logits.shape[:-1]
     scale: Tensor | None = None
     if isinstance(row_scale, Tensor):
