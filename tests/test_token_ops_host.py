@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import re
+
 import pytest
 import torch
 
@@ -70,3 +72,14 @@ def test_c_entries_refuse_before_any_device_work(lib) -> None:
         assert status() == kind
         assert text in nat.last_error()
     assert recurrence(batch=0) == distill(rows=0) == sample(rows=0) == nat.OK
+
+
+def test_no_kernel_ignores_that_a_wait_ran_out() -> None:
+    """Each bounded wait for a copy says whether it arrived; a kernel that went on would leave copies on their
+    way into shared memory that is not its own any more."""
+    ignored = re.compile(r"^\s*(if( constexpr)? \([^()]*\)\s*)?(sm100::)?mbar_wait(_sleep)?\(")
+    sources = sorted(b200_build.CSRC_DIR.glob("*.cu"))
+    assert sources
+    for path in sources:
+        for number, line in enumerate(path.read_text().splitlines(), 1):
+            assert not ignored.match(line), f"{path.name}:{number}"

@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kBlock, RESIDENT ? 3 : 4) distill_row_kernel(c
   if (warp < kWarps) {
     for (int from = whole0, c = 0; from < whole1; from += per_chunk, ++c) {
       const int to = min(from + per_chunk, whole1);
-      if (RESIDENT) sm100::mbar_wait(&full[c], 0, &abort, &g_distill_error);
+      if (RESIDENT && !sm100::mbar_wait(&full[c], 0, &abort, &g_distill_error)) break;
       int v = from + tid;
       // Full batches without checks where a slice is in shared memory: 2048 x 131072 bf16 at T = 2 243 ->
       // 235 us. From global memory two loops cost registers: the loss of 4096 x 32000 56.5 -> 59 us.
@@ -651,6 +651,9 @@ __global__ void __launch_bounds__(kBlock, RESIDENT ? 3 : 4) distill_row_kernel(c
     g.losses[row] = loss;
     if (MODE == kLoss && g.stats != nullptr)
       g.stats[row] = make_float4(st.m, inv_t, inv_1, static_cast<float>((has_teacher ? 1 : 0) + (has_label ? 2 : 0)));
+  }
+  if (RESIDENT && tid == kThreads && abort != 0) {  // a wait ran out: the copies are seen out first
+    for (int from = whole0, c = 0; from < whole1; from += per_chunk, ++c) sm100::mbar_drain(&full[c], 0);
   }
 }
 

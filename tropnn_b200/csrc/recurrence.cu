@@ -325,7 +325,7 @@ struct Stream {
   const CUtensorMap *maps[TENSORS];
   int ch0, batch, s = 0;
   uint32_t parity = 0;
-  bool stored = false;
+  bool stored = false, alive = true;
   // plain
   const T *from[TENSORS];
   int64_t stride[TENSORS];
@@ -336,7 +336,7 @@ struct Stream {
   // Starts the loads of the tensors in `which` (a bit each) of the run at t0, `ahead` stages on.
   __device__ __forceinline__ void fetch(int t0, uint32_t which, int ahead) {
     if constexpr (TMA) {
-      if ((threadIdx.x & 31) == 0) {
+      if ((threadIdx.x & 31) == 0 && alive) {
         int at = s + ahead;
         if (at >= kDeep) at -= kDeep;
         sm100::mbar_expect_tx(&full[at], __popc(which) * kRun * kChan * sizeof(T));
@@ -362,8 +362,22 @@ struct Stream {
       }
     }
   }
-  __device__ __forceinline__ void wait() {
-    if constexpr (TMA) sm100::mbar_wait(&full[s], parity, abort, &g_recurrence_error);
+  // The stage of the run with `left` runs (it included) to come has arrived. Where a wait runs out, a lane
+  // waits no more, and lane 0, which issues the copies, sees those on their way out and starts no others;
+  // the warp goes on with what lies in its ring, so that it meets the block at every barrier.
+  __device__ __forceinline__ void wait(int left) {
+    if constexpr (TMA) {
+      if (!alive || sm100::mbar_wait(&full[s], parity, abort, &g_recurrence_error)) return;
+      alive = false;
+      if ((threadIdx.x & 31) != 0) return;
+      for (int n = min(kDeep - (stored ? 1 : 0), left), at = s, p = parity; n > 0; --n) {
+        sm100::mbar_drain(&full[at], p);
+        if (++at == kDeep) {
+          at = 0;
+          p ^= 1;
+        }
+      }
+    }
   }
   __device__ __forceinline__ float2 get(int tensor, int j) {
     if constexpr (TMA) return stage_pair<T>(rows(tensor) + j * kChan, threadIdx.x & 31);
@@ -449,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
   int item = 0;
   // One run: step(j, a, c x) for each of its steps, then the loads of a later one.
   auto gates_of = [&](float2 (&a)[kRun], float2 (&b)[kRun]) {
-    in.wait();
+    in.wait(total - item);
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
       float2 c;
@@ -536,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
       sm100::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        tma_store_3d(&maps.out_value, in.rows(1), in.ch0, t0, in.batch);
+        if (in.alive) tma_store_3d(&maps.out_value, in.rows(1), in.ch0, t0, in.batch);
         sm100::bulk_commit();
         bulk_wait_read<1>();  // the stage before this one has been read by its store
       }
@@ -811,12 +825,25 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   int buf = 0, s = 0;
   uint32_t parity = 0;
+  bool alive = true;
   for (int64_t tile = first, t0 = t_first; tile < stop; tile += stride, t0 += stride, buf ^= 1) {
     const int n = static_cast<int>(t0 >= stop ? 0 : min64(kLong, stop - t0));
     const uint32_t cut = __ballot_sync(0xffffffffu, flag != 0);
     flag = flag_of(t0 + stride);
     const bool plain = n == kLong && cut == 0;
-    if (n > 0) sm100::mbar_wait(&full[warp][s], parity, &abort, &g_recurrence_error);
+    if (n > 0 && alive) {
+      // A wait that runs out, as in Stream::wait.
+      alive = sm100::mbar_wait(&full[warp][s], parity, &abort, &g_recurrence_error);
+      if (!alive && lane == 0) {
+        for (int i = 0, at = s, p = parity; i < kStages - (tile > first ? 1 : 0) && t0 + i * stride < stop; ++i) {
+          sm100::mbar_drain(&full[warp][at], p);
+          if (++at == kStages) {
+            at = 0;
+            p ^= 1;
+          }
+        }
+      }
+    }
     T *rows = stage(s);
     float2 a[kLong], b[kLong], p, h;
 #pragma unroll
@@ -835,11 +862,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     sm100::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      if (n > 0) tma_store_3d(&maps.out_value, rows + kLong * kChan, ch0, static_cast<int>(t0), batch);
+      if (n > 0 && alive) tma_store_3d(&maps.out_value, rows + kLong * kChan, ch0, static_cast<int>(t0), batch);
       sm100::bulk_commit();
       // The stage before this one has been read by its store: its next tile comes in.
       bulk_wait_read<1>();
-      if (tile > first) fetch(t0 + (kStages - 1) * stride, s == 0 ? kStages - 1 : s - 1);
+      if (tile > first && alive) fetch(t0 + (kStages - 1) * stride, s == 0 ? kStages - 1 : s - 1);
     }
     if (++s == kStages) {
       s = 0;
@@ -923,7 +950,7 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
       const int t0 = items.start(item);
       const int n = min(kRun, steps - t0);
       const uint32_t cut = flags();
-      in.wait();
+      in.wait(total - item);
       float2 a[kRun], gt[kRun];
 #pragma unroll
       for (int j = 0; j < kRun; ++j) {
@@ -973,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
     const uint32_t cut = flags();
     float2 h = before;
     before = before_of(item + 1);
-    in.wait();
+    in.wait(total - item);
     float2 a[kRun], c[kRun], u[kRun], gt[kRun];
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
@@ -1035,8 +1062,10 @@ __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
       sm100::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        tma_store_3d(&maps.out_gate, in.rows(0), in.ch0, t0, in.batch);
-        tma_store_3d(&maps.out_value, in.rows(1), in.ch0, t0, in.batch);
+        if (in.alive) {
+          tma_store_3d(&maps.out_gate, in.rows(0), in.ch0, t0, in.batch);
+          tma_store_3d(&maps.out_value, in.rows(1), in.ch0, t0, in.batch);
+        }
         sm100::bulk_commit();
         bulk_wait_read<1>();  // the stage before this one has been read by its stores
       }

@@ -57,7 +57,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
 
 // Bounded wait for phase `parity` of `bar`. Returns false (raising *abort and
 // *error_word) after kWaitLimitNs, or false at once once another role has aborted.
-__device__ inline bool mbar_wait(uint64_t *bar, uint32_t parity, int *abort, int *error_word) {
+[[nodiscard]] __device__ inline bool mbar_wait(uint64_t *bar, uint32_t parity, int *abort, int *error_word) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t start = global_ns();
   volatile int *ab = abort;
@@ -77,7 +77,7 @@ __device__ inline bool mbar_wait(uint64_t *bar, uint32_t parity, int *abort, int
 // Bounded wait as mbar_wait, polling with the mbarrier suspend-time hint `hint_ns`: the thread
 // sleeps between polls until the phase completes (or the hint expires), so that whole warps
 // can wait without taking issue slots from the TMA and MMA threads.
-__device__ inline bool mbar_wait_sleep(uint64_t *bar, uint32_t parity, int *abort, int *error_word, uint32_t hint_ns) {
+[[nodiscard]] __device__ inline bool mbar_wait_sleep(uint64_t *bar, uint32_t parity, int *abort, int *error_word, uint32_t hint_ns) {
   const uint64_t start = global_ns();
   volatile int *ab = abort;
   for (;;) {
