@@ -125,6 +125,25 @@ def test_loss_and_gradient(shape, dtype, T, w) -> None:
     _close_grad(g, grad, mass, scale.double()[:, None], dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize(("T", "w"), [(0.5, 0.0), (0.5, 0.3), (0.25, 0.5), (2.0, 0.3)])
+def test_teacher_entries_of_the_lowest_value(dtype, T, w) -> None:
+    """A logit of the type's lowest value is a value, below T = 1 too: alone it is a uniform teacher,
+    beside others it weighs nothing."""
+    for top in (6, 300):
+        logits, teacher, at, labels = _inputs(3, 777, top, torch.float32, 34, ragged=False, teacher_dtype=dtype)
+        teacher[0] = torch.finfo(dtype).min
+        teacher[1, 2:] = torch.finfo(dtype).min
+        losses, grad, mass, _ = _reference(logits, teacher, at, labels, T, w)
+        got, got_grad = tropnn_b200.distill_loss_grad_b200(logits, teacher, at, labels, temperature=T, label_weight=w)
+        _close_loss(got, losses, T)
+        _close_grad(got_grad, grad, mass, torch.ones(3, 1, dtype=torch.float64), torch.float32)
+        leaf = logits.detach().requires_grad_()
+        loss = tropnn_b200.distill_loss_b200(leaf, teacher, at, labels, temperature=T, label_weight=w, reduction="none")
+        _close_loss(loss, losses, T)
+        _close_grad(torch.autograd.grad(loss.sum(), leaf)[0], grad, mass, torch.ones(3, 1, dtype=torch.float64), torch.float32)
+
+
 def test_gradient_against_differences() -> None:
     """Along a random direction; f32 losses of about 3 are good to 1e-6, over a step of 1e-2: 1e-4."""
     logits, teacher, at, labels = _inputs(6, 500, 16, torch.float32, 21)

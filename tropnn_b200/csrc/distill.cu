@@ -267,13 +267,13 @@ __device__ __forceinline__ RowStats joined(RowStats a, float k_t) {
 // that the row's sums take anyway, each thread has the parts at hand.
 constexpr int kEntriesPerWarp = kMaxTop / kWarps, kEntriesPerLane = kEntriesPerWarp / 32;
 struct TeacherPart {
-  float t_max, total;         // sum of e = exp(t - t_max), t = teacher logit / T
-  float entropy, cross, from; // sums of e (t - t_max) and of e (s - from) / T
+  float t_max, total;         // sum of e = exp((t - t_max) / T)
+  float entropy, cross, from; // sums of e (t - t_max) / T and of e (s - from) / T
   int count;                  // of its entries in the CTA's part of the row
 };
 struct EntryTable {
   alignas(16) int at[kMaxTop];   // -1: none
-  alignas(16) float q[kMaxTop];  // t, later its share exp(t - t_max) / total
+  alignas(16) float q[kMaxTop];  // t, later its share exp((t - t_max) / T) / total
   uint16_t mine[kMaxTop];        // numbers of the entries in the CTA's part, a stretch a warp
   TeacherPart part[kWarps];
   int label;  // -1: none
@@ -311,7 +311,6 @@ __device__ __forceinline__ void load_targets(const DistillArgs &g, int64_t row, 
     s[i] = -INFINITY;
     if (at[i] < 0 || at[i] >= g.vocab || t[i] == -INFINITY) at[i] = -1;
     if (at[i] >= 0) {
-      t[i] *= g.inv_temperature;
       p.t_max = fmaxf(p.t_max, t[i]);
       if (for_loss) s[i] = to_f32<T>(x[at[i]]);
     }
@@ -338,7 +337,7 @@ __device__ __forceinline__ void load_targets(const DistillArgs &g, int64_t row, 
 #pragma unroll
   for (int i = 0; i < kEntriesPerLane; ++i) {
     if (at[i] >= 0) {
-      const float d = t[i] - p.t_max, e = expf(d);
+      const float d = (t[i] - p.t_max) * g.inv_temperature, e = expf(d);
       p.total += e;
       if (e != 0.f) {
         p.entropy += e * d;
@@ -366,7 +365,7 @@ struct Teacher {
     t_max = kLowest;
     total = 0.f;
     for (int w = 0; w < parts; ++w) t_max = fmaxf(t_max, table.part[w].t_max);
-    for (int w = 0; w < parts; ++w) total += table.part[w].total * expf(table.part[w].t_max - t_max);
+    for (int w = 0; w < parts; ++w) total += table.part[w].total * expf((table.part[w].t_max - t_max) * g.inv_temperature);
     if (total == 0.f) parts = 0;  // NaN stays
   }
 };
@@ -375,9 +374,9 @@ __device__ __forceinline__ float teacher_loss(const DistillArgs &g, const EntryT
   float entropy = 0.f, cross = 0.f;
   for (int w = 0; w < teacher.parts; ++w) {
     const TeacherPart &p = table.part[w];
-    const float f = expf(p.t_max - teacher.t_max);
-    if (p.total == 0.f) continue;
-    entropy += f * (p.entropy + p.total * (p.t_max - teacher.t_max));
+    const float d = (p.t_max - teacher.t_max) * g.inv_temperature, f = expf(d);
+    if (p.total == 0.f || f == 0.f) continue;  // no part of the sum, however far off d or the logits are
+    entropy += f * (p.entropy + p.total * d);
     cross += f * (p.cross + p.total * ((p.from - m) * g.inv_temperature));
   }
   return (entropy - cross) / teacher.total - logf(teacher.total) + logf(s_t);
@@ -387,7 +386,7 @@ __device__ __forceinline__ void form_shares(const DistillArgs &g, const Teacher 
   if (teacher.parts == 0) return;
   const float inv_total = 1.f / teacher.total;
   for (int k = threadIdx.x; k < (g.top + 31 & ~31); k += kBlock)
-    table.q[k] = table.at[k] >= 0 ? expf(table.q[k] - teacher.t_max) * inv_total : 0.f;
+    table.q[k] = table.at[k] >= 0 ? expf((table.q[k] - teacher.t_max) * g.inv_temperature) * inv_total : 0.f;
 }
 
 struct GradScale {
