@@ -125,6 +125,85 @@ def test_loss_and_gradient(shape, dtype, T, w) -> None:
     _close_grad(g, grad, mass, scale.double()[:, None], dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize(("T", "w"), [(1.5, 0.3), (0.7, 0.5), (4.0, 0.25)])
+def test_labels_at_a_temperature_of_its_own(shape, dtype, T, w) -> None:
+    """Two sums an element whose exponentials have nothing to do with one another."""
+    test_loss_and_gradient(shape, dtype, T, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_exponentials_of_the_labels(dtype) -> None:
+    """A row with a label alone has the gradient w p1, here relative to its largest entry w / sum: a
+    power of two to 2^-22 of it, its argument d log2(e) to 1.5 * 2^-24 of that (the product and the
+    constant), and two roundings of 2^-24, in the type that it is stored in."""
+    vocab = 4096
+    logits = torch.linspace(-75.0, 0.0, vocab, dtype=torch.float64).to(dtype)
+    logits = torch.stack([logits, logits.flip(0), logits.roll(1), logits.roll(3)]).cuda()  # each place in a vector
+    label = 5
+    at = torch.full((4, 1), -1, dtype=torch.int64, device="cuda")
+    _, grad = tropnn_b200.distill_loss_grad_b200(
+        logits, torch.zeros(4, 1, device="cuda"), at, torch.full((4,), label, device="cuda"), temperature=1.5, label_weight=0.5)
+    x, g = logits.double().cpu(), grad.double().cpu()
+    want = x.exp()
+    rest = torch.arange(vocab) != label
+    ratio = g / g.amax(dim=1, keepdim=True)
+    bound = 2.0**-22 + 1.5 * 2.0**-24 * x.abs() + 3 * 2.0**-24 + 2 * (UNIT[dtype] if dtype != torch.float32 else 0.0)
+    assert bool(((ratio / want - 1).abs() <= bound)[:, rest].all()), float(((ratio / want - 1).abs() - bound)[:, rest].max())
+
+
+@pytest.mark.parametrize("top", [129, 500, 1024])
+@pytest.mark.parametrize(("T", "w"), [(1.0, 0.0), (2.0, 0.3), (1.5, 0.4)])
+def test_long_teacher_lists(top, T, w) -> None:
+    """More than 128 entries are read by several warps: entries of one index in the shares of two, the
+    label among them, shares without an entry."""
+    logits, teacher, at, labels = _inputs(6, 5003, top, torch.float32, 31 + top, ragged=False)
+    at[:, top - 1] = at[:, 0]
+    at[:, 128] = at[:, 127]
+    labels[:3] = at[:3, 0]
+    labels[3] = at[3, top - 1]
+    labels[4] = -100
+    at[4, :128] = -1  # the first share has none
+    at[5, 1:] = -1
+    teacher[2, 64:] -= 200.0  # shares that weigh nothing
+    losses, grad, mass, _ = _reference(logits, teacher, at, labels, T, w)
+    got, got_grad = tropnn_b200.distill_loss_grad_b200(logits, teacher, at, labels, temperature=T, label_weight=w)
+    _close_loss(got, losses, T)
+    _close_grad(got_grad, grad, mass, torch.ones(6, 1, dtype=torch.float64), torch.float32)
+    leaf = logits.detach().requires_grad_()
+    loss = tropnn_b200.distill_loss_b200(leaf, teacher, at, labels, temperature=T, label_weight=w, reduction="none")
+    _close_loss(loss, losses, T)
+    (got_grad,) = torch.autograd.grad(loss.sum(), leaf)
+    _close_grad(got_grad, grad, mass, torch.ones(6, 1, dtype=torch.float64), torch.float32)
+
+
+@pytest.mark.parametrize(("dtype", "vocab"), [(torch.float32, 450_001), (torch.bfloat16, 900_001), (torch.float16, 850_006)])
+@pytest.mark.parametrize(("T", "w"), [(1.0, 0.0), (2.0, 0.3), (1.5, 0.4)])
+def test_rows_that_shared_memory_does_not_hold(dtype, vocab, T, w) -> None:
+    logits, teacher, at, labels = _inputs(2, vocab, 40, dtype, 32, ragged=False)
+    losses, grad, mass, _ = _reference(logits, teacher, at, labels, T, w)
+    got, got_grad = tropnn_b200.distill_loss_grad_b200(logits, teacher, at, labels, temperature=T, label_weight=w)
+    _close_loss(got, losses, T)
+    _close_grad(got_grad, grad, mass, torch.ones(2, 1, dtype=torch.float64), dtype)
+
+
+@pytest.mark.parametrize(("rows", "vocab", "dtype"), [(900, 3001, torch.float16), (115, 131072, torch.bfloat16), (460, 16001, torch.float32)])
+def test_more_rows_than_the_gpu_holds(rows, vocab, dtype) -> None:
+    """And a few of the rows by themselves: the sums' order may differ with the rows' number, so as close
+    to the formulas, not bit for bit."""
+    logits, teacher, at, labels = _inputs(rows, vocab, 16, dtype, 33)
+    args = dict(temperature=1.5, label_weight=0.25)
+    losses, grad, mass, _ = _reference(logits, teacher, at, labels, 1.5, 0.25)
+    got, got_grad = tropnn_b200.distill_loss_grad_b200(logits, teacher, at, labels, **args)
+    _close_loss(got, losses, 1.5)
+    _close_grad(got_grad, grad, mass, torch.ones(rows, 1, dtype=torch.float64), dtype)
+    some = slice(rows - 4, rows - 1)
+    got, got_grad = tropnn_b200.distill_loss_grad_b200(logits[some], teacher[some], at[some], labels[some], **args)
+    _close_loss(got, losses[some], 1.5)
+    _close_grad(got_grad, grad[some], mass[some], torch.ones(3, 1, dtype=torch.float64), dtype)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize(("T", "w"), [(0.5, 0.0), (0.5, 0.3), (0.25, 0.5), (2.0, 0.3)])
 def test_teacher_entries_of_the_lowest_value(dtype, T, w) -> None:
