@@ -102,6 +102,52 @@ def test_a_large_vocabulary() -> None:
         assert torch.equal(tropnn_b200.sample_tokens_b200(logits, u, **settings).cpu(), _reference(logits, u, **settings))
 
 
+def _compare_some(logits, u, settings, some) -> None:
+    """Some rows of a batch against the definition, and against each of them alone."""
+    got = tropnn_b200.sample_tokens_b200(logits, u, **settings)
+    pick = lambda v: v[some] if isinstance(v, torch.Tensor) else v  # noqa: E731
+    want = _reference(logits[some], u[some], **{name: pick(v) for name, v in settings.items()})
+    assert torch.equal(got[some].cpu(), want), settings
+    for n in some[:2]:
+        one = {name: v[n : n + 1] if isinstance(v, torch.Tensor) else v for name, v in settings.items()}
+        alone = tropnn_b200.sample_tokens_b200(logits[n : n + 1], u[n : n + 1], **one)
+        assert int(alone) == int(got[n]), settings
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [9001, 70001])
+def test_more_rows_than_the_gpu_holds(vocab, dtype) -> None:
+    """Rows that are streamed, a CTA each (of more than 2^16 tokens, or fewer), at odd offsets."""
+    rows = 330
+    whole, u = _inputs(rows, vocab + 2, dtype, vocab, spread=1.5)
+    logits = whole[:, 1 : vocab + 1]
+    logits[7] = logits[7].round()  # many tokens of one logit
+    logits[8, 100:] = -math.inf
+    logits[9] = -math.inf
+    logits[10, vocab - 1] = float("nan")
+    some = [3, 328, 7, 8, 9, 10, 200]
+    for settings in ({"top_p": 0.9}, {"top_p": 0.9999, "temperature": 3.0}, {"top_k": 50}, {"top_k": 3000, "top_p": 0.9, "min_p": 0.001},
+                     {"top_k": 1}, {}, {"min_p": 0.05}, {"temperature": 0.0}):
+        _compare_some(logits, u, settings, some)
+    gen = torch.Generator().manual_seed(12)
+    pick = lambda values, t: torch.tensor(values)[torch.randint(0, len(values), (rows,), generator=gen)].to(t).cuda()  # noqa: E731
+    for _ in range(3):
+        settings = {
+            "temperature": pick([0.0, 0.6, 1.0, 1.5], torch.float32),
+            "top_k": pick([0, 1, 20, 1000], torch.int32),
+            "top_p": pick([1.0, 0.8, 0.99], torch.float32),
+            "min_p": pick([0.0, 0.01, 0.2], torch.float32),
+        }
+        _compare_some(logits, u, settings, some)
+
+
+@pytest.mark.parametrize(("dtype", "vocab"), [(torch.float32, 2_300_001), (torch.bfloat16, 4_600_003), (torch.float16, 4_600_003)])
+def test_rows_of_more_batches_than_maxima_are_kept_for(dtype, vocab) -> None:
+    logits, u = _inputs(1, vocab, dtype, 20)
+    for settings in ({}, {"top_k": 50}, {"top_p": 0.9}, {"top_k": 5000, "top_p": 0.7}, {"min_p": 0.1}, {"temperature": 0.0}):
+        assert torch.equal(tropnn_b200.sample_tokens_b200(logits, u, **settings).cpu(), _reference(logits, u, **settings))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_settings_of_each_row(dtype) -> None:
     rows, vocab = 64, 5003
