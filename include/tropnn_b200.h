@@ -660,9 +660,9 @@ TROPNN_B200_API int tropnn_b200_recurrence_step(const void *gate, int64_t gate_s
  *   q = softmax(teacher / T) over the row's entries with an index in [0, vocab) and a logit above
  *   -inf, p = softmax(logits / T), p1 = softmax(logits)
  *   loss = (1 - w) T^2 sum_k q_k (log q_k - log p[index_k]) + w (-log p1[label])
- * w = label_weight. A label that is ignore_index or outside [0, vocab) gives no label term, a row
- * without entries no teacher term; a row with neither ("without a target") has loss 0 and gradient
- * 0. Entries of one index add up. logits: row n of `vocab` elements at
+ * w = label_weight, T in [2^-60, 2^60] (any positive T where w is 1). A label that is ignore_index or
+ * outside [0, vocab) gives no label term, a row without entries no teacher term; a row with neither
+ * ("without a target") has loss 0 and gradient 0. Entries of one index add up. logits: row n of `vocab` elements at
  * (n / inner) * outer_stride + (n % inner) * inner_stride; teacher [rows, top] and indices
  * [rows, top] (I32/I64) contiguous, top <= 1024; labels int64 [rows] or NULL. losses f32 [rows];
  * stats f32 [rows, 4], 16-byte aligned (NULL: not kept), for distill_reduce and distill_grad.

@@ -418,6 +418,15 @@ def test_no_rows() -> None:
     assert torch.autograd.grad(loss, logits)[0].shape == (0, 10)
 
 
+def test_temperatures_that_f32_cannot_square_are_refused() -> None:
+    logits, teacher, at, labels = _inputs(2, 50, 3, torch.float32, 35)
+    for T in (1e-40, 1e-25, 1e25, 3e38):
+        for op in (tropnn_b200.distill_loss_b200, tropnn_b200.distill_loss_grad_b200):
+            with pytest.raises(ValueError, match="temperature"):
+                op(logits, teacher, at, labels, temperature=T, label_weight=0.5)
+            op(logits, teacher, at, labels, temperature=T, label_weight=1.0)  # the labels have none
+
+
 @pytest.mark.parametrize("grad_mode", [True, False])
 def test_forward_mode_is_refused(grad_mode) -> None:
     """A tangent is not lost, which would be a derivative of 0."""

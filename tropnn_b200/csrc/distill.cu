@@ -786,6 +786,9 @@ int run_rows(const char *what, DistillArgs g, int dtype, int64_t rows, int64_t v
              kMaxTop, g.top);
   TB_REQUIRE(temperature > 0.f && temperature < INFINITY, TROPNN_B200_ERR_INVALID,
              "%s: temperature must be positive and finite", what);
+  // f32 holds 1 / T and (1 - w) T^2 with room for what they multiply.
+  TB_REQUIRE(label_weight == 1.f || (temperature >= 0x1p-60f && temperature <= 0x1p60f), TROPNN_B200_ERR_INVALID,
+             "%s: temperature must be in [2^-60, 2^60] for a teacher", what);
   TB_REQUIRE(label_weight >= 0.f && label_weight <= 1.f, TROPNN_B200_ERR_INVALID, "%s: label_weight must be in [0, 1]", what);
   TB_REQUIRE(label_weight == 0.f || g.labels != nullptr, TROPNN_B200_ERR_INVALID, "%s: label_weight without labels", what);
   if (rows == 0) return clear_error();

@@ -280,6 +280,8 @@ def _distill_check(
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     if not (0.0 <= label_weight <= 1.0):
         raise ValueError(f"label_weight must be in [0, 1], got {label_weight}")
+    if label_weight < 1.0 and not (2.0**-60 <= temperature <= 2.0**60):
+        raise ValueError(f"temperature must be in [2**-60, 2**60] for a teacher, got {temperature}")
     if label_weight > 0.0 and labels is None:
         raise ValueError("label_weight > 0 needs labels")
     if teacher.requires_grad or not teacher.is_contiguous():
@@ -365,8 +367,9 @@ def distill_loss_b200(
     A row without entries has no teacher term; a label that is ``ignore_index`` or outside ``[0,
     vocab)`` gives no label term; a row with neither has loss 0 and gradient 0 and does not count in
     the "mean" (which is 0 where no row counts). ``reduction`` is "mean", "sum" or "none" (a loss a
-    row). Everything is computed in f32 and the loss is f32; logits of f32/f16/bf16, sliced rows and
-    steps in place. Differentiable (once, in reverse mode) in the logits; the teacher gets no gradient.
+    row). ``temperature`` is in ``[2**-60, 2**60]``, whose squares f32 holds (any positive number where
+    ``label_weight`` is 1). Everything is computed in f32 and the loss is f32; logits of f32/f16/bf16,
+    sliced rows and steps in place. Differentiable (once, in reverse mode) in the logits; the teacher gets no gradient.
     The backward reads the logits again: ``distill_loss_grad_b200`` does both in one pass.
     """
     if reduction not in _REDUCTIONS:
