@@ -83,3 +83,15 @@ def test_no_kernel_ignores_that_a_wait_ran_out() -> None:
     for path in sources:
         for number, line in enumerate(path.read_text().splitlines(), 1):
             assert not ignored.match(line), f"{path.name}:{number}"
+
+
+def test_sizes_whose_product_overflows_are_refused(lib) -> None:
+    for batch, dim in ((1 << 61, 64), (1 << 40, 1 << 40), (1, 1 << 62)):
+        status = lib.tropnn_b200_recurrence_step(16, dim, 16, dim, nat.F32, None, batch, dim, 16, dim, 16, None)
+        assert status != 0 and "too large" in nat.last_error()
+        status = lib.tropnn_b200_recurrence_forward(16, dim, dim, 16, dim, dim, nat.F32, None, None, batch, 1, dim, 16, 16,
+                                                    None, 0, None, 0, None)
+        assert status != 0 and "too large" in nat.last_error()
+    for batch, dim in ((1 << 62, 256), (1 << 61, 64), (1, (1 << 63) - 1)):
+        assert lib.tropnn_b200_recurrence_workspace_size(batch, 100, dim, nat.F32) == 0
+        assert lib.tropnn_b200_recurrence_saved_size(batch, 100, dim) == 0

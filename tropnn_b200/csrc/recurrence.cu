@@ -1124,11 +1124,16 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(const T *__restric
 inline size_t elem_bytes(int dtype) { return dtype == TROPNN_B200_F32 ? 4 : 2; }
 inline bool paired(const void *p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (2 * elem_bytes(dtype)) == 0; }
 
+// Blocks of channels of all rows, by 8 chunks each, below 2^31: tested so that nothing overflows.
+bool fits_grid(int64_t batch, int64_t dim) {
+  const int64_t most = 0x7fffffffLL / kMaxCluster;
+  return dim <= most * kChan && (batch == 0 || ceil_div(dim, kChan) <= most / batch);
+}
 int check_sizes(const char *what, int dtype, int64_t batch, int64_t steps, int64_t dim) {
   TB_REQUIRE(is_float_dtype(dtype), TROPNN_B200_ERR_DTYPE, "%s: dtype %d is not f32/f16/bf16", what, dtype);
   TB_REQUIRE(batch >= 0 && steps >= 0 && dim >= 0, TROPNN_B200_ERR_INVALID, "%s: bad sizes (batch %lld, steps %lld, dim %lld)",
              what, (long long)batch, (long long)steps, (long long)dim);
-  TB_REQUIRE(batch * ceil_div(dim, kChan) * kMaxCluster <= 0x7fffffffLL, TROPNN_B200_ERR_INVALID, "%s: batch x dim too large", what);
+  TB_REQUIRE(fits_grid(batch, dim), TROPNN_B200_ERR_INVALID, "%s: batch x dim too large", what);
   TB_REQUIRE(steps <= 0x7fffffffLL - kRun, TROPNN_B200_ERR_INVALID, "%s: %lld steps are too many", what, (long long)steps);
   return TROPNN_B200_OK;
 }
@@ -1290,12 +1295,12 @@ using namespace tropnn_b200;
 extern "C" {
 
 size_t tropnn_b200_recurrence_saved_size(int64_t batch, int64_t steps, int64_t dim) {
-  if (batch <= 0 || steps <= 0 || dim <= 0) return 0;
+  if (batch <= 0 || steps <= 0 || dim <= 0 || !fits_grid(batch, dim)) return 0;
   return static_cast<size_t>(batch * ceil_div(steps, kRun) * dim) * sizeof(float);
 }
 
 size_t tropnn_b200_recurrence_workspace_size(int64_t batch, int64_t steps, int64_t dim, int dtype) {
-  if (batch <= 0 || steps <= 0 || dim <= 0 || !is_float_dtype(dtype)) return 0;
+  if (batch <= 0 || steps <= 0 || dim <= 0 || !is_float_dtype(dtype) || !fits_grid(batch, dim)) return 0;
   const int64_t units = units_of(batch, dim), runs = ceil_div(steps, kRun);
   return std::max(maps_bytes(plan_for(units, runs, slots_of(true, dtype)), batch, dim),
                   maps_bytes(plan_for(units, runs, slots_of(false, dtype)), batch, dim));
