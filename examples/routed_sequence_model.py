@@ -73,12 +73,13 @@ class RoutedSequenceModel(nn.Module):
 
     @torch.no_grad()
     def generate(self, prompt: Tensor, uniforms: Tensor, **sampling: float) -> Tensor:
-        """``uniforms.shape[1]`` tokens after ``prompt``: a prefill, then a step and a draw a token."""
+        """``uniforms.shape[1]`` tokens after ``prompt``: a prefill, then a step and a draw a token. A row
+        whose logits are no distribution draws -1."""
         logits, states = self(prompt)
         logits, tokens = logits[:, -1], []
         for t in range(uniforms.shape[1]):
             tokens.append(sample_tokens_b200(logits, uniforms[:, t], **sampling))
-            x = self.embed(tokens[-1])
+            x = self.embed(tokens[-1].clamp(min=0))
             for block, state in zip(self.blocks, states):
                 x = block.step(x, state)
             logits = self.head(self.norm(x))[:, 0]

@@ -49,3 +49,11 @@ def test_steps_follow_the_whole_sequence(example) -> None:
                 x = block.step(x, state)
             logits = model.head(model.norm(x))[:, 0]
             assert float((logits - whole[:, t]).abs().max()) <= 1e-3 * float(whole[:, t].abs().max())
+
+
+def test_a_row_without_a_distribution_goes_on(example, monkeypatch) -> None:
+    """The sampler's -1 is no row of the embedding."""
+    model = example.RoutedSequenceModel(60, dim=64, depth=1).cuda().eval()
+    monkeypatch.setattr(example, "sample_tokens_b200", lambda logits, u, **_: torch.full_like(u, -1, dtype=torch.int64))
+    tokens = model.generate(torch.zeros(2, 3, dtype=torch.int64, device="cuda"), torch.rand(2, 4, device="cuda"))
+    assert bool((tokens == -1).all())
