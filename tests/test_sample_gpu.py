@@ -238,6 +238,16 @@ def test_masked_rows(dtype) -> None:
         assert int(got[3]) in (300, 700) and int(got[5]) == 123
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_temperatures_whose_inverse_is_subnormal(dtype) -> None:
+    lowest = torch.finfo(dtype).min
+    logits = torch.tensor([0.0, lowest, lowest / 2, lowest / 4, -1.0, -math.inf, lowest / 3], dtype=dtype).cuda().expand(64, 7)
+    u = ((torch.arange(64) + 0.5) / 64).cuda()
+    for settings in ({"temperature": 1e38}, {"temperature": 3.3e38}, {"temperature": 3e38, "top_p": 0.8}, {"temperature": 2e38, "top_k": 4}):
+        got = tropnn_b200.sample_tokens_b200(logits, u, **settings)
+        assert torch.equal(got.cpu(), _reference(logits, u, **settings)), settings
+
+
 def test_uniforms_at_the_ends() -> None:
     logits = torch.randn(5, 300, generator=torch.Generator().manual_seed(11)).cuda()
     u = torch.tensor([0.0, 1.0, 1.0 - 2.0**-24, -0.5, 2.0], device="cuda")

@@ -28,8 +28,6 @@
 // 24 us (5.5 TB/s); min-p .05 512 rows 40 us, .5 2048 rows 100 us (5.4 TB/s); no cut 512 rows 82 us;
 // top-p .95 64 rows 51 us, .9 512 rows 238 us; top-k 50 256 rows 34 us; one row of 32000 f32 with top-k
 // 50 and top-p .9 12.7 us.
-#include <cfloat>
-
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -472,7 +470,7 @@ __global__ void __launch_bounds__(kBlock<SEARCH>, SEARCH ? 2 : 4) sample_kernel(
     return;
   }
   scale.temperature = temperature;
-  scale.inv_t = fmaxf(1.f / temperature, FLT_MIN);  // not 0: -inf has to stay at -inf
+  scale.inv_t = fmaxf(1.f / temperature, __int_as_float(1));  // not 0 of an infinite T: -inf has to stay at -inf
   const float uniform = g.uniforms[row];
   auto target_of = [&](uint64_t total) -> uint64_t {
     const double place = floor(static_cast<double>(uniform) * static_cast<double>(total));
