@@ -6,8 +6,8 @@
 // The recurrence is linear, so a stretch of steps maps the state before it to P h + H with P the
 // product of its gates (marked where a reset cuts it). A lane has two neighbouring channels, a warp 64; both are computed in f32x2
 // instructions. Two schemes, each bound by issue slots and latencies before HBM:
-//  - tiles (the forward where the channels fill the GPU: 28 blocks of 64 and more, rows of the batch counted): a warp scans a run
-//    of steps in registers, the runs' maps are exchanged, and the run is scanned again from the state
+//  - tiles (the forward where the channels fill the GPU: 28 blocks of 64 and more, in f32 19, rows of the
+//    batch counted; and of short sequences): a warp scans a run of steps in registers, the runs' maps are exchanged, and the run is scanned again from the state
 //    before it. Gate and value are read and turned into gates once; every tile waits for a barrier.
 //  - segments (the backward, and the forward of few channels): each warp has a stretch of the sequence
 //    of its own and goes over it twice without waiting for any other, first for the stretch's map, then,
@@ -131,8 +131,9 @@ __device__ __forceinline__ void store_pair(T *p, float2 v, bool on0, bool on1) {
   }
 }
 
-// a and c = 1 - a. The smaller one, m = e / (1 + e) with e = exp(-|f|), has its full relative
-// accuracy; the larger is 1 - m, the f32 next to it.
+// a and c = 1 - a. The smaller one, m = e / (1 + e) with e = exp(-|f|), does not cancel: it is off by
+// |f| 2^-24 of itself (the rounding of exp's argument) and some 2^-22 (the approximate units), and is 0
+// where e is below 2^-126. The larger is 1 - m, the f32 next to it.
 __device__ __forceinline__ void gates1(float f, float &a, float &c) {
   const float e = exp2_approx(fabsf(f) * -1.4426950408889634f);
   const float m = e * rcp_approx(1.f + e), o = 1.f - m;
@@ -178,7 +179,8 @@ struct RecurrenceArgs {
   float *grad_h0;
 };
 
-// What a launch does: both passes with a cluster's exchange between them, or one of the two.
+// What a launch does: both passes with a cluster's exchange between them (the backward), or one of the
+// two.
 enum Pass { kBoth = 0, kMaps = 1, kApply = 2 };
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -414,6 +416,7 @@ struct Items {
 template <typename T, bool TMA, bool PAIRED, int PASS>
 __global__ void __launch_bounds__(kThreads, TMA && sizeof(T) == 2 ? 3 : 2)
     recurrence_forward_kernel(const RecurrenceArgs g, const __grid_constant__ SequenceMaps maps) {
+  static_assert(PASS != kBoth, "a forward in one launch goes by tiles");
   extern __shared__ __align__(128) uint8_t dynamic[];
   __shared__ Exchange ex;
   __shared__ uint64_t full[kWarps][4];
@@ -602,8 +605,7 @@ __device__ __forceinline__ float2 tile_exchange(TileExchange &ex, int buf, float
   float2 in = state;
   if (ranks == 1) {
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const int w = i;
+    for (int w = 0; w < kWarps; ++w) {
       if (w == warp) in = state;
       state = apply_run(ex.p[buf][w][lane], state, ex.h[buf][w][lane], cuts);
     }
@@ -612,8 +614,7 @@ __device__ __forceinline__ float2 tile_exchange(TileExchange &ex, int buf, float
   if (warp < ranks) {  // the CTA's map, to one CTA a warp
     float2 cp = make_float2(1.f, 1.f), ch = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const int w = i;
+    for (int w = 0; w < kWarps; ++w) {
       const float2 pw = ex.p[buf][w][lane];
       ch = apply_run(pw, ch, ex.h[buf][w][lane], cuts);
       cp = join_runs(cp, pw, cuts);
@@ -628,8 +629,7 @@ __device__ __forceinline__ float2 tile_exchange(TileExchange &ex, int buf, float
     state = apply_run(make_float2(m.x, m.y), state, make_float2(m.z, m.w), cuts);
   }
 #pragma unroll
-  for (int i = 0; i < kWarps - 1; ++i) {
-    const int w = i;
+  for (int w = 0; w < kWarps - 1; ++w) {
     if (w < warp) in = apply_run(ex.p[buf][w][lane], in, ex.h[buf][w][lane], cuts);
   }
   return in;
@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_tiles_kernel(const Rec
   const T *value = static_cast<const T *>(g.value) + batch * g.value_batch + at.from;
   T *out = static_cast<T *>(g.h) + batch * g.steps * g.dim + ch;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
-  const int64_t first = 0, stop = g.steps;
+  const int64_t stop = g.steps;
   if (g.chunks > 1) cluster_arrive();
 
   Raw<T> rf[kLong], rx[kLong];
@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_tiles_kernel(const Rec
       }
     }
   };
-  load(first + rank * kTile + warp * kLong);
+  load(rank * kTile + warp * kLong);
   float2 state = make_float2(0.f, 0.f);  // the state before the cluster's tiles, the same in every warp
   if (g.h0 != nullptr) {
     const float *p = g.h0 + batch * g.dim + ch;
@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_tiles_kernel(const Rec
   if (g.chunks > 1) cluster_wait();
 
   int buf = 0;
-  for (int64_t tile = first; tile < stop; tile += int64_t(g.chunks) * kTile, buf ^= 1) {
+  for (int64_t tile = 0; tile < stop; tile += int64_t(g.chunks) * kTile, buf ^= 1) {
     const int64_t t0 = tile + rank * kTile + warp * kLong;
     const int n = static_cast<int>(t0 >= stop ? 0 : min64(kLong, stop - t0));
     const uint32_t cut = reset_bits(reset, t0, n);
@@ -792,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int64_t ch = ch0 + 2 * lane;
   const bool on = ch < g.dim;
   const uint8_t *reset = g.reset != nullptr ? g.reset + batch * g.steps : nullptr;
-  const int64_t first = 0, stop = g.steps;
+  const int64_t stop = g.steps;
   const int64_t stride = int64_t(g.chunks) * kTile;
   T *ring = reinterpret_cast<T *>(dynamic) + size_t(warp) * kStages * 2 * kLong * kChan;
   auto stage = [&](int s) -> T * { return ring + s * 2 * kLong * kChan; };
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
   if (g.chunks > 1) cluster_arrive();
   if (threadIdx.x == 0) abort = 0;
-  const int64_t t_first = first + rank * kTile + warp * kLong;
+  const int64_t t_first = rank * kTile + warp * kLong;
   if (lane == 0) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) sm100::mbar_init(&full[warp][s], 1);
@@ -826,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   int buf = 0, s = 0;
   uint32_t parity = 0;
   bool alive = true;
-  for (int64_t tile = first, t0 = t_first; tile < stop; tile += stride, t0 += stride, buf ^= 1) {
+  for (int64_t tile = 0, t0 = t_first; tile < stop; tile += stride, t0 += stride, buf ^= 1) {
     const int n = static_cast<int>(t0 >= stop ? 0 : min64(kLong, stop - t0));
     const uint32_t cut = __ballot_sync(0xffffffffu, flag != 0);
     flag = flag_of(t0 + stride);
@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       // A wait that runs out, as in Stream::wait.
       alive = sm100::mbar_wait(&full[warp][s], parity, &abort, &g_recurrence_error);
       if (!alive && lane == 0) {
-        for (int i = 0, at = s, p = parity; i < kStages - (tile > first ? 1 : 0) && t0 + i * stride < stop; ++i) {
+        for (int i = 0, at = s, p = parity; i < kStages - (tile > 0 ? 1 : 0) && t0 + i * stride < stop; ++i) {
           sm100::mbar_drain(&full[warp][at], p);
           if (++at == kStages) {
             at = 0;
@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       sm100::bulk_commit();
       // The stage before this one has been read by its store: its next tile comes in.
       bulk_wait_read<1>();
-      if (tile > first && alive) fetch(t0 + (kStages - 1) * stride, s == 0 ? kStages - 1 : s - 1);
+      if (tile > 0 && alive) fetch(t0 + (kStages - 1) * stride, s == 0 ? kStages - 1 : s - 1);
     }
     if (++s == kStages) {
       s = 0;
@@ -1162,7 +1162,9 @@ Plan plan_for(int64_t units, int64_t runs, int64_t slots) {
   return p;
 }
 int64_t units_of(int64_t batch, int64_t dim) { return batch * ceil_div(dim, kChan); }
-int64_t slots_of(bool forward, int dtype) { return 148 * (dtype == TROPNN_B200_F32 || !forward ? 2 : 3); }
+// CTAs on the GPU at once. The SMs are a constant: the workspace query must not need a device.
+constexpr int kSms = 148;
+int64_t slots_of(bool forward, int dtype) { return kSms * (dtype == TROPNN_B200_F32 || !forward ? 2 : 3); }
 size_t maps_bytes(const Plan &p, int64_t batch, int64_t dim) {
   return p.two_launches ? static_cast<size_t>(batch * p.chunks * kMapSlots * dim) * sizeof(float2) : 0;
 }
@@ -1225,7 +1227,7 @@ template <typename T, bool TMA, bool PAIRED>
 int launch_tiles(const char *what, RecurrenceArgs g, SequenceMaps &maps, int64_t units, cudaStream_t stream) {
   const int64_t tiles = ceil_div(g.steps, kWarps * kTileRun<T>);
   g.chunks = 1;  // CTAs of a cluster, two of them an SM in all
-  while (g.chunks < kMaxCluster && units * g.chunks * 2 <= 2 * 148 && g.chunks * 2 <= tiles) g.chunks *= 2;
+  while (g.chunks < kMaxCluster && units * g.chunks * 2 <= 2 * kSms && g.chunks * 2 <= tiles) g.chunks *= 2;
   const void *kernel = TMA ? reinterpret_cast<const void *>(recurrence_tiles_tma_kernel<T>)
                            : reinterpret_cast<const void *>(recurrence_tiles_kernel<T, PAIRED>);
   return launch_clusters(what, kernel, TMA ? kTileRingBytes<T> : 0, units * g.chunks, g.chunks, g, maps, stream);
