@@ -21,10 +21,11 @@
 // a row's maximum below 2^-126 are 0, in the sums as in the gradient.
 //
 // Measured (bf16): the loss of 8192 x 131072 335 us (6.4 TB/s, 98 % of a copy's rate), the gradient 683 us
-// (6.3 TB/s), both HBM-bound; in one call 877 us (4.9 TB/s), bound by how the three CTAs of an SM overlap
-// their loads, exponentials (476 us of that unit) and stores. 4096 x 32000 with labels at T = 2: 56 us,
-// 84 us and 106 us. In one call four CTAs an SM with six slices a row take 975 us, eight slices 1141; with
-// the row read again instead of kept 2048 x 131072 takes 247 us and not 227, 1 x 131072 7.4 and not 6.6.
+// (6.3 TB/s), both HBM-bound; in one call 905 to 950 us by the box (4.5 to 4.7 TB/s), bound by how the
+// three CTAs of an SM overlap their loads, exponentials (476 us of that unit) and stores. 4096 x 32000 with
+// labels at T = 2: 56 us, 84 us and 106 us. In one call, where it took 875 us, four CTAs an SM with six
+// slices a row took 975 and eight slices 1141; with the row read again instead of kept 2048 x 131072 takes
+// 247 us and not 227, 1 x 131072 7.4 and not 6.6.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
