@@ -447,6 +447,47 @@ def test_forward_mode_is_refused(grad_mode) -> None:
                 call()
 
 
+def test_saved_tensors_may_come_back_with_other_strides() -> None:
+    from .test_recurrence_gpu import _elsewhere
+
+    logits, teacher, at, labels = _inputs(5, 700, 9, torch.float32, 37)
+    leaf = logits.requires_grad_()
+    kw = dict(temperature=2.0, label_weight=0.25)
+    (want,) = torch.autograd.grad(tropnn_b200.distill_loss_b200(leaf, teacher, at, labels, **kw), leaf)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _elsewhere):
+        (got,) = torch.autograd.grad(tropnn_b200.distill_loss_b200(leaf, teacher, at, labels, **kw), leaf)
+    assert torch.equal(got, want)
+
+
+def test_calls_in_a_cuda_graph() -> None:
+    """Loss, gradient, both in one call and a draw captured once and replayed on other inputs."""
+    logits, teacher, at, labels = _inputs(6, 3001, 9, torch.bfloat16, 38)
+    leaf, u = logits.clone().requires_grad_(), torch.rand(6, generator=torch.Generator().manual_seed(1)).cuda()
+    kw = dict(temperature=2.0, label_weight=0.25)
+
+    def calls():
+        loss = tropnn_b200.distill_loss_b200(leaf, teacher, at, labels, **kw)
+        (grad,) = torch.autograd.grad(loss, leaf)
+        tokens = tropnn_b200.sample_tokens_b200(leaf, u, top_k=40, top_p=0.9)
+        return [loss.detach(), grad, *tropnn_b200.distill_loss_grad_b200(leaf.detach(), teacher, at, labels, **kw), tokens]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        calls()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    with torch.no_grad():
+        leaf.copy_(logits.roll(1, dims=0))
+        teacher.neg_()
+        u.copy_(1 - u)
+    graph.replay()
+    got = [t.clone() for t in out]
+    assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+
+
 def test_refusals() -> None:
     op = tropnn_b200.distill_loss_b200
     x, t = torch.zeros(2, 9, device="cuda"), torch.zeros(2, 3, device="cuda")

@@ -395,6 +395,57 @@ def test_forward_mode_is_refused(grad_mode) -> None:
                 tropnn_b200.gated_recurrence_step_b200(*row)
 
 
+def _elsewhere(t):
+    """The same numbers with other strides, as a saved-tensor hook may bring them back."""
+    room = torch.full((2, *reversed(t.shape)), 0, dtype=t.dtype, device=t.device)
+    return room[0].permute(tuple(reversed(range(t.ndim)))).copy_(t.detach())
+
+
+def test_saved_tensors_may_come_back_with_other_strides() -> None:
+    gate, value, h0 = _inputs(2, 90, 48, torch.float32, 18)
+    reset = (torch.rand(2, 90, generator=torch.Generator().manual_seed(4)) < 0.1).cuda()
+    leaves = [t.requires_grad_() for t in (gate, value, h0)]
+    want = torch.autograd.grad(tropnn_b200.gated_recurrence_b200(*leaves, reset=reset)[0].sum(), leaves)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _elsewhere):
+        h, _ = tropnn_b200.gated_recurrence_b200(*leaves, reset=reset)
+        got = torch.autograd.grad(h.sum(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_in_a_cuda_graph() -> None:
+    """Forward, backward and steps captured once and replayed on other inputs."""
+    gate, value, h0 = _inputs(2, 400, 64, torch.bfloat16, 19)
+    long_gate, long_value, _ = _inputs(1, 12000, 32, torch.bfloat16, 20)
+    leaves = [t.clone().requires_grad_() for t in (gate, value, h0)]
+    state = h0.clone()
+
+    def calls():
+        h, last = tropnn_b200.gated_recurrence_b200(*leaves)
+        grads = torch.autograd.grad(h, leaves, torch.ones_like(h))
+        with torch.no_grad():
+            far, _ = tropnn_b200.gated_recurrence_b200(long_gate, long_value)
+            step = tropnn_b200.gated_recurrence_step_b200(leaves[0][:, 0], leaves[1][:, 0], state)
+        return [h.detach(), last.detach(), *grads, far, step]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        calls()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    with torch.no_grad():
+        for t in leaves:
+            t.neg_()
+        long_value.neg_()
+        state.copy_(h0)
+    graph.replay()
+    got = [t.clone() for t in out]
+    state.copy_(h0)
+    assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+
+
 def test_refusals() -> None:
     op, step = tropnn_b200.gated_recurrence_b200, tropnn_b200.gated_recurrence_step_b200
     t = torch.zeros(2, 3, 4, device="cuda")

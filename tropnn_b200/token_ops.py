@@ -114,6 +114,14 @@ class _GatedRecurrenceFunction(torch.autograd.Function):
             return None, None, None, None
         gate, value, reset, saved = ctx.saved_tensors
         batch, steps, dim = shape = tuple(gate.shape)
+        # Hooks may bring a saved tensor back with other strides.
+        gate_batch, gate_step, unit = gate.stride()
+        value_batch, value_step, value_unit = value.stride()
+        if unit != 1 or value_unit != 1:
+            gate, value = gate.contiguous(), value.contiguous()
+            gate_batch, gate_step = value_batch, value_step = steps * dim, dim
+        saved = saved.contiguous()
+        reset = None if reset is None else reset.contiguous()
         lib = nat.load()
         grad_h = None if grad_h is None else grad_h.contiguous()
         grad_last = None if grad_last is None else grad_last.contiguous()
@@ -122,9 +130,9 @@ class _GatedRecurrenceFunction(torch.autograd.Function):
         grad_h0 = saved.new_empty((batch, dim)) if ctx.needs_input_grad[2] else None
         ws, ws_bytes = _recurrence_workspace(lib, gate, shape)
         _call(
-            gate.device, "recurrence_backward", lib.tropnn_b200_recurrence_backward, gate.data_ptr(), gate.stride(0),
-            gate.stride(1), value.data_ptr(), value.stride(0), value.stride(1), nat.float_code(gate.dtype),
-            nat.ptr(reset), batch, steps, dim, saved.data_ptr(), saved.numel() * 4, nat.ptr(grad_h), nat.ptr(grad_last),
+            gate.device, "recurrence_backward", lib.tropnn_b200_recurrence_backward, gate.data_ptr(), gate_batch,
+            gate_step, value.data_ptr(), value_batch, value_step, nat.float_code(gate.dtype), nat.ptr(reset), batch,
+            steps, dim, saved.data_ptr(), saved.numel() * 4, nat.ptr(grad_h), nat.ptr(grad_last),
             grad_gate.data_ptr(), grad_value.data_ptr(), nat.ptr(grad_h0), nat.ptr(ws), ws_bytes,
         )
         return grad_gate, grad_value, grad_h0, None
@@ -336,6 +344,9 @@ class _DistillLossFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx: Any, grad_loss: Tensor) -> tuple[Any, ...]:
         logits, stats, count, teacher, indices, labels = ctx.saved_tensors
+        # Hooks may bring a saved tensor back with other strides.
+        stats, teacher, indices = stats.contiguous(), teacher.contiguous(), indices.contiguous()
+        labels = None if labels is None else labels.contiguous()
         read, _, args = _distill_args(logits, teacher, indices, labels, ctx.settings)
         grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
         scale = grad_loss.contiguous()
